@@ -250,6 +250,22 @@ int hp_philox(hp_ctx* ctx, int dtype, int dist, void* out, int64_t count, uint64
  * Replaces: _random.py:19-31 (_philox_numpy) on the device. */
 int hp_philox_words(hp_ctx* ctx, uint32_t* out, int64_t count, uint64_t seed, uint64_t start);
 
+/* ---- operators of model training ----------------------------------------- */
+
+/* Gated linear recurrence over `time` of x (batch, time, channels):
+ * h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(gate_t), with gates (batch,
+ * time, gates) each shared by channels / gates neighbouring channels. `initial`
+ * (batch, channels) is h_{-1}, zero if NULL; where the bool `resets` (batch,
+ * time) is set, h_{t-1} counts as zero (NULL: nowhere). float32 or float64. */
+int hp_gated_recurrence(hp_ctx* ctx, int dtype, const void* x, const void* gate, const void* initial,
+                        const void* resets, void* h, int64_t batch, int64_t time, int64_t channels, int64_t gates);
+
+/* Its gradients: dx, dgate (summed over the channels of a gate) and, unless
+ * NULL, dinitial, from the gradient `grad` of the states h. */
+int hp_gated_recurrence_grad(hp_ctx* ctx, int dtype, const void* grad, const void* x, const void* gate, const void* h,
+                             const void* initial, const void* resets, void* dx, void* dgate, void* dinitial,
+                             int64_t batch, int64_t time, int64_t channels, int64_t gates);
+
 /* ---- runtime compilation for fused elementwise / map-reduce kernels ------ */
 
 /* Compile HIP source with hipRTC for gfx950 and load `name` from it.

@@ -686,6 +686,18 @@ class HIPBackend:
             )
         return out
 
+    # ---- operators of nn ---------------------------------------------------------------
+
+    def gated_recurrence(self, *args):
+        from ._hip_nn import gated_recurrence
+
+        return gated_recurrence(self, *args)
+
+    def gated_recurrence_grad(self, *args):
+        from ._hip_nn import gated_recurrence_grad
+
+        return gated_recurrence_grad(self, *args)
+
     # ---- protocol: compilation and lifetime -------------------------------------------
 
     def create_lowering(self):

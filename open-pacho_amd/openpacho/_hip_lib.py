@@ -64,6 +64,8 @@ PROTOTYPES = {
     "hp_reduce": [_ptr, _i32, _i32, _ptr, _ptr, _i64, _i64, _i64],
     "hp_philox": [_ptr, _i32, _i32, _ptr, _i64, _u64, _u64, ctypes.c_double, ctypes.c_double, ctypes.c_double],
     "hp_philox_words": [_ptr, _ptr, _i64, _u64, _u64],
+    "hp_gated_recurrence": [_ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64],
+    "hp_gated_recurrence_grad": [_ptr, _i32] + [_ptr] * 9 + [_i64] * 4,
     "hp_rtc_compile": [_ptr, _cstr, _cstr, _pptr],
     "hp_rtc_launch": [_ptr, _ptr, _i64, _i32, _i32, _pptr],
     "hp_rtc_launch_packed": [_ptr, _ptr, _i64, _i32, _cstr, _i64],

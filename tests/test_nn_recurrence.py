@@ -1,0 +1,134 @@
+"""``nn.gated_recurrence`` on the NumPy backend: values against the definition,
+gradients against it and against differences, and what it refuses."""
+
+import numpy as np
+import pytest
+
+import openpacho as p
+from oracle import training
+
+SIZES = [(1, 1, 1, 1), (3, 1, 5, 5), (2, 7, 6, 6), (2, 9, 6, 2), (1, 30, 4, 1), (0, 3, 4, 2), (2, 0, 4, 4), (2, 3, 0, 0)]
+# Units of rounding a step: 4 of each gate, 2 products and a sum, and as many again for steps composed in another order.
+UNITS = 20
+
+
+def make(sizes, dtype, seed=0, state=True, resets=True):
+    batch, time, channels, gates = sizes
+    rng = np.random.default_rng(seed)
+    x, d = (rng.standard_normal((batch, time, channels)).astype(dtype) for _ in range(2))
+    gate = (2 * rng.standard_normal((batch, time, gates)) + 1).astype(dtype)
+    initial = rng.standard_normal((batch, channels)).astype(dtype) if state else None
+    starts = rng.random((batch, time)) < 0.15 if resets else None
+    return x, gate, initial, starts, d
+
+
+def put(backend, *values):
+    return [None if v is None else p.asarray(v, backend=backend) for v in values]
+
+
+def near(got, want, size, dtype, units=UNITS):
+    bound = units * np.finfo(dtype).eps / 2 * size + np.finfo(dtype).tiny
+    error = np.abs(got.astype(training.WIDE) - want)
+    assert got.dtype == dtype and got.shape == want.shape
+    assert np.all(error <= bound), float(np.max(error / bound))
+
+
+def check(backend, sizes, dtype, state, resets):
+    x, gate, initial, starts, d = make(sizes, dtype, sum(sizes), state, resets)
+    xs, gs, first, rs, ds = put(backend, x, gate, initial, starts, d)
+    want, size = training.recurrence(x, gate, initial, starts)
+    h = p.nn.gated_recurrence(xs, gs, first, resets=rs)
+    near(p.asnumpy(h), want, size, dtype)
+    states = p.asnumpy(h)
+    values, bounds = training.recurrence_grad(d, x, gate, states, initial, starts)
+    found = p.nn.gated_recurrence_grad(ds, xs, gs, h, first, resets=rs)
+    assert (found[2] is None) == (initial is None)
+    for got, want, size in zip(found, values, bounds):
+        if got is not None:
+            near(p.asnumpy(got), want, size, dtype)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("state,resets", [(True, True), (False, False), (True, False)])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_values_and_gradients(numpy_backend, sizes, state, resets, dtype):
+    check(numpy_backend, sizes, dtype, state, resets)
+
+
+def test_gradients_match_differences(numpy_backend):
+    x, gate, initial, starts, d = make((2, 6, 4, 2), np.float64, 3)
+
+    def value(x, gate, initial):
+        return float((d * p.asnumpy(p.nn.gated_recurrence(*put(numpy_backend, x, gate, initial), resets=p.asarray(starts)))).sum())
+
+    given = [x, gate, initial]
+    h = p.nn.gated_recurrence(*put(numpy_backend, *given), resets=p.asarray(starts))
+    found = p.nn.gated_recurrence_grad(p.asarray(d), *put(numpy_backend, x, gate), h, p.asarray(initial), resets=p.asarray(starts))
+    step = 1e-6
+    for which, got in enumerate(found):
+        got = p.asnumpy(got)
+        for at in np.ndindex(got.shape):
+            ends = []
+            for sign in (1, -1):
+                moved = [v.copy() for v in given]
+                moved[which][at] += sign * step
+                ends.append(value(*moved))
+            # Central differences: third derivatives of order 1 times step^2, rounding of the sum over the step.
+            assert abs(got[at] - (ends[0] - ends[1]) / (2 * step)) < 1e-8
+
+
+def test_a_step_is_one_token_of_the_recurrence(numpy_backend):
+    x, gate, initial, _, _ = make((3, 1, 6, 2), np.float32)
+    whole = p.asnumpy(p.nn.gated_recurrence(*put(numpy_backend, x, gate, initial)))
+    step = p.nn.gated_recurrence_step(*put(numpy_backend, x[:, 0], gate[:, 0], initial))
+    np.testing.assert_array_equal(p.asnumpy(step), whole[:, 0])
+
+
+def test_leading_axes_and_host_values(numpy_backend):
+    x, gate, initial, starts, _ = make((6, 5, 4, 4), np.float32)
+    flat = p.asnumpy(p.nn.gated_recurrence(*put(numpy_backend, x, gate, initial), resets=p.asarray(starts)))
+    shaped = [v.reshape((2, 3) + v.shape[1:]) for v in (x, gate, initial)]
+    got = p.nn.gated_recurrence(p.asarray(shaped[0]), shaped[1], shaped[2], resets=starts.reshape(2, 3, 5))
+    np.testing.assert_array_equal(p.asnumpy(got), flat.reshape(2, 3, 5, 4))
+    alone = p.nn.gated_recurrence(p.asarray(x[0]), p.asarray(gate[0]), p.asarray(initial[0]), resets=starts[0])
+    np.testing.assert_array_equal(p.asnumpy(alone), flat[0])
+
+
+def test_refusals(numpy_backend):
+    x, gate = p.zeros((2, 3, 4), dtype="float32"), p.zeros((2, 3, 4), dtype="float32")
+    f = p.nn.gated_recurrence
+    for bad in (p.zeros((4,), dtype="float32"), p.zeros((2, 3, 6), dtype="float32")):
+        with pytest.raises(ValueError):
+            f(bad, gate)
+    with pytest.raises(ValueError, match="do not divide"):
+        f(x, p.zeros((2, 3, 3), dtype="float32"))
+    with pytest.raises(ValueError, match="without channels"):
+        f(p.zeros((2, 3, 0), dtype="float32"), gate)
+    with pytest.raises(ValueError, match="gates"):
+        f(x, p.zeros((2, 3, 0), dtype="float32"))
+    with pytest.raises(ValueError):
+        f(x, p.zeros((2, 4, 4), dtype="float32"))
+    with pytest.raises(ValueError, match="initial"):
+        f(x, gate, p.zeros((4,), dtype="float32"))
+    with pytest.raises(ValueError, match="resets"):
+        f(x, gate, resets=np.zeros((2,), bool))
+    with pytest.raises(p.UnsupportedDtypeError):
+        f(x, gate, resets=p.zeros((2, 3), dtype="int32"))
+    with pytest.raises(p.UnsupportedDtypeError):
+        f(x, gate, resets=np.zeros((2, 3)))
+    with pytest.raises(p.UnsupportedDtypeError):
+        f(x, p.zeros((2, 3, 4), dtype="float64"))
+    with pytest.raises(p.UnsupportedDtypeError):
+        f(p.zeros((2, 3, 4), dtype="int32"), gate)
+    with pytest.raises(ValueError, match="grad"):
+        p.nn.gated_recurrence_grad(p.zeros((2, 3), dtype="float32"), x, gate, x)
+    with pytest.raises(ValueError, match="h must"):
+        p.nn.gated_recurrence_grad(x, x, gate, p.zeros((2, 3), dtype="float32"))
+    with pytest.raises(ValueError):
+        p.nn.gated_recurrence_step(p.zeros((), dtype="float32"), p.zeros((), dtype="float32"), x)
+    with pytest.raises(ValueError, match="initial"):
+        p.nn.gated_recurrence_step(x, gate, p.zeros((2, 3), dtype="float32"))
+    with pytest.raises(NotImplementedError, match="not captured"):
+        p.compile(lambda x, g: f(x, g))(x, gate)
+    with pytest.raises(NotImplementedError, match="not captured"):
+        p.fuse(lambda x, g: f(x, g))(x, gate)
