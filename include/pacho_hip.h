@@ -266,6 +266,32 @@ int hp_gated_recurrence_grad(hp_ctx* ctx, int dtype, const void* grad, const voi
                              const void* initial, const void* resets, void* dx, void* dgate, void* dinitial,
                              int64_t batch, int64_t time, int64_t channels, int64_t gates);
 
+/* log softmax(logits) of rows x vocab logits at their `targets` (index_dtype
+ * HP_I32 or HP_I64); 0 for rows whose byte of `mask` (NULL: none) is 0, which
+ * are not read; NaN for another target outside the vocabulary. */
+int hp_token_log_probs(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, const void* targets,
+                       const void* mask, void* log_probs, int64_t rows, int64_t vocab);
+
+/* Clipped policy loss over the rows that `mask` keeps: the sum of
+ * -min(r A, clip(r, 1 - low, 1 + high) A) + kl_weight (exp(d) - d - 1) divided by
+ * `count`, or by the number of rows kept (at least 1) if count is 0, where r =
+ * exp(log_prob - old) and d = reference - log_prob (reference NULL: no such term).
+ * Writes the 0-d loss, the log-probabilities as hp_token_log_probs, and unless
+ * NULL the gradient of the logits. */
+int hp_policy_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, const void* actions, const void* old,
+                   const void* advantages, const void* reference, const void* mask, void* loss, void* log_probs,
+                   void* grad, int64_t rows, int64_t vocab, double low, double high, double kl_weight, double count);
+
+/* Preference loss of (2, pairs, time, vocab) logits, the chosen responses and
+ * then the rejected ones: the mean over pairs (0 of none) of
+ * -(1 - smoothing) log sigmoid(m) - smoothing log sigmoid(-m) with m = beta times
+ * the difference of the responses' summed log-probabilities less their
+ * `reference` (2, pairs). Writes the 0-d loss, the sums (2, pairs) and unless
+ * NULL the gradient of the logits. */
+int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, const void* targets,
+                       const void* reference, const void* mask, void* loss, void* sums, void* grad, int64_t pairs,
+                       int64_t time, int64_t vocab, double beta, double smoothing);
+
 /* ---- runtime compilation for fused elementwise / map-reduce kernels ------ */
 
 /* Compile HIP source with hipRTC for gfx950 and load `name` from it.

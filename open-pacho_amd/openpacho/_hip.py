@@ -698,6 +698,21 @@ class HIPBackend:
 
         return gated_recurrence_grad(self, *args)
 
+    def token_log_probs(self, *args):
+        from ._hip_nn import token_log_probs
+
+        return token_log_probs(self, *args)
+
+    def policy_loss(self, *args):
+        from ._hip_nn import policy_loss
+
+        return policy_loss(self, *args)
+
+    def preference_loss(self, *args):
+        from ._hip_nn import preference_loss
+
+        return preference_loss(self, *args)
+
     # ---- protocol: compilation and lifetime -------------------------------------------
 
     def create_lowering(self):

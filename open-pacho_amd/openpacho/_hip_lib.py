@@ -66,6 +66,9 @@ PROTOTYPES = {
     "hp_philox_words": [_ptr, _ptr, _i64, _u64, _u64],
     "hp_gated_recurrence": [_ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64],
     "hp_gated_recurrence_grad": [_ptr, _i32] + [_ptr] * 9 + [_i64] * 4,
+    "hp_token_log_probs": [_ptr, _i32, _i32] + [_ptr] * 4 + [_i64] * 2,
+    "hp_policy_loss": [_ptr, _i32, _i32] + [_ptr] * 9 + [_i64] * 2 + [ctypes.c_double] * 4,
+    "hp_preference_loss": [_ptr, _i32, _i32] + [_ptr] * 7 + [_i64] * 3 + [ctypes.c_double] * 2,
     "hp_rtc_compile": [_ptr, _cstr, _cstr, _pptr],
     "hp_rtc_launch": [_ptr, _ptr, _i64, _i32, _i32, _pptr],
     "hp_rtc_launch_packed": [_ptr, _ptr, _i64, _i32, _cstr, _i64],

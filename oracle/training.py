@@ -69,3 +69,102 @@ def recurrence_grad(grad, x, gate, h, initial=None, resets=None):
         if resets is not None:
             carried, size = (np.where(resets[:, t, None], 0, v) for v in (carried, size))
     return (dx, d_gate, carried), (dx_size, gate_size, size)
+
+
+# ---- losses from logits ----------------------------------------------------------
+#
+# Bounds are in units of rounding u of the operator's type. A row's sum of
+# exponentials loses 50 u in its terms' own rounding and the sum's order (an
+# exponential 4, a tree and chains of at most some tens of additions), and
+# D = sum_j p_j |z_j - max| u from the subtractions; its logarithm and the
+# differences add their own sizes.
+
+
+class Row:
+    """One row of logits and its target."""
+
+    def __init__(self, logits, target):
+        z = np.asarray(logits).astype(WIDE)
+        top = z.max()
+        terms = np.exp(z - top)
+        total = terms.sum()
+        self.p, self.target = terms / total, target
+        self.distance = np.where(self.p > 0, np.abs(z - top), 0)
+        self.total_units = 50 + (self.p * self.distance).sum()
+        self.log_prob = z[target] - top - np.log(total)
+        self.units = self.total_units + 3 * abs(np.log(total)) + 2 * abs(z[target] - top) + abs(self.log_prob)
+
+    def grad(self, weight, weight_units):
+        """weight (1[target] - p), and its bound for a weight that is off by weight_units."""
+        one = np.zeros_like(self.p)
+        one[self.target] = 1
+        p_units = 6 + self.distance + self.total_units
+        bound = weight_units * np.abs(one - self.p) + abs(weight) * (self.p * p_units + 2 * one)
+        return weight * (one - self.p), bound
+
+
+def token_log_probs(logits, targets, mask=None):
+    """(values, bounds in units of rounding) over rows of logits (rows, vocabulary)."""
+    values, units = np.zeros(len(logits), WIDE), np.zeros(len(logits), WIDE)
+    for i in range(len(logits)):
+        if mask is None or mask[i]:
+            row = Row(logits[i], targets[i])
+            values[i], units[i] = row.log_prob, row.units
+    return values, units
+
+
+def policy_loss(logits, actions, old, advantages, reference=None, mask=None, clip=(0.2, 0.2), kl_weight=0.0, count=None):
+    """((loss, log_probs, gradient), their bounds, rows whose ratio is so near an end of the clip
+    that rounding decides between the sides), over rows of logits."""
+    old, advantages, reference = _wide(old, advantages, reference)
+    n = len(logits)
+    log_probs, units = np.zeros(n, WIDE), np.zeros(n, WIDE)
+    grad, bounds = np.zeros(np.shape(logits), WIDE), np.zeros(np.shape(logits), WIDE)
+    loss, loss_units, undecided = WIDE(0), WIDE(0), np.zeros(n, bool)
+    kept = range(n) if mask is None else np.flatnonzero(mask)
+    if count is None:
+        count = max(1, len(kept))
+    low, high = 1 - WIDE(clip[0]), 1 + WIDE(clip[1])
+    for i in kept:
+        row = Row(logits[i], actions[i])
+        log_probs[i], units[i] = row.log_prob, row.units
+        ratio = np.exp(row.log_prob - old[i])
+        ratio_units = ratio * (row.units + abs(row.log_prob - old[i]) + 3)
+        undecided[i] = min(abs(ratio - low), abs(ratio - high)) <= ratio_units * 2.0**-23 + 2.0**-22
+        free, held = ratio * advantages[i], min(max(ratio, low), high) * advantages[i]
+        stopped = free > held
+        each, slope = -min(free, held), 0 if stopped else -free
+        each_units = abs(advantages[i]) * ratio_units + 4 * abs(free)
+        if reference is not None and kl_weight:
+            apart = reference[i] - row.log_prob
+            apart_units = row.units + abs(apart)
+            each = each + kl_weight * (np.expm1(apart) - apart)
+            slope = slope - kl_weight * np.expm1(apart)
+            each_units += kl_weight * ((np.exp(apart) + 1) * apart_units + 4 * abs(np.expm1(apart)) + 2 * abs(apart))
+        loss, loss_units = loss + each, loss_units + each_units + abs(each)
+        grad[i], bounds[i] = row.grad(slope / count, (each_units + 4 * abs(slope)) / count)
+    return (loss / count, log_probs, grad), (loss_units / count, units, bounds), undecided
+
+
+def preference_loss(logits, targets, reference, mask=None, beta=0.1, smoothing=0.0):
+    """((loss, sums, gradient), their bounds) of logits (2, pairs, time, vocabulary)."""
+    _, pairs, time = np.shape(targets)
+    (reference,) = _wide(reference)
+    rows, sums, units = {}, np.zeros((2, pairs), WIDE), np.zeros((2, pairs), WIDE)
+    for at in np.ndindex(2, pairs, time):
+        if mask is None or mask[at]:
+            rows[at] = row = Row(logits[at], targets[at])
+            sums[at[:2]] += row.log_prob
+            # Twenty additions deep in float, or one rounding of a double sum.
+            units[at[:2]] += row.units + 20 * abs(row.log_prob)
+    margin = WIDE(beta) * ((sums[0] - reference[0]) - (sums[1] - reference[1]))
+    margin_units = abs(beta) * (units.sum(0) + 2 * np.abs(sums).sum(0) + 2 * np.abs(reference).sum(0)) + 4 * np.abs(margin)
+    losses = (1 - smoothing) * np.log1p(np.exp(-margin)) + smoothing * np.log1p(np.exp(margin))
+    loss_units = margin_units + 4 * (np.abs(margin) + 1)
+    n = max(1, pairs)
+    slope = beta * (smoothing * sigmoid(margin) - (1 - smoothing) * sigmoid(-margin)) / n
+    slope_units = abs(beta) * (margin_units + 8) / n
+    grad, bounds = np.zeros(np.shape(logits), WIDE), np.zeros(np.shape(logits), WIDE)
+    for at, row in rows.items():
+        grad[at], bounds[at] = row.grad(slope[at[1]] * (1 if at[0] == 0 else -1), slope_units[at[1]])
+    return (losses.sum() / n, sums, grad), (loss_units.sum() / n, units + 4 * np.abs(sums), bounds)
