@@ -292,6 +292,34 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
                        const void* reference, const void* mask, void* loss, void* sums, void* grad, int64_t pairs,
                        int64_t time, int64_t vocab, double beta, double smoothing);
 
+/* AdamW over `count` tensors of sizes[i] elements, float32 or float64. The
+ * state holds both moments in the tensors' type (bits 0) or in 8 bits with a
+ * float32 scale for every 256 elements of a tensor (bits 8, float32 tensors):
+ * the first moment's share in the block's largest in a sign, 3 exponent and 4
+ * further bits, the second's root in 4 exponent and 4 further bits. A state of
+ * zero bytes holds moments of zero.
+ *
+ * Sizes without a device: offsets[i], in elements, of each tensor within an
+ * array of *elements, as new parameters, values of moments and, for bits 0, the
+ * two arrays of a state hold them; *state_bytes of one state. */
+int hp_adamw_layout(int dtype, int bits, int64_t count, const int64_t* sizes, int64_t* offsets, int64_t* elements,
+                    int64_t* state_bytes);
+
+/* A state that holds the given moments. */
+int hp_adamw_load(hp_ctx* ctx, int dtype, int bits, int64_t count, const void* const* first, const void* const* second,
+                  const int64_t* sizes, void* state);
+
+/* The float32 values of the first (which 0) or second (1) moments of a state of
+ * 8 bits, an array of `elements`. */
+int hp_adamw_values(hp_ctx* ctx, int64_t elements, const void* state, int which, void* values);
+
+/* One step: m' = beta1 m + (1 - beta1) g, v' = beta2 v + (1 - beta2) g g and
+ * p' = p - (decays[i] p + step m' / (root sqrt(v') + eps)), into a new state and
+ * an array of new parameters. */
+int hp_adamw_step(hp_ctx* ctx, int dtype, int bits, int64_t count, const void* const* params, const void* const* grads,
+                  const int64_t* sizes, const double* decays, const void* state, void* new_state, void* new_params,
+                  double beta1, double beta2, double step, double root, double eps);
+
 /* ---- runtime compilation for fused elementwise / map-reduce kernels ------ */
 
 /* Compile HIP source with hipRTC for gfx950 and load `name` from it.

@@ -320,7 +320,10 @@ class HIPBackend:
         count = prod(shape)
         if count > _MAX_ELEMENTS:
             raise ValueError("Array exceeds GPU indexing limits")
-        capacity = max(1, count * dtype.itemsize)
+        return self.block(max(1, count * dtype.itemsize))
+
+    def block(self, capacity):
+        """Storage of `capacity` (>= 1) bytes."""
         with self._guard:
             if capacity <= _SMALL_BLOCK:
                 if self._small:
@@ -712,6 +715,21 @@ class HIPBackend:
         from ._hip_nn import preference_loss
 
         return preference_loss(self, *args)
+
+    def adamw_load(self, *args):
+        from ._hip_nn import adamw_load
+
+        return adamw_load(self, *args)
+
+    def adamw_moments(self, *args):
+        from ._hip_nn import adamw_moments
+
+        return adamw_moments(self, *args)
+
+    def adamw_step(self, *args):
+        from ._hip_nn import adamw_step
+
+        return adamw_step(self, *args)
 
     # ---- protocol: compilation and lifetime -------------------------------------------
 

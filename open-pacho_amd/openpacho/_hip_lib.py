@@ -31,7 +31,7 @@ REDUCTIONS = {"sum": 0, "min": 1, "max": 2}
 
 _i32, _i64, _u32, _u64 = ctypes.c_int, ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint64
 _ptr, _pptr, _cstr = ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p), ctypes.c_char_p
-_i64p = ctypes.POINTER(ctypes.c_int64)
+_i64p, _f64p = ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_double)
 
 # name -> argument types (every function returns int unless listed in _RESTYPES)
 PROTOTYPES = {
@@ -69,6 +69,10 @@ PROTOTYPES = {
     "hp_token_log_probs": [_ptr, _i32, _i32] + [_ptr] * 4 + [_i64] * 2,
     "hp_policy_loss": [_ptr, _i32, _i32] + [_ptr] * 9 + [_i64] * 2 + [ctypes.c_double] * 4,
     "hp_preference_loss": [_ptr, _i32, _i32] + [_ptr] * 7 + [_i64] * 3 + [ctypes.c_double] * 2,
+    "hp_adamw_layout": [_i32, _i32, _i64] + [_i64p] * 4,
+    "hp_adamw_load": [_ptr, _i32, _i32, _i64, _pptr, _pptr, _i64p, _ptr],
+    "hp_adamw_values": [_ptr, _i64, _ptr, _i32, _ptr],
+    "hp_adamw_step": [_ptr, _i32, _i32, _i64, _pptr, _pptr, _i64p, _f64p, _ptr, _ptr, _ptr] + [ctypes.c_double] * 5,
     "hp_rtc_compile": [_ptr, _cstr, _cstr, _pptr],
     "hp_rtc_launch": [_ptr, _ptr, _i64, _i32, _i32, _pptr],
     "hp_rtc_launch_packed": [_ptr, _ptr, _i64, _i32, _cstr, _i64],

@@ -320,7 +320,7 @@ def adamw_state(params, *, state_bits=None, steps=0, first=None, second=None):
     half a step of its code.
     """
     what = "adamw_state"
-    if not params:
+    if isinstance(params, (list, tuple)) and not params:
         raise ValueError(f"{what}: no tensors")
     backend, dtype, shapes = _tensors(what, "params", params)
     if state_bits not in (None, 8):

@@ -168,3 +168,59 @@ def preference_loss(logits, targets, reference, mask=None, beta=0.1, smoothing=0
     for at, row in rows.items():
         grad[at], bounds[at] = row.grad(slope[at[1]] * (1 if at[0] == 0 else -1), slope_units[at[1]])
     return (losses.sum() / n, sums, grad), (loss_units.sum() / n, units + 4 * np.abs(sums), bounds)
+
+
+# ---- AdamW ---------------------------------------------------------------------
+
+BLOCK = 256
+
+
+def adamw(p, g, m, v, steps, learning_rate, betas, eps, weight_decay):
+    """((p', m', v'), their bounds in units of rounding) of one tensor in its step `steps`, as the definition has it."""
+    p, g, m, v = _wide(p, g, m, v)
+    b1, b2, rate, decay = (WIDE(x) for x in (*betas, learning_rate, weight_decay))
+    # Constants, products and a sum: one rounding each.
+    m_units, v_units = 4 * (np.abs(b1 * m) + np.abs((1 - b1) * g)), 5 * (np.abs(b2 * v) + (1 - b2) * g * g)
+    m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    size = np.sqrt(v / (1 - b2**steps)) + eps
+    move = rate * (m / (1 - b1**steps)) / size
+    # The moment's own error, the root's (half of v's, which only sums terms >= 0), and some ten further roundings.
+    p_units = rate / (1 - b1**steps) * m_units / size + (5 + 10) * np.abs(move) + 4 * np.abs(rate * decay * p)
+    p = p - (rate * decay * p + move)
+    return (p, m, v), (p_units + np.abs(p), m_units, v_units)
+
+
+def _grid(codes, low):
+    return np.array([c * 2.0**-low if c < 16 else (16 + c % 16) * 2.0 ** (c // 16 - 1 - low) for c in range(codes + 1)])
+
+
+def _nearest(values, codes, low, positive):
+    """float32 values >= 0 by the codes' shares of their block's largest; ties between codes go to the even one."""
+    grid = _grid(codes, low)
+    held = np.empty_like(values)
+    for start in range(0, len(values), BLOCK):
+        block = values[start : start + BLOCK]
+        top = block.max()
+        if not np.isfinite(top):
+            held[start : start + BLOCK] = np.nan
+            continue
+        share = (block / top).astype(np.float64) if top > 0 else np.zeros(len(block))
+        above = np.clip(np.searchsorted(grid, share), 1, codes)
+        lower, upper = share - grid[above - 1], grid[above] - share
+        code = np.where((upper < lower) | ((upper == lower) & (above % 2 == 0)), above, above - 1)
+        if positive:
+            code = np.where(block > 0, np.maximum(code, 1), code)
+        held[start : start + BLOCK] = grid[code].astype(np.float32) * top
+    return held
+
+
+def held_first(m):
+    """What a float32 first moment stands for in 8 bits."""
+    flat = np.asarray(m, np.float32).reshape(-1)
+    held = _nearest(np.abs(flat), 112, 10, False)
+    return np.where(np.signbit(flat), -held, held).reshape(np.shape(m))
+
+
+def held_second(v):
+    flat = np.asarray(v, np.float32).reshape(-1)
+    return np.square(_nearest(np.sqrt(flat), 240, 18, True)).reshape(np.shape(v))
