@@ -41,13 +41,6 @@ struct Vec<double> {
   static constexpr int width = 2;
 };
 
-__device__ __forceinline__ float log_of(float x) { return logf(x); }
-__device__ __forceinline__ double log_of(double x) { return log(x); }
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-__device__ __forceinline__ float expm1_of(float x) { return expm1f(x); }
-__device__ __forceinline__ double expm1_of(double x) { return expm1(x); }
-__device__ __forceinline__ double log1p_of(double x) { return log1p(x); }
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
 
@@ -61,9 +54,10 @@ struct Call {
   int64_t rows, vocab;
   T* log_probs;
   T* grad;
+  double* exact;  // the log-probabilities in 64 bits (null: not wanted)
   // Policy loss (old set).
   const T *old, *advantages, *reference;
-  T low, high, kl;  // 1 - clip below, 1 + clip above, weight of the KL term
+  double low, high, kl;  // 1 - clip below, 1 + clip above, weight of the KL term
   const double* scale;  // 1 / count in device memory, or
   double scale_value;   // on the host
   double* sums;         // a workgroup's sum of losses each
@@ -76,29 +70,41 @@ struct Call {
   __device__ int64_t target(int64_t row) const {
     return wide_targets ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
   }
-  // The logit at the row's target; NaN outside the vocabulary.
-  __device__ T at_target(int64_t row, int64_t y) const {
-    return y >= 0 && y < vocab ? logits[row * vocab + y] : T(__builtin_nan(""));
+  // The log-probability of the row's target, NaN outside the vocabulary. From
+  // here on a token's terms are computed in 64 bits and rounded once: its ratio
+  // and the margin of a pair are differences of such values, and exp of them.
+  __device__ double log_prob(int64_t row, int64_t y, T top, T total) const {
+    const T at = y >= 0 && y < vocab ? logits[row * vocab + y] : T(__builtin_nan(""));
+    return (double(at) - double(top)) - log(double(total));
   }
-  __device__ T scaled(T w) const { return w * T(scale ? *scale : scale_value); }
+  __device__ void keep(int64_t row, double value, T top, T total) const {
+    log_probs[row] = T(value);
+    if (exact) exact[row] = value;
+    if (tops) tops[row] = top, inverses[row] = T(1) / total;
+  }
+  __device__ void leave_out(int64_t row) const {
+    log_probs[row] = T(0);
+    if (exact) exact[row] = 0;
+  }
+  __device__ T scaled(double w) const { return T(w * (scale ? *scale : scale_value)); }
 };
 
 // The policy loss of a token and its derivative by the log-probability.
 // expm1 keeps the KL term's digits where the two policies nearly agree.
 template <typename T>
-__device__ __forceinline__ void policy_token(const Call<T>& c, int64_t row, T log_prob, T& loss, T& slope) {
-  const T advantage = c.advantages[row];
-  const T ratio = exp_of(log_prob - c.old[row]);
-  const T free = ratio * advantage;
+__device__ __forceinline__ void policy_token(const Call<T>& c, int64_t row, double log_prob, double& loss, double& slope) {
+  const double advantage = c.advantages[row];
+  const double ratio = exp(log_prob - double(c.old[row]));
+  const double free = ratio * advantage;
   // Not fmin/fmax: a NaN ratio stays NaN.
-  const T within = ratio < c.low ? c.low : ratio > c.high ? c.high : ratio;
-  const T held = within * advantage;
+  const double within = ratio < c.low ? c.low : ratio > c.high ? c.high : ratio;
+  const double held = within * advantage;
   const bool stopped = free > held;
   loss = -(stopped ? held : free);
-  slope = stopped ? T(0) : -free;
+  slope = stopped ? 0.0 : -free;
   if (c.reference) {
-    const T apart = c.reference[row] - log_prob;
-    const T grown = expm1_of(apart);
+    const double apart = double(c.reference[row]) - log_prob;
+    const double grown = expm1(apart);
     loss += c.kl * (grown - apart);
     slope -= c.kl * grown;
   }
@@ -221,7 +227,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Call<T> c, const T* __restr
   double sum = 0;
   for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); row < c.rows; row += int64_t(gridDim.x) * 4) {
     if (!c.kept(row)) {
-      if (lane == 0) c.log_probs[row] = T(0);
+      if (lane == 0) c.leave_out(row);
       continue;
     }
     const T* tops = part_tops + row * pieces;
@@ -233,17 +239,13 @@ __global__ __launch_bounds__(256) void finish_kernel(Call<T> c, const T* __restr
     T total = T(0);
     for (int k = lane; k < pieces; k += 64) total += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - top);
     total = team_reduce<64>(total, static_cast<T*>(nullptr), [](T a, T b) { return a + b; });
-    const int64_t y = c.target(row);
-    const T log_prob = c.at_target(row, y) - top - log_of(total);
-    if (lane == 0) {
-      c.log_probs[row] = log_prob;
-      if (c.tops) c.tops[row] = top, c.inverses[row] = T(1) / total;
-    }
+    const double log_prob = c.log_prob(row, c.target(row), top, total);
+    if (lane == 0) c.keep(row, log_prob, top, total);
     if (!c.old) continue;
-    T loss, slope;
+    double loss, slope;
     policy_token(c, row, log_prob, loss, slope);
     if (lane == 0) {
-      sum += double(loss);
+      sum += loss;
       if (c.weights) c.weights[row] = c.scaled(slope);
     }
   }
@@ -320,7 +322,7 @@ __global__ __launch_bounds__(256) void pair_kernel(Call<T> c, const T* __restric
   double sum[2] = {0, 0};
   for (int side = 0; side < 2; ++side) {
     const int64_t first = (side * pairs + blockIdx.x) * c.tokens;
-    for (int64_t t = threadIdx.x; t < c.tokens; t += 256) sum[side] += double(c.log_probs[first + t]);
+    for (int64_t t = threadIdx.x; t < c.tokens; t += 256) sum[side] += c.exact[first + t];
     sum[side] = hpd::wave_sum(sum[side]);
     if ((threadIdx.x & 63) == 0) meet[side][threadIdx.x >> 6] = sum[side];
   }
@@ -329,14 +331,13 @@ __global__ __launch_bounds__(256) void pair_kernel(Call<T> c, const T* __restric
   double ratio[2];
   for (int side = 0; side < 2; ++side) {
     const int64_t at = side * pairs + blockIdx.x;
-    // The responses' sums are a result of their own, and the margin is theirs as returned.
-    const T total = T(meet[side][0] + meet[side][1] + meet[side][2] + meet[side][3]);
-    sums_out[at] = total;
-    ratio[side] = double(total) - double(reference[at]);
+    const double total = meet[side][0] + meet[side][1] + meet[side][2] + meet[side][3];
+    sums_out[at] = T(total);
+    ratio[side] = total - double(reference[at]);
   }
   const double margin = beta * (ratio[0] - ratio[1]);
   // -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)), with a NaN margin kept.
-  const double small = exp(-fabs(margin)), soft = log1p_of(small), large = 1.0 / (1.0 + small);
+  const double small = exp(-fabs(margin)), soft = log1p(small), large = 1.0 / (1.0 + small);
   const double yes = margin >= 0 ? large : small * large, no = margin >= 0 ? small * large : large;
   const double loss = (1 - smoothing) * ((margin < 0 ? -margin : 0.0) + soft) + smoothing * ((margin > 0 ? margin : 0.0) + soft);
   c.sums[blockIdx.x] = loss;
@@ -471,9 +472,9 @@ int hp_policy_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, 
       c.old = static_cast<const T*>(old);
       c.advantages = static_cast<const T*>(advantages);
       c.reference = static_cast<const T*>(reference);
-      c.low = T(1 - low);
-      c.high = T(1 + high);
-      c.kl = T(kl_weight);
+      c.low = 1 - low;
+      c.high = 1 + high;
+      c.kl = kl_weight;
       c.log_probs = static_cast<T*>(log_probs);
       c.grad = static_cast<T*>(grad);
       if (count > 0) {
@@ -520,6 +521,7 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
       c.scale_value = 1.0 / double(std::max<int64_t>(pairs, 1));
       if (pairs) {
         c.log_probs = scratch.take<T>(rows);
+        c.exact = scratch.take<double>(rows);
         if (grad) {
           c.tops = scratch.take<T>(rows);
           c.inverses = scratch.take<T>(rows);
