@@ -275,12 +275,14 @@ int hp_token_log_probs(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
 /* Clipped policy loss over the rows that `mask` keeps: the sum of
  * -min(r A, clip(r, 1 - low, 1 + high) A) + kl_weight (exp(d) - d - 1) divided by
  * `count`, or by the number of rows kept (at least 1) if count is 0, where r =
- * exp(log_prob - old) and d = reference - log_prob (reference NULL: no such term).
+ * exp(log_prob - old), A of row i is advantages[(i / divide) % period] and d =
+ * reference - log_prob (reference NULL: no such term).
  * Writes the 0-d loss, the log-probabilities as hp_token_log_probs, and unless
  * NULL the gradient of the logits. */
 int hp_policy_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, const void* actions, const void* old,
-                   const void* advantages, const void* reference, const void* mask, void* loss, void* log_probs,
-                   void* grad, int64_t rows, int64_t vocab, double low, double high, double kl_weight, double count);
+                   const void* advantages, int64_t divide, int64_t period, const void* reference, const void* mask,
+                   void* loss, void* log_probs, void* grad, int64_t rows, int64_t vocab, double low, double high,
+                   double kl_weight, double count);
 
 /* Preference loss of (2, pairs, time, vocab) logits, the chosen responses and
  * then the rejected ones: the mean over pairs (0 of none) of

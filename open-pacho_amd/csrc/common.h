@@ -89,6 +89,7 @@ struct hp_ctx {
   size_t pool_limit = 0;
   int fail_next = 0;
   bool staged_products = false;  // hp_debug_staged_products
+  unsigned* ticket = nullptr;  // zero in device memory between launches: workgroups that have ended
 };
 
 namespace hp {

@@ -176,9 +176,13 @@ int hp_init(int device, hp_ctx** out) {
     HP_CHECK(hipStreamCreateWithFlags(&ctx->side, hipStreamNonBlocking));
     HP_CHECK(hipEventCreateWithFlags(&ctx->fork, hipEventDisableTiming));
     HP_CHECK(hipEventCreateWithFlags(&ctx->join, hipEventDisableTiming));
+    HP_CHECK(hipMalloc(reinterpret_cast<void**>(&ctx->ticket), 256));
+    const unsigned zero = 0;
+    HP_CHECK(hipMemcpy(ctx->ticket, &zero, sizeof(zero), hipMemcpyHostToDevice));
     *out = ctx;
   });
   if (status != HP_OK && ctx != nullptr) {
+    if (ctx->ticket) (void)hipFree(ctx->ticket);
     if (ctx->join) (void)hipEventDestroy(ctx->join);
     if (ctx->fork) (void)hipEventDestroy(ctx->fork);
     if (ctx->side) (void)hipStreamDestroy(ctx->side);
@@ -200,6 +204,7 @@ int hp_destroy(hp_ctx* ctx) {
     for (auto& entry : ctx->live) HP_CHECK(hipFree(entry.first));
     ctx->free_blocks.clear();
     ctx->live.clear();
+    HP_CHECK(hipFree(ctx->ticket));
     HP_CHECK(hipEventDestroy(ctx->join));
     HP_CHECK(hipEventDestroy(ctx->fork));
     HP_CHECK(hipStreamDestroy(ctx->side));

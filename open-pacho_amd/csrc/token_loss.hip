@@ -7,25 +7,33 @@
 // so that a row needs its statistics (m, S), one scalar w that follows from
 // log p_y, and a pass that writes. Bound: HBM, each logit read once and each
 // gradient written once where a row can stay in registers meanwhile:
-//   - rows are cut into pieces of kPieceThreads x kPieceLoads vectors (stats_kernel),
-//     whose (m, S) meet per row (finish_kernel), and are read again for the
-//     gradient (grad_kernel). The preference loss needs the second reading in any
-//     case: w depends on every token of both responses.
+//   - row_kernel: a team of L threads holds a whole row in K vectors of 16 bytes
+//     each and computes m and S from registers (the terms exp(z - m) replace the
+//     logits there), then the loss of its token and the gradient;
+//   - rows that no team holds, or so few of them that teams would leave the chip
+//     idle, are cut into pieces (stats_kernel), whose (m, S) meet per row
+//     (finish_kernel), and are read again for the gradient (grad_kernel). The
+//     preference loss needs this second reading in any case: w depends on every
+//     token of both responses.
 // Sums over a row are float (double of doubles) in a tree; the loss sums are
-// double. No atomics: every order is fixed, so results repeat bit for bit.
+// double. Every order is fixed, so results repeat bit for bit.
 //
 // A row that the mask leaves out is not read. Pieces and teams pad with -inf,
 // which adds nothing to S; the reference of a piece that is all -inf is 0, so
 // that it adds 0 and no NaN. NaN and +inf logits make S NaN.
+#include <type_traits>
+
 #include "common.h"
 #include "exponential.h"
 
 namespace {
 
 constexpr int kPieceThreads = 256, kPieceLoads = 8;
+constexpr unsigned kTicketBlocks = 1024;
+constexpr int64_t kCountedBytes = int64_t(1) << 25;
 
-// What is left of a row from a piece on, as far as a piece can reach.
-__device__ __forceinline__ int piece_end(int64_t left) { return left < (1 << 20) ? int(left) : 1 << 20; }
+// Elements of a piece, of which the last one of a row may have fewer.
+__device__ __forceinline__ int piece_end(int64_t left, int piece) { return left < piece ? int(left) : piece; }
 
 template <typename T>
 struct Vec;
@@ -44,6 +52,22 @@ struct Vec<double> {
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
 
+// log x in 64 bits. Of a float, the exponent's part exactly and the log of the
+// rest, below 0.35, to a float's precision: the error is 3e-8 whatever x is.
+__device__ __forceinline__ double log_wide(float x) {
+  int exponent;
+  float rest = frexpf(x, &exponent);
+  if (rest < 0.70710678f) rest *= 2, --exponent;
+  return double(exponent) * 0.6931471805599453 + double(logf(rest));
+}
+__device__ __forceinline__ double log_wide(double x) { return log(x); }
+// exp and exp - 1 of a difference of log-probabilities formed in 64 bits: a
+// float's precision loses no more than the rounding of the result.
+__device__ __forceinline__ double exp_difference(float, double x) { return expf(float(x)); }
+__device__ __forceinline__ double exp_difference(double, double x) { return exp(x); }
+__device__ __forceinline__ double expm1_difference(float, double x) { return expm1f(float(x)); }
+__device__ __forceinline__ double expm1_difference(double, double x) { return expm1(x); }
+
 // The values of one call; pointers that it does not have are null.
 template <typename T>
 struct Call {
@@ -57,10 +81,17 @@ struct Call {
   double* exact;  // the log-probabilities in 64 bits (null: not wanted)
   // Policy loss (old set).
   const T *old, *advantages, *reference;
-  double low, high, kl;  // 1 - clip below, 1 + clip above, weight of the KL term
-  const double* scale;  // 1 / count in device memory, or
-  double scale_value;   // on the host
-  double* sums;         // a workgroup's sum of losses each
+  unsigned divide, period;  // row r's advantage is number (r / divide) % period
+  double low, high, kl;     // 1 - clip below, 1 + clip above, weight of the KL term
+  // What the sum of losses is multiplied by: a value in device memory, or the
+  // one here, or where count_here is set one over the rows that the mask keeps,
+  // which every workgroup counts for itself.
+  const double* scale;
+  double scale_value;
+  bool count_here;
+  double* sums;      // a workgroup's sum of losses each
+  T* loss;           // their scaled sum, by the last workgroup to end, if
+  unsigned* ticket;  // not null: counts the workgroups that have ended
   // Statistics of every row for a later gradient pass (null: not wanted).
   T *tops, *inverses, *weights;
   // Preference loss: a weight for every `tokens` rows in place of one each.
@@ -71,11 +102,11 @@ struct Call {
     return wide_targets ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
   }
   // The log-probability of the row's target, NaN outside the vocabulary. From
-  // here on a token's terms are computed in 64 bits and rounded once: its ratio
-  // and the margin of a pair are differences of such values, and exp of them.
+  // here on a token's terms are differences in 64 bits: float32 would lose
+  // digits of the ratio and of a pair's margin.
   __device__ double log_prob(int64_t row, int64_t y, T top, T total) const {
     const T at = y >= 0 && y < vocab ? logits[row * vocab + y] : T(__builtin_nan(""));
-    return (double(at) - double(top)) - log(double(total));
+    return (double(at) - double(top)) - log_wide(total);
   }
   __device__ void keep(int64_t row, double value, T top, T total) const {
     log_probs[row] = T(value);
@@ -86,15 +117,18 @@ struct Call {
     log_probs[row] = T(0);
     if (exact) exact[row] = 0;
   }
-  __device__ T scaled(double w) const { return T(w * (scale ? *scale : scale_value)); }
+  __device__ T advantage(int64_t row) const {
+    if (divide == 1 && period == rows) return advantages[row];
+    return advantages[unsigned(row) / divide % period];
+  }
 };
 
 // The policy loss of a token and its derivative by the log-probability.
 // expm1 keeps the KL term's digits where the two policies nearly agree.
 template <typename T>
 __device__ __forceinline__ void policy_token(const Call<T>& c, int64_t row, double log_prob, double& loss, double& slope) {
-  const double advantage = c.advantages[row];
-  const double ratio = exp(log_prob - double(c.old[row]));
+  const double advantage = c.advantage(row);
+  const double ratio = exp_difference(T(0), log_prob - double(c.old[row]));
   const double free = ratio * advantage;
   // Not fmin/fmax: a NaN ratio stays NaN.
   const double within = ratio < c.low ? c.low : ratio > c.high ? c.high : ratio;
@@ -104,7 +138,7 @@ __device__ __forceinline__ void policy_token(const Call<T>& c, int64_t row, doub
   slope = stopped ? 0.0 : -free;
   if (c.reference) {
     const double apart = double(c.reference[row]) - log_prob;
-    const double grown = expm1(apart);
+    const double grown = expm1_difference(T(0), apart);
     loss += c.kl * (grown - apart);
     slope -= c.kl * grown;
   }
@@ -126,95 +160,191 @@ __device__ __forceinline__ T team_reduce(T v, T* meet, Op op) {
   return v;
 }
 
-// Vectors k * L + lane of a row of `length` elements, -inf past its end. All but
-// the last L vectors of a row are whole, which the team's index k alone tells.
+// A team's share of a row of `length` elements: the whole vectors k * L + lane,
+// and of the elements after the last whole vector one for each of the first
+// lanes. Places past the row's end hold -inf.
 template <typename T, int L, int K>
-__device__ __forceinline__ void load_row(const T* row, int length, int lane, T (&z)[K][Vec<T>::width]) {
-  constexpr int W = Vec<T>::width;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int i = (k * L + lane) * W;
-    if ((k + 1) * L * W <= length || i + W <= length) {
-      const auto v = *reinterpret_cast<const typename Vec<T>::type*>(row + i);
-#pragma unroll
-      for (int j = 0; j < W; ++j) z[k][j] = v[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < W; ++j) z[k][j] = i + j < length ? row[i + j] : -T(__builtin_huge_val());
-    }
-  }
-}
+struct Share {
+  static constexpr int W = Vec<T>::width;
+  using V = typename Vec<T>::type;
+  T z[K][W], rest;
 
-template <typename T, int L, int K>
-__device__ __forceinline__ void store_row(T* row, int length, int lane, const T (&z)[K][Vec<T>::width]) {
-  constexpr int W = Vec<T>::width;
+  __device__ __forceinline__ static int index(int k, int lane) { return (k * L + lane) * W; }
+  __device__ __forceinline__ static int rest_index(int length, int lane) { return length / W * W + lane; }
+
+  __device__ __forceinline__ void load(const T* row, int length, int lane) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int i = (k * L + lane) * W;
-    if ((k + 1) * L * W <= length || i + W <= length) {
-      typename Vec<T>::type v;
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) v[j] = z[k][j];
-      *reinterpret_cast<typename Vec<T>::type*>(row + i) = v;
-    } else {
+      for (int j = 0; j < W; ++j) z[k][j] = -T(__builtin_huge_val());
+      if (index(k, lane) + W <= length) {
+        const V v = *reinterpret_cast<const V*>(row + index(k, lane));
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        if (i + j < length) row[i + j] = z[k][j];
+        for (int j = 0; j < W; ++j) z[k][j] = v[j];
       }
     }
+    rest = -T(__builtin_huge_val());
+    if (rest_index(length, lane) < length) rest = row[rest_index(length, lane)];
   }
-}
 
-// z becomes exp(z - top); top and total are those of the team's values.
-template <typename T, int L, int K>
-__device__ __forceinline__ void statistics(T (&z)[K][Vec<T>::width], T* meet, T& top, T& total) {
-  constexpr int W = Vec<T>::width;
-  T m = z[0][0];
+  __device__ __forceinline__ void store(T* row, int length, int lane) const {
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+      if (index(k, lane) + W <= length) {
+        V v;
 #pragma unroll
-    for (int j = 0; j < W; ++j) m = larger(m, z[k][j]);
-  top = team_reduce<L>(m, meet, [](T a, T b) { return larger(a, b); });
-  const T reference = top == -T(__builtin_huge_val()) ? T(0) : top;
-  T s[W] = {};
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      z[k][j] = hpd::exp_down(z[k][j] - reference);
-      s[j] += z[k][j];
+        for (int j = 0; j < W; ++j) v[j] = z[k][j];
+        *reinterpret_cast<V*>(row + index(k, lane)) = v;
+      }
     }
-  T sum = s[0];
-#pragma unroll
-  for (int j = 1; j < W; ++j) sum += s[j];
-  total = team_reduce<L>(sum, meet + 16, [](T a, T b) { return a + b; });
-}
+    if (rest_index(length, lane) < length) row[rest_index(length, lane)] = rest;
+  }
 
-// Adds each thread's `sum` over the workgroup and leaves it at sums[blockIdx.x].
-__device__ __forceinline__ void leave_sum(double sum, double* sums) {
+  // f(value, its index in the row) for every value.
+  template <typename F>
+  __device__ __forceinline__ void each(int length, int lane, F&& f) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < W; ++j) f(z[k][j], index(k, lane) + j);
+    f(rest, rest_index(length, lane));
+  }
+
+  // The values become exp(z - top); top and total are those of the team.
+  __device__ __forceinline__ void statistics(int length, int lane, T* meet, T& top, T& total) {
+    T m = rest;
+    each(length, lane, [&](T& v, int) { m = larger(m, v); });
+    top = team_reduce<L>(m, meet, [](T a, T b) { return larger(a, b); });
+    const T reference = top == -T(__builtin_huge_val()) ? T(0) : top;
+    rest = hpd::exp_down(rest - reference);
+    T sum = rest;
+    T s[W] = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        z[k][j] = hpd::exp_down(z[k][j] - reference);
+        s[j] += z[k][j];
+      }
+#pragma unroll
+    for (int j = 0; j < W; ++j) sum += s[j];
+    total = team_reduce<L>(sum, meet + 16, [](T a, T b) { return a + b; });
+  }
+};
+
+// The sum of every thread's value, for thread 0 of the workgroup.
+__device__ __forceinline__ double workgroup_sum(double sum) {
   __shared__ double meet[16];
   sum = hpd::wave_sum(sum);
+  __syncthreads();  // an earlier sum's values have been read
   if ((threadIdx.x & 63) == 0) meet[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (unsigned w = 1; w < blockDim.x / 64; ++w) sum += meet[w];
-    sums[blockIdx.x] = sum;
+  sum = meet[0];
+  for (unsigned w = 1; w < blockDim.x / 64; ++w) sum += meet[w];
+  return sum;
+}
+
+// The factor of the losses.
+template <typename T>
+__device__ __forceinline__ double scale_of(const Call<T>& c) {
+  if (!c.count_here) return c.scale ? *c.scale : c.scale_value;
+  // Sixteen bytes at a time: the top bit of a byte is set where it is not 0.
+  typedef uint32_t U4 __attribute__((ext_vector_type(4), aligned(1)));
+  const int64_t vectors = c.rows / 16;
+  int count = 0;
+  for (int64_t i = threadIdx.x; i < vectors; i += blockDim.x) {
+    const U4 v = reinterpret_cast<const U4*>(c.mask)[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) count += __popc((((v[j] & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | v[j]) & 0x80808080u);
   }
+  const int64_t tail = vectors * 16 + threadIdx.x;
+  if (threadIdx.x < 16 && tail < c.rows) count += c.mask[tail] != 0;
+  const double sum = workgroup_sum(count);
+  return 1.0 / (sum > 1.0 ? sum : 1.0);
+}
+
+// Leaves the workgroup's sum of losses. With a ticket, the last workgroup adds
+// all of them in their order, whichever it is, and sets the ticket back.
+template <typename T>
+__device__ __forceinline__ void leave_loss(const Call<T>& c, double sum, double scale) {
+  __shared__ bool last;
+  sum = workgroup_sum(sum);
+  if (threadIdx.x == 0) {
+    __hip_atomic_store(&c.sums[blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (c.ticket) last = __hip_atomic_fetch_add(c.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  }
+  if (!c.ticket) return;
+  __syncthreads();
+  if (!last) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  double total = 0;
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += blockDim.x) {
+    total += __hip_atomic_load(&c.sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  total = workgroup_sum(total);
+  if (threadIdx.x == 0) {
+    *c.loss = T(total * scale);
+    __hip_atomic_store(c.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
+
+// At 16 vectors a lane, four waves per SIMD (128 registers) keep a second
+// workgroup's loads in flight while one waits at its barriers.
+template <typename T, int L, int K>
+__global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? 4 : 1) void row_kernel(Call<T> c) {
+  constexpr int kTeams = L > 256 ? 1 : 256 / L;
+  __shared__ T meet[32];
+  const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : threadIdx.x / L;
+  const int length = int(c.vocab);
+  const double factor = c.old ? scale_of(c) : 1.0;
+  double sum = 0;
+  // Teams of several waves are alone in their workgroup: the loop and the
+  // branches on a row are uniform where they pass a barrier.
+  for (int64_t row = int64_t(blockIdx.x) * kTeams + team; row < c.rows; row += int64_t(gridDim.x) * kTeams) {
+    T* out = c.grad && c.old ? c.grad + row * c.vocab : nullptr;
+    Share<T, L, K> share;
+    if (!c.kept(row)) {
+      if (lane == 0) c.leave_out(row);
+      if (out) {
+        share.each(length, lane, [](T& v, int) { v = T(0); });
+        share.store(out, length, lane);
+      }
+      continue;
+    }
+    share.load(c.logits + row * c.vocab, length, lane);
+    const int64_t y = c.target(row);
+    T top, total;
+    share.statistics(length, lane, meet, top, total);
+    const double log_prob = c.log_prob(row, y, top, total);
+    if (lane == 0) c.keep(row, log_prob, top, total);
+    if (!c.old) continue;
+    double loss, slope;
+    policy_token(c, row, log_prob, loss, slope);
+    if (lane == 0) sum += loss;
+    if (!out) continue;
+    const T w = T(slope * factor), scale = -w * (T(1) / total);
+    const int at = y >= 0 && y < c.vocab ? int(y) : -1;
+    share.each(length, lane, [&](T& v, int i) { v = v * scale + (i == at ? w : T(0)); });
+    share.store(out, length, lane);
+  }
+  if (c.old) leave_loss(c, sum, factor);
 }
 
 // (m, S) of one piece of a row: parts[row * pieces + piece].
 template <typename T>
 __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __restrict__ part_tops,
-                                                              T* __restrict__ part_totals, int pieces) {
-  constexpr int W = Vec<T>::width, K = kPieceLoads;
+                                                              T* __restrict__ part_totals, int pieces,
+                                                              int piece) {
   __shared__ T meet[32];
   for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
     const int64_t row = part / pieces;
     if (!c.kept(row)) continue;
-    const int64_t start = (part - row * pieces) * (kPieceThreads * K * W);
-    T z[K][W], top, total;
-    load_row<T, kPieceThreads, K>(c.logits + row * c.vocab + start, piece_end(c.vocab - start), threadIdx.x, z);
-    statistics<T, kPieceThreads, K>(z, meet, top, total);
+    const int64_t start = (part - row * pieces) * piece;
+    const int length = piece_end(c.vocab - start, piece);
+    T top, total;
+    Share<T, kPieceThreads, kPieceLoads> share;
+    share.load(c.logits + row * c.vocab + start, length, threadIdx.x);
+    share.statistics(length, threadIdx.x, meet, top, total);
     if (threadIdx.x == 0) part_tops[part] = top, part_totals[part] = total;
   }
 }
@@ -224,6 +354,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void finish_kernel(Call<T> c, const T* __restrict__ part_tops,
                                                      const T* __restrict__ part_totals, int pieces) {
   const int lane = threadIdx.x & 63;
+  const double factor = c.old ? scale_of(c) : 1.0;
   double sum = 0;
   for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); row < c.rows; row += int64_t(gridDim.x) * 4) {
     if (!c.kept(row)) {
@@ -246,71 +377,49 @@ __global__ __launch_bounds__(256) void finish_kernel(Call<T> c, const T* __restr
     policy_token(c, row, log_prob, loss, slope);
     if (lane == 0) {
       sum += loss;
-      if (c.weights) c.weights[row] = c.scaled(slope);
+      if (c.weights) c.weights[row] = T(slope * factor);
     }
   }
-  if (c.old) leave_sum(sum, c.sums);
+  if (c.old) leave_loss(c, sum, factor);
 }
 
 // The gradient of one piece of a row from the row's statistics and weight.
-template <typename T>
-__global__ __launch_bounds__(kPieceThreads) void grad_kernel(Call<T> c, int pieces) {
-  constexpr int W = Vec<T>::width, K = kPieceLoads;
-  for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
+template <typename T, int L, int K>
+__global__ __launch_bounds__(256) void grad_kernel(Call<T> c, int pieces, int piece) {
+  constexpr int kTeams = 256 / L;
+  const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : threadIdx.x / L;
+  for (int64_t part = int64_t(blockIdx.x) * kTeams + team; part < c.rows * pieces; part += int64_t(gridDim.x) * kTeams) {
     const int64_t row = part / pieces;
-    const int64_t start = (part - row * pieces) * (kPieceThreads * K * W);
-    T* out = c.grad + row * c.vocab + start;
-    T z[K][W];
+    const int64_t start = (part - row * pieces) * piece;
+    const int length = piece_end(c.vocab - start, piece);
+    Share<T, L, K> share;
     if (c.kept(row)) {
-      load_row<T, kPieceThreads, K>(c.logits + row * c.vocab + start, piece_end(c.vocab - start), threadIdx.x, z);
+      share.load(c.logits + row * c.vocab + start, length, lane);
       const int64_t y = c.target(row) - start;
-    const int at = y >= 0 && y < piece_end(c.vocab - start) ? int(y) : -1;
-      const T w = c.weights[row / c.tokens], share = -w * c.inverses[row], top = c.tops[row];
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const int i = (k * kPieceThreads + int(threadIdx.x)) * W + j;
-          z[k][j] = hpd::exp_down(z[k][j] - top) * share + (i == at ? w : T(0));
-        }
+      const int at = y >= 0 && y < length ? int(y) : -1;
+      const T w = c.weights[row / c.tokens], scale = -w * c.inverses[row], top = c.tops[row];
+      share.each(length, lane, [&](T& v, int i) { v = hpd::exp_down(v - top) * scale + (i == at ? w : T(0)); });
     } else {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < W; ++j) z[k][j] = T(0);
+      share.each(length, lane, [](T& v, int) { v = T(0); });
     }
-    store_row<T, kPieceThreads, K>(out, piece_end(c.vocab - start), threadIdx.x, z);
+    share.store(c.grad + row * c.vocab + start, length, lane);
   }
 }
 
-// 1 / max(1, set bytes of the mask), by one workgroup.
-__global__ __launch_bounds__(1024) void count_kernel(const uint8_t* __restrict__ mask, int64_t rows, double* __restrict__ scale) {
-  __shared__ double meet[16];
-  unsigned count = 0;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) count += mask[i] != 0;
-  double sum = hpd::wave_sum(double(count));
-  if ((threadIdx.x & 63) == 0) meet[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) sum += meet[w];
-    *scale = 1.0 / (sum > 1.0 ? sum : 1.0);
-  }
+// 1 / max(1, rows that the mask keeps), by one workgroup.
+template <typename T>
+__global__ __launch_bounds__(1024) void count_kernel(Call<T> c, double* __restrict__ scale) {
+  const double found = scale_of(c);
+  if (threadIdx.x == 0) *scale = found;
 }
 
 // loss = scale x the sum of the workgroups' sums, by one workgroup.
 template <typename T>
-__global__ __launch_bounds__(1024) void loss_kernel(const double* __restrict__ sums, int64_t n, const double* __restrict__ scale,
-                                                    double scale_value, T* __restrict__ loss) {
-  __shared__ double meet[16];
+__global__ __launch_bounds__(1024) void loss_kernel(Call<T> c, int64_t n) {
   double sum = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) sum += sums[i];
-  sum = hpd::wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) meet[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) sum += meet[w];
-    *loss = T(sum * (scale ? *scale : scale_value));
-  }
+  for (int64_t i = threadIdx.x; i < n; i += 1024) sum += c.sums[i];
+  sum = workgroup_sum(sum);
+  if (threadIdx.x == 0) *c.loss = T(sum * (c.scale ? *c.scale : c.scale_value));
 }
 
 // A workgroup per pair: the responses' log-probabilities, the pair's loss and
@@ -318,34 +427,26 @@ __global__ __launch_bounds__(1024) void loss_kernel(const double* __restrict__ s
 template <typename T>
 __global__ __launch_bounds__(256) void pair_kernel(Call<T> c, const T* __restrict__ reference, int64_t pairs, double beta,
                                                    double smoothing, T* __restrict__ sums_out) {
-  __shared__ double meet[2][4];
-  double sum[2] = {0, 0};
-  for (int side = 0; side < 2; ++side) {
-    const int64_t first = (side * pairs + blockIdx.x) * c.tokens;
-    for (int64_t t = threadIdx.x; t < c.tokens; t += 256) sum[side] += c.exact[first + t];
-    sum[side] = hpd::wave_sum(sum[side]);
-    if ((threadIdx.x & 63) == 0) meet[side][threadIdx.x >> 6] = sum[side];
-  }
-  __syncthreads();
-  if (threadIdx.x != 0) return;
   double ratio[2];
   for (int side = 0; side < 2; ++side) {
     const int64_t at = side * pairs + blockIdx.x;
-    const double total = meet[side][0] + meet[side][1] + meet[side][2] + meet[side][3];
-    sums_out[at] = T(total);
-    ratio[side] = total - double(reference[at]);
+    double sum = 0;
+    for (int64_t t = threadIdx.x; t < c.tokens; t += 256) sum += c.exact[at * c.tokens + t];
+    sum = workgroup_sum(sum);
+    if (threadIdx.x == 0) sums_out[at] = T(sum);
+    ratio[side] = sum - double(reference[at]);
   }
   const double margin = beta * (ratio[0] - ratio[1]);
   // -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)), with a NaN margin kept.
   const double small = exp(-fabs(margin)), soft = log1p(small), large = 1.0 / (1.0 + small);
   const double yes = margin >= 0 ? large : small * large, no = margin >= 0 ? small * large : large;
   const double loss = (1 - smoothing) * ((margin < 0 ? -margin : 0.0) + soft) + smoothing * ((margin > 0 ? margin : 0.0) + soft);
-  c.sums[blockIdx.x] = loss;
-  if (c.weights) {
+  if (c.weights && threadIdx.x == 0) {
     const double slope = beta * (smoothing * yes - (1 - smoothing) * no) / double(pairs);
     c.weights[blockIdx.x] = T(slope);
     c.weights[pairs + blockIdx.x] = T(-slope);
   }
+  leave_loss(c, threadIdx.x == 0 ? loss : 0.0, c.scale_value);
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -374,40 +475,124 @@ class Scratch {
   std::vector<void*> held_;
 };
 
-template <typename T>
-constexpr int64_t piece_length() {
-  return int64_t(kPieceThreads) * kPieceLoads * Vec<T>::width;
+// Calls f with the team (L, K) that holds rows of `vocab` logits, or returns
+// false: none does.
+template <typename T, typename F>
+bool with_team(int64_t vocab, F&& f) {
+  const int64_t vectors = hp::ceil_div(vocab, Vec<T>::width);
+#define TEAM(L, K) \
+  if (vectors <= L * K) return f(std::integral_constant<int, L>{}, std::integral_constant<int, K>{}), true;
+  TEAM(4, 1)
+  TEAM(8, 1)
+  TEAM(16, 1)
+  TEAM(32, 1)
+  TEAM(64, 1)
+  TEAM(64, 2)
+  TEAM(64, 4)
+  TEAM(64, 8)
+  TEAM(256, 4)
+  TEAM(256, 8)
+  TEAM(256, 16)
+  TEAM(512, 16)
+  if constexpr (sizeof(T) == 4) {
+    TEAM(1024, 16)
+  }
+#undef TEAM
+  return false;
 }
 
-unsigned pieces_grid(int64_t rows, int64_t pieces) { return unsigned(std::min(rows * pieces, hp::kMaxGrid)); }
+// Equal pieces of whole vectors, as few as hold the row.
+template <typename T>
+struct Pieces {
+  int count, length;
+  explicit Pieces(int64_t vocab) {
+    const int64_t vectors = hp::ceil_div(vocab, Vec<T>::width);
+    const int64_t least = hp::ceil_div(vectors, kPieceThreads * kPieceLoads);
+    length = int(hp::ceil_div(vectors, least)) * Vec<T>::width;
+    count = int(hp::ceil_div(vocab, length));
+  }
+};
+
+unsigned loop_grid(int64_t groups) { return unsigned(std::min(groups, hp::kMaxGrid)); }
+
+// Whether a policy loss or log-probabilities take teams: not for rows so few and
+// so long that they would leave most of the chip idle.
+template <typename T>
+bool teams_serve(int64_t rows, int64_t vocab) {
+  return vocab <= 256 * 16 * Vec<T>::width || rows >= 128;
+}
+
+// The sum of the losses where the kernel that made them does not leave it.
+template <typename T>
+void final_loss(hp_ctx* ctx, const Call<T>& c, int64_t sums) {
+  if (c.ticket && sums) return;
+  loss_kernel<T><<<1, 1024, 0, ctx->stream>>>(c, sums);
+  hp::check_launch("loss sum");
+}
+
+// Prepares a launch of `blocks` workgroups that leave sums of losses. Few of them
+// count the mask and add the sums themselves, which saves two launches: each
+// ends with a fence of the caches between the dies, and reads the whole mask.
+template <typename T>
+void plan_losses(hp_ctx* ctx, Scratch& scratch, Call<T>& c, unsigned blocks) {
+  c.sums = scratch.take<double>(blocks);
+  if (blocks <= kTicketBlocks) c.ticket = ctx->ticket;
+  if (!c.count_here || (c.ticket && int64_t(blocks) * c.rows <= kCountedBytes)) return;
+  double* scale = scratch.take<double>(1);
+  count_kernel<T><<<1, 1024, 0, ctx->stream>>>(c, scale);
+  hp::check_launch("token count");
+  c.scale = scale;
+  c.count_here = false;
+}
 
 // The statistics, log-probabilities and, for the policy loss, the losses of
-// every row, their sums in c.sums; returns how many sums.
+// every row, their sums in c.sums; returns how many sums. `done`: whether the
+// gradient is written, too.
 template <typename T>
-int64_t rows_pass(hp_ctx* ctx, Scratch& scratch, Call<T>& c) {
-  const int64_t pieces = hp::ceil_div(c.vocab, piece_length<T>());
-  T* tops = scratch.take<T>(c.rows * pieces);
-  T* totals = scratch.take<T>(c.rows * pieces);
-  const unsigned blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, 4), 4096));
-  if (c.old) c.sums = scratch.take<double>(blocks);
-  stats_kernel<T><<<pieces_grid(c.rows, pieces), kPieceThreads, 0, ctx->stream>>>(c, tops, totals, int(pieces));
+int64_t rows_pass(hp_ctx* ctx, Scratch& scratch, Call<T>& c, bool& done) {
+  done = false;
+  unsigned blocks = 0;
+  if (teams_serve<T>(c.rows, c.vocab) && with_team<T>(c.vocab, [&](auto l, auto k) {
+        constexpr int L = l, K = k, kTeams = L > 256 ? 1 : 256 / L;
+        blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, kTeams), 16384));
+        if (c.old) plan_losses(ctx, scratch, c, blocks);
+        row_kernel<T, L, K><<<blocks, L > 256 ? L : 256, 0, ctx->stream>>>(c);
+        hp::check_launch("token rows");
+      })) {
+    done = c.old && c.grad;
+    return blocks;
+  }
+  const Pieces<T> pieces(c.vocab);
+  T* tops = scratch.take<T>(c.rows * pieces.count);
+  T* totals = scratch.take<T>(c.rows * pieces.count);
+  if (c.grad && c.old) {
+    c.tops = scratch.take<T>(c.rows);
+    c.inverses = scratch.take<T>(c.rows);
+    c.weights = scratch.take<T>(c.rows);
+  }
+  blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, 4), 4096));
+  if (c.old) plan_losses(ctx, scratch, c, blocks);
+  stats_kernel<T><<<loop_grid(c.rows * pieces.count), kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
   hp::check_launch("token statistics");
-  finish_kernel<T><<<blocks, 256, 0, ctx->stream>>>(c, tops, totals, int(pieces));
+  finish_kernel<T><<<blocks, 256, 0, ctx->stream>>>(c, tops, totals, pieces.count);
   hp::check_launch("token losses");
   return blocks;
 }
 
 template <typename T>
 void grad_pass(hp_ctx* ctx, const Call<T>& c) {
-  const int64_t pieces = hp::ceil_div(c.vocab, piece_length<T>());
-  grad_kernel<T><<<pieces_grid(c.rows, pieces), kPieceThreads, 0, ctx->stream>>>(c, int(pieces));
-  hp::check_launch("logits gradient");
-}
-
-template <typename T>
-void final_loss(hp_ctx* ctx, const Call<T>& c, int64_t sums, void* loss) {
-  loss_kernel<T><<<1, 1024, 0, ctx->stream>>>(c.sums, sums, c.scale, c.scale_value, static_cast<T*>(loss));
-  hp::check_launch("loss sum");
+  const auto launch = [&](auto l, auto k, int pieces, int piece) {
+    constexpr int L = l, K = k;
+    const int64_t groups = hp::ceil_div(c.rows * pieces, 256 / L);
+    grad_kernel<T, L, K><<<loop_grid(groups), 256, 0, ctx->stream>>>(c, pieces, piece);
+    hp::check_launch("logits gradient");
+  };
+  const bool held = c.vocab <= kPieceThreads * kPieceLoads * Vec<T>::width && with_team<T>(c.vocab, [&](auto l, auto k) {
+    if constexpr (l * k <= kPieceThreads * kPieceLoads) launch(l, k, 1, int(c.vocab));
+  });
+  if (held) return;
+  const Pieces<T> pieces(c.vocab);
+  launch(std::integral_constant<int, kPieceThreads>{}, std::integral_constant<int, kPieceLoads>{}, pieces.count, pieces.length);
 }
 
 template <typename T>
@@ -452,18 +637,22 @@ int hp_token_log_probs(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
       Scratch scratch(ctx);
       Call<T> c = call_of<T>(index_dtype, logits, targets, mask, rows, vocab);
       c.log_probs = static_cast<T*>(log_probs);
-      rows_pass(ctx, scratch, c);
+      bool done;
+      rows_pass(ctx, scratch, c, done);
     });
   });
 }
 
 int hp_policy_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, const void* actions, const void* old,
-                   const void* advantages, const void* reference, const void* mask, void* loss, void* log_probs,
-                   void* grad, int64_t rows, int64_t vocab, double low, double high, double kl_weight, double count) {
+                   const void* advantages, int64_t divide, int64_t period, const void* reference, const void* mask,
+                   void* loss, void* log_probs, void* grad, int64_t rows, int64_t vocab, double low, double high,
+                   double kl_weight, double count) {
   return hp::guarded([&] {
     hp::enter(ctx);
     check_call(dtype, index_dtype, rows, vocab);
     hp::require(low >= 0 && high >= 0, "clip out of range");
+    hp::require(divide > 0 && period > 0 && divide <= INT32_MAX && period <= INT32_MAX, "advantages repeat out of range");
+    hp::require(rows <= INT32_MAX, "too many rows");
     hp::require(loss && (rows == 0 || (logits && actions && old && advantages && log_probs)), "null pointer");
     by_type(dtype, [&](auto zero) {
       using T = decltype(zero);
@@ -477,27 +666,19 @@ int hp_policy_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, 
       c.kl = kl_weight;
       c.log_probs = static_cast<T*>(log_probs);
       c.grad = static_cast<T*>(grad);
-      if (count > 0) {
-        c.scale_value = 1 / count;
-      } else if (!mask) {
-        c.scale_value = 1.0 / double(std::max<int64_t>(rows, 1));
-      } else if (rows) {
-        double* scale = scratch.take<double>(1);
-        count_kernel<<<1, 1024, 0, ctx->stream>>>(c.mask, rows, scale);
-        hp::check_launch("token count");
-        c.scale = scale;
-      }
+      c.loss = static_cast<T*>(loss);
+      c.divide = unsigned(divide);
+      c.period = unsigned(period);
+      if (count > 0) c.scale_value = 1 / count;
+      else if (!mask) c.scale_value = 1.0 / double(std::max<int64_t>(rows, 1));
+      else c.count_here = rows > 0;
       int64_t sums = 0;
       if (rows) {
-        if (grad) {
-          c.tops = scratch.take<T>(rows);
-          c.inverses = scratch.take<T>(rows);
-          c.weights = scratch.take<T>(rows);
-        }
-        sums = rows_pass(ctx, scratch, c);
-        if (grad) grad_pass(ctx, c);
+        bool done;
+        sums = rows_pass(ctx, scratch, c, done);
+        if (grad && !done) grad_pass(ctx, c);
       }
-      final_loss(ctx, c, sums, loss);
+      final_loss(ctx, c, sums);
     });
   });
 }
@@ -518,6 +699,7 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
       Call<T> c = call_of<T>(index_dtype, logits, targets, mask, rows, vocab);
       c.grad = static_cast<T*>(grad);
       c.tokens = time;
+      c.loss = static_cast<T*>(loss);
       c.scale_value = 1.0 / double(std::max<int64_t>(pairs, 1));
       if (pairs) {
         c.log_probs = scratch.take<T>(rows);
@@ -526,15 +708,16 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
           c.tops = scratch.take<T>(rows);
           c.inverses = scratch.take<T>(rows);
         }
-        if (rows) rows_pass(ctx, scratch, c);
+        bool done;
+        if (rows) rows_pass(ctx, scratch, c, done);
         if (grad) c.weights = scratch.take<T>(2 * pairs);
-        c.sums = scratch.take<double>(pairs);
+        plan_losses(ctx, scratch, c, unsigned(pairs));
         pair_kernel<T><<<unsigned(pairs), 256, 0, ctx->stream>>>(c, static_cast<const T*>(reference), pairs, beta,
                                                                  smoothing, static_cast<T*>(sums));
         hp::check_launch("preference pairs");
         if (grad && rows) grad_pass(ctx, c);
       }
-      final_loss(ctx, c, pairs, loss);
+      final_loss(ctx, c, pairs);
     });
   });
 }

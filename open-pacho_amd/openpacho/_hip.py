@@ -30,6 +30,7 @@ import weakref
 import numpy as np
 
 from . import _hip_lib as lib_
+from . import _hip_nn
 from ._hip_lowering import BLOCK, HIPLowering, eager_source
 from .backends import DeviceInfo, check_dtype
 from .exceptions import BackendUnavailableError, UnsupportedDtypeError
@@ -691,45 +692,14 @@ class HIPBackend:
 
     # ---- operators of nn ---------------------------------------------------------------
 
-    def gated_recurrence(self, *args):
-        from ._hip_nn import gated_recurrence
-
-        return gated_recurrence(self, *args)
-
-    def gated_recurrence_grad(self, *args):
-        from ._hip_nn import gated_recurrence_grad
-
-        return gated_recurrence_grad(self, *args)
-
-    def token_log_probs(self, *args):
-        from ._hip_nn import token_log_probs
-
-        return token_log_probs(self, *args)
-
-    def policy_loss(self, *args):
-        from ._hip_nn import policy_loss
-
-        return policy_loss(self, *args)
-
-    def preference_loss(self, *args):
-        from ._hip_nn import preference_loss
-
-        return preference_loss(self, *args)
-
-    def adamw_load(self, *args):
-        from ._hip_nn import adamw_load
-
-        return adamw_load(self, *args)
-
-    def adamw_moments(self, *args):
-        from ._hip_nn import adamw_moments
-
-        return adamw_moments(self, *args)
-
-    def adamw_step(self, *args):
-        from ._hip_nn import adamw_step
-
-        return adamw_step(self, *args)
+    gated_recurrence = _hip_nn.gated_recurrence
+    gated_recurrence_grad = _hip_nn.gated_recurrence_grad
+    token_log_probs = _hip_nn.token_log_probs
+    policy_loss = _hip_nn.policy_loss
+    preference_loss = _hip_nn.preference_loss
+    adamw_load = _hip_nn.adamw_load
+    adamw_moments = _hip_nn.adamw_moments
+    adamw_step = _hip_nn.adamw_step
 
     # ---- protocol: compilation and lifetime -------------------------------------------
 

@@ -67,7 +67,7 @@ PROTOTYPES = {
     "hp_gated_recurrence": [_ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64],
     "hp_gated_recurrence_grad": [_ptr, _i32] + [_ptr] * 9 + [_i64] * 4,
     "hp_token_log_probs": [_ptr, _i32, _i32] + [_ptr] * 4 + [_i64] * 2,
-    "hp_policy_loss": [_ptr, _i32, _i32] + [_ptr] * 9 + [_i64] * 2 + [ctypes.c_double] * 4,
+    "hp_policy_loss": [_ptr, _i32, _i32] + [_ptr] * 4 + [_i64] * 2 + [_ptr] * 5 + [_i64] * 2 + [ctypes.c_double] * 4,
     "hp_preference_loss": [_ptr, _i32, _i32] + [_ptr] * 7 + [_i64] * 3 + [ctypes.c_double] * 2,
     "hp_adamw_layout": [_i32, _i32, _i64] + [_i64p] * 4,
     "hp_adamw_load": [_ptr, _i32, _i32, _i64, _pptr, _pptr, _i64p, _ptr],

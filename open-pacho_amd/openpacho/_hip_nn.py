@@ -12,65 +12,91 @@ def _ptr(array):
     return None if array is None else array._data.ptr
 
 
+def _run(backend, name, *args):
+    with backend._guard:
+        backend._call(name, *args)
+
+
 def gated_recurrence(backend, x, gate, initial, resets, batch, time, channels, gates):
-    h = backend.empty(x.shape, x.dtype)
-    with backend._active():
-        backend._call(
-            "hp_gated_recurrence", lib_.DTYPE_CODES[x.dtype], _ptr(x), _ptr(gate), _ptr(initial), _ptr(resets), h.ptr,
-            batch, time, channels, gates,
-        )
+    h = backend.empty(x._shape, x._dtype)
+    _run(
+        backend, "hp_gated_recurrence", lib_.DTYPE_CODES[x._dtype], x._data.ptr, gate._data.ptr, _ptr(initial), _ptr(resets),
+        h.ptr, batch, time, channels, gates,
+    )
     return h
 
 
 def gated_recurrence_grad(backend, grad, x, gate, h, initial, resets, batch, time, channels, gates):
-    dx, d_gate = backend.empty(x.shape, x.dtype), backend.empty(gate.shape, gate.dtype)
+    dx, d_gate = backend.empty(x._shape, x._dtype), backend.empty(gate._shape, x._dtype)
     d_initial = None
     if initial is not None:
-        # Of no steps the state does not depend on it.
-        d_initial = backend.empty(initial.shape, x.dtype) if time else backend.full(initial.shape, 0, x.dtype)
-    with backend._active():
-        backend._call(
-            "hp_gated_recurrence_grad", lib_.DTYPE_CODES[x.dtype], _ptr(grad), _ptr(x), _ptr(gate), _ptr(h), _ptr(initial),
-            _ptr(resets), dx.ptr, d_gate.ptr, None if d_initial is None else d_initial.ptr, batch, time, channels, gates,
-        )
+        # Of no steps the states do not depend on it.
+        d_initial = backend.empty(initial._shape, x._dtype) if time else backend.full(initial._shape, 0, x._dtype)
+    _run(
+        backend, "hp_gated_recurrence_grad", lib_.DTYPE_CODES[x._dtype], grad._data.ptr, x._data.ptr, gate._data.ptr,
+        h._data.ptr, _ptr(initial), _ptr(resets), dx.ptr, d_gate.ptr, None if d_initial is None else d_initial.ptr,
+        batch, time, channels, gates,
+    )
     return dx, d_gate, d_initial
 
 
 def _codes(logits, targets):
-    return lib_.DTYPE_CODES[logits.dtype], lib_.DTYPE_CODES[targets.dtype]
+    return lib_.DTYPE_CODES[logits._dtype], lib_.DTYPE_CODES[targets._dtype]
 
 
 def token_log_probs(backend, logits, targets, mask):
-    log_probs = backend.empty(targets.shape, logits.dtype)
-    with backend._active():
-        backend._call(
-            "hp_token_log_probs", *_codes(logits, targets), _ptr(logits), _ptr(targets), _ptr(mask), log_probs.ptr,
-            targets.size, logits.shape[-1],
-        )
+    log_probs = backend.empty(targets._shape, logits._dtype)
+    _run(
+        backend, "hp_token_log_probs", *_codes(logits, targets), logits._data.ptr, targets._data.ptr, _ptr(mask), log_probs.ptr,
+        targets.size, logits._shape[-1],
+    )
     return log_probs
 
 
+def _period(shape, whole):
+    """(divide, period) such that element (i // divide) % period of an array of
+    `shape` stands at element i of it broadcast to `whole`; None where the axes
+    that it has are not next to each other."""
+    shape = (1,) * (len(whole) - len(shape)) + shape
+    kept = [axis for axis, (own, d) in enumerate(zip(shape, whole)) if own == d != 1]
+    if not kept:
+        return 1, 1
+    if any(whole[axis] != 1 for axis in range(kept[0], kept[-1]) if axis not in kept):
+        return None
+    return prod(whole[kept[-1] + 1 :]), prod(shape)
+
+
+def _broadcast(backend, array, whole):
+    """Storage of `array`, and how it repeats over `whole` (_period)."""
+    if array._shape == whole:
+        return array._data, 1, max(1, array.size)
+    found = _period(array._shape, whole)
+    if found is None:
+        strides = [prod(array._shape[axis + 1 :]) if d != 1 else 0 for axis, d in enumerate(array._shape)]
+        return backend.gather(array, whole, 0, (0,) * (len(whole) - len(strides)) + tuple(strides)), 1, prod(whole)
+    return array._data, *(max(1, n) for n in found)
+
+
 def policy_loss(backend, logits, actions, old, advantages, reference, mask, low, high, kl_weight, count, gradient):
-    loss, log_probs = backend.empty((), logits.dtype), backend.empty(actions.shape, logits.dtype)
-    grad = backend.empty(logits.shape, logits.dtype) if gradient else None
-    with backend._active():
-        backend._call(
-            "hp_policy_loss", *_codes(logits, actions), _ptr(logits), _ptr(actions), _ptr(old), _ptr(advantages),
-            _ptr(reference), _ptr(mask), loss.ptr, log_probs.ptr, None if grad is None else grad.ptr, actions.size,
-            logits.shape[-1], low, high, kl_weight, count or 0.0,
-        )
+    loss, log_probs = backend.empty((), logits._dtype), backend.empty(actions._shape, logits._dtype)
+    grad = backend.empty(logits._shape, logits._dtype) if gradient else None
+    gains, divide, period = _broadcast(backend, advantages, actions._shape)
+    _run(
+        backend, "hp_policy_loss", *_codes(logits, actions), logits._data.ptr, actions._data.ptr, old._data.ptr, gains.ptr,
+        divide, period, _ptr(reference), _ptr(mask), loss.ptr, log_probs.ptr, None if grad is None else grad.ptr,
+        actions.size, logits._shape[-1], low, high, kl_weight, count or 0.0,
+    )
     return loss, log_probs, grad
 
 
 def preference_loss(backend, logits, targets, reference, mask, beta, smoothing, gradient):
-    loss, sums = backend.empty((), logits.dtype), backend.empty(reference.shape, logits.dtype)
-    grad = backend.empty(logits.shape, logits.dtype) if gradient else None
-    _, pairs, time = targets.shape
-    with backend._active():
-        backend._call(
-            "hp_preference_loss", *_codes(logits, targets), _ptr(logits), _ptr(targets), _ptr(reference), _ptr(mask),
-            loss.ptr, sums.ptr, None if grad is None else grad.ptr, pairs, time, logits.shape[-1], beta, smoothing,
-        )
+    loss, sums = backend.empty((), logits._dtype), backend.empty(reference._shape, logits._dtype)
+    grad = backend.empty(logits._shape, logits._dtype) if gradient else None
+    _, pairs, time = targets._shape
+    _run(
+        backend, "hp_preference_loss", *_codes(logits, targets), logits._data.ptr, targets._data.ptr, reference._data.ptr,
+        _ptr(mask), loss.ptr, sums.ptr, None if grad is None else grad.ptr, pairs, time, logits._shape[-1], beta, smoothing,
+    )
     return loss, sums, grad
 
 
@@ -124,14 +150,13 @@ class _State:
 def adamw_load(backend, first, second, shapes, dtype, bits):
     layout = _Layout(backend, shapes, dtype, bits)
     block = backend.block(layout.state_bytes)
-    with backend._active():
-        if first is None:
-            backend._call("hp_fill", block.ptr, layout.state_bytes, 1, 0)
-        else:
-            backend._call(
-                "hp_adamw_load", layout.code, layout.bits, layout.count, layout.addresses(first), layout.addresses(second),
-                layout.sizes, block.ptr,
-            )
+    if first is None:
+        _run(backend, "hp_fill", block.ptr, layout.state_bytes, 1, 0)
+    else:
+        _run(
+            backend, "hp_adamw_load", layout.code, layout.bits, layout.count, layout.addresses(first), layout.addresses(second),
+            layout.sizes, block.ptr,
+        )
     return _State(layout, block)
 
 
@@ -140,17 +165,15 @@ def adamw_moments(backend, state, which, shapes, dtype, bits):
     if not bits:
         return layout.spans(state.block, which * layout.bytes)
     values = backend.block(max(1, layout.bytes))
-    with backend._active():
-        backend._call("hp_adamw_values", layout.elements, state.block.ptr, which, values.ptr)
+    _run(backend, "hp_adamw_values", layout.elements, state.block.ptr, which, values.ptr)
     return layout.spans(values)
 
 
 def adamw_step(backend, params, grads, state, shapes, dtype, bits, decays, scalars):
     layout = state.layout
     block, new = backend.block(layout.state_bytes), backend.block(max(1, layout.bytes))
-    with backend._active():
-        backend._call(
-            "hp_adamw_step", layout.code, layout.bits, layout.count, layout.addresses(params), layout.addresses(grads),
-            layout.sizes, layout.numbers(*decays), state.block.ptr, block.ptr, new.ptr, *scalars,
-        )
+    _run(
+        backend, "hp_adamw_step", layout.code, layout.bits, layout.count, layout.addresses(params), layout.addresses(grads),
+        layout.sizes, layout.numbers(*decays), state.block.ptr, block.ptr, new.ptr, *scalars,
+    )
     return layout.spans(new), _State(layout, block)

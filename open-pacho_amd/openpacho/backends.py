@@ -18,6 +18,7 @@ from functools import lru_cache
 
 import numpy as np
 
+from . import _nn_host
 from .exceptions import BackendUnavailableError, UnsupportedDtypeError
 
 SUPPORTED_DTYPES = tuple(
@@ -134,45 +135,15 @@ class NumpyBackend:
 
         return two_pass_norm(a._data.reshape(a.shape), axes, dtype)
 
-    def gated_recurrence(self, *args):
-        from ._nn_host import recurrence
-
-        return recurrence(*args)
-
-    def gated_recurrence_grad(self, *args):
-        from ._nn_host import recurrence_grad
-
-        return recurrence_grad(*args)
-
-    def token_log_probs(self, *args):
-        from ._nn_host import token_log_probs
-
-        return token_log_probs(*args)
-
-    def policy_loss(self, *args):
-        from ._nn_host import policy_loss
-
-        return policy_loss(*args)
-
-    def preference_loss(self, *args):
-        from ._nn_host import preference_loss
-
-        return preference_loss(*args)
-
-    def adamw_load(self, *args):
-        from ._nn_host import adamw_load
-
-        return adamw_load(*args)
-
-    def adamw_moments(self, *args):
-        from ._nn_host import adamw_moments
-
-        return adamw_moments(*args)
-
-    def adamw_step(self, *args):
-        from ._nn_host import adamw_step
-
-        return adamw_step(*args)
+    # The operators of nn.
+    gated_recurrence = staticmethod(_nn_host.recurrence)
+    gated_recurrence_grad = staticmethod(_nn_host.recurrence_grad)
+    token_log_probs = staticmethod(_nn_host.token_log_probs)
+    policy_loss = staticmethod(_nn_host.policy_loss)
+    preference_loss = staticmethod(_nn_host.preference_loss)
+    adamw_load = staticmethod(_nn_host.adamw_load)
+    adamw_moments = staticmethod(_nn_host.adamw_moments)
+    adamw_step = staticmethod(_nn_host.adamw_step)
 
     def synchronize(self):
         return None

@@ -19,7 +19,7 @@ from math import prod
 import numpy as np
 
 from . import _array as xp
-from .backends import get_backend
+from .backends import _DEFAULT
 from .exceptions import BackendMismatchError, UnsupportedDtypeError
 
 _FLOATS = (np.dtype("float32"), np.dtype("float64"))
@@ -30,19 +30,23 @@ _BOOL = np.dtype("bool")
 # ---- arguments -----------------------------------------------------------------
 
 
+def _refuse_capture(what, backend):
+    if backend._is_tracing or _DEFAULT.get()._is_tracing:
+        raise NotImplementedError(f"{what} is not captured; call it between compiled functions")
+
+
 class _Operands:
     """The arrays of one call: their backend, and their float dtype, which the first one gives."""
 
+    __slots__ = ("what", "backend", "dtype")
+
     def __init__(self, what, lead, *others):
-        given = [lead, *others]
-        if getattr(get_backend(), "_is_tracing", False) or any(
-            getattr(v, "_backend", None) is not None and v._backend._is_tracing for v in given
-        ):
-            raise NotImplementedError(f"{what} is not captured; call it between compiled functions")
-        self.what, self.backend = what, xp._common_backend(given)
-        if not hasattr(self.backend, "gated_recurrence"):
-            raise NotImplementedError(f"the {self.backend.name} backend does not offer {what}")
-        self.dtype = lead.dtype if isinstance(lead, xp.ndarray) else np.asarray(lead).dtype
+        self.what, self.backend = what, xp._common_backend((lead, *others)) if not isinstance(lead, xp.ndarray) else lead._backend
+        for value in others:
+            if value is not None and isinstance(value, xp.ndarray) and value._backend is not self.backend:
+                raise BackendMismatchError("Arrays belong to different backends/devices; use to_backend()")
+        _refuse_capture(what, self.backend)
+        self.dtype = lead._dtype if isinstance(lead, xp.ndarray) else np.asarray(lead).dtype
         if self.dtype not in _FLOATS:
             raise UnsupportedDtypeError(f"{what} requires float32 or float64, got {self.dtype}")
 
@@ -52,11 +56,11 @@ class _Operands:
         if not isinstance(value, xp.ndarray):
             host = np.asarray(value)
             value = xp.asarray(host if host.dtype in dtypes else self._converted(name, host, dtypes[-1]), backend=self.backend)
-        if value.dtype not in dtypes:
+        if value._dtype not in dtypes:
             wanted = " or ".join(map(str, dtypes))
             raise UnsupportedDtypeError(f"{self.what}: {name} must be {wanted}, got {value.dtype}")
-        if shape is not None and value.shape != tuple(shape):
-            raise ValueError(f"{self.what}: {name} must have shape {tuple(shape)}, got {value.shape}")
+        if shape is not None and value._shape != shape:
+            raise ValueError(f"{self.what}: {name} must have shape {shape}, got {value.shape}")
         return value
 
     def _converted(self, name, host, dtype):
@@ -68,21 +72,26 @@ class _Operands:
         return None if value is None else self.array(name, value, shape, dtypes)
 
     def broadcast(self, name, value, shape):
-        """`value` at every place of `shape`."""
+        """`value`, which has to broadcast to `shape`."""
         value = self.array(name, value)
-        if value.shape == tuple(shape):
-            return value
-        try:
-            if np.broadcast_shapes(value.shape, shape) != tuple(shape):
-                raise ValueError
-        except ValueError:
-            raise ValueError(f"{self.what}: {name} of shape {value.shape} does not broadcast to {tuple(shape)}") from None
-        own, lead = xp._strides(value.shape), len(shape) - value.ndim
-        strides = (0,) * lead + tuple(s if d != 1 else 0 for s, d in zip(own, value.shape))
-        return self.result(self.backend.gather(value, shape, 0, strides), shape)
+        if value._shape != shape:
+            try:
+                whole = np.broadcast_shapes(value._shape, shape) == shape
+            except ValueError:
+                whole = False
+            if not whole:
+                raise ValueError(f"{self.what}: {name} of shape {value.shape} does not broadcast to {shape}")
+        return value
 
-    def result(self, data, shape, dtype=None):
-        return xp.ndarray._wrap(data, shape, self.dtype if dtype is None else dtype, self.backend)
+    def result(self, data, shape):
+        return _wrapped(data, shape, self.dtype, self.backend)
+
+
+def _wrapped(data, shape, dtype, backend):
+    """ndarray._wrap of storage whose shape and dtype are as an array keeps them."""
+    array = object.__new__(xp.ndarray)
+    array._data, array._shape, array._dtype, array._backend = data, shape, dtype, backend
+    return array
 
 
 def _number(what, value, least=None, below=None, infinite=False):
@@ -97,20 +106,25 @@ def _number(what, value, least=None, below=None, infinite=False):
 # ---- gated recurrence ----------------------------------------------------------
 
 
-def _recurrence_operands(what, x, gate, initial, resets, *others):
-    ops = _Operands(what, x, gate, initial, resets, *others)
-    x = ops.array("x", x)
-    if x.ndim < 2:
-        raise ValueError(f"{what}: x must have axes (..., time, channels), got {x.shape}")
-    lead, (time, channels) = x.shape[:-2], x.shape[-2:]
-    gate = ops.array("gate", gate)
-    if gate.ndim != x.ndim or gate.shape[:-1] != x.shape[:-1]:
-        raise ValueError(f"{what}: gate must have shape {x.shape[:-1]} and an axis of gates, got {gate.shape}")
-    gates = gate.shape[-1]
+def _gates_divide(what, channels, gates):
     if channels and (not gates or channels % gates):
         raise ValueError(f"{what}: {gates} gates do not divide {channels} channels")
     if not channels and gates:
         raise ValueError(f"{what}: {gates} gates without channels")
+
+
+def _recurrence_operands(what, x, gate, initial, resets, *others):
+    ops = _Operands(what, x, gate, initial, resets, *others)
+    x = ops.array("x", x)
+    if len(x._shape) < 2:
+        raise ValueError(f"{what}: x must have axes (..., time, channels), got {x.shape}")
+    lead, (time, channels) = x._shape[:-2], x._shape[-2:]
+    gate = ops.array("gate", gate)
+    if not gate._shape or gate._shape[:-1] != x._shape[:-1]:
+        raise ValueError(f"{what}: gate must have shape {x.shape[:-1]} and an axis of gates, got {gate.shape}")
+    gates = gate._shape[-1]
+    if gates != channels:
+        _gates_divide(what, channels, gates)
     initial = ops.optional("initial", initial, lead + (channels,))
     resets = ops.optional("resets", resets, lead + (time,), (_BOOL,))
     return ops, x, gate, initial, resets, (prod(lead), time, channels, gates)
@@ -126,17 +140,20 @@ def gated_recurrence(x, gate, initial=None, *, resets=None):
     counts as zero, whatever it holds. Returns every state, of x's shape.
     """
     ops, x, gate, initial, resets, sizes = _recurrence_operands("gated_recurrence", x, gate, initial, resets)
-    return ops.result(ops.backend.gated_recurrence(x, gate, initial, resets, *sizes), x.shape)
+    return ops.result(ops.backend.gated_recurrence(x, gate, initial, resets, *sizes), x._shape)
 
 
 def gated_recurrence_step(x, gate, state):
     """The next state of one token: ``gated_recurrence`` of a single step, without its time axis."""
-    ops = _Operands("gated_recurrence_step", x, gate, state)
+    what = "gated_recurrence_step"
+    ops = _Operands(what, x, gate, state)
     x, gate = ops.array("x", x), ops.array("gate", gate)
-    if not x.ndim or gate.ndim != x.ndim:
-        raise ValueError(f"gated_recurrence_step: x and gate must have axes (..., channels), got {x.shape} and {gate.shape}")
-    step = gated_recurrence(x.reshape(x.shape[:-1] + (1, x.shape[-1])), gate.reshape(gate.shape[:-1] + (1, gate.shape[-1])), state)
-    return step.reshape(x.shape)
+    if not x._shape or not gate._shape or gate._shape[:-1] != x._shape[:-1]:
+        raise ValueError(f"{what}: x and gate must have axes (..., channels) and (..., gates), got {x.shape} and {gate.shape}")
+    lead, channels, gates = x._shape[:-1], x._shape[-1], gate._shape[-1]
+    _gates_divide(what, channels, gates)
+    state = ops.array("state", state, x._shape)
+    return ops.result(ops.backend.gated_recurrence(x, gate, state, None, prod(lead), 1, channels, gates), x._shape)
 
 
 def gated_recurrence_grad(grad, x, gate, h, initial=None, *, resets=None):
@@ -147,10 +164,10 @@ def gated_recurrence_grad(grad, x, gate, h, initial=None, *, resets=None):
     """
     what = "gated_recurrence_grad"
     ops, x, gate, initial, resets, sizes = _recurrence_operands(what, x, gate, initial, resets, grad, h)
-    grad, h = ops.array("grad", grad, x.shape), ops.array("h", h, x.shape)
+    grad, h = ops.array("grad", grad, x._shape), ops.array("h", h, x._shape)
     dx, d_gate, d_initial = ops.backend.gated_recurrence_grad(grad, x, gate, h, initial, resets, *sizes)
-    first = None if initial is None else ops.result(d_initial, initial.shape)
-    return ops.result(dx, x.shape), ops.result(d_gate, gate.shape), first
+    first = None if initial is None else ops.result(d_initial, initial._shape)
+    return ops.result(dx, x._shape), ops.result(d_gate, gate._shape), first
 
 
 # ---- losses from logits ----------------------------------------------------------
@@ -271,7 +288,7 @@ class AdamWState:
 
     def _moments(self, which):
         storages = self._backend.adamw_moments(self._data, which, self._shapes, self._dtype, self.state_bits)
-        return [xp.ndarray._wrap(d, s, self._dtype, self._backend) for d, s in zip(storages, self._shapes)]
+        return _wrapped_list(storages, self._shapes, self._dtype, self._backend)
 
     @property
     def first(self):
@@ -285,27 +302,21 @@ class AdamWState:
         return f"AdamWState(tensors={len(self._shapes)}, steps={self.steps}, state_bits={self.state_bits}, dtype={self._dtype})"
 
 
-def _tensors(what, name, values, backend=None, dtype=None, shapes=None):
-    """A list of arrays of one backend and dtype (those given, if any), and their shapes."""
-    if not isinstance(values, (list, tuple)) or not all(isinstance(v, xp.ndarray) for v in values):
+def _wrapped_list(storages, shapes, dtype, backend):
+    return [_wrapped(data, shape, dtype, backend) for data, shape in zip(storages, shapes)]
+
+
+def _check_tensors(what, name, values, backend, dtype, shapes):
+    """Refuse what is not a list of arrays of this backend, dtype and these shapes."""
+    if not isinstance(values, (list, tuple)) or not all([isinstance(v, xp.ndarray) for v in values]):
         raise TypeError(f"{what}: {name} must be a list of arrays")
-    backend = values[0]._backend if backend is None else backend
-    if getattr(backend, "_is_tracing", False) or getattr(get_backend(), "_is_tracing", False):
-        raise NotImplementedError(f"{what} is not captured; call it between compiled functions")
-    if not hasattr(backend, "adamw_step"):
-        raise NotImplementedError(f"the {backend.name} backend does not offer {what}")
-    dtype = values[0]._dtype if dtype is None else dtype
-    if dtype not in _FLOATS:
-        raise UnsupportedDtypeError(f"{what} requires float32 or float64, got {dtype}")
     for value in values:
         if value._backend is not backend:
             raise BackendMismatchError("Arrays belong to different backends/devices; use to_backend()")
-        if value._dtype != dtype:
-            raise UnsupportedDtypeError(f"{what}: {name} must be {dtype}, got {value._dtype}")
-    found = [v._shape for v in values]
-    if shapes is not None and found != shapes:
-        raise ValueError(f"{what}: the shapes of {name} do not match those of the state: {len(found)} and {len(shapes)} tensors")
-    return backend, dtype, found
+        if value._dtype is not dtype and value._dtype != dtype:
+            raise UnsupportedDtypeError(f"{what}: {name} must be {dtype}, got {value.dtype}")
+    if [v._shape for v in values] != shapes:
+        raise ValueError(f"{what}: the shapes of {name} do not match those of the state's {len(shapes)} tensors")
 
 
 def adamw_state(params, *, state_bits=None, steps=0, first=None, second=None):
@@ -322,7 +333,14 @@ def adamw_state(params, *, state_bits=None, steps=0, first=None, second=None):
     what = "adamw_state"
     if isinstance(params, (list, tuple)) and not params:
         raise ValueError(f"{what}: no tensors")
-    backend, dtype, shapes = _tensors(what, "params", params)
+    if not isinstance(params, (list, tuple)) or not isinstance(params[0], xp.ndarray):
+        raise TypeError(f"{what}: params must be a list of arrays")
+    backend, dtype = params[0]._backend, params[0]._dtype
+    _refuse_capture(what, backend)
+    if dtype not in _FLOATS:
+        raise UnsupportedDtypeError(f"{what} requires float32 or float64, got {dtype}")
+    shapes = [getattr(p, "_shape", None) for p in params]
+    _check_tensors(what, "params", params, backend, dtype, shapes)
     if state_bits not in (None, 8):
         raise ValueError(f"state_bits must be None or 8, got {state_bits!r}")
     if state_bits == 8 and dtype != _FLOATS[0]:
@@ -334,7 +352,7 @@ def adamw_state(params, *, state_bits=None, steps=0, first=None, second=None):
         raise ValueError("first and second come together")
     for name, moments in (("first", first), ("second", second)):
         if moments is not None:
-            _tensors(what, name, moments, backend, dtype, shapes)
+            _check_tensors(what, name, moments, backend, dtype, shapes)
     return AdamWState(backend, dtype, shapes, state_bits, steps, backend.adamw_load(first, second, shapes, dtype, state_bits))
 
 
@@ -349,8 +367,10 @@ def adamw(params, grads, state, *, learning_rate=1e-3, betas=(0.9, 0.999), eps=1
     what = "adamw"
     if not isinstance(state, AdamWState):
         raise TypeError(f"{what}: state must come from adamw_state or a step")
-    backend, dtype, shapes = _tensors(what, "params", params, state._backend, state._dtype, state._shapes)
-    _tensors(what, "grads", grads, backend, dtype, shapes)
+    backend, dtype, shapes = state._backend, state._dtype, state._shapes
+    _refuse_capture(what, backend)
+    _check_tensors(what, "params", params, backend, dtype, shapes)
+    _check_tensors(what, "grads", grads, backend, dtype, shapes)
     learning_rate = _number("learning_rate", learning_rate, 0)
     beta1, beta2 = (_number("betas", b, 0, 1) for b in betas)
     eps = _number("eps", eps)
@@ -367,5 +387,4 @@ def adamw(params, grads, state, *, learning_rate=1e-3, betas=(0.9, 0.999), eps=1
     scalars = (beta1, beta2, learning_rate / (1 - beta1**steps), 1 / math.sqrt(1 - beta2**steps), eps)
     decays = [learning_rate * d for d in decays]
     storages, data = backend.adamw_step(params, grads, state._data, shapes, dtype, state.state_bits, decays, scalars)
-    new = [xp.ndarray._wrap(d, s, dtype, backend) for d, s in zip(storages, shapes)]
-    return new, AdamWState(backend, dtype, shapes, state.state_bits, steps, data)
+    return _wrapped_list(storages, shapes, dtype, backend), AdamWState(backend, dtype, shapes, state.state_bits, steps, data)

@@ -41,6 +41,17 @@ def test_preference_loss(hip, pairs, time, vocab, dtype):
     check_preference(hip, pairs, time, vocab, dtype, seed=time, beta=0.5, smoothing=0.1, index=np.int32)
 
 
+def test_advantages_broadcast(hip):
+    rng = np.random.default_rng(0)
+    logits, actions = p.asarray(rng.standard_normal((3, 4, 5, 6)), backend=hip), rng.integers(0, 6, (3, 4, 5))
+    old = rng.standard_normal((3, 4, 5)) - 2
+    for shape in ((3, 4, 5), (3, 4, 1), (3, 1, 1), (1, 4, 1), (4, 5), (5,), (1,), (), (3, 1, 5), (1, 4, 5)):
+        narrow = rng.standard_normal(shape)
+        full = np.broadcast_to(narrow, (3, 4, 5)).copy()
+        for one, two in zip(p.nn.policy_loss_grad(logits, actions, old, narrow), p.nn.policy_loss_grad(logits, actions, old, full)):
+            np.testing.assert_array_equal(p.asnumpy(one), p.asnumpy(two))
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 def test_edges(hip, dtype):
     check_edges(hip, dtype)
@@ -81,9 +92,11 @@ def test_refusals_at_the_library(hip):
             with pytest.raises(ValueError):
                 hip._call("hp_token_log_probs", code, index, logits, z, None, z, rows, vocab)
             with pytest.raises(ValueError):
-                hip._call("hp_policy_loss", code, index, logits, *[z] * 3, None, None, z, z, z, rows, vocab, 0.2, 0.2, 0.0, 0.0)
+                hip._call("hp_policy_loss", code, index, logits, *[z] * 3, 1, 1, None, None, z, z, z, rows, vocab, 0.2, 0.2, 0.0, 0.0)
         with pytest.raises(ValueError, match="clip"):
-            hip._call("hp_policy_loss", 5, 2, *[z] * 4, None, None, z, z, z, 1, 4, -0.2, 0.2, 0.0, 0.0)
+            hip._call("hp_policy_loss", 5, 2, *[z] * 4, 1, 1, None, None, z, z, z, 1, 4, -0.2, 0.2, 0.0, 0.0)
+        with pytest.raises(ValueError, match="repeat"):
+            hip._call("hp_policy_loss", 5, 2, *[z] * 4, 1, 0, None, None, z, z, z, 1, 4, 0.2, 0.2, 0.0, 0.0)
         with pytest.raises(ValueError):
             hip._call("hp_preference_loss", 5, 2, *[z] * 3, None, z, z, z, -1, 1, 4, 0.1, 0.0)
         with pytest.raises(ValueError):

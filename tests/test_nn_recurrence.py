@@ -126,7 +126,7 @@ def test_refusals(numpy_backend):
         p.nn.gated_recurrence_grad(x, x, gate, p.zeros((2, 3), dtype="float32"))
     with pytest.raises(ValueError):
         p.nn.gated_recurrence_step(p.zeros((), dtype="float32"), p.zeros((), dtype="float32"), x)
-    with pytest.raises(ValueError, match="initial"):
+    with pytest.raises(ValueError, match="state"):
         p.nn.gated_recurrence_step(x, gate, p.zeros((2, 3), dtype="float32"))
     with pytest.raises(NotImplementedError, match="not captured"):
         p.compile(lambda x, g: f(x, g))(x, gate)
