@@ -27,14 +27,13 @@ __device__ __forceinline__ float inverse(float x) {
 __device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
 
 // keep = sigmoid(g) and take = 1 - keep, each to full precision: one of them is
-// 1 / (1 + exp(-|g|)), the other exp(-|g|) times it.
+// 1 / (1 + exp(-|g|)), the other exp(-|g|) times it. Of a NaN both are NaN.
 template <typename T>
 __device__ __forceinline__ void gates(T g, T& keep, T& take) {
   const T small = exp_down(-__builtin_elementwise_abs(g));
   const T large = inverse(T(1) + small);
   keep = g >= T(0) ? large : small * large;
   take = g >= T(0) ? small * large : large;
-  if (g != g) keep = take = g;
 }
 
 }  // namespace hpd

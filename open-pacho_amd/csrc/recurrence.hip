@@ -13,18 +13,24 @@
 // Bound: HBM. Forward reads x and the gates and writes h, backward reads four
 // arrays and writes two, each once. A lane owns a channel, so that a wave reads
 // 64 neighbouring channels of a step at once whatever their number and
-// alignment; a workgroup owns 64 channels, and its waves consecutive runs of R
+// alignment; a workgroup owns 64 channels, and its W waves consecutive runs of R
 // steps. Each wave loads its run into registers, composes it, leaves (A, B) in
 // LDS, takes what the waves before it left, and then computes and stores its
-// states: one pass over the data, one barrier for each R x waves steps. The next
-// run's loads are issued before the barrier.
+// states: one pass over the data, one barrier for each R x W steps. Two sets of
+// registers take turns, so that the next run's loads are in flight while a run
+// is computed.
+//
+// Few channels would leave compute units idle: then time is cut into segments
+// for workgroups of their own, and a kernel before composes each segment, at the
+// price of reading the gates and x (backward: the gradient) twice.
+#include <type_traits>
+
 #include "common.h"
 #include "exponential.h"
 
 namespace {
 
-constexpr int kMaxWaves = 8;
-
+// Steps of a wave's run.
 template <typename T>
 struct Steps;
 template <>
@@ -36,12 +42,16 @@ struct Steps<double> {
   static constexpr int forward = 8, backward = 4;
 };
 
+constexpr unsigned kDies = 8;  // of the chip, each with a cache of its own
+
 struct Extents {
   int64_t time;      // steps of a row
   int64_t total;     // rows x channels
   int64_t channels;  // of a step
   int64_t gates;     // of a step
   int64_t width;     // channels that share a gate: channels / gates
+  int64_t groups;    // of 64 lanes
+  int64_t segment;   // steps of a segment
   // Backward with shared gates: lanes are laid out by heads.
   int64_t heads;  // rows x gates
   int pack;       // whole heads in a wave (width <= 64), else 1
@@ -89,8 +99,9 @@ __device__ __forceinline__ T apply(T a, T b, T h) {
 template <typename T, int R>
 __device__ __forceinline__ void load_steps(const T* column, int64_t stride, int64_t t, int64_t end, T outside, T (&v)[R]) {
   if (t >= 0 && t + R <= end) {
+    const T* p = column + t * stride;
 #pragma unroll
-    for (int i = 0; i < R; ++i) v[i] = column[(t + i) * stride];
+    for (int i = 0; i < R; ++i) v[i] = p[i * stride];
   } else {
 #pragma unroll
     for (int i = 0; i < R; ++i) v[i] = t + i >= 0 && t + i < end ? column[(t + i) * stride] : outside;
@@ -101,6 +112,17 @@ __device__ __forceinline__ void load_steps(const T* column, int64_t stride, int6
 template <int R>
 __device__ __forceinline__ unsigned load_resets(const uint8_t* row, int64_t t, int64_t end) {
   unsigned bits = 0;
+  if (R % 4 == 0 && t >= 0 && t + R <= end) {
+    typedef uint32_t U __attribute__((ext_vector_type(R < 4 ? 1 : R / 4), aligned(1)));
+    const U v = *reinterpret_cast<const U*>(row + t);
+    // The top bit of a byte is set where it is not 0; a product gathers four of them.
+#pragma unroll
+    for (int j = 0; j < R / 4; ++j) {
+      const unsigned set = (((v[j] & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | v[j]) >> 7 & 0x01010101u;
+      bits |= (set * 0x01020408u >> 24 & 15) << 4 * j;
+    }
+    return bits;
+  }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (t + i >= 0 && t + i < end) bits |= unsigned(row[t + i] != 0) << i;
@@ -108,160 +130,371 @@ __device__ __forceinline__ unsigned load_resets(const uint8_t* row, int64_t t, i
   return bits;
 }
 
-template <typename T, int R, bool RESETS>
-__global__ __launch_bounds__(kMaxWaves * 64) void forward_kernel(const T* __restrict__ x, const T* __restrict__ gate,
-                                                                 const T* __restrict__ initial,
-                                                                 const uint8_t* __restrict__ resets,
-                                                                 T* __restrict__ h, Extents e) {
-  __shared__ T left_a[2][kMaxWaves][64], left_b[2][kMaxWaves][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const Place at = flat_place(e, blockIdx.x, lane);
+// What the waves of a workgroup leave for each other; two sets, so that one
+// barrier is enough.
+template <typename T, int W>
+struct Left {
+  T a[2][W][64], b[2][W][64];
+};
+
+// Takes `before` through the runs of all waves in their order: `before` becomes
+// the value after the last one, the result is the one before this wave's run.
+template <typename T, int W>
+__device__ __forceinline__ T through(const Run<T>& run, Left<T, W>& left, int turn, int wave, int lane, T& before) {
+  if constexpr (W == 1) {
+    const T now = before;
+    before = apply(run.cut ? T(-1) : run.a, run.b, before);
+    return now;
+  }
+  left.a[turn][wave][lane] = run.cut ? T(-1) : run.a;
+  left.b[turn][wave][lane] = run.b;
+  __syncthreads();
+  T now = before;
+#pragma unroll
+  for (int first = 0; first < W; first += 4) {  // four waves' at a time: two registers each
+    T a[4], b[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) a[w] = left.a[turn][first + w][lane], b[w] = left.b[turn][first + w][lane];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (first + w == wave) now = before;
+      before = apply(a[w], b[w], before);
+    }
+  }
+  return now;
+}
+
+// The state before a segment: the value before the row through the segments
+// before it, whose compositions stand in parts (A, then B) by segment.
+template <typename T>
+__device__ __forceinline__ T through_segments(const T* parts, int64_t total, int64_t q, int64_t segments, int64_t before, T state) {
+  const T *a = parts + q, *b = parts + segments * total + q;
+  int64_t s = 0;
+  for (; s + 8 <= before; s += 8) {
+    T av[8], bv[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) av[k] = a[(s + k) * total], bv[k] = b[(s + k) * total];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) state = apply(av[k], bv[k], state);
+  }
+  for (; s < before; ++s) state = apply(a[s * total], b[s * total], state);
+  return state;
+}
+
+// A workgroup's channels and steps.
+struct Part {
+  int64_t group, segment, begin, end;
+};
+
+__device__ __forceinline__ Part part_of(const Extents& e) {
+  // Consecutive workgroups start on different dies; consecutive groups of a
+  // segment, which share lines where rows are not whole lines, go to one.
+  const unsigned die = blockIdx.x % kDies, least = gridDim.x / kDies, more = gridDim.x % kDies;
+  const int64_t place = die * least + (die < more ? die : more) + blockIdx.x / kDies;
+  const int64_t segment = place / e.groups, begin = segment * e.segment;
+  return {place - segment * e.groups, segment, begin, begin + e.segment < e.time ? begin + e.segment : e.time};
+}
+
+// ---- forward ---------------------------------------------------------------------
+
+template <typename T, int R>
+struct ForwardLoads {
+  T x[R], gate[R];
+  unsigned resets = 0;
+
+  // Steps past the end keep the state: their gate is +inf.
+  template <bool RESETS>
+  __device__ __forceinline__ void load(const T* xs, const T* gs, const uint8_t* rs, const Extents& e, int64_t t, int64_t end) {
+    load_steps<T, R>(xs, e.channels, t, end, T(0), x);
+    load_steps<T, R>(gs, e.gates, t, end, T(__builtin_huge_val()), gate);
+    if (RESETS) resets = load_resets<R>(rs, t, end);
+  }
+
+  // x and gate become (1 - a) x and a; `run` goes on through the steps.
+  template <bool RESETS>
+  __device__ __forceinline__ void compose(Run<T>& run) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      T keep, take;
+      hpd::gates(gate[i], keep, take);
+      gate[i] = keep;
+      x[i] *= take;
+      const bool cut = RESETS && (resets >> i & 1);
+      run.b = (cut ? T(0) : keep * run.b) + x[i];
+      run.a *= keep;
+    }
+    run.cut = run.cut || (RESETS && resets);
+  }
+};
+
+template <typename T, int R, int W, bool RESETS>
+__global__ __launch_bounds__(W * 64) void forward_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                         const T* __restrict__ initial, const uint8_t* __restrict__ resets,
+                                                         T* __restrict__ h, const T* __restrict__ parts, Extents e) {
+  __shared__ Left<T, W> left;
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Part part = part_of(e);
+  const Place at = flat_place(e, part.group, lane);
   const T* xs = x + at.row * e.time * e.channels + at.channel;
   const T* gs = gate + at.row * e.time * e.gates + at.gate;
   const uint8_t* rs = RESETS ? resets + at.row * e.time : nullptr;
   T* hs = h + at.row * e.time * e.channels + at.channel;
-  T state = initial ? initial[at.row * e.channels + at.channel] : T(0);
+  const int64_t q = at.row * e.channels + at.channel;
+  T state = initial ? initial[q] : T(0);
+  if (parts) state = through_segments(parts, e.total, q, gridDim.x / e.groups, part.segment, state);
 
-  // Steps past the end keep the state: their gate is +inf.
-  const T open = __builtin_huge_val();
-  T nx[R], ng[R];
-  unsigned nr = 0;
-  int64_t t = int64_t(wave) * R;
-  const int64_t stride = int64_t(waves) * R;
-  load_steps<T, R>(xs, e.channels, t, e.time, T(0), nx);
-  load_steps<T, R>(gs, e.gates, t, e.time, open, ng);
-  if (RESETS) nr = load_resets<R>(rs, t, e.time);
-
-  int turn = 0;
-  for (int64_t base = 0; base < e.time; base += stride, t += stride, turn ^= 1) {
-    T a[R], b[R];
-    const unsigned reset = nr;
+  constexpr int64_t stride = int64_t(W) * R;
+  int64_t t = part.begin + int64_t(wave) * R;
+  ForwardLoads<T, R> one, two;
+  const auto steps = [&](ForwardLoads<T, R>& now, ForwardLoads<T, R>& next, int turn) {
+    if (t + stride < part.end) next.template load<RESETS>(xs, gs, rs, e, t + stride, part.end);
     Run<T> run{T(1), T(0), false};
+    now.template compose<RESETS>(run);
+    T value = through<T, W>(run, left, turn, wave, lane, state);
+    const bool whole = t + R <= part.end;
+    T* out = hs + t * e.channels;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      T take;
-      hpd::gates(ng[i], a[i], take);
-      b[i] = take * nx[i];
-      const bool cut = RESETS && (reset >> i & 1);
-      run.cut = run.cut || cut;
-      run.b = (cut ? T(0) : a[i] * run.b) + b[i];
-      run.a *= a[i];
+      const bool cut = RESETS && (now.resets >> i & 1);
+      now.x[i] = value = (cut ? T(0) : now.gate[i] * value) + now.x[i];
     }
-    if (base + stride < e.time) {
-      load_steps<T, R>(xs, e.channels, t + stride, e.time, T(0), nx);
-      load_steps<T, R>(gs, e.gates, t + stride, e.time, open, ng);
-      if (RESETS) nr = load_resets<R>(rs, t + stride, e.time);
-    }
-    left_a[turn][wave][lane] = run.cut ? T(-1) : run.a;
-    left_b[turn][wave][lane] = run.b;
-    __syncthreads();
-    T now = state;
-    for (int w = 0; w < waves; ++w) {
-      if (w == wave) now = state;
-      state = apply(left_a[turn][w][lane], left_b[turn][w][lane], state);
-    }
+    if (at.valid) {
+      if (whole) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const bool cut = RESETS && (reset >> i & 1);
-      now = (cut ? T(0) : a[i] * now) + b[i];
-      if (at.valid && t + i < e.time) hs[(t + i) * e.channels] = now;
+        for (int i = 0; i < R; ++i) out[i * e.channels] = now.x[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (t + i < part.end) out[i * e.channels] = now.x[i];
+        }
+      }
     }
+    t += stride;
+  };
+  one.template load<RESETS>(xs, gs, rs, e, t, part.end);
+  for (int64_t base = part.begin; base < part.end; base += 2 * stride) {
+    steps(one, two, 0);
+    if (base + stride < part.end) steps(two, one, 1);
   }
 }
 
+// ---- backward --------------------------------------------------------------------
+
+template <typename T, int R>
+struct BackwardLoads {
+  T x[R], gate[R], h[R], grad[R];
+  unsigned resets = 0;
+
+  // Steps outside the segment pass the gradient on: their gate is +inf and their
+  // gradient 0. h is that of the step before. STATES: with x and h.
+  template <bool RESETS, bool STATES = true>
+  __device__ __forceinline__ void load(const T* xs, const T* gs, const T* hs, const T* ds, const uint8_t* rs, T before,
+                                       const Extents& e, int64_t t, int64_t begin) {
+    load_steps<T, R>(gs, e.gates, t, e.time, T(__builtin_huge_val()), gate);
+    load_steps<T, R>(ds, e.channels, t, e.time, T(0), grad);
+    if constexpr (STATES) {
+      load_steps<T, R>(xs, e.channels, t, e.time, T(0), x);
+      load_steps<T, R>(hs, e.channels, t - 1, e.time, before, h);
+    } else {
+#pragma unroll
+      for (int i = 0; i < R; ++i) x[i] = h[i] = T(0);
+    }
+    if (RESETS) resets = load_resets<R>(rs, t, e.time);
+    if (t < begin) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (t + i < begin) gate[i] = T(__builtin_huge_val()), grad[i] = T(0), resets &= ~(1u << i);
+      }
+    }
+  }
+
+  // gate becomes a, h - x (0 - x at a reset) stands in h and 1 - a in x; `run`
+  // goes on through the steps, from the last.
+  template <bool RESETS>
+  __device__ __forceinline__ void compose(Run<T>& run) {
+#pragma unroll
+    for (int i = R - 1; i >= 0; --i) {
+      T keep, take;
+      hpd::gates(gate[i], keep, take);
+      gate[i] = keep;
+      const bool cut = RESETS && (resets >> i & 1);
+      h[i] = (cut ? T(0) : h[i]) - x[i];
+      x[i] = take;
+      run.b = cut ? T(0) : keep * (grad[i] + run.b);
+      run.a *= keep;
+    }
+    run.cut = run.cut || (RESETS && resets);
+  }
+};
+
+// Lanes that share one of a wave's R x pack sums of gate gradients: a power of two.
+template <int R>
+struct SumLanes {
+  __device__ __forceinline__ static int of(int pack) {
+    int lanes = 1;
+    while (lanes * 2 * R * pack <= 64) lanes *= 2;
+    return lanes;
+  }
+};
+
 // SHARED: gates that heads share; dgate then holds e.pieces partial sums.
-template <typename T, int R, bool RESETS, bool SHARED>
-__global__ __launch_bounds__(kMaxWaves * 64) void backward_kernel(
-    const T* __restrict__ grad, const T* __restrict__ x, const T* __restrict__ gate, const T* __restrict__ h,
-    const T* __restrict__ initial, const uint8_t* __restrict__ resets, T* __restrict__ dx, T* __restrict__ dgate,
-    T* __restrict__ dinitial, Extents e) {
-  __shared__ T left_a[2][kMaxWaves][64], left_b[2][kMaxWaves][64];
-  __shared__ T shares[SHARED ? kMaxWaves : 1][SHARED ? R : 1][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const Place at = SHARED ? head_place(e, blockIdx.x, lane) : flat_place(e, blockIdx.x, lane);
+template <typename T, int R, int W, bool RESETS, bool SHARED>
+__global__ __launch_bounds__(W * 64) void backward_kernel(const T* __restrict__ grad, const T* __restrict__ x,
+                                                          const T* __restrict__ gate, const T* __restrict__ h,
+                                                          const T* __restrict__ initial, const uint8_t* __restrict__ resets,
+                                                          T* __restrict__ dx, T* __restrict__ dgate, T* __restrict__ dinitial,
+                                                          const T* __restrict__ parts, Extents e) {
+  __shared__ Left<T, W> left;
+  __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];  // rows of a task's lanes in banks of their own
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Part part = part_of(e);
+  const Place at = SHARED ? head_place(e, part.group, lane) : flat_place(e, part.group, lane);
   const int64_t column = at.row * e.time * e.channels + at.channel;
   const int64_t gate_column = at.row * e.time * e.gates + at.gate;
   const T *xs = x + column, *hs = h + column, *ds = grad + column, *gs = gate + gate_column;
   const uint8_t* rs = RESETS ? resets + at.row * e.time : nullptr;
-  const int64_t first = at.row * e.channels + at.channel;
-  const T before = initial ? initial[first] : T(0);
+  const int64_t q = at.row * e.channels + at.channel;
+  const T before = initial ? initial[q] : T(0);
+  const int64_t segments = gridDim.x / e.groups;
+  T carried = T(0);
+  // Segments are kept from the last one on, in the order of this pass.
+  if (parts) carried = through_segments(parts, e.total, q, segments, segments - 1 - part.segment, carried);
 
   // Wave 0 takes the last R steps, wave 1 those before them: t is the first
-  // step of a wave's run, below zero at the start of the row. Steps outside
-  // the row pass the gradient on: their gate is +inf and their gradient 0.
-  const T open = __builtin_huge_val();
-  T nx[R], ng[R], nh[R], nd[R];
-  unsigned nr = 0;
-  int64_t t = e.time - int64_t(wave + 1) * R;
-  const int64_t stride = int64_t(waves) * R;
-  const auto load = [&](int64_t from) {
-    load_steps<T, R>(xs, e.channels, from, e.time, T(0), nx);
-    load_steps<T, R>(gs, e.gates, from, e.time, open, ng);
-    load_steps<T, R>(ds, e.channels, from, e.time, T(0), nd);
-    load_steps<T, R>(hs, e.channels, from - 1, e.time, before, nh);
-    if (RESETS) nr = load_resets<R>(rs, from, e.time);
-  };
-  load(t);
-
-  T carried = T(0);
-  int turn = 0;
-  for (int64_t base = 0; base < e.time; base += stride, t -= stride, turn ^= 1) {
-    T a[R], take[R], d[R], apart[R];
-    const unsigned reset = nr;
+  // step of a wave's run, before the segment at its start.
+  constexpr int64_t stride = int64_t(W) * R;
+  int64_t t = part.end - int64_t(wave + 1) * R;
+  BackwardLoads<T, R> one, two;
+  const auto steps = [&](BackwardLoads<T, R>& now, BackwardLoads<T, R>& next, int turn, bool more) {
+    if (more) next.template load<RESETS>(xs, gs, hs, ds, rs, before, e, t - stride, part.begin);
     Run<T> run{T(1), T(0), false};
+    now.template compose<RESETS>(run);
+    T value = through<T, W>(run, left, turn, wave, lane, carried);
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
-      const bool cut = RESETS && (reset >> i & 1);
-      hpd::gates(ng[i], a[i], take[i]);
-      d[i] = nd[i];
-      apart[i] = (cut ? T(0) : nh[i]) - nx[i];
-      run.cut = run.cut || cut;
-      run.b = cut ? T(0) : a[i] * (d[i] + run.b);
-      run.a *= a[i];
+      const bool cut = RESETS && (now.resets >> i & 1);
+      const T slope = now.grad[i] + value;
+      value = cut ? T(0) : now.gate[i] * slope;
+      now.h[i] = slope * now.h[i] * (now.gate[i] * now.x[i]);
+      now.x[i] = slope * now.x[i];
     }
-    if (base + stride < e.time) load(t - stride);
-    left_a[turn][wave][lane] = run.cut ? T(-1) : run.a;
-    left_b[turn][wave][lane] = run.b;
-    __syncthreads();
-    T now = carried;
-    for (int w = 0; w < waves; ++w) {
-      if (w == wave) now = carried;
-      carried = apply(left_a[turn][w][lane], left_b[turn][w][lane], carried);
-    }
+    T* out = dx + column + t * e.channels;
+    T* out_gate = dgate + gate_column + t * e.gates;
+    if (at.valid) {
+      if (t >= part.begin) {
 #pragma unroll
-    for (int i = R - 1; i >= 0; --i) {
-      const bool cut = RESETS && (reset >> i & 1);
-      const bool inside = at.valid && t + i >= 0;
-      const T slope = d[i] + now;
-      now = cut ? T(0) : a[i] * slope;
-      const T share = slope * apart[i] * (a[i] * take[i]);
-      if (inside) dx[column + (t + i) * e.channels] = slope * take[i];
-      if constexpr (SHARED) shares[wave][i][lane] = share;
-      else if (inside) dgate[gate_column + (t + i) * e.gates] = share;
+        for (int i = 0; i < R; ++i) {
+          out[i * e.channels] = now.x[i];
+          if (!SHARED) out_gate[i * e.gates] = now.h[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (t + i >= part.begin) {
+            out[i * e.channels] = now.x[i];
+            if (!SHARED) out_gate[i * e.gates] = now.h[i];
+          }
+        }
+      }
     }
     if constexpr (SHARED) {
       // The wave's own rows of LDS: its stores are in order before its loads.
+#pragma unroll
+      for (int i = 0; i < R; ++i) shares[wave][i][lane] = now.h[i];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      const int64_t group = blockIdx.x;
-      const int64_t head0 = group / e.pieces * e.pack;
-      const int64_t left = e.width - (group % e.pieces) * e.piece;
-      const int count = int(left < e.piece ? left : e.piece);
-      T* out = dgate + (group % e.pieces) * (e.heads * e.time);
-      for (int task = lane; task < R * e.pack; task += 64) {
-        const int i = task / e.pack, slot = task - i * e.pack;
-        const int64_t head = head0 + slot;
-        if (head >= e.heads || t + i < 0) continue;
+      const int64_t piece = part.group % e.pieces, head0 = part.group / e.pieces * e.pack;
+      const int64_t rest = e.width - piece * e.piece;
+      const int count = int(rest < e.piece ? rest : e.piece);
+      T* sums = dgate + piece * (e.heads * e.time);
+      // One sum for each step and head of the wave, by neighbouring lanes.
+      const int lanes = SumLanes<R>::of(e.pack), sub = lane % lanes;
+      for (int first = 0; first < R * e.pack; first += 64 / lanes) {
+        const int task = first + lane / lanes, i = task / e.pack, slot = task - i * e.pack;
         T sum = T(0);
-        for (int k = 0; k < count; ++k) sum += shares[wave][i][slot * e.piece + k];
+        if (i < R) {
+          for (int k = sub; k < count; k += lanes) sum += shares[wave][i][slot * e.piece + k];
+        }
+        for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        const int64_t head = head0 + slot;
+        if (sub != 0 || i >= R || head >= e.heads || t + i < part.begin) continue;
         const int64_t row = head / e.gates;
-        out[(row * e.time + t + i) * e.gates + (head - row * e.gates)] = sum;
+        sums[(row * e.time + t + i) * e.gates + (head - row * e.gates)] = sum;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
+    t -= stride;
+  };
+  one.template load<RESETS>(xs, gs, hs, ds, rs, before, e, t, part.begin);
+  for (int64_t base = part.begin; base < part.end; base += 2 * stride) {
+    const bool second = base + stride < part.end;
+    steps(one, two, 0, second);
+    if (second) steps(two, one, 1, base + 2 * stride < part.end);
   }
-  if (dinitial && wave == 0 && at.valid) dinitial[first] = carried;
+  if (dinitial && part.segment == 0 && wave == 0 && at.valid) dinitial[q] = carried;
+}
+
+// ---- segments --------------------------------------------------------------------
+
+// The composition of every segment but the last one in the pass's order, per
+// channel. A wave composes one W-th of a segment.
+template <typename T, int R, int W, bool RESETS, bool BACKWARD>
+__global__ __launch_bounds__(W * 64) void segments_kernel(const T* __restrict__ values, const T* __restrict__ gate,
+                                                          const uint8_t* __restrict__ resets, T* __restrict__ parts,
+                                                          Extents e) {
+  __shared__ T left_a[W][64], left_b[W][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Part part = part_of(e);
+  const int64_t place = part.segment, composed = gridDim.x / e.groups;  // one less than segments
+  if (BACKWARD) {
+    part.begin = (composed - place) * e.segment;
+    part.end = part.begin + e.segment < e.time ? part.begin + e.segment : e.time;
+  }
+  const Place at = flat_place(e, part.group, lane);
+  const T* vs = values + at.row * e.time * e.channels + at.channel;
+  const T* gs = gate + at.row * e.time * e.gates + at.gate;
+  const uint8_t* rs = RESETS ? resets + at.row * e.time : nullptr;
+  const int64_t share = (e.segment + W * R - 1) / (W * R) * R;
+  Run<T> run{T(1), T(0), false};
+  if (!BACKWARD) {
+    const int64_t begin = part.begin + wave * share, end = begin + share < part.end ? begin + share : part.end;
+    ForwardLoads<T, R> one, two;
+    one.template load<RESETS>(vs, gs, rs, e, begin, end);
+    for (int64_t t = begin; t < end; t += 2 * R) {
+      two.template load<RESETS>(vs, gs, rs, e, t + R, end);
+      one.template compose<RESETS>(run);
+      one.template load<RESETS>(vs, gs, rs, e, t + 2 * R, end);
+      two.template compose<RESETS>(run);
+    }
+  } else {
+    const int64_t end = part.end - wave * share, begin = end - share > part.begin ? end - share : part.begin;
+    BackwardLoads<T, R> one, two;
+    const auto load = [&](BackwardLoads<T, R>& to, int64_t t) {
+      to.template load<RESETS, false>(nullptr, gs, nullptr, vs, rs, T(0), e, t, begin);
+    };
+    load(one, end - R);
+    for (int64_t t = end - R; t + R > begin; t -= 2 * R) {
+      load(two, t - R);
+      one.template compose<RESETS>(run);
+      load(one, t - 2 * R);
+      two.template compose<RESETS>(run);
+    }
+  }
+  left_a[wave][lane] = run.cut ? T(-1) : run.a;
+  left_b[wave][lane] = run.b;
+  __syncthreads();
+  if (wave != 0 || !at.valid) return;
+  Run<T> all{T(1), T(0), false};
+  for (int w = 0; w < W; ++w) {
+    const T a = left_a[w][lane];
+    all.b = apply(a, left_b[w][lane], all.b);
+    all.cut = all.cut || a < T(0);
+    all.a *= a;
+  }
+  const int64_t q = at.row * e.channels + at.channel, segments = composed + 1;
+  parts[place * e.total + q] = all.cut ? T(-1) : all.a;
+  parts[(segments + place) * e.total + q] = all.b;
 }
 
 // out[i] = sum over k of parts[k][i], in order.
@@ -296,46 +529,88 @@ unsigned checked_grid(int64_t groups, int threads) {
   return unsigned(groups);
 }
 
-int waves_for(int64_t time, int steps) {
-  int waves = 1;
-  while (waves < kMaxWaves && waves * steps < time) waves *= 2;
-  return waves;
+constexpr int kWaves = 16, kSegmentWaves = 8;
+
+// Cuts time where groups are too few to fill the chip; returns the number of
+// segments.
+int64_t plan_segments(const hp_ctx* ctx, Extents& e, int steps) {
+  const int64_t least = int64_t(kWaves) * steps;  // of a segment
+  int64_t segments = 1;
+  if (e.groups * 2 <= ctx->compute_units) segments = std::min(ctx->compute_units / e.groups, e.time / least);
+  e.segment = segments > 1 ? hp::ceil_div(hp::ceil_div(e.time, segments), least) * least : e.time;
+  return hp::ceil_div(e.time, e.segment);
+}
+
+// Calls f with the waves of a workgroup and the steps of a run.
+template <int R, typename F>
+void with_shape(int64_t time, F&& f) {
+  using Int = std::integral_constant<int, R>;
+  if (time == 1) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  else if (time <= R) f(std::integral_constant<int, 1>{}, Int{});
+  else if (time <= 4 * R) f(std::integral_constant<int, 4>{}, Int{});
+  else f(std::integral_constant<int, kWaves>{}, Int{});
+}
+
+// The compositions of the segments, in scratch memory; null for one segment.
+template <typename T, int R, bool BACKWARD>
+T* compose_segments(hp_ctx* ctx, const T* values, const T* gate, const uint8_t* resets, Extents e, int64_t segments) {
+  if (segments == 1) return nullptr;
+  e.groups = hp::ceil_div(e.total, 64);
+  T* parts = static_cast<T*>(hp::scratch_alloc(ctx, size_t(2 * segments) * size_t(e.total) * sizeof(T)));
+  constexpr int W = kSegmentWaves;
+  const unsigned grid = checked_grid(e.groups * (segments - 1), 64 * W);
+  const auto kernel = resets ? segments_kernel<T, R, W, true, BACKWARD> : segments_kernel<T, R, W, false, BACKWARD>;
+  kernel<<<grid, 64 * W, 0, ctx->stream>>>(values, gate, resets, parts, e);
+  return parts;
+}
+
+// Returns a call's scratch memory, then reports a failed launch.
+void finish(hp_ctx* ctx, const char* name, void* one, void* two) {
+  const hipError_t status = hipGetLastError();
+  if (one) hp::scratch_free(ctx, one);
+  if (two) hp::scratch_free(ctx, two);
+  hp::check_hip(status, name);
 }
 
 template <typename T>
-void forward(hp_ctx* ctx, const T* x, const T* gate, const T* initial, const uint8_t* resets, T* h, const Extents& e) {
+void forward(hp_ctx* ctx, const T* x, const T* gate, const T* initial, const uint8_t* resets, T* h, Extents e) {
   constexpr int R = Steps<T>::forward;
-  const int threads = 64 * waves_for(e.time, R);
-  const unsigned grid = checked_grid(hp::ceil_div(e.total, 64), threads);
-  const auto kernel = resets ? forward_kernel<T, R, true> : forward_kernel<T, R, false>;
-  kernel<<<grid, threads, 0, ctx->stream>>>(x, gate, initial, resets, h, e);
-  hp::check_launch("recurrence forward");
+  e.groups = hp::ceil_div(e.total, 64);
+  const int64_t segments = plan_segments(ctx, e, R);
+  T* parts = nullptr;
+  with_shape<R>(e.time, [&](auto waves, auto steps) {
+    constexpr int W = waves, S = steps;
+    const unsigned grid = checked_grid(e.groups * segments, 64 * W);
+    parts = compose_segments<T, R, false>(ctx, x, gate, resets, e, segments);
+    const auto kernel = resets ? forward_kernel<T, S, W, true> : forward_kernel<T, S, W, false>;
+    kernel<<<grid, 64 * W, 0, ctx->stream>>>(x, gate, initial, resets, h, parts, e);
+  });
+  finish(ctx, "launch of the recurrence", parts, nullptr);
 }
 
 template <typename T>
 void backward(hp_ctx* ctx, const T* grad, const T* x, const T* gate, const T* h, const T* initial,
-              const uint8_t* resets, T* dx, T* dgate, T* dinitial, const Extents& e) {
+              const uint8_t* resets, T* dx, T* dgate, T* dinitial, Extents e) {
   constexpr int R = Steps<T>::backward;
   const bool shared = e.width > 1;
-  const int64_t groups = shared ? hp::ceil_div(e.heads, e.pack) * e.pieces : hp::ceil_div(e.total, 64);
-  const int threads = 64 * waves_for(e.time, R);
-  const unsigned grid = checked_grid(groups, threads);
+  e.groups = shared ? hp::ceil_div(e.heads, e.pack) * e.pieces : hp::ceil_div(e.total, 64);
+  const int64_t segments = plan_segments(ctx, e, R);
   const int64_t count = e.heads * e.time;
-  T* parts = dgate;
-  if (e.pieces > 1) parts = static_cast<T*>(hp::scratch_alloc(ctx, size_t(e.pieces) * size_t(count) * sizeof(T)));
-  const auto kernel = shared ? (resets ? backward_kernel<T, R, true, true> : backward_kernel<T, R, false, true>)
-                             : (resets ? backward_kernel<T, R, true, false> : backward_kernel<T, R, false, false>);
-  kernel<<<grid, threads, 0, ctx->stream>>>(grad, x, gate, h, initial, resets, dx, parts, dinitial, e);
-  const hipError_t status = hipGetLastError();
+  T *parts = nullptr, *sums = dgate;
+  with_shape<R>(e.time, [&](auto waves, auto steps) {
+    constexpr int W = waves, S = steps;
+    const unsigned grid = checked_grid(e.groups * segments, 64 * W);
+    if (e.pieces > 1) sums = static_cast<T*>(hp::scratch_alloc(ctx, size_t(e.pieces) * size_t(count) * sizeof(T)));
+    parts = compose_segments<T, R, true>(ctx, grad, gate, resets, e, segments);
+    const auto kernel = shared ? (resets ? backward_kernel<T, S, W, true, true> : backward_kernel<T, S, W, false, true>)
+                               : (resets ? backward_kernel<T, S, W, true, false> : backward_kernel<T, S, W, false, false>);
+    kernel<<<grid, 64 * W, 0, ctx->stream>>>(grad, x, gate, h, initial, resets, dx, sums, dinitial, parts, e);
+  });
   if (e.pieces > 1) {
-    if (status == hipSuccess) {
-      const int64_t blocks = std::min<int64_t>(hp::ceil_div(count, 256), 4096);
-      add_parts_kernel<T><<<unsigned(blocks), 256, 0, ctx->stream>>>(parts, dgate, count, e.pieces);
-    }
-    hp::scratch_free(ctx, parts);
+    const int64_t blocks = std::min<int64_t>(hp::ceil_div(count, 256), 4096);
+    add_parts_kernel<T><<<unsigned(blocks), 256, 0, ctx->stream>>>(sums, dgate, count, e.pieces);
   }
-  hp::check_hip(status, "launch of recurrence backward");
-  hp::check_launch("recurrence gate sums");
+  finish(ctx, "launch of the recurrence's gradient", parts, e.pieces > 1 ? sums : nullptr);
 }
 
 }  // namespace
