@@ -102,6 +102,33 @@ void enter(hp_ctx* ctx);
 void* scratch_alloc(hp_ctx* ctx, size_t bytes);
 void scratch_free(hp_ctx* ctx, void* ptr);
 
+// Temporaries of one call, returned to the pool when it ends (stream ordered:
+// also while the kernels that use them are queued).
+class Scratch {
+ public:
+  explicit Scratch(hp_ctx* ctx) : ctx_(ctx) {}
+  Scratch(const Scratch&) = delete;
+  Scratch& operator=(const Scratch&) = delete;
+  ~Scratch() {
+    for (void* p : held_) {
+      try {
+        scratch_free(ctx_, p);
+      } catch (...) {  // must not leave a destructor; the context frees the block when it ends
+      }
+    }
+  }
+  template <typename T>
+  T* take(int64_t count) {
+    held_.reserve(held_.size() + 1);
+    held_.push_back(scratch_alloc(ctx_, size_t(count) * sizeof(T)));
+    return static_cast<T*>(held_.back());
+  }
+
+ private:
+  hp_ctx* ctx_;
+  std::vector<void*> held_;
+};
+
 inline void require(bool condition, const std::string& message) {
   if (!condition) fail(HP_E_INVALID, message);
 }

@@ -20,9 +20,16 @@
 // registers take turns, so that the next run's loads are in flight while a run
 // is computed.
 //
-// Few channels would leave compute units idle: then time is cut into segments
-// for workgroups of their own, and a kernel before composes each segment, at the
-// price of reading the gates and x (backward: the gradient) twice.
+// Few channels would leave compute units idle: then every W x R steps of 64
+// channels are a tile with a workgroup of its own (the chained kernels), still in
+// one pass. A tile publishes its composition as soon as it has it. Tiles count in
+// blocks of `span`: the state before a tile is the one before its block, which
+// the last tile of the block before publishes, through the compositions of the
+// block's earlier tiles, always in the same order, so that results repeat bit
+// for bit. Workgroups take tiles in time order from queues, so a tile only ever
+// waits for tiles whose workgroups have started, and those for earlier ones: every
+// wait ends. A published word is valid by itself, without fences: memory is all
+// ones before, which no published value is.
 #include <type_traits>
 
 #include "common.h"
@@ -51,7 +58,8 @@ struct Extents {
   int64_t gates;     // of a step
   int64_t width;     // channels that share a gate: channels / gates
   int64_t groups;    // of 64 lanes
-  int64_t segment;   // steps of a segment
+  int64_t tiles;     // of a group (chained kernels)
+  int span;          // tiles of a block
   // Backward with shared gates: lanes are laid out by heads.
   int64_t heads;  // rows x gates
   int pack;       // whole heads in a wave (width <= 64), else 1
@@ -164,35 +172,152 @@ __device__ __forceinline__ T through(const Run<T>& run, Left<T, W>& left, int tu
   return now;
 }
 
-// The state before a segment: the value before the row through the segments
-// before it, whose compositions stand in parts (A, then B) by segment.
-template <typename T>
-__device__ __forceinline__ T through_segments(const T* parts, int64_t total, int64_t q, int64_t segments, int64_t before, T state) {
-  const T *a = parts + q, *b = parts + segments * total + q;
-  int64_t s = 0;
-  for (; s + 8 <= before; s += 8) {
-    T av[8], bv[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) av[k] = a[(s + k) * total], bv[k] = b[(s + k) * total];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) state = apply(av[k], bv[k], state);
-  }
-  for (; s < before; ++s) state = apply(a[s * total], b[s * total], state);
-  return state;
+// Workgroup b as number b' such that consecutive b' run on one die: workgroups
+// start on the dies in turn, and neighbouring groups share lines where rows are
+// not whole lines.
+__device__ __forceinline__ int64_t by_die() {
+  const unsigned die = blockIdx.x % kDies, least = gridDim.x / kDies, more = gridDim.x % kDies;
+  return int64_t(die) * least + (die < more ? die : more) + blockIdx.x / kDies;
 }
 
-// A workgroup's channels and steps.
-struct Part {
-  int64_t group, segment, begin, end;
+// ---- chained tiles -----------------------------------------------------------------
+
+template <typename T>
+struct Word;
+template <>
+struct Word<float> {
+  using type = uint32_t;
+};
+template <>
+struct Word<double> {
+  using type = uint64_t;
 };
 
-__device__ __forceinline__ Part part_of(const Extents& e) {
-  // Consecutive workgroups start on different dies; consecutive groups of a
-  // segment, which share lines where rows are not whole lines, go to one.
-  const unsigned die = blockIdx.x % kDies, least = gridDim.x / kDies, more = gridDim.x % kDies;
-  const int64_t place = die * least + (die < more ? die : more) + blockIdx.x / kDies;
-  const int64_t segment = place / e.groups, begin = segment * e.segment;
-  return {place - segment * e.groups, segment, begin, begin + e.segment < e.time ? begin + e.segment : e.time};
+constexpr int kTicketWords = 32;  // of 4 bytes, apart for each die's queue
+
+// Memory of a chained launch, all ones at its start: a queue for each die, the
+// compositions of the tiles (A of 64 lanes, then B), and the states after blocks.
+template <typename T>
+struct Chain {
+  unsigned* tickets;
+  typename Word<T>::type *runs, *states;
+
+  __device__ __forceinline__ static void publish(typename Word<T>::type* at, T value) {
+    typename Word<T>::type bits;
+    __builtin_memcpy(&bits, &value, sizeof(T));
+    if (bits == ~typename Word<T>::type(0)) bits = ~typename Word<T>::type(0) - 1;  // a NaN as well
+    __hip_atomic_store(at, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __device__ __forceinline__ static typename Word<T>::type peek(const typename Word<T>::type* at) {
+    return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  // The value at `at`, first seen as `bits`, once it is there.
+  __device__ __forceinline__ static T await(const typename Word<T>::type* at, typename Word<T>::type bits) {
+    while (bits == ~typename Word<T>::type(0)) {
+      __builtin_amdgcn_s_sleep(1);
+      bits = peek(at);
+    }
+    T value;
+    __builtin_memcpy(&value, &bits, sizeof(T));
+    return value;
+  }
+};
+
+// Groups of a die's queue: [first(die), first(die + 1)).
+__device__ __forceinline__ int64_t first_group(const Extents& e, int die) { return die * e.groups / kDies; }
+
+struct Tile {
+  int64_t group, number;
+};
+
+// The next tile of this die's queue, or of another's when it is empty. There are as
+// many workgroups as tiles, so each finds one (a number below 0 would be none).
+__device__ __forceinline__ Tile take_tile(unsigned* tickets, const Extents& e) {
+  __shared__ int64_t found[2];
+  if (threadIdx.x == 0) {
+    found[1] = -1;
+    for (unsigned turn = 0; turn < kDies; ++turn) {
+      const int die = (blockIdx.x + turn) % kDies;
+      const int64_t first = first_group(e, die), groups = first_group(e, die + 1) - first;
+      if (groups == 0) continue;
+      // All ones counts as -1.
+      const unsigned ticket = 1 + __hip_atomic_fetch_add(tickets + die * kTicketWords, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (ticket >= uint64_t(groups) * uint64_t(e.tiles)) continue;
+      const int64_t number = ticket / groups;
+      found[0] = first + (ticket - number * groups);
+      found[1] = number;
+      break;
+    }
+  }
+  __syncthreads();
+  return {found[0], found[1]};
+}
+
+// a composed with what came before it: `before` where a < 0 is dropped.
+template <typename T>
+__device__ __forceinline__ void then(T& all_a, T& all_b, T a, T b) {
+  all_b = apply(a, b, all_b);
+  all_a = a < T(0) || all_a < T(0) ? T(-1) : all_a * a;
+}
+
+template <typename T, int W>
+struct ChainLeft {
+  T a[W][64], b[W][64], earlier_a[W][64], earlier_b[W][64], state[64];
+};
+
+// The value before this wave's run; `after` becomes the value after the tile.
+// `first` is the value before the row.
+template <typename T, int W>
+__device__ __forceinline__ T through_chain(const Run<T>& run, ChainLeft<T, W>& left, const Chain<T>& chain, const Extents& e,
+                                           const Tile& tile, int wave, int lane, T first, T& after) {
+  using C = Chain<T>;
+  using Bits = typename Word<T>::type;
+  const int64_t block = tile.number / e.span;
+  const int inner = int(tile.number - block * e.span);
+  const bool last = inner == e.span - 1;
+  left.a[wave][lane] = run.cut ? T(-1) : run.a;
+  left.b[wave][lane] = run.b;
+  __syncthreads();
+  T all_a = T(1), all_b = T(0), own_a = T(1), own_b = T(0);
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w == wave) own_a = all_a, own_b = all_b;
+    then(all_a, all_b, left.a[w][lane], left.b[w][lane]);
+  }
+  Bits* const runs = chain.runs + (tile.number * e.groups + tile.group) * 128 + lane;
+  if (wave == 0 && !last) C::publish(runs, all_a), C::publish(runs + 64, all_b);
+  // Each wave takes a run of the block's earlier tiles.
+  const int each = (inner + W - 1) / W, low = wave * each, high = low + each < inner ? low + each : inner;
+  T win_a = T(1), win_b = T(0);
+  for (int p = low; p < high; p += 4) {
+    Bits a[4], b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const Bits* at = runs - (inner - (p + k < high ? p + k : high - 1)) * e.groups * 128;
+      a[k] = C::peek(at), b[k] = C::peek(at + 64);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (p + k >= high) break;
+      const Bits* at = runs - (inner - (p + k)) * e.groups * 128;
+      const T va = C::await(at, a[k]);
+      then(win_a, win_b, va, C::await(at + 64, b[k]));
+    }
+  }
+  left.earlier_a[wave][lane] = win_a;
+  left.earlier_b[wave][lane] = win_b;
+  Bits* const states = chain.states + (block * e.groups + tile.group) * 64 + lane;
+  if (wave == W - 1) {
+    const Bits* at = states - e.groups * 64;
+    left.state[lane] = block == 0 ? first : C::await(at, C::peek(at));
+  }
+  __syncthreads();
+  T state = left.state[lane];
+#pragma unroll
+  for (int w = 0; w < W; ++w) state = apply(left.earlier_a[w][lane], left.earlier_b[w][lane], state);
+  after = apply(all_a, all_b, state);
+  if (wave == 0 && last) C::publish(states, after);
+  return apply(own_a, own_b, state);
 }
 
 // ---- forward ---------------------------------------------------------------------
@@ -227,55 +352,94 @@ struct ForwardLoads {
   }
 };
 
-template <typename T, int R, int W, bool RESETS>
-__global__ __launch_bounds__(W * 64) void forward_kernel(const T* __restrict__ x, const T* __restrict__ gate,
-                                                         const T* __restrict__ initial, const uint8_t* __restrict__ resets,
-                                                         T* __restrict__ h, const T* __restrict__ parts, Extents e) {
-  __shared__ Left<T, W> left;
-  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Part part = part_of(e);
-  const Place at = flat_place(e, part.group, lane);
-  const T* xs = x + at.row * e.time * e.channels + at.channel;
-  const T* gs = gate + at.row * e.time * e.gates + at.gate;
-  const uint8_t* rs = RESETS ? resets + at.row * e.time : nullptr;
-  T* hs = h + at.row * e.time * e.channels + at.channel;
-  const int64_t q = at.row * e.channels + at.channel;
-  T state = initial ? initial[q] : T(0);
-  if (parts) state = through_segments(parts, e.total, q, gridDim.x / e.groups, part.segment, state);
+// The arrays of a call.
+template <typename T>
+struct Forward {
+  const T *x, *gate, *initial;
+  const uint8_t* resets;
+  T* h;
+};
 
-  constexpr int64_t stride = int64_t(W) * R;
-  int64_t t = part.begin + int64_t(wave) * R;
-  ForwardLoads<T, R> one, two;
-  const auto steps = [&](ForwardLoads<T, R>& now, ForwardLoads<T, R>& next, int turn) {
-    if (t + stride < part.end) next.template load<RESETS>(xs, gs, rs, e, t + stride, part.end);
-    Run<T> run{T(1), T(0), false};
-    now.template compose<RESETS>(run);
-    T value = through<T, W>(run, left, turn, wave, lane, state);
-    const bool whole = t + R <= part.end;
-    T* out = hs + t * e.channels;
+// A lane's columns of them.
+template <typename T>
+struct ForwardColumns {
+  const T *x, *gate;
+  const uint8_t* resets;
+  T *h, first;
+  bool valid;
+
+  __device__ __forceinline__ ForwardColumns(const Forward<T>& f, const Extents& e, int64_t group, int lane) {
+    const Place at = flat_place(e, group, lane);
+    const int64_t column = at.row * e.time * e.channels + at.channel;
+    x = f.x + column;
+    h = f.h + column;
+    gate = f.gate + at.row * e.time * e.gates + at.gate;
+    resets = f.resets + at.row * e.time;
+    first = f.initial ? f.initial[at.row * e.channels + at.channel] : T(0);
+    valid = at.valid;
+  }
+
+  // The states of composed steps from t on.
+  template <int R, bool RESETS>
+  __device__ __forceinline__ void finish(ForwardLoads<T, R>& now, const Extents& e, int64_t t, T value) const {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const bool cut = RESETS && (now.resets >> i & 1);
       now.x[i] = value = (cut ? T(0) : now.gate[i] * value) + now.x[i];
     }
-    if (at.valid) {
-      if (whole) {
+    if (!valid) return;
+    T* out = h + t * e.channels;
+    if (t + R <= e.time) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) out[i * e.channels] = now.x[i];
-      } else {
+      for (int i = 0; i < R; ++i) out[i * e.channels] = now.x[i];
+    } else {
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-          if (t + i < part.end) out[i * e.channels] = now.x[i];
-        }
+      for (int i = 0; i < R; ++i) {
+        if (t + i < e.time) out[i * e.channels] = now.x[i];
       }
     }
+  }
+};
+
+template <typename T, int R, int W, bool RESETS>
+__global__ __launch_bounds__(W * 64) void forward_kernel(Forward<T> f, Extents e) {
+  __shared__ Left<T, W> left;
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const ForwardColumns<T> c(f, e, by_die(), lane);
+  T state = c.first;
+  constexpr int64_t stride = int64_t(W) * R;
+  int64_t t = int64_t(wave) * R;
+  ForwardLoads<T, R> one, two;
+  const auto steps = [&](ForwardLoads<T, R>& now, ForwardLoads<T, R>& next, int turn) {
+    if (t + stride < e.time) next.template load<RESETS>(c.x, c.gate, c.resets, e, t + stride, e.time);
+    Run<T> run{T(1), T(0), false};
+    now.template compose<RESETS>(run);
+    const T value = through<T, W>(run, left, turn, wave, lane, state);
+    c.template finish<R, RESETS>(now, e, t, value);
     t += stride;
   };
-  one.template load<RESETS>(xs, gs, rs, e, t, part.end);
-  for (int64_t base = part.begin; base < part.end; base += 2 * stride) {
+  one.template load<RESETS>(c.x, c.gate, c.resets, e, t, e.time);
+  for (int64_t base = 0; base < e.time; base += 2 * stride) {
     steps(one, two, 0);
-    if (base + stride < part.end) steps(two, one, 1);
+    if (base + stride < e.time) steps(two, one, 1);
   }
+}
+
+template <typename T, int R, int W, bool RESETS>
+__global__ __launch_bounds__(W * 64) void forward_chained_kernel(Forward<T> f, Extents e, Chain<T> chain) {
+  __shared__ ChainLeft<T, W> left;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Tile tile = take_tile(chain.tickets, e);
+  if (tile.number < 0) return;
+  const ForwardColumns<T> c(f, e, tile.group, lane);
+  const int64_t t = (tile.number * W + wave) * R;
+  ForwardLoads<T, R> now;
+  now.template load<RESETS>(c.x, c.gate, c.resets, e, t, e.time);
+  Run<T> run{T(1), T(0), false};
+  now.template compose<RESETS>(run);
+  T after;
+  const T value = through_chain<T, W>(run, left, chain, e, tile, wave, lane, c.first, after);
+  c.template finish<R, RESETS>(now, e, t, value);
 }
 
 // ---- backward --------------------------------------------------------------------
@@ -285,27 +449,16 @@ struct BackwardLoads {
   T x[R], gate[R], h[R], grad[R];
   unsigned resets = 0;
 
-  // Steps outside the segment pass the gradient on: their gate is +inf and their
-  // gradient 0. h is that of the step before. STATES: with x and h.
-  template <bool RESETS, bool STATES = true>
+  // Steps before the row pass the gradient on: their gate is +inf and their
+  // gradient 0. h is that of the step before.
+  template <bool RESETS>
   __device__ __forceinline__ void load(const T* xs, const T* gs, const T* hs, const T* ds, const uint8_t* rs, T before,
-                                       const Extents& e, int64_t t, int64_t begin) {
+                                       const Extents& e, int64_t t) {
     load_steps<T, R>(gs, e.gates, t, e.time, T(__builtin_huge_val()), gate);
     load_steps<T, R>(ds, e.channels, t, e.time, T(0), grad);
-    if constexpr (STATES) {
-      load_steps<T, R>(xs, e.channels, t, e.time, T(0), x);
-      load_steps<T, R>(hs, e.channels, t - 1, e.time, before, h);
-    } else {
-#pragma unroll
-      for (int i = 0; i < R; ++i) x[i] = h[i] = T(0);
-    }
+    load_steps<T, R>(xs, e.channels, t, e.time, T(0), x);
+    load_steps<T, R>(hs, e.channels, t - 1, e.time, before, h);
     if (RESETS) resets = load_resets<R>(rs, t, e.time);
-    if (t < begin) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        if (t + i < begin) gate[i] = T(__builtin_huge_val()), grad[i] = T(0), resets &= ~(1u << i);
-      }
-    }
   }
 
   // gate becomes a, h - x (0 - x at a reset) stands in h and 1 - a in x; `run`
@@ -337,39 +490,47 @@ struct SumLanes {
   }
 };
 
-// SHARED: gates that heads share; dgate then holds e.pieces partial sums.
-template <typename T, int R, int W, bool RESETS, bool SHARED>
-__global__ __launch_bounds__(W * 64) void backward_kernel(const T* __restrict__ grad, const T* __restrict__ x,
-                                                          const T* __restrict__ gate, const T* __restrict__ h,
-                                                          const T* __restrict__ initial, const uint8_t* __restrict__ resets,
-                                                          T* __restrict__ dx, T* __restrict__ dgate, T* __restrict__ dinitial,
-                                                          const T* __restrict__ parts, Extents e) {
-  __shared__ Left<T, W> left;
-  __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];  // rows of a task's lanes in banks of their own
-  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Part part = part_of(e);
-  const Place at = SHARED ? head_place(e, part.group, lane) : flat_place(e, part.group, lane);
-  const int64_t column = at.row * e.time * e.channels + at.channel;
-  const int64_t gate_column = at.row * e.time * e.gates + at.gate;
-  const T *xs = x + column, *hs = h + column, *ds = grad + column, *gs = gate + gate_column;
-  const uint8_t* rs = RESETS ? resets + at.row * e.time : nullptr;
-  const int64_t q = at.row * e.channels + at.channel;
-  const T before = initial ? initial[q] : T(0);
-  const int64_t segments = gridDim.x / e.groups;
-  T carried = T(0);
-  // Segments are kept from the last one on, in the order of this pass.
-  if (parts) carried = through_segments(parts, e.total, q, segments, segments - 1 - part.segment, carried);
+// The arrays of a call. dgate holds e.pieces partial sums where heads share gates.
+template <typename T>
+struct Backward {
+  const T *grad, *x, *gate, *h, *initial;
+  const uint8_t* resets;
+  T *dx, *dgate, *dinitial;
+};
 
-  // Wave 0 takes the last R steps, wave 1 those before them: t is the first
-  // step of a wave's run, before the segment at its start.
-  constexpr int64_t stride = int64_t(W) * R;
-  int64_t t = part.end - int64_t(wave + 1) * R;
-  BackwardLoads<T, R> one, two;
-  const auto steps = [&](BackwardLoads<T, R>& now, BackwardLoads<T, R>& next, int turn, bool more) {
-    if (more) next.template load<RESETS>(xs, gs, hs, ds, rs, before, e, t - stride, part.begin);
-    Run<T> run{T(1), T(0), false};
-    now.template compose<RESETS>(run);
-    T value = through<T, W>(run, left, turn, wave, lane, carried);
+// SHARED: gates that heads share.
+template <typename T, bool SHARED>
+struct BackwardColumns {
+  const T *x, *gate, *h, *grad;
+  const uint8_t* resets;
+  T *dx, *dgate, *dinitial, before;
+  bool valid;
+
+  __device__ __forceinline__ BackwardColumns(const Backward<T>& f, const Extents& e, int64_t group, int lane) {
+    const Place at = SHARED ? head_place(e, group, lane) : flat_place(e, group, lane);
+    const int64_t column = at.row * e.time * e.channels + at.channel;
+    const int64_t gate_column = at.row * e.time * e.gates + at.gate, q = at.row * e.channels + at.channel;
+    x = f.x + column;
+    h = f.h + column;
+    grad = f.grad + column;
+    dx = f.dx + column;
+    gate = f.gate + gate_column;
+    dgate = SHARED ? f.dgate : f.dgate + gate_column;
+    resets = f.resets + at.row * e.time;
+    before = f.initial ? f.initial[q] : T(0);
+    dinitial = f.dinitial ? f.dinitial + q : nullptr;
+    valid = at.valid;
+  }
+
+  template <bool RESETS, int R>
+  __device__ __forceinline__ void load(BackwardLoads<T, R>& to, const Extents& e, int64_t t) const {
+    to.template load<RESETS>(x, gate, h, grad, resets, before, e, t);
+  }
+
+  // The gradients of composed steps from t on; `shares`: LDS of this wave.
+  template <int R, bool RESETS>
+  __device__ __forceinline__ void finish(BackwardLoads<T, R>& now, const Extents& e, int64_t group, int64_t t, int lane,
+                                         T (*shares)[65], T value) const {
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
       const bool cut = RESETS && (now.resets >> i & 1);
@@ -378,10 +539,10 @@ __global__ __launch_bounds__(W * 64) void backward_kernel(const T* __restrict__ 
       now.h[i] = slope * now.h[i] * (now.gate[i] * now.x[i]);
       now.x[i] = slope * now.x[i];
     }
-    T* out = dx + column + t * e.channels;
-    T* out_gate = dgate + gate_column + t * e.gates;
-    if (at.valid) {
-      if (t >= part.begin) {
+    T* out = dx + t * e.channels;
+    T* out_gate = dgate + t * e.gates;
+    if (valid) {
+      if (t >= 0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           out[i * e.channels] = now.x[i];
@@ -390,111 +551,102 @@ __global__ __launch_bounds__(W * 64) void backward_kernel(const T* __restrict__ 
       } else {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          if (t + i >= part.begin) {
+          if (t + i >= 0) {
             out[i * e.channels] = now.x[i];
             if (!SHARED) out_gate[i * e.gates] = now.h[i];
           }
         }
       }
     }
-    if constexpr (SHARED) {
-      // The wave's own rows of LDS: its stores are in order before its loads.
+    if constexpr (SHARED) add_shares<R>(now, e, group, t, lane, shares);
+  }
+
+  // One sum for each step and head of the wave, by neighbouring lanes.
+  template <int R>
+  __device__ __forceinline__ void add_shares(const BackwardLoads<T, R>& now, const Extents& e, int64_t group, int64_t t,
+                                             int lane, T (*shares)[65]) const {
+    // The wave's own rows of LDS: its stores are in order before its loads.
 #pragma unroll
-      for (int i = 0; i < R; ++i) shares[wave][i][lane] = now.h[i];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      const int64_t piece = part.group % e.pieces, head0 = part.group / e.pieces * e.pack;
-      const int64_t rest = e.width - piece * e.piece;
-      const int count = int(rest < e.piece ? rest : e.piece);
-      T* sums = dgate + piece * (e.heads * e.time);
-      // One sum for each step and head of the wave, by neighbouring lanes.
-      const int lanes = SumLanes<R>::of(e.pack), sub = lane % lanes;
-      for (int first = 0; first < R * e.pack; first += 64 / lanes) {
-        const int task = first + lane / lanes, i = task / e.pack, slot = task - i * e.pack;
-        T sum = T(0);
-        if (i < R) {
-          for (int k = sub; k < count; k += lanes) sum += shares[wave][i][slot * e.piece + k];
-        }
-        for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        const int64_t head = head0 + slot;
-        if (sub != 0 || i >= R || head >= e.heads || t + i < part.begin) continue;
-        const int64_t row = head / e.gates;
-        sums[(row * e.time + t + i) * e.gates + (head - row * e.gates)] = sum;
+    for (int i = 0; i < R; ++i) shares[i][lane] = now.h[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int64_t piece = group % e.pieces, head0 = group / e.pieces * e.pack;
+    const int64_t rest = e.width - piece * e.piece;
+    const int count = int(rest < e.piece ? rest : e.piece);
+    T* sums = dgate + piece * (e.heads * e.time);
+    int lanes = 1;  // that share a sum: a power of two
+    while (lanes * 2 * R * e.pack <= 64) lanes *= 2;
+    const int sub = lane % lanes;
+    for (int first = 0; first < R * e.pack; first += 64 / lanes) {
+      const int task = first + lane / lanes, i = task / e.pack, slot = task - i * e.pack;
+      T sum = T(0);
+      if (i < R) {
+        for (int k = sub; k < count; k += lanes) sum += shares[i][slot * e.piece + k];
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      const int64_t head = head0 + slot;
+      if (sub != 0 || i >= R || head >= e.heads || t + i < 0) continue;
+      const int64_t row = head / e.gates;
+      sums[(row * e.time + t + i) * e.gates + (head - row * e.gates)] = sum;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// Wave 0 takes the last R steps, wave 1 those before them: t is the first step
+// of a wave's run, below zero at the start of the row.
+template <typename T, int R, int W, bool RESETS, bool SHARED>
+__global__ __launch_bounds__(W * 64) void backward_kernel(Backward<T> f, Extents e) {
+  __shared__ Left<T, W> left;
+  __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];  // rows of a sum's lanes in banks of their own
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t group = by_die();
+  const BackwardColumns<T, SHARED> c(f, e, group, lane);
+  T carried = T(0);
+  constexpr int64_t stride = int64_t(W) * R;
+  int64_t t = e.time - int64_t(wave + 1) * R;
+  BackwardLoads<T, R> one, two;
+  const auto steps = [&](BackwardLoads<T, R>& now, BackwardLoads<T, R>& next, int turn, bool more) {
+    if (more) c.template load<RESETS>(next, e, t - stride);
+    Run<T> run{T(1), T(0), false};
+    now.template compose<RESETS>(run);
+    const T value = through<T, W>(run, left, turn, wave, lane, carried);
+    c.template finish<R, RESETS>(now, e, group, t, lane, shares[SHARED ? wave : 0], value);
     t -= stride;
   };
-  one.template load<RESETS>(xs, gs, hs, ds, rs, before, e, t, part.begin);
-  for (int64_t base = part.begin; base < part.end; base += 2 * stride) {
-    const bool second = base + stride < part.end;
+  c.template load<RESETS>(one, e, t);
+  for (int64_t base = 0; base < e.time; base += 2 * stride) {
+    const bool second = base + stride < e.time;
     steps(one, two, 0, second);
-    if (second) steps(two, one, 1, base + 2 * stride < part.end);
+    if (second) steps(two, one, 1, base + 2 * stride < e.time);
   }
-  if (dinitial && part.segment == 0 && wave == 0 && at.valid) dinitial[q] = carried;
+  if (c.dinitial && wave == 0 && c.valid) *c.dinitial = carried;
 }
 
-// ---- segments --------------------------------------------------------------------
-
-// The composition of every segment but the last one in the pass's order, per
-// channel. A wave composes one W-th of a segment.
-template <typename T, int R, int W, bool RESETS, bool BACKWARD>
-__global__ __launch_bounds__(W * 64) void segments_kernel(const T* __restrict__ values, const T* __restrict__ gate,
-                                                          const uint8_t* __restrict__ resets, T* __restrict__ parts,
-                                                          Extents e) {
-  __shared__ T left_a[W][64], left_b[W][64];
+template <typename T, int R, int W, bool RESETS, bool SHARED>
+__global__ __launch_bounds__(W * 64) void backward_chained_kernel(Backward<T> f, Extents e, Chain<T> chain) {
+  __shared__ ChainLeft<T, W> left;
+  __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Part part = part_of(e);
-  const int64_t place = part.segment, composed = gridDim.x / e.groups;  // one less than segments
-  if (BACKWARD) {
-    part.begin = (composed - place) * e.segment;
-    part.end = part.begin + e.segment < e.time ? part.begin + e.segment : e.time;
-  }
-  const Place at = flat_place(e, part.group, lane);
-  const T* vs = values + at.row * e.time * e.channels + at.channel;
-  const T* gs = gate + at.row * e.time * e.gates + at.gate;
-  const uint8_t* rs = RESETS ? resets + at.row * e.time : nullptr;
-  const int64_t share = (e.segment + W * R - 1) / (W * R) * R;
+  const Tile tile = take_tile(chain.tickets, e);
+  if (tile.number < 0) return;
+  const BackwardColumns<T, SHARED> c(f, e, tile.group, lane);
+  const int64_t t = e.time - (tile.number * W + wave + 1) * R;
+  BackwardLoads<T, R> now;
+  c.template load<RESETS>(now, e, t);
   Run<T> run{T(1), T(0), false};
-  if (!BACKWARD) {
-    const int64_t begin = part.begin + wave * share, end = begin + share < part.end ? begin + share : part.end;
-    ForwardLoads<T, R> one, two;
-    one.template load<RESETS>(vs, gs, rs, e, begin, end);
-    for (int64_t t = begin; t < end; t += 2 * R) {
-      two.template load<RESETS>(vs, gs, rs, e, t + R, end);
-      one.template compose<RESETS>(run);
-      one.template load<RESETS>(vs, gs, rs, e, t + 2 * R, end);
-      two.template compose<RESETS>(run);
-    }
-  } else {
-    const int64_t end = part.end - wave * share, begin = end - share > part.begin ? end - share : part.begin;
-    BackwardLoads<T, R> one, two;
-    const auto load = [&](BackwardLoads<T, R>& to, int64_t t) {
-      to.template load<RESETS, false>(nullptr, gs, nullptr, vs, rs, T(0), e, t, begin);
-    };
-    load(one, end - R);
-    for (int64_t t = end - R; t + R > begin; t -= 2 * R) {
-      load(two, t - R);
-      one.template compose<RESETS>(run);
-      load(one, t - 2 * R);
-      two.template compose<RESETS>(run);
-    }
+  now.template compose<RESETS>(run);
+  T after;
+  const T value = through_chain<T, W>(run, left, chain, e, tile, wave, lane, T(0), after);
+  c.template finish<R, RESETS>(now, e, tile.group, t, lane, shares[SHARED ? wave : 0], value);
+  if (c.dinitial && tile.number == e.tiles - 1 && wave == 0 && c.valid) *c.dinitial = after;
+}
+
+__global__ __launch_bounds__(256) void ones_kernel(uint4* __restrict__ to, int64_t n) {
+  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+    to[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
   }
-  left_a[wave][lane] = run.cut ? T(-1) : run.a;
-  left_b[wave][lane] = run.b;
-  __syncthreads();
-  if (wave != 0 || !at.valid) return;
-  Run<T> all{T(1), T(0), false};
-  for (int w = 0; w < W; ++w) {
-    const T a = left_a[w][lane];
-    all.b = apply(a, left_b[w][lane], all.b);
-    all.cut = all.cut || a < T(0);
-    all.a *= a;
-  }
-  const int64_t q = at.row * e.channels + at.channel, segments = composed + 1;
-  parts[place * e.total + q] = all.cut ? T(-1) : all.a;
-  parts[(segments + place) * e.total + q] = all.b;
 }
 
 // out[i] = sum over k of parts[k][i], in order.
@@ -529,88 +681,89 @@ unsigned checked_grid(int64_t groups, int threads) {
   return unsigned(groups);
 }
 
-constexpr int kWaves = 16, kSegmentWaves = 8;
-
-// Cuts time where groups are too few to fill the chip; returns the number of
-// segments.
-int64_t plan_segments(const hp_ctx* ctx, Extents& e, int steps) {
-  const int64_t least = int64_t(kWaves) * steps;  // of a segment
-  int64_t segments = 1;
-  if (e.groups * 2 <= ctx->compute_units) segments = std::min(ctx->compute_units / e.groups, e.time / least);
-  e.segment = segments > 1 ? hp::ceil_div(hp::ceil_div(e.time, segments), least) * least : e.time;
-  return hp::ceil_div(e.time, e.segment);
-}
+constexpr int kWaves = 8;
 
 // Calls f with the waves of a workgroup and the steps of a run.
 template <int R, typename F>
 void with_shape(int64_t time, F&& f) {
-  using Int = std::integral_constant<int, R>;
-  if (time == 1) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-  else if (time <= R) f(std::integral_constant<int, 1>{}, Int{});
-  else if (time <= 4 * R) f(std::integral_constant<int, 4>{}, Int{});
-  else f(std::integral_constant<int, kWaves>{}, Int{});
+  const auto shape = [&](auto waves, auto steps) { f(waves, steps); };
+  if (time == 1) shape(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  else if (time <= 4) shape(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+  else if (time <= R) shape(std::integral_constant<int, 1>{}, std::integral_constant<int, R>{});
+  else if (time <= 4 * R) shape(std::integral_constant<int, 4>{}, std::integral_constant<int, R>{});
+  else shape(std::integral_constant<int, kWaves>{}, std::integral_constant<int, R>{});
 }
 
-// The compositions of the segments, in scratch memory; null for one segment.
-template <typename T, int R, bool BACKWARD>
-T* compose_segments(hp_ctx* ctx, const T* values, const T* gate, const uint8_t* resets, Extents e, int64_t segments) {
-  if (segments == 1) return nullptr;
-  e.groups = hp::ceil_div(e.total, 64);
-  T* parts = static_cast<T*>(hp::scratch_alloc(ctx, size_t(2 * segments) * size_t(e.total) * sizeof(T)));
-  constexpr int W = kSegmentWaves;
-  const unsigned grid = checked_grid(e.groups * (segments - 1), 64 * W);
-  const auto kernel = resets ? segments_kernel<T, R, W, true, BACKWARD> : segments_kernel<T, R, W, false, BACKWARD>;
-  kernel<<<grid, 64 * W, 0, ctx->stream>>>(values, gate, resets, parts, e);
-  return parts;
+// Whether tiles are chained: where one workgroup for each group leaves compute
+// units idle and time is long enough to give them some.
+bool plan_chain(const hp_ctx* ctx, Extents& e, int steps) {
+  e.tiles = hp::ceil_div(e.time, int64_t(kWaves) * steps);
+  if (e.groups * 2 > ctx->compute_units || e.tiles < 4) return false;
+  e.span = e.groups >= 16 ? 16 : 64;
+  return true;
 }
 
-// Returns a call's scratch memory, then reports a failed launch.
-void finish(hp_ctx* ctx, const char* name, void* one, void* two) {
-  const hipError_t status = hipGetLastError();
-  if (one) hp::scratch_free(ctx, one);
-  if (two) hp::scratch_free(ctx, two);
-  hp::check_hip(status, name);
+// Memory of a chained launch, all ones.
+template <typename T>
+Chain<T> make_chain(hp_ctx* ctx, hp::Scratch& scratch, const Extents& e) {
+  const int64_t tickets = int64_t(kDies) * kTicketWords * 4, runs = e.tiles * e.groups * 128 * int64_t(sizeof(T));
+  const int64_t states = hp::ceil_div(e.tiles, e.span) * e.groups * 64 * int64_t(sizeof(T));
+  char* memory = scratch.take<char>(tickets + runs + states);
+  const int64_t n = (tickets + runs + states) / 16;
+  ones_kernel<<<unsigned(std::min<int64_t>(hp::ceil_div(n, 256), 2048)), 256, 0, ctx->stream>>>(reinterpret_cast<uint4*>(memory), n);
+  hp::check_launch("recurrence memory");
+  using Bits = typename Word<T>::type;
+  return {reinterpret_cast<unsigned*>(memory), reinterpret_cast<Bits*>(memory + tickets), reinterpret_cast<Bits*>(memory + tickets + runs)};
 }
 
 template <typename T>
-void forward(hp_ctx* ctx, const T* x, const T* gate, const T* initial, const uint8_t* resets, T* h, Extents e) {
+void forward(hp_ctx* ctx, const Forward<T>& f, Extents e) {
   constexpr int R = Steps<T>::forward;
+  hp::Scratch scratch(ctx);
   e.groups = hp::ceil_div(e.total, 64);
-  const int64_t segments = plan_segments(ctx, e, R);
-  T* parts = nullptr;
-  with_shape<R>(e.time, [&](auto waves, auto steps) {
-    constexpr int W = waves, S = steps;
-    const unsigned grid = checked_grid(e.groups * segments, 64 * W);
-    parts = compose_segments<T, R, false>(ctx, x, gate, resets, e, segments);
-    const auto kernel = resets ? forward_kernel<T, S, W, true> : forward_kernel<T, S, W, false>;
-    kernel<<<grid, 64 * W, 0, ctx->stream>>>(x, gate, initial, resets, h, parts, e);
-  });
-  finish(ctx, "launch of the recurrence", parts, nullptr);
+  if (plan_chain(ctx, e, R)) {
+    const unsigned grid = checked_grid(e.groups * e.tiles, 64 * kWaves);
+    const Chain<T> chain = make_chain<T>(ctx, scratch, e);
+    const auto kernel = f.resets ? forward_chained_kernel<T, R, kWaves, true> : forward_chained_kernel<T, R, kWaves, false>;
+    kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
+  } else {
+    with_shape<R>(e.time, [&](auto waves, auto steps) {
+      constexpr int W = waves, S = steps;
+      const unsigned grid = checked_grid(e.groups, 64 * W);
+      const auto kernel = f.resets ? forward_kernel<T, S, W, true> : forward_kernel<T, S, W, false>;
+      kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
+    });
+  }
+  hp::check_launch("recurrence");
 }
 
-template <typename T>
-void backward(hp_ctx* ctx, const T* grad, const T* x, const T* gate, const T* h, const T* initial,
-              const uint8_t* resets, T* dx, T* dgate, T* dinitial, Extents e) {
+template <typename T, bool SHARED>
+void backward(hp_ctx* ctx, Backward<T> f, Extents e) {
   constexpr int R = Steps<T>::backward;
-  const bool shared = e.width > 1;
-  e.groups = shared ? hp::ceil_div(e.heads, e.pack) * e.pieces : hp::ceil_div(e.total, 64);
-  const int64_t segments = plan_segments(ctx, e, R);
+  hp::Scratch scratch(ctx);
+  e.groups = SHARED ? hp::ceil_div(e.heads, e.pack) * e.pieces : hp::ceil_div(e.total, 64);
+  T* const dgate = f.dgate;
   const int64_t count = e.heads * e.time;
-  T *parts = nullptr, *sums = dgate;
-  with_shape<R>(e.time, [&](auto waves, auto steps) {
-    constexpr int W = waves, S = steps;
-    const unsigned grid = checked_grid(e.groups * segments, 64 * W);
-    if (e.pieces > 1) sums = static_cast<T*>(hp::scratch_alloc(ctx, size_t(e.pieces) * size_t(count) * sizeof(T)));
-    parts = compose_segments<T, R, true>(ctx, grad, gate, resets, e, segments);
-    const auto kernel = shared ? (resets ? backward_kernel<T, S, W, true, true> : backward_kernel<T, S, W, false, true>)
-                               : (resets ? backward_kernel<T, S, W, true, false> : backward_kernel<T, S, W, false, false>);
-    kernel<<<grid, 64 * W, 0, ctx->stream>>>(grad, x, gate, h, initial, resets, dx, sums, dinitial, parts, e);
-  });
+  if (e.pieces > 1) f.dgate = scratch.take<T>(e.pieces * count);
+  if (plan_chain(ctx, e, R)) {
+    const unsigned grid = checked_grid(e.groups * e.tiles, 64 * kWaves);
+    const Chain<T> chain = make_chain<T>(ctx, scratch, e);
+    const auto kernel = f.resets ? backward_chained_kernel<T, R, kWaves, true, SHARED> : backward_chained_kernel<T, R, kWaves, false, SHARED>;
+    kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
+  } else {
+    with_shape<R>(e.time, [&](auto waves, auto steps) {
+      constexpr int W = waves, S = steps;
+      const unsigned grid = checked_grid(e.groups, 64 * W);
+      const auto kernel = f.resets ? backward_kernel<T, S, W, true, SHARED> : backward_kernel<T, S, W, false, SHARED>;
+      kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
+    });
+  }
+  hp::check_launch("recurrence gradient");
   if (e.pieces > 1) {
     const int64_t blocks = std::min<int64_t>(hp::ceil_div(count, 256), 4096);
-    add_parts_kernel<T><<<unsigned(blocks), 256, 0, ctx->stream>>>(sums, dgate, count, e.pieces);
+    add_parts_kernel<T><<<unsigned(blocks), 256, 0, ctx->stream>>>(f.dgate, dgate, count, e.pieces);
+    hp::check_launch("recurrence gate sums");
   }
-  finish(ctx, "launch of the recurrence's gradient", parts, e.pieces > 1 ? sums : nullptr);
 }
 
 }  // namespace
@@ -626,13 +779,12 @@ int hp_gated_recurrence(hp_ctx* ctx, int dtype, const void* x, const void* gate,
     if (e.total == 0 || time == 0) return;
     hp::require(x && gate && h, "null pointer");
     const auto r = static_cast<const uint8_t*>(resets);
-    if (dtype == HP_F32) {
-      forward(ctx, static_cast<const float*>(x), static_cast<const float*>(gate), static_cast<const float*>(initial), r,
-              static_cast<float*>(h), e);
-    } else {
-      forward(ctx, static_cast<const double*>(x), static_cast<const double*>(gate), static_cast<const double*>(initial),
-              r, static_cast<double*>(h), e);
-    }
+    const auto run = [&](auto zero) {
+      using T = decltype(zero);
+      forward<T>(ctx, {static_cast<const T*>(x), static_cast<const T*>(gate), static_cast<const T*>(initial), r, static_cast<T*>(h)}, e);
+    };
+    if (dtype == HP_F32) run(float(0));
+    else run(double(0));
   });
 }
 
@@ -648,9 +800,11 @@ int hp_gated_recurrence_grad(hp_ctx* ctx, int dtype, const void* grad, const voi
     const auto r = static_cast<const uint8_t*>(resets);
     const auto run = [&](auto zero) {
       using T = decltype(zero);
-      backward<T>(ctx, static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const T*>(gate),
-                  static_cast<const T*>(h), static_cast<const T*>(initial), r, static_cast<T*>(dx),
-                  static_cast<T*>(dgate), static_cast<T*>(dinitial), e);
+      const Backward<T> f{static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const T*>(gate),
+                          static_cast<const T*>(h), static_cast<const T*>(initial), r, static_cast<T*>(dx),
+                          static_cast<T*>(dgate), static_cast<T*>(dinitial)};
+      if (e.width > 1) backward<T, true>(ctx, f, e);
+      else backward<T, false>(ctx, f, e);
     };
     if (dtype == HP_F32) run(float(0));
     else run(double(0));

@@ -451,30 +451,6 @@ __global__ __launch_bounds__(256) void pair_kernel(Call<T> c, const T* __restric
 
 // ---- host ----------------------------------------------------------------------
 
-// Temporaries of one call, returned to the pool when it ends.
-class Scratch {
- public:
-  explicit Scratch(hp_ctx* ctx) : ctx_(ctx) {}
-  ~Scratch() {
-    for (void* p : held_) {
-      try {
-        hp::scratch_free(ctx_, p);
-      } catch (...) {  // a failing free would leave a destructor: the block stays allocated
-      }
-    }
-  }
-  template <typename T>
-  T* take(int64_t count) {
-    held_.reserve(held_.size() + 1);
-    held_.push_back(hp::scratch_alloc(ctx_, size_t(count) * sizeof(T)));
-    return static_cast<T*>(held_.back());
-  }
-
- private:
-  hp_ctx* ctx_;
-  std::vector<void*> held_;
-};
-
 // Calls f with the team (L, K) that holds rows of `vocab` logits, or returns
 // false: none does.
 template <typename T, typename F>
@@ -534,7 +510,7 @@ void final_loss(hp_ctx* ctx, const Call<T>& c, int64_t sums) {
 // count the mask and add the sums themselves, which saves two launches: each
 // ends with a fence of the caches between the dies, and reads the whole mask.
 template <typename T>
-void plan_losses(hp_ctx* ctx, Scratch& scratch, Call<T>& c, unsigned blocks) {
+void plan_losses(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, unsigned blocks) {
   c.sums = scratch.take<double>(blocks);
   if (blocks <= kTicketBlocks) c.ticket = ctx->ticket;
   if (!c.count_here || (c.ticket && int64_t(blocks) * c.rows <= kCountedBytes)) return;
@@ -549,7 +525,7 @@ void plan_losses(hp_ctx* ctx, Scratch& scratch, Call<T>& c, unsigned blocks) {
 // every row, their sums in c.sums; returns how many sums. `done`: whether the
 // gradient is written, too.
 template <typename T>
-int64_t rows_pass(hp_ctx* ctx, Scratch& scratch, Call<T>& c, bool& done) {
+int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, bool& done) {
   done = false;
   unsigned blocks = 0;
   if (teams_serve<T>(c.rows, c.vocab) && with_team<T>(c.vocab, [&](auto l, auto k) {
@@ -634,7 +610,7 @@ int hp_token_log_probs(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
     hp::require(logits && targets && log_probs, "null pointer");
     by_type(dtype, [&](auto zero) {
       using T = decltype(zero);
-      Scratch scratch(ctx);
+      hp::Scratch scratch(ctx);
       Call<T> c = call_of<T>(index_dtype, logits, targets, mask, rows, vocab);
       c.log_probs = static_cast<T*>(log_probs);
       bool done;
@@ -656,7 +632,7 @@ int hp_policy_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, 
     hp::require(loss && (rows == 0 || (logits && actions && old && advantages && log_probs)), "null pointer");
     by_type(dtype, [&](auto zero) {
       using T = decltype(zero);
-      Scratch scratch(ctx);
+      hp::Scratch scratch(ctx);
       Call<T> c = call_of<T>(index_dtype, logits, actions, mask, rows, vocab);
       c.old = static_cast<const T*>(old);
       c.advantages = static_cast<const T*>(advantages);
@@ -695,7 +671,7 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
     hp::require(pairs <= hp::kMaxGrid, "too many pairs for one launch");
     by_type(dtype, [&](auto zero) {
       using T = decltype(zero);
-      Scratch scratch(ctx);
+      hp::Scratch scratch(ctx);
       Call<T> c = call_of<T>(index_dtype, logits, targets, mask, rows, vocab);
       c.grad = static_cast<T*>(grad);
       c.tokens = time;
