@@ -89,7 +89,10 @@ struct hp_ctx {
   size_t pool_limit = 0;
   int fail_next = 0;
   bool staged_products = false;  // hp_debug_staged_products
-  unsigned* ticket = nullptr;  // zero in device memory between launches: workgroups that have ended
+  // Device memory for sums that the last workgroup of a launch adds: the number of
+  // workgroups that have ended, 0 between launches, and 256 bytes further
+  // kTicketPlaces 8-byte places, all ones between launches.
+  unsigned* ticket = nullptr;
 };
 
 namespace hp {
@@ -141,6 +144,8 @@ inline void check_launch(const char* name) {
     fail(HP_E_HIP, std::string("launch of ") + name + " failed: " + hipGetErrorString(status));
   }
 }
+
+constexpr unsigned kTicketPlaces = 1024;  // at hp_ctx::ticket
 
 // Most workgroups of a 1-D launch of 256 threads each: a launch takes fewer
 // than 2^32 threads, and drops the workgroups past them without an error.

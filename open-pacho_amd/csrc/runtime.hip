@@ -176,9 +176,10 @@ int hp_init(int device, hp_ctx** out) {
     HP_CHECK(hipStreamCreateWithFlags(&ctx->side, hipStreamNonBlocking));
     HP_CHECK(hipEventCreateWithFlags(&ctx->fork, hipEventDisableTiming));
     HP_CHECK(hipEventCreateWithFlags(&ctx->join, hipEventDisableTiming));
-    HP_CHECK(hipMalloc(reinterpret_cast<void**>(&ctx->ticket), 256));
-    const unsigned zero = 0;
-    HP_CHECK(hipMemcpy(ctx->ticket, &zero, sizeof(zero), hipMemcpyHostToDevice));
+    std::vector<uint64_t> places(32 + hp::kTicketPlaces, ~uint64_t(0));
+    std::fill_n(places.begin(), 32, uint64_t(0));
+    HP_CHECK(hipMalloc(reinterpret_cast<void**>(&ctx->ticket), places.size() * 8));
+    HP_CHECK(hipMemcpy(ctx->ticket, places.data(), places.size() * 8, hipMemcpyHostToDevice));
     *out = ctx;
   });
   if (status != HP_OK && ctx != nullptr) {

@@ -12,9 +12,9 @@
 //     logits there), then the loss of its token and the gradient;
 //   - rows that no team holds, or so few of them that teams would leave the chip
 //     idle, are cut into pieces (stats_kernel), whose (m, S) meet per row
-//     (finish_kernel), and are read again for the gradient (grad_kernel). The
-//     preference loss needs this second reading in any case: w depends on every
-//     token of both responses.
+//     (finish_kernel, policy_grad_kernel), and are read again for the gradient.
+//     The preference loss needs this second reading (grad_kernel) in any case: w
+//     depends on every token of both responses.
 // Sums over a row are float (double of doubles) in a tree; the loss sums are
 // double. Every order is fixed, so results repeat bit for bit.
 //
@@ -29,7 +29,7 @@
 namespace {
 
 constexpr int kPieceThreads = 256, kPieceLoads = 8;
-constexpr unsigned kTicketBlocks = 1024;
+constexpr int64_t kFewPieces = 1024;
 constexpr int64_t kCountedBytes = int64_t(1) << 25;
 
 // Elements of a piece, of which the last one of a row may have fewer.
@@ -263,23 +263,35 @@ __device__ __forceinline__ double scale_of(const Call<T>& c) {
   return 1.0 / (sum > 1.0 ? sum : 1.0);
 }
 
-// Leaves the workgroup's sum of losses. With a ticket, the last workgroup adds
-// all of them in their order, whichever it is, and sets the ticket back.
+// Leaves `sum`, which thread 0 has, as number `index` of `count`. With a ticket the
+// last one to come adds all of them in their order, whichever workgroup it is. No
+// fences: a sum is valid by itself, the places being all ones (which no sum is)
+// between launches, and each is on its way before its ticket is taken.
 template <typename T>
-__device__ __forceinline__ void leave_loss(const Call<T>& c, double sum, double scale) {
+__device__ __forceinline__ void leave_loss(const Call<T>& c, double sum, double scale, unsigned index, unsigned count) {
   __shared__ bool last;
-  sum = workgroup_sum(sum);
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(&c.sums[blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (c.ticket) last = __hip_atomic_fetch_add(c.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  if (!c.ticket) {
+    if (threadIdx.x == 0) c.sums[index] = sum;
+    return;
   }
-  if (!c.ticket) return;
+  uint64_t* const places = reinterpret_cast<uint64_t*>(c.ticket + 64);
+  if (threadIdx.x == 0) {
+    uint64_t bits = __builtin_bit_cast(uint64_t, sum);
+    if (bits == ~uint64_t(0)) --bits;  // a NaN as well
+    __hip_atomic_store(&places[index], bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = __hip_atomic_fetch_add(c.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == count - 1;
+  }
   __syncthreads();
-  if (!last) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  const bool adds = last;
+  __syncthreads();
+  if (!adds) return;
   double total = 0;
-  for (unsigned i = threadIdx.x; i < gridDim.x; i += blockDim.x) {
-    total += __hip_atomic_load(&c.sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (unsigned i = threadIdx.x; i < count; i += blockDim.x) {
+    uint64_t bits;
+    do bits = __hip_atomic_load(&places[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    while (bits == ~uint64_t(0));
+    total += __builtin_bit_cast(double, bits);
+    __hip_atomic_store(&places[i], ~uint64_t(0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   total = workgroup_sum(total);
   if (threadIdx.x == 0) {
@@ -327,7 +339,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? 4 : 
     share.each(length, lane, [&](T& v, int i) { v = v * scale + (i == at ? w : T(0)); });
     share.store(out, length, lane);
   }
-  if (c.old) leave_loss(c, sum, factor);
+  if (c.old) leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
 }
 
 // (m, S) of one piece of a row: parts[row * pieces + piece].
@@ -349,38 +361,38 @@ __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __re
   }
 }
 
-// A wave per row: its pieces' statistics meet, and with them its token's loss.
+// (m, S) of a row from its pieces', by every wave for itself.
 template <typename T>
-__global__ __launch_bounds__(256) void finish_kernel(Call<T> c, const T* __restrict__ part_tops,
-                                                     const T* __restrict__ part_totals, int pieces) {
+__device__ __forceinline__ void join_pieces(const T* tops, const T* totals, int pieces, T& top, T& total) {
   const int lane = threadIdx.x & 63;
+  const T none = -T(__builtin_huge_val());
+  top = none;
+  for (int k = lane; k < pieces; k += 64) top = larger(top, tops[k]);
+  top = team_reduce<64>(top, static_cast<T*>(nullptr), [](T a, T b) { return larger(a, b); });
+  total = T(0);
+  for (int k = lane; k < pieces; k += 64) total += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - top);
+  total = team_reduce<64>(total, static_cast<T*>(nullptr), [](T a, T b) { return a + b; });
+}
+
+// A workgroup per row: its pieces' statistics meet, and with them its token's
+// loss. As wide as policy_grad_kernel, so that both add the losses in one order.
+template <typename T>
+__global__ __launch_bounds__(kPieceThreads) void finish_kernel(Call<T> c, const T* __restrict__ part_tops,
+                                                               const T* __restrict__ part_totals, int pieces) {
   const double factor = c.old ? scale_of(c) : 1.0;
-  double sum = 0;
-  for (int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); row < c.rows; row += int64_t(gridDim.x) * 4) {
-    if (!c.kept(row)) {
-      if (lane == 0) c.leave_out(row);
-      continue;
-    }
-    const T* tops = part_tops + row * pieces;
-    const T* totals = part_totals + row * pieces;
-    const T none = -T(__builtin_huge_val());
-    T top = none;
-    for (int k = lane; k < pieces; k += 64) top = larger(top, tops[k]);
-    top = team_reduce<64>(top, static_cast<T*>(nullptr), [](T a, T b) { return larger(a, b); });
-    T total = T(0);
-    for (int k = lane; k < pieces; k += 64) total += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - top);
-    total = team_reduce<64>(total, static_cast<T*>(nullptr), [](T a, T b) { return a + b; });
+  const int64_t row = blockIdx.x;
+  double loss = 0;
+  if (c.kept(row)) {
+    T top, total;
+    join_pieces(part_tops + row * pieces, part_totals + row * pieces, pieces, top, total);
     const double log_prob = c.log_prob(row, c.target(row), top, total);
-    if (lane == 0) c.keep(row, log_prob, top, total);
-    if (!c.old) continue;
-    double loss, slope;
-    policy_token(c, row, log_prob, loss, slope);
-    if (lane == 0) {
-      sum += loss;
-      if (c.weights) c.weights[row] = T(slope * factor);
-    }
+    if (threadIdx.x == 0) c.keep(row, log_prob, top, total);
+    double slope;
+    if (c.old) policy_token(c, row, log_prob, loss, slope);
+  } else if (threadIdx.x == 0) {
+    c.leave_out(row);
   }
-  if (c.old) leave_loss(c, sum, factor);
+  if (c.old) leave_loss(c, loss, factor, blockIdx.x, gridDim.x);
 }
 
 // The gradient of one piece of a row from the row's statistics and weight.
@@ -406,6 +418,42 @@ __global__ __launch_bounds__(256) void grad_kernel(Call<T> c, int pieces, int pi
   }
 }
 
+// The same for the policy loss, from the statistics of the row's pieces: every
+// workgroup joins them and forms the token's terms for itself, and that of the
+// first piece leaves the token's log-probability and loss.
+template <typename T>
+__global__ __launch_bounds__(kPieceThreads) void policy_grad_kernel(Call<T> c, const T* __restrict__ part_tops,
+                                                                    const T* __restrict__ part_totals, int pieces, int piece) {
+  const double factor = scale_of(c);
+  for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
+    const int64_t row = part / pieces;
+    const bool first = part == row * pieces;
+    const int64_t start = (part - row * pieces) * piece;
+    const int length = piece_end(c.vocab - start, piece), lane = threadIdx.x;
+    T* out = c.grad + row * c.vocab + start;
+    double loss = 0;
+    Share<T, kPieceThreads, kPieceLoads> share;
+    if (c.kept(row)) {
+      share.load(c.logits + row * c.vocab + start, length, lane);
+      T top, total;
+      join_pieces(part_tops + row * pieces, part_totals + row * pieces, pieces, top, total);
+      const int64_t y = c.target(row);
+      const double log_prob = c.log_prob(row, y, top, total);
+      if (first && lane == 0) c.keep(row, log_prob, top, total);
+      double slope;
+      policy_token(c, row, log_prob, loss, slope);
+      const int at = y >= start && y < start + length ? int(y - start) : -1;
+      const T w = T(slope * factor), scale = -w * (T(1) / total);
+      share.each(length, lane, [&](T& v, int i) { v = hpd::exp_down(v - top) * scale + (i == at ? w : T(0)); });
+    } else {
+      if (first && lane == 0) c.leave_out(row);
+      share.each(length, lane, [](T& v, int) { v = T(0); });
+    }
+    share.store(out, length, lane);
+    if (first) leave_loss(c, loss, factor, unsigned(row), unsigned(c.rows));
+  }
+}
+
 // 1 / max(1, rows that the mask keeps), by one workgroup.
 template <typename T>
 __global__ __launch_bounds__(1024) void count_kernel(Call<T> c, double* __restrict__ scale) {
@@ -418,8 +466,9 @@ template <typename T>
 __global__ __launch_bounds__(1024) void loss_kernel(Call<T> c, int64_t n) {
   double sum = 0;
   for (int64_t i = threadIdx.x; i < n; i += 1024) sum += c.sums[i];
+  const double factor = scale_of(c);
   sum = workgroup_sum(sum);
-  if (threadIdx.x == 0) *c.loss = T(sum * (c.scale ? *c.scale : c.scale_value));
+  if (threadIdx.x == 0) *c.loss = T(sum * factor);
 }
 
 // A workgroup per pair: the responses' log-probabilities, the pair's loss and
@@ -446,7 +495,7 @@ __global__ __launch_bounds__(256) void pair_kernel(Call<T> c, const T* __restric
     c.weights[blockIdx.x] = T(slope);
     c.weights[pairs + blockIdx.x] = T(-slope);
   }
-  leave_loss(c, threadIdx.x == 0 ? loss : 0.0, c.scale_value);
+  leave_loss(c, loss, c.scale_value, blockIdx.x, gridDim.x);
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -477,14 +526,16 @@ bool with_team(int64_t vocab, F&& f) {
   return false;
 }
 
-// Equal pieces of whole vectors, as few as hold the row.
+// Equal pieces of whole vectors: as few as hold the row, or as many as rows need
+// to make kFewPieces workgroups, with a vector for every thread.
 template <typename T>
 struct Pieces {
   int count, length;
-  explicit Pieces(int64_t vocab) {
+  Pieces(int64_t rows, int64_t vocab) {
     const int64_t vectors = hp::ceil_div(vocab, Vec<T>::width);
     const int64_t least = hp::ceil_div(vectors, kPieceThreads * kPieceLoads);
-    length = int(hp::ceil_div(vectors, least)) * Vec<T>::width;
+    const int64_t wanted = std::min(hp::ceil_div(kFewPieces, rows), hp::ceil_div(vectors, kPieceThreads));
+    length = int(hp::ceil_div(vectors, std::max(least, wanted))) * Vec<T>::width;
     count = int(hp::ceil_div(vocab, length));
   }
 };
@@ -506,14 +557,14 @@ void final_loss(hp_ctx* ctx, const Call<T>& c, int64_t sums) {
   hp::check_launch("loss sum");
 }
 
-// Prepares a launch of `blocks` workgroups that leave sums of losses. Few of them
-// count the mask and add the sums themselves, which saves two launches: each
-// ends with a fence of the caches between the dies, and reads the whole mask.
+// Prepares a launch of `blocks` workgroups that leave `sums` sums of losses. Few
+// sums are added by the last workgroup, and few workgroups count the mask
+// themselves, which saves a launch each.
 template <typename T>
-void plan_losses(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, unsigned blocks) {
-  c.sums = scratch.take<double>(blocks);
-  if (blocks <= kTicketBlocks) c.ticket = ctx->ticket;
-  if (!c.count_here || (c.ticket && int64_t(blocks) * c.rows <= kCountedBytes)) return;
+void plan_losses(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, unsigned sums, unsigned blocks) {
+  if (sums <= hp::kTicketPlaces) c.ticket = ctx->ticket;
+  else c.sums = scratch.take<double>(sums);
+  if (!c.count_here || int64_t(blocks) * c.rows <= kCountedBytes) return;
   double* scale = scratch.take<double>(1);
   count_kernel<T><<<1, 1024, 0, ctx->stream>>>(c, scale);
   hp::check_launch("token count");
@@ -522,35 +573,31 @@ void plan_losses(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, unsigned blocks)
 }
 
 // The statistics, log-probabilities and, for the policy loss, the losses of
-// every row, their sums in c.sums; returns how many sums. `done`: whether the
-// gradient is written, too.
+// every row and the gradient; returns how many sums of losses there are.
 template <typename T>
-int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, bool& done) {
-  done = false;
+int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   unsigned blocks = 0;
   if (teams_serve<T>(c.rows, c.vocab) && with_team<T>(c.vocab, [&](auto l, auto k) {
         constexpr int L = l, K = k, kTeams = L > 256 ? 1 : 256 / L;
         blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, kTeams), 16384));
-        if (c.old) plan_losses(ctx, scratch, c, blocks);
+        if (c.old) plan_losses(ctx, scratch, c, blocks, blocks);
         row_kernel<T, L, K><<<blocks, L > 256 ? L : 256, 0, ctx->stream>>>(c);
         hp::check_launch("token rows");
       })) {
-    done = c.old && c.grad;
     return blocks;
   }
-  const Pieces<T> pieces(c.vocab);
+  const Pieces<T> pieces(c.rows, c.vocab);
   T* tops = scratch.take<T>(c.rows * pieces.count);
   T* totals = scratch.take<T>(c.rows * pieces.count);
-  if (c.grad && c.old) {
-    c.tops = scratch.take<T>(c.rows);
-    c.inverses = scratch.take<T>(c.rows);
-    c.weights = scratch.take<T>(c.rows);
-  }
-  blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, 4), 4096));
-  if (c.old) plan_losses(ctx, scratch, c, blocks);
-  stats_kernel<T><<<loop_grid(c.rows * pieces.count), kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
+  const unsigned grid = loop_grid(c.rows * pieces.count);
+  const bool done = c.old && c.grad;  // the gradient follows from the pieces at once
+  hp::require(c.rows <= hp::kMaxGrid, "too many long rows for one launch");
+  blocks = unsigned(c.rows);
+  if (c.old) plan_losses(ctx, scratch, c, blocks, done ? grid : blocks);
+  stats_kernel<T><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
   hp::check_launch("token statistics");
-  finish_kernel<T><<<blocks, 256, 0, ctx->stream>>>(c, tops, totals, pieces.count);
+  if (done) policy_grad_kernel<T><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
+  else finish_kernel<T><<<blocks, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count);
   hp::check_launch("token losses");
   return blocks;
 }
@@ -567,7 +614,7 @@ void grad_pass(hp_ctx* ctx, const Call<T>& c) {
     if constexpr (l * k <= kPieceThreads * kPieceLoads) launch(l, k, 1, int(c.vocab));
   });
   if (held) return;
-  const Pieces<T> pieces(c.vocab);
+  const Pieces<T> pieces(c.rows, c.vocab);
   launch(std::integral_constant<int, kPieceThreads>{}, std::integral_constant<int, kPieceLoads>{}, pieces.count, pieces.length);
 }
 
@@ -613,8 +660,7 @@ int hp_token_log_probs(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
       hp::Scratch scratch(ctx);
       Call<T> c = call_of<T>(index_dtype, logits, targets, mask, rows, vocab);
       c.log_probs = static_cast<T*>(log_probs);
-      bool done;
-      rows_pass(ctx, scratch, c, done);
+      rows_pass(ctx, scratch, c);
     });
   });
 }
@@ -650,9 +696,7 @@ int hp_policy_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, 
       else c.count_here = rows > 0;
       int64_t sums = 0;
       if (rows) {
-        bool done;
-        sums = rows_pass(ctx, scratch, c, done);
-        if (grad && !done) grad_pass(ctx, c);
+        sums = rows_pass(ctx, scratch, c);
       }
       final_loss(ctx, c, sums);
     });
@@ -684,10 +728,9 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
           c.tops = scratch.take<T>(rows);
           c.inverses = scratch.take<T>(rows);
         }
-        bool done;
-        if (rows) rows_pass(ctx, scratch, c, done);
+        if (rows) rows_pass(ctx, scratch, c);
         if (grad) c.weights = scratch.take<T>(2 * pairs);
-        plan_losses(ctx, scratch, c, unsigned(pairs));
+        plan_losses(ctx, scratch, c, unsigned(pairs), unsigned(pairs));
         pair_kernel<T><<<unsigned(pairs), 256, 0, ctx->stream>>>(c, static_cast<const T*>(reference), pairs, beta,
                                                                  smoothing, static_cast<T*>(sums));
         hp::check_launch("preference pairs");

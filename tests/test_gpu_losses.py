@@ -76,6 +76,25 @@ def test_forbidden_logits_at_the_ends_of_rows(hip, vocab):
     assert p.asnumpy(found[1])[2] == 0 and not grad[2].any()
 
 
+@pytest.mark.parametrize("rows,vocab", [(1030, 4097), (1500, 6000), (4200, 65), (1100, 66000), (40000, 9)])
+def test_more_sums_than_one_launch_adds(hip, rows, vocab):
+    # Losses of rows and workgroups beyond what the last workgroup adds, with and without a mask.
+    rng = np.random.default_rng(rows)
+    z = p.random.default_rng(3, backend=hip).normal(0, 1, (rows, vocab), dtype=np.float32)
+    actions, advantages = rng.integers(0, vocab, rows), rng.standard_normal(rows).astype(np.float32)
+    mask = rng.random(rows) < 0.6
+    logs = p.asnumpy(p.nn.token_log_probs(z, actions)).astype(np.float64)
+    old = (logs + 0.1 * rng.standard_normal(rows)).astype(np.float32)
+    ratio = np.exp(logs - old)
+    each = -np.minimum(ratio * advantages, np.clip(ratio, 0.8, 1.2) * advantages)
+    for kept in (None, mask):
+        want = each[mask].mean() if kept is not None else each.mean()
+        found = p.nn.policy_loss_grad(z, actions, old, advantages, mask=kept)
+        # A mean of terms of size up to 3, each off by some 1e-6 of the log-probability's rounding.
+        assert abs(found[0].item() - want) < 5e-6
+        assert abs(p.nn.policy_loss(z, actions, old, advantages, mask=kept)[0].item() - want) < 5e-6
+
+
 def test_repeated_calls_give_the_same_bits(hip):
     for rows, vocab in ((700, 18), (300, 5000), (3, 100003)):
         given = put(hip, *policy_inputs(rows, vocab, np.float32))
