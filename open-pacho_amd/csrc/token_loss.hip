@@ -144,41 +144,63 @@ __device__ __forceinline__ void policy_token(const Call<T>& c, int64_t row, doub
   }
 }
 
-// Reductions over a team of L neighbouring threads, every thread getting the
-// result. Teams of several waves are a whole workgroup and meet in `meet`.
+// A reduction over L <= 64 neighbouring lanes, all of them getting the result.
 template <int L, typename T, typename Op>
-__device__ __forceinline__ T team_reduce(T v, T* meet, Op op) {
+__device__ __forceinline__ T team_reduce(T v, Op op) {
 #pragma unroll
-  for (int o = (L < 64 ? L : 64) / 2; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
-  if constexpr (L > 64) {
-    if ((threadIdx.x & 63) == 0) meet[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = meet[0];
-#pragma unroll
-    for (int w = 1; w < L / 64; ++w) v = op(v, meet[w]);
-  }
+  for (int o = L / 2; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
   return v;
 }
 
-// A team's share of a row of `length` elements: the whole vectors k * L + lane,
-// and of the elements after the last whole vector one for each of the first
-// lanes. Places past the row's end hold -inf.
+// (m, S) of a row from its pieces', by every wave for itself.
+template <typename T>
+__device__ __forceinline__ void join_pieces(const T* tops, const T* totals, int pieces, T& top, T& total) {
+  const int lane = threadIdx.x & 63;
+  const T none = -T(__builtin_huge_val());
+  top = none;
+  for (int k = lane; k < pieces; k += 64) top = larger(top, tops[k]);
+  top = team_reduce<64>(top, [](T a, T b) { return larger(a, b); });
+  total = T(0);
+  for (int k = lane; k < pieces; k += 64) total += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - top);
+  total = team_reduce<64>(total, [](T a, T b) { return a + b; });
+}
+
+// A team's share of a row of `length` elements, which it takes in pieces of
+// kPieceThreads x kPieceLoads vectors: kSide pieces side by side by 256 threads each,
+// kDeep one after the other, a lane's vectors of a piece 256 apart. Of the elements
+// after the last whole vector, the first lanes of the last piece have one each.
+// Places past the row's end hold -inf. Each piece's sum is formed as stats_kernel
+// forms it and they meet as there, so that a row's statistics have the same bits
+// whichever kernel makes them.
 template <typename T, int L, int K>
 struct Share {
   static constexpr int W = Vec<T>::width;
+  static constexpr int kSide = L > kPieceThreads ? L / kPieceThreads : 1, kDeep = K > kPieceLoads ? K / kPieceLoads : 1;
+  static constexpr int kStep = L > kPieceThreads ? kPieceThreads : L, kLoads = K / kDeep;  // of a piece
   using V = typename Vec<T>::type;
   T z[K][W], rest;
 
-  __device__ __forceinline__ static int index(int k, int lane) { return (k * L + lane) * W; }
-  __device__ __forceinline__ static int rest_index(int length, int lane) { return length / W * W + lane; }
+  __device__ __forceinline__ static int index(int k, int lane) {
+    const int piece = k / kLoads * kSide + lane / kStep;
+    return (piece * kStep * kLoads + k % kLoads * kStep + lane % kStep) * W;
+  }
+  __device__ __forceinline__ static int rest_piece(int length) { return (length - 1) / (kStep * kLoads * W); }
+  __device__ __forceinline__ static int rest_index(int length, int lane) {
+    if (kSide > 1 && lane / kStep != rest_piece(length) % kSide) return length;
+    return length / W * W + lane % kStep;
+  }
 
+  // STREAM: past the caches, for a last reading.
+  template <bool STREAM>
   __device__ __forceinline__ void load(const T* row, int length, int lane) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int j = 0; j < W; ++j) z[k][j] = -T(__builtin_huge_val());
       if (index(k, lane) + W <= length) {
-        const V v = *reinterpret_cast<const V*>(row + index(k, lane));
+        V v;
+        if constexpr (STREAM) v = __builtin_nontemporal_load(reinterpret_cast<const V*>(row + index(k, lane)));
+        else v = *reinterpret_cast<const V*>(row + index(k, lane));
 #pragma unroll
         for (int j = 0; j < W; ++j) z[k][j] = v[j];
       }
@@ -187,6 +209,7 @@ struct Share {
     if (rest_index(length, lane) < length) rest = row[rest_index(length, lane)];
   }
 
+  // Past the caches: the gradient is larger than they are, or read by other kernels.
   __device__ __forceinline__ void store(T* row, int length, int lane) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -194,41 +217,96 @@ struct Share {
         V v;
 #pragma unroll
         for (int j = 0; j < W; ++j) v[j] = z[k][j];
-        *reinterpret_cast<V*>(row + index(k, lane)) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<V*>(row + index(k, lane)));
       }
     }
     if (rest_index(length, lane) < length) row[rest_index(length, lane)] = rest;
   }
 
-  // f(value, its index in the row) for every value.
+  // f(value, its index in the row, which of the lane's pieces) for every value.
   template <typename F>
   __device__ __forceinline__ void each(int length, int lane, F&& f) {
+    const int last = kDeep > 1 ? rest_piece(length) / kSide : 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int d = 0; d < kDeep; ++d) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) f(z[k][j], index(k, lane) + j);
-    f(rest, rest_index(length, lane));
+      for (int k = d * kLoads; k < (d + 1) * kLoads; ++k)
+#pragma unroll
+        for (int j = 0; j < W; ++j) f(z[k][j], index(k, lane) + j, d);
+      if (d == last) f(rest, rest_index(length, lane), d);
+    }
   }
 
-  // The values become exp(z - top); top and total are those of the team.
-  __device__ __forceinline__ void statistics(int length, int lane, T* meet, T& top, T& total) {
-    T m = rest;
-    each(length, lane, [&](T& v, int) { m = larger(m, v); });
-    top = team_reduce<L>(m, meet, [](T a, T b) { return larger(a, b); });
-    const T reference = top == -T(__builtin_huge_val()) ? T(0) : top;
-    rest = hpd::exp_down(rest - reference);
-    T sum = rest;
-    T s[W] = {};
+  // The values become exp(z - tops[d]) in the d-th piece of the lane; top and total
+  // are those of the row. `meet` has room for 16 waves twice and pieces twice.
+  __device__ __forceinline__ void statistics(int length, int lane, T* meet, T (&tops)[kDeep], T& top, T& total) {
+    constexpr T kNone = -T(__builtin_huge_val());
+    const auto greater = [](T a, T b) { return larger(a, b); };
+    const auto plus = [](T a, T b) { return a + b; };
+    const int last = kDeep > 1 ? rest_piece(length) / kSide : 0;  // the piece that has the rest
+    T totals[kDeep];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int d = 0; d < kDeep; ++d) {
+      T m = d == last ? rest : kNone;
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        z[k][j] = hpd::exp_down(z[k][j] - reference);
-        s[j] += z[k][j];
+      for (int k = d * kLoads; k < (d + 1) * kLoads; ++k)
+#pragma unroll
+        for (int j = 0; j < W; ++j) m = larger(m, z[k][j]);
+      tops[d] = piece_reduce(m, meet, greater);
+      const T reference = tops[d] == kNone ? T(0) : tops[d];
+      T sum = T(0);
+      if (d == last) sum = rest = hpd::exp_down(rest - reference);
+      T s[W] = {};
+#pragma unroll
+      for (int k = d * kLoads; k < (d + 1) * kLoads; ++k)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          z[k][j] = hpd::exp_down(z[k][j] - reference);
+          s[j] += z[k][j];
+        }
+#pragma unroll
+      for (int j = 0; j < W; ++j) sum += s[j];
+      totals[d] = piece_reduce(sum, meet + 16, plus);
+    }
+    if constexpr (kSide * kDeep == 1) {
+      top = tops[0];
+      total = totals[0];
+    } else {
+      T *all_tops = meet + 32, *all_totals = meet + 32 + kSide * kDeep;
+      if (lane % kStep == 0) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+          all_tops[d * kSide + lane / kStep] = tops[d];
+          all_totals[d * kSide + lane / kStep] = totals[d];
+        }
       }
+      __syncthreads();
+      const int pieces = rest_piece(length) + 1;
+      join_pieces(all_tops, all_totals, pieces, top, total);
+      __syncthreads();  // before the next row's
+    }
+  }
+
+  // The share of each piece's values in the row: exp(tops[d] - top), exactly 1 of one piece.
+  __device__ __forceinline__ static T part(T piece_top, T top) {
+    return kSide * kDeep == 1 ? T(1) : hpd::exp_down(piece_top - top);
+  }
+
+ private:
+  template <typename Op>
+  __device__ __forceinline__ static T piece_reduce(T v, T* meet, Op op) {
+    if constexpr (L <= 64) return team_reduce<L>(v, op);
 #pragma unroll
-    for (int j = 0; j < W; ++j) sum += s[j];
-    total = team_reduce<L>(sum, meet + 16, [](T a, T b) { return a + b; });
+    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();  // an earlier reduction's values have been read
+    if ((threadIdx.x & 63) == 0) meet[wave] = v;
+    __syncthreads();
+    const T* own = meet + wave / 4 * 4;
+    v = own[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) v = op(v, own[w]);
+    return v;
   }
 };
 
@@ -305,7 +383,8 @@ __device__ __forceinline__ void leave_loss(const Call<T>& c, double sum, double 
 template <typename T, int L, int K>
 __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? 4 : 1) void row_kernel(Call<T> c) {
   constexpr int kTeams = L > 256 ? 1 : 256 / L;
-  __shared__ T meet[32];
+  using S = Share<T, L, K>;
+  __shared__ T meet[32 + 2 * S::kSide * S::kDeep];
   const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : threadIdx.x / L;
   const int length = int(c.vocab);
   const double factor = c.old ? scale_of(c) : 1.0;
@@ -314,19 +393,19 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? 4 : 
   // branches on a row are uniform where they pass a barrier.
   for (int64_t row = int64_t(blockIdx.x) * kTeams + team; row < c.rows; row += int64_t(gridDim.x) * kTeams) {
     T* out = c.grad && c.old ? c.grad + row * c.vocab : nullptr;
-    Share<T, L, K> share;
+    S share;
     if (!c.kept(row)) {
       if (lane == 0) c.leave_out(row);
       if (out) {
-        share.each(length, lane, [](T& v, int) { v = T(0); });
+        share.each(length, lane, [](T& v, int, int) { v = T(0); });
         share.store(out, length, lane);
       }
       continue;
     }
-    share.load(c.logits + row * c.vocab, length, lane);
+    share.template load<true>(c.logits + row * c.vocab, length, lane);
     const int64_t y = c.target(row);
-    T top, total;
-    share.statistics(length, lane, meet, top, total);
+    T tops[S::kDeep], top, total;
+    share.statistics(length, lane, meet, tops, top, total);
     const double log_prob = c.log_prob(row, y, top, total);
     if (lane == 0) c.keep(row, log_prob, top, total);
     if (!c.old) continue;
@@ -336,14 +415,14 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? 4 : 
     if (!out) continue;
     const T w = T(slope * factor), scale = -w * (T(1) / total);
     const int at = y >= 0 && y < c.vocab ? int(y) : -1;
-    share.each(length, lane, [&](T& v, int i) { v = v * scale + (i == at ? w : T(0)); });
+    share.each(length, lane, [&](T& v, int i, int d) { v = v * (scale * S::part(tops[d], top)) + (i == at ? w : T(0)); });
     share.store(out, length, lane);
   }
   if (c.old) leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
 }
 
 // (m, S) of one piece of a row: parts[row * pieces + piece].
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __restrict__ part_tops,
                                                               T* __restrict__ part_totals, int pieces,
                                                               int piece) {
@@ -353,25 +432,12 @@ __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __re
     if (!c.kept(row)) continue;
     const int64_t start = (part - row * pieces) * piece;
     const int length = piece_end(c.vocab - start, piece);
-    T top, total;
+    T tops[1], top, total;
     Share<T, kPieceThreads, kPieceLoads> share;
-    share.load(c.logits + row * c.vocab + start, length, threadIdx.x);
-    share.statistics(length, threadIdx.x, meet, top, total);
+    share.template load<STREAM>(c.logits + row * c.vocab + start, length, threadIdx.x);
+    share.statistics(length, threadIdx.x, meet, tops, top, total);
     if (threadIdx.x == 0) part_tops[part] = top, part_totals[part] = total;
   }
-}
-
-// (m, S) of a row from its pieces', by every wave for itself.
-template <typename T>
-__device__ __forceinline__ void join_pieces(const T* tops, const T* totals, int pieces, T& top, T& total) {
-  const int lane = threadIdx.x & 63;
-  const T none = -T(__builtin_huge_val());
-  top = none;
-  for (int k = lane; k < pieces; k += 64) top = larger(top, tops[k]);
-  top = team_reduce<64>(top, static_cast<T*>(nullptr), [](T a, T b) { return larger(a, b); });
-  total = T(0);
-  for (int k = lane; k < pieces; k += 64) total += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - top);
-  total = team_reduce<64>(total, static_cast<T*>(nullptr), [](T a, T b) { return a + b; });
 }
 
 // A workgroup per row: its pieces' statistics meet, and with them its token's
@@ -406,13 +472,13 @@ __global__ __launch_bounds__(256) void grad_kernel(Call<T> c, int pieces, int pi
     const int length = piece_end(c.vocab - start, piece);
     Share<T, L, K> share;
     if (c.kept(row)) {
-      share.load(c.logits + row * c.vocab + start, length, lane);
+      share.template load<true>(c.logits + row * c.vocab + start, length, lane);
       const int64_t y = c.target(row) - start;
       const int at = y >= 0 && y < length ? int(y) : -1;
       const T w = c.weights[row / c.tokens], scale = -w * c.inverses[row], top = c.tops[row];
-      share.each(length, lane, [&](T& v, int i) { v = hpd::exp_down(v - top) * scale + (i == at ? w : T(0)); });
+      share.each(length, lane, [&](T& v, int i, int) { v = hpd::exp_down(v - top) * scale + (i == at ? w : T(0)); });
     } else {
-      share.each(length, lane, [](T& v, int) { v = T(0); });
+      share.each(length, lane, [](T& v, int, int) { v = T(0); });
     }
     share.store(c.grad + row * c.vocab + start, length, lane);
   }
@@ -434,7 +500,7 @@ __global__ __launch_bounds__(kPieceThreads) void policy_grad_kernel(Call<T> c, c
     double loss = 0;
     Share<T, kPieceThreads, kPieceLoads> share;
     if (c.kept(row)) {
-      share.load(c.logits + row * c.vocab + start, length, lane);
+      share.template load<true>(c.logits + row * c.vocab + start, length, lane);
       T top, total;
       join_pieces(part_tops + row * pieces, part_totals + row * pieces, pieces, top, total);
       const int64_t y = c.target(row);
@@ -444,10 +510,10 @@ __global__ __launch_bounds__(kPieceThreads) void policy_grad_kernel(Call<T> c, c
       policy_token(c, row, log_prob, loss, slope);
       const int at = y >= start && y < start + length ? int(y - start) : -1;
       const T w = T(slope * factor), scale = -w * (T(1) / total);
-      share.each(length, lane, [&](T& v, int i) { v = hpd::exp_down(v - top) * scale + (i == at ? w : T(0)); });
+      share.each(length, lane, [&](T& v, int i, int) { v = hpd::exp_down(v - top) * scale + (i == at ? w : T(0)); });
     } else {
       if (first && lane == 0) c.leave_out(row);
-      share.each(length, lane, [](T& v, int) { v = T(0); });
+      share.each(length, lane, [](T& v, int, int) { v = T(0); });
     }
     share.store(out, length, lane);
     if (first) leave_loss(c, loss, factor, unsigned(row), unsigned(c.rows));
@@ -526,27 +592,40 @@ bool with_team(int64_t vocab, F&& f) {
   return false;
 }
 
-// Equal pieces of whole vectors: as few as hold the row, or as many as rows need
-// to make kFewPieces workgroups, with a vector for every thread.
+// Whether teams take the rows of a call with the gradient: not rows so few and so
+// long that they would leave most of the chip idle.
+template <typename T>
+bool teams_hold(int64_t rows, int64_t vocab) {
+  const int64_t vectors = hp::ceil_div(vocab, Vec<T>::width);
+  return vectors <= 256 * 16 || (vectors <= (sizeof(T) == 4 ? 1024 : 512) * 16 && rows >= 128);
+}
+
+// Pieces of a row, of whole vectors: the teams' where teams would take the rows, so
+// that the statistics have the same bits; else equal ones, as few as hold the row or
+// as many as rows need to make kFewPieces workgroups, with a vector for every thread.
 template <typename T>
 struct Pieces {
   int count, length;
   Pieces(int64_t rows, int64_t vocab) {
-    const int64_t vectors = hp::ceil_div(vocab, Vec<T>::width);
-    const int64_t least = hp::ceil_div(vectors, kPieceThreads * kPieceLoads);
+    const int64_t vectors = hp::ceil_div(vocab, Vec<T>::width), most = kPieceThreads * kPieceLoads;
+    const int64_t least = hp::ceil_div(vectors, most);
     const int64_t wanted = std::min(hp::ceil_div(kFewPieces, rows), hp::ceil_div(vectors, kPieceThreads));
-    length = int(hp::ceil_div(vectors, std::max(least, wanted))) * Vec<T>::width;
+    const int64_t each = teams_hold<T>(rows, vocab) ? most : hp::ceil_div(vectors, std::max(least, wanted));
+    length = int(each) * Vec<T>::width;
     count = int(hp::ceil_div(vocab, length));
   }
 };
 
 unsigned loop_grid(int64_t groups) { return unsigned(std::min(groups, hp::kMaxGrid)); }
 
-// Whether a policy loss or log-probabilities take teams: not for rows so few and
-// so long that they would leave most of the chip idle.
+// Whether a call takes teams. Without the gradient only for rows that a piece
+// holds: more and smaller workgroups overlap better where nothing has to stay in
+// registers (4096 x 32000 float32: pieces 101 us, teams 122; 2048 x 50257: 77 and
+// 132; 8192 x 6000, one piece: 59).
 template <typename T>
-bool teams_serve(int64_t rows, int64_t vocab) {
-  return vocab <= 256 * 16 * Vec<T>::width || rows >= 128;
+bool teams_serve(const Call<T>& c) {
+  if (c.vocab <= kPieceThreads * kPieceLoads * Vec<T>::width) return true;
+  return c.old && c.grad && teams_hold<T>(c.rows, c.vocab);
 }
 
 // The sum of the losses where the kernel that made them does not leave it.
@@ -577,7 +656,7 @@ void plan_losses(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, unsigned sums, u
 template <typename T>
 int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   unsigned blocks = 0;
-  if (teams_serve<T>(c.rows, c.vocab) && with_team<T>(c.vocab, [&](auto l, auto k) {
+  if (teams_serve(c) && with_team<T>(c.vocab, [&](auto l, auto k) {
         constexpr int L = l, K = k, kTeams = L > 256 ? 1 : 256 / L;
         blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, kTeams), 16384));
         if (c.old) plan_losses(ctx, scratch, c, blocks, blocks);
@@ -594,7 +673,8 @@ int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   hp::require(c.rows <= hp::kMaxGrid, "too many long rows for one launch");
   blocks = unsigned(c.rows);
   if (c.old) plan_losses(ctx, scratch, c, blocks, done ? grid : blocks);
-  stats_kernel<T><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
+  const auto stats = c.grad ? stats_kernel<T, false> : stats_kernel<T, true>;
+  stats<<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
   hp::check_launch("token statistics");
   if (done) policy_grad_kernel<T><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
   else finish_kernel<T><<<blocks, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count);
