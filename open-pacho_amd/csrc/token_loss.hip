@@ -152,18 +152,37 @@ __device__ __forceinline__ T team_reduce(T v, Op op) {
   return v;
 }
 
-// (m, S) of a row from its pieces', by every wave for itself.
+// (m, S) of a row from those of pieces in the lanes that have one.
+template <typename T>
+__device__ __forceinline__ void join(bool has, T piece_top, T piece_total, T& top, T& total) {
+  const T none = -T(__builtin_huge_val());
+  top = team_reduce<64>(has ? piece_top : none, [](T a, T b) { return larger(a, b); });
+  T part = T(0);
+  if (has) part = piece_top == none ? piece_total : piece_total * hpd::exp_down(piece_top - top);
+  total = team_reduce<64>(part, [](T a, T b) { return a + b; });
+}
+
+// The same from memory, by every wave for itself; a lane's pieces join first.
 template <typename T>
 __device__ __forceinline__ void join_pieces(const T* tops, const T* totals, int pieces, T& top, T& total) {
   const int lane = threadIdx.x & 63;
   const T none = -T(__builtin_huge_val());
-  top = none;
-  for (int k = lane; k < pieces; k += 64) top = larger(top, tops[k]);
-  top = team_reduce<64>(top, [](T a, T b) { return larger(a, b); });
-  total = T(0);
-  for (int k = lane; k < pieces; k += 64) total += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - top);
-  total = team_reduce<64>(total, [](T a, T b) { return a + b; });
+  T own = lane < pieces ? tops[lane] : none, sum = lane < pieces ? totals[lane] : T(0);
+  for (int k = lane + 64; k < pieces; k += 64) {
+    const T next = larger(own, tops[k]);
+    if (own != none) sum *= hpd::exp_down(own - next);
+    sum += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - next);
+    own = next;
+  }
+  join(lane < pieces, own, sum, top, total);
 }
+
+// What the waves of a workgroup leave for each other, for two rows in turn: of
+// each of D pieces in depth.
+template <typename T, int D>
+struct Meet {
+  T tops[2][D][16], totals[2][D][16];
+};
 
 // A team's share of a row of `length` elements, which it takes in pieces of
 // kPieceThreads x kPieceLoads vectors: kSide pieces side by side by 256 threads each,
@@ -238,13 +257,13 @@ struct Share {
   }
 
   // The values become exp(z - tops[d]) in the d-th piece of the lane; top and total
-  // are those of the row. `meet` has room for 16 waves twice and pieces twice.
-  __device__ __forceinline__ void statistics(int length, int lane, T* meet, T (&tops)[kDeep], T& top, T& total) {
+  // are those of the row. A barrier each after the maxima and the sums; rows take
+  // the two sets of `meet` in turn.
+  __device__ __forceinline__ void statistics(int length, int lane, Meet<T, kDeep>& meet, int turn, T (&tops)[kDeep], T& top, T& total) {
     constexpr T kNone = -T(__builtin_huge_val());
     const auto greater = [](T a, T b) { return larger(a, b); };
     const auto plus = [](T a, T b) { return a + b; };
     const int last = kDeep > 1 ? rest_piece(length) / kSide : 0;  // the piece that has the rest
-    T totals[kDeep];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       T m = d == last ? rest : kNone;
@@ -252,7 +271,12 @@ struct Share {
       for (int k = d * kLoads; k < (d + 1) * kLoads; ++k)
 #pragma unroll
         for (int j = 0; j < W; ++j) m = larger(m, z[k][j]);
-      tops[d] = piece_reduce(m, meet, greater);
+      tops[d] = team_reduce<L < 64 ? L : 64>(m, greater);
+    }
+    share_out(tops, meet.tops[turn], greater);
+    T totals[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
       const T reference = tops[d] == kNone ? T(0) : tops[d];
       T sum = T(0);
       if (d == last) sum = rest = hpd::exp_down(rest - reference);
@@ -266,24 +290,21 @@ struct Share {
         }
 #pragma unroll
       for (int j = 0; j < W; ++j) sum += s[j];
-      totals[d] = piece_reduce(sum, meet + 16, plus);
+      totals[d] = team_reduce<L < 64 ? L : 64>(sum, plus);
     }
-    if constexpr (kSide * kDeep == 1) {
-      top = tops[0];
-      total = totals[0];
-    } else {
-      T *all_tops = meet + 32, *all_totals = meet + 32 + kSide * kDeep;
-      if (lane % kStep == 0) {
-#pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-          all_tops[d * kSide + lane / kStep] = tops[d];
-          all_totals[d * kSide + lane / kStep] = totals[d];
-        }
+    share_out(totals, meet.totals[turn], plus);
+    top = tops[0];
+    total = totals[0];
+    if constexpr (kSide * kDeep > 1) {
+      // Lane k joins in for piece k, as in join_pieces.
+      const int k = threadIdx.x & 63, d = k / kSide, side = k % kSide;
+      const bool has = k <= rest_piece(length);
+      T piece_top = kNone, piece_total = T(0);
+      if (has) {
+        piece_top = of_waves(meet.tops[turn][d], side, greater);
+        piece_total = of_waves(meet.totals[turn][d], side, plus);
       }
-      __syncthreads();
-      const int pieces = rest_piece(length) + 1;
-      join_pieces(all_tops, all_totals, pieces, top, total);
-      __syncthreads();  // before the next row's
+      join(has, piece_top, piece_total, top, total);
     }
   }
 
@@ -293,20 +314,27 @@ struct Share {
   }
 
  private:
+  // The four waves' values of the piece at `side`.
   template <typename Op>
-  __device__ __forceinline__ static T piece_reduce(T v, T* meet, Op op) {
-    if constexpr (L <= 64) return team_reduce<L>(v, op);
+  __device__ __forceinline__ static T of_waves(const T* waves, int side, Op op) {
+    T v = waves[4 * side];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
-    const int wave = threadIdx.x >> 6;
-    __syncthreads();  // an earlier reduction's values have been read
-    if ((threadIdx.x & 63) == 0) meet[wave] = v;
-    __syncthreads();
-    const T* own = meet + wave / 4 * 4;
-    v = own[0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) v = op(v, own[w]);
+    for (int w = 1; w < 4; ++w) v = op(v, waves[4 * side + w]);
     return v;
+  }
+  // From each wave's values the pieces'.
+  template <typename Op>
+  __device__ __forceinline__ static void share_out(T (&v)[kDeep], T (*waves)[16], Op op) {
+    if constexpr (L > 64) {
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) waves[d][wave] = v[d];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) v[d] = of_waves(waves[d], wave / 4, op);
+    }
   }
 };
 
@@ -378,21 +406,24 @@ __device__ __forceinline__ void leave_loss(const Call<T>& c, double sum, double 
   }
 }
 
+// LOSS: the policy loss and, unless c.grad is null, its gradient; else the
+// statistics alone, which leave the logits in the caches for the gradient's pass.
 // At 16 vectors a lane, four waves per SIMD (128 registers) keep a second
 // workgroup's loads in flight while one waits at its barriers.
-template <typename T, int L, int K>
-__global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? 4 : 1) void row_kernel(Call<T> c) {
+template <typename T, int L, int K, bool LOSS>
+__global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? (L > 256 ? 4 : 3) : 1) void row_kernel(Call<T> c) {
   constexpr int kTeams = L > 256 ? 1 : 256 / L;
   using S = Share<T, L, K>;
-  __shared__ T meet[32 + 2 * S::kSide * S::kDeep];
+  __shared__ Meet<T, S::kDeep> meet;
   const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : threadIdx.x / L;
   const int length = int(c.vocab);
-  const double factor = c.old ? scale_of(c) : 1.0;
+  const double factor = LOSS ? scale_of(c) : 1.0;
   double sum = 0;
+  int turn = 0;
   // Teams of several waves are alone in their workgroup: the loop and the
   // branches on a row are uniform where they pass a barrier.
   for (int64_t row = int64_t(blockIdx.x) * kTeams + team; row < c.rows; row += int64_t(gridDim.x) * kTeams) {
-    T* out = c.grad && c.old ? c.grad + row * c.vocab : nullptr;
+    T* out = LOSS && c.grad ? c.grad + row * c.vocab : nullptr;
     S share;
     if (!c.kept(row)) {
       if (lane == 0) c.leave_out(row);
@@ -402,23 +433,25 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? 4 : 
       }
       continue;
     }
-    share.template load<true>(c.logits + row * c.vocab, length, lane);
+    share.template load<LOSS>(c.logits + row * c.vocab, length, lane);
     const int64_t y = c.target(row);
     T tops[S::kDeep], top, total;
-    share.statistics(length, lane, meet, tops, top, total);
+    share.statistics(length, lane, meet, turn, tops, top, total);
+    turn ^= 1;
     const double log_prob = c.log_prob(row, y, top, total);
     if (lane == 0) c.keep(row, log_prob, top, total);
-    if (!c.old) continue;
-    double loss, slope;
-    policy_token(c, row, log_prob, loss, slope);
-    if (lane == 0) sum += loss;
-    if (!out) continue;
-    const T w = T(slope * factor), scale = -w * (T(1) / total);
-    const int at = y >= 0 && y < c.vocab ? int(y) : -1;
-    share.each(length, lane, [&](T& v, int i, int d) { v = v * (scale * S::part(tops[d], top)) + (i == at ? w : T(0)); });
-    share.store(out, length, lane);
+    if constexpr (LOSS) {
+      double loss, slope;
+      policy_token(c, row, log_prob, loss, slope);
+      if (lane == 0) sum += loss;
+      if (!out) continue;
+      const T w = T(slope * factor), scale = -w * (T(1) / total);
+      const int at = y >= 0 && y < c.vocab ? int(y) : -1;
+      share.each(length, lane, [&](T& v, int i, int d) { v = v * (scale * S::part(tops[d], top)) + (i == at ? w : T(0)); });
+      share.store(out, length, lane);
+    }
   }
-  if (c.old) leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
+  if constexpr (LOSS) leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
 }
 
 // (m, S) of one piece of a row: parts[row * pieces + piece].
@@ -426,7 +459,8 @@ template <typename T, bool STREAM>
 __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __restrict__ part_tops,
                                                               T* __restrict__ part_totals, int pieces,
                                                               int piece) {
-  __shared__ T meet[32];
+  __shared__ Meet<T, 1> meet;
+  int turn = 0;
   for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
     const int64_t row = part / pieces;
     if (!c.kept(row)) continue;
@@ -435,7 +469,8 @@ __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __re
     T tops[1], top, total;
     Share<T, kPieceThreads, kPieceLoads> share;
     share.template load<STREAM>(c.logits + row * c.vocab + start, length, threadIdx.x);
-    share.statistics(length, threadIdx.x, meet, tops, top, total);
+    share.statistics(length, threadIdx.x, meet, turn, tops, top, total);
+    turn ^= 1;
     if (threadIdx.x == 0) part_tops[part] = top, part_totals[part] = total;
   }
 }
@@ -659,8 +694,13 @@ int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   if (teams_serve(c) && with_team<T>(c.vocab, [&](auto l, auto k) {
         constexpr int L = l, K = k, kTeams = L > 256 ? 1 : 256 / L;
         blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, kTeams), 16384));
-        if (c.old) plan_losses(ctx, scratch, c, blocks, blocks);
-        row_kernel<T, L, K><<<blocks, L > 256 ? L : 256, 0, ctx->stream>>>(c);
+        constexpr int threads = L > 256 ? L : 256;
+        if (c.old) {
+          plan_losses(ctx, scratch, c, blocks, blocks);
+          row_kernel<T, L, K, true><<<blocks, threads, 0, ctx->stream>>>(c);
+        } else if constexpr (L * K <= kPieceThreads * kPieceLoads) {  // teams_serve()
+          row_kernel<T, L, K, false><<<blocks, threads, 0, ctx->stream>>>(c);
+        }
         hp::check_launch("token rows");
       })) {
     return blocks;
