@@ -16,20 +16,26 @@
 // alignment; a workgroup owns 64 channels, and its W waves consecutive runs of R
 // steps. Each wave loads its run into registers, composes it, leaves (A, B) in
 // LDS, takes what the waves before it left, and then computes and stores its
-// states: one pass over the data, one barrier for each R x W steps. Two sets of
-// registers take turns, so that the next run's loads are in flight while a run
-// is computed.
+// states: one pass over the data.
 //
-// Few channels would leave compute units idle: then every W x R steps of 64
-// channels are a tile with a workgroup of its own (the chained kernels), still in
-// one pass. A tile publishes its composition as soon as it has it. Tiles count in
-// blocks of `span`: the state before a tile is the one before its block, which
-// the last tile of the block before publishes, through the compositions of the
-// block's earlier tiles, always in the same order, so that results repeat bit
+// Longer rows are cut into tiles of W x R steps with a workgroup each (the chained
+// kernels), still in one pass. A tile publishes its composition as soon as it has
+// it. Tiles count in blocks of `span`: the state before a tile is the one before its
+// block, which the last tile of the block before publishes, through the compositions
+// of the block's earlier tiles, always in the same order, so that results repeat bit
 // for bit. Workgroups take tiles in time order from queues, so a tile only ever
 // waits for tiles whose workgroups have started, and those for earlier ones: every
 // wait ends. A published word is valid by itself, without fences: memory is all
-// ones before, which no published value is.
+// ones before, which no published value is. One workgroup that walks all tiles of
+// its channels with the next tile's loads in flight took 163 us forward and 327
+// backward for 8 x 4096 x 2048 float32 where chained tiles take 150 and 294 (5.4 and
+// 5.5 TB/s of 5.5 that reads and writes together reach here): its waves wait for
+// each other every tile. For 1 x 65536 x 1024, segments of time in two passes took
+// 278 and 448 us, chained tiles 174 and 331.
+//
+// Runs of 16 and 8 steps (forward, backward; half as many float64) fill 72 and 90
+// registers, so that three and two workgroups share a compute unit. Half as many
+// steps take 2 to 25% longer, twice as many backward 4 to 8%, four waves 3 to 15%.
 #include <type_traits>
 
 #include "common.h"
@@ -401,27 +407,25 @@ struct ForwardColumns {
   }
 };
 
-template <typename T, int R, int W, bool RESETS>
+// Rows of at most W x R steps, or of two times as many where DOUBLE.
+template <typename T, int R, int W, bool DOUBLE, bool RESETS>
 __global__ __launch_bounds__(W * 64) void forward_kernel(Forward<T> f, Extents e) {
   __shared__ Left<T, W> left;
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ForwardColumns<T> c(f, e, by_die(), lane);
   T state = c.first;
-  constexpr int64_t stride = int64_t(W) * R;
-  int64_t t = int64_t(wave) * R;
-  ForwardLoads<T, R> one, two;
-  const auto steps = [&](ForwardLoads<T, R>& now, ForwardLoads<T, R>& next, int turn) {
-    if (t + stride < e.time) next.template load<RESETS>(c.x, c.gate, c.resets, e, t + stride, e.time);
+  constexpr int stride = W * R;
+  ForwardLoads<T, R> loads[DOUBLE ? 2 : 1];
+#pragma unroll
+  for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) {
+    loads[n].template load<RESETS>(c.x, c.gate, c.resets, e, n * stride + wave * R, e.time);
+  }
+#pragma unroll
+  for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) {
     Run<T> run{T(1), T(0), false};
-    now.template compose<RESETS>(run);
-    const T value = through<T, W>(run, left, turn, wave, lane, state);
-    c.template finish<R, RESETS>(now, e, t, value);
-    t += stride;
-  };
-  one.template load<RESETS>(c.x, c.gate, c.resets, e, t, e.time);
-  for (int64_t base = 0; base < e.time; base += 2 * stride) {
-    steps(one, two, 0);
-    if (base + stride < e.time) steps(two, one, 1);
+    loads[n].template compose<RESETS>(run);
+    const T value = through<T, W>(run, left, n, wave, lane, state);
+    c.template finish<R, RESETS>(loads[n], e, n * stride + wave * R, value);
   }
 }
 
@@ -594,9 +598,9 @@ struct BackwardColumns {
   }
 };
 
-// Wave 0 takes the last R steps, wave 1 those before them: t is the first step
-// of a wave's run, below zero at the start of the row.
-template <typename T, int R, int W, bool RESETS, bool SHARED>
+// Rows as in forward_kernel. Wave 0 takes the last R steps, wave 1 those before them:
+// a wave's first step is below zero at the start of the row.
+template <typename T, int R, int W, bool DOUBLE, bool RESETS, bool SHARED>
 __global__ __launch_bounds__(W * 64) void backward_kernel(Backward<T> f, Extents e) {
   __shared__ Left<T, W> left;
   __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];  // rows of a sum's lanes in banks of their own
@@ -604,22 +608,16 @@ __global__ __launch_bounds__(W * 64) void backward_kernel(Backward<T> f, Extents
   const int64_t group = by_die();
   const BackwardColumns<T, SHARED> c(f, e, group, lane);
   T carried = T(0);
-  constexpr int64_t stride = int64_t(W) * R;
-  int64_t t = e.time - int64_t(wave + 1) * R;
-  BackwardLoads<T, R> one, two;
-  const auto steps = [&](BackwardLoads<T, R>& now, BackwardLoads<T, R>& next, int turn, bool more) {
-    if (more) c.template load<RESETS>(next, e, t - stride);
+  const int64_t t = e.time - int64_t(wave + 1) * R;
+  BackwardLoads<T, R> loads[DOUBLE ? 2 : 1];
+#pragma unroll
+  for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) c.template load<RESETS>(loads[n], e, t - n * W * R);
+#pragma unroll
+  for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) {
     Run<T> run{T(1), T(0), false};
-    now.template compose<RESETS>(run);
-    const T value = through<T, W>(run, left, turn, wave, lane, carried);
-    c.template finish<R, RESETS>(now, e, group, t, lane, shares[SHARED ? wave : 0], value);
-    t -= stride;
-  };
-  c.template load<RESETS>(one, e, t);
-  for (int64_t base = 0; base < e.time; base += 2 * stride) {
-    const bool second = base + stride < e.time;
-    steps(one, two, 0, second);
-    if (second) steps(two, one, 1, base + 2 * stride < e.time);
+    loads[n].template compose<RESETS>(run);
+    const T value = through<T, W>(run, left, n, wave, lane, carried);
+    c.template finish<R, RESETS>(loads[n], e, group, t - n * W * R, lane, shares[SHARED ? wave : 0], value);
   }
   if (c.dinitial && wave == 0 && c.valid) *c.dinitial = carried;
 }
@@ -683,15 +681,21 @@ unsigned checked_grid(int64_t groups, int threads) {
 
 constexpr int kWaves = 8;
 
-// Calls f with the waves of a workgroup and the steps of a run.
+// Calls f with the steps of a run, the waves of a workgroup, and whether it takes
+// two runs of each.
 template <int R, typename F>
 void with_shape(int64_t time, F&& f) {
-  const auto shape = [&](auto waves, auto steps) { f(waves, steps); };
-  if (time == 1) shape(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-  else if (time <= 4) shape(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-  else if (time <= R) shape(std::integral_constant<int, 1>{}, std::integral_constant<int, R>{});
-  else if (time <= 4 * R) shape(std::integral_constant<int, 4>{}, std::integral_constant<int, R>{});
-  else shape(std::integral_constant<int, kWaves>{}, std::integral_constant<int, R>{});
+  const auto shape = [&](auto steps, auto waves, auto twice) { f(steps, waves, twice); };
+  using Int = std::integral_constant<int, R>;
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  using All = std::integral_constant<int, kWaves>;
+  if (time == 1) shape(One{}, One{}, std::false_type{});
+  else if (time <= 4) shape(Four{}, One{}, std::false_type{});
+  else if (time <= R) shape(Int{}, One{}, std::false_type{});
+  else if (time <= 4 * R) shape(Int{}, Four{}, std::false_type{});
+  else if (time <= kWaves * R) shape(Int{}, All{}, std::false_type{});
+  else shape(Int{}, All{}, std::true_type{});
 }
 
 // Whether tiles are chained: from three on. (With one workgroup that walks two
@@ -728,10 +732,10 @@ void forward(hp_ctx* ctx, const Forward<T>& f, Extents e) {
     const auto kernel = f.resets ? forward_chained_kernel<T, R, kWaves, true> : forward_chained_kernel<T, R, kWaves, false>;
     kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
   } else {
-    with_shape<R>(e.time, [&](auto waves, auto steps) {
-      constexpr int W = waves, S = steps;
+    with_shape<R>(e.time, [&](auto steps, auto waves, auto twice) {
+      constexpr int S = steps, W = waves;
       const unsigned grid = checked_grid(e.groups, 64 * W);
-      const auto kernel = f.resets ? forward_kernel<T, S, W, true> : forward_kernel<T, S, W, false>;
+      const auto kernel = f.resets ? forward_kernel<T, S, W, twice, true> : forward_kernel<T, S, W, twice, false>;
       kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
     });
   }
@@ -752,10 +756,10 @@ void backward(hp_ctx* ctx, Backward<T> f, Extents e) {
     const auto kernel = f.resets ? backward_chained_kernel<T, R, kWaves, true, SHARED> : backward_chained_kernel<T, R, kWaves, false, SHARED>;
     kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
   } else {
-    with_shape<R>(e.time, [&](auto waves, auto steps) {
-      constexpr int W = waves, S = steps;
+    with_shape<R>(e.time, [&](auto steps, auto waves, auto twice) {
+      constexpr int S = steps, W = waves;
       const unsigned grid = checked_grid(e.groups, 64 * W);
-      const auto kernel = f.resets ? backward_kernel<T, S, W, true, SHARED> : backward_kernel<T, S, W, false, SHARED>;
+      const auto kernel = f.resets ? backward_kernel<T, S, W, twice, true, SHARED> : backward_kernel<T, S, W, twice, false, SHARED>;
       kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
     });
   }

@@ -17,6 +17,9 @@ SIZES = [
     (1, 1, 1, 1), (3, 1, 65, 65), (5, 2, 13, 13), (2, 17, 64, 64), (1, 1000, 3, 3), (2, 129, 70, 70), (4, 257, 130, 130),
     (33, 65, 2, 2), (2, 33, 12, 4), (3, 5, 64, 1), (2, 9, 66, 1), (1, 515, 200, 2), (2, 130, 125, 1), (2, 40, 256, 2),
     (1, 300, 96, 96), (7, 31, 40, 8), (0, 3, 4, 2), (2, 0, 4, 4), (2, 3, 0, 0),
+    # the ends of runs, of workgroups and of two of them, and tiles beyond
+    (2, 4, 5, 5), (2, 5, 5, 1), (1, 8, 70, 70), (1, 16, 70, 35), (1, 32, 9, 9), (1, 63, 9, 3), (1, 64, 66, 66), (1, 128, 9, 1),
+    (1, 192, 65, 65), (1, 193, 6, 6), (1, 256, 6, 2), (1, 384, 3, 3), (1, 385, 3, 1), (1, 513, 130, 1),
 ]  # fmt: skip
 
 
@@ -28,7 +31,8 @@ def test_values_and_gradients(hip, sizes, state, resets, dtype):
     check(hip, sizes, dtype, state, resets)
 
 
-@pytest.mark.parametrize("sizes", [(1, 20000, 5, 5), (1, 5001, 130, 2), (2, 4099, 65, 65)])
+# Several blocks of tiles, of 16 (from 16 groups of channels on) and of 64.
+@pytest.mark.parametrize("sizes", [(1, 20000, 5, 5), (1, 5001, 130, 2), (2, 4099, 65, 65), (1, 2100, 1030, 1030), (3, 2049, 400, 4)])
 def test_long_rows(hip, sizes):
     print(sizes, flush=True)
     check(hip, sizes, np.float32, True, True)
