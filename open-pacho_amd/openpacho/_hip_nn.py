@@ -70,6 +70,8 @@ def _broadcast(backend, array, whole):
     """Storage of `array`, and how it repeats over `whole` (_period)."""
     if array._shape == whole:
         return array._data, 1, max(1, array.size)
+    if whole and array._shape == whole[:-1] + (1,):  # one for each row, the usual one
+        return array._data, max(1, whole[-1]), max(1, array.size)
     found = _period(array._shape, whole)
     if found is None:
         strides = [prod(array._shape[axis + 1 :]) if d != 1 else 0 for axis, d in enumerate(array._shape)]
@@ -108,9 +110,6 @@ class _Span:
 
     __slots__ = ("block", "offset")
 
-    def __init__(self, block, offset):
-        self.block, self.offset = block, offset
-
     @property
     def ptr(self):
         start = self.block.ptr  # 0 once the backend is closed
@@ -137,7 +136,12 @@ class _Layout:
         return self.pointers(*[a._data.ptr for a in arrays])
 
     def spans(self, block, start=0):
-        return [_Span(block, start + offset) for offset in self.offsets]
+        spans, new = [], object.__new__
+        for offset in self.offsets:
+            span = new(_Span)
+            span.block, span.offset = block, start + offset
+            spans.append(span)
+        return spans
 
 
 class _State:

@@ -74,7 +74,7 @@ class _Operands:
     def broadcast(self, name, value, shape):
         """`value`, which has to broadcast to `shape`."""
         value = self.array(name, value)
-        if value._shape != shape:
+        if value._shape != shape and not (shape and value._shape == shape[:-1] + (1,)):
             try:
                 whole = np.broadcast_shapes(value._shape, shape) == shape
             except ValueError:
@@ -95,6 +95,8 @@ def _wrapped(data, shape, dtype, backend):
 
 
 def _number(what, value, least=None, below=None, infinite=False):
+    if type(value) is float and least == 0 and 0 <= value < (math.inf if below is None else below):
+        return value
     value = float(value)
     if math.isnan(value) or (math.isinf(value) and not infinite):
         raise ValueError(f"{what} must be a finite number")
@@ -303,11 +305,21 @@ class AdamWState:
 
 
 def _wrapped_list(storages, shapes, dtype, backend):
-    return [_wrapped(data, shape, dtype, backend) for data, shape in zip(storages, shapes)]
+    arrays, new, kind = [], object.__new__, xp.ndarray
+    for data, shape in zip(storages, shapes):  # _wrapped, without a call for each of many tensors
+        array = new(kind)
+        array._data, array._shape, array._dtype, array._backend = data, shape, dtype, backend
+        arrays.append(array)
+    return arrays
 
 
 def _check_tensors(what, name, values, backend, dtype, shapes):
     """Refuse what is not a list of arrays of this backend, dtype and these shapes."""
+    try:
+        if [v._shape for v in values if v._backend is backend and v._dtype is dtype] == shapes and type(values) in (list, tuple):
+            return
+    except (AttributeError, TypeError):
+        pass  # something in it is no array
     if not isinstance(values, (list, tuple)) or not all([isinstance(v, xp.ndarray) for v in values]):
         raise TypeError(f"{what}: {name} must be a list of arrays")
     for value in values:
