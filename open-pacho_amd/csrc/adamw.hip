@@ -4,8 +4,11 @@
 //   p' = p - (decay p + step m' / (root sqrt(v') + eps)),  step = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
 //
 // Bound: HBM. Four arrays are read and three written (float32: 28 bytes a
-// parameter), with 8-bit moments two arrays and two bytes read, one array and two
-// bytes written and 16 bytes of scales for every 256 parameters.
+// parameter: 201 million in 948 us, 5.9 TB/s), with 8-bit moments two arrays and two
+// bytes read, one array and two bytes written and 16 bytes of scales for every 256
+// parameters (98 million: 1.6 GB in 264-306 us). There the vector unit comes
+// next: divisions and roots as the compiler expands them took 131 instructions a
+// parameter and bound the kernel at 340 us, the ones below take about 80.
 //
 // A launch takes up to kTensors tensors: the table of their addresses is a
 // kernel argument, so that no table has to be copied to the device first. A
@@ -64,13 +67,15 @@ struct Pack {
   T v[W];
 };
 
-// W values from `p`; one access if `whole`, else those below `count`.
+// W values from `p`; one access if `whole`, else those below `count`. Past the
+// caches, as the stores: everything is read and written once (201 million float32
+// parameters 998 -> 948 us, 98 million with 8-bit states 483 -> 419).
 template <typename T, int W>
 __device__ __forceinline__ Pack<T, W> load_pack(const T* p, bool whole, int64_t count) {
   typedef T V __attribute__((ext_vector_type(W), aligned(sizeof(T))));
   Pack<T, W> r;
   if (whole) {
-    const V v = *reinterpret_cast<const V*>(p);
+    const V v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
 #pragma unroll
     for (int j = 0; j < W; ++j) r.v[j] = v[j];
   } else {
@@ -86,44 +91,88 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, W>& r) {
   V v;
 #pragma unroll
   for (int j = 0; j < W; ++j) v[j] = r.v[j];
-  *reinterpret_cast<V*>(p) = v;
+  __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
 }
 
+// 1 / x of a normal x > 0 or infinity to a unit in the last place: the hardware's
+// estimate, which is 0 from 2^126 on, and a Newton step.
+__device__ __forceinline__ float reciprocal(float x) {
+  const float r = __builtin_amdgcn_rcpf(x);
+  return r == 0.0f ? 0.0f : __builtin_fmaf(r, __builtin_fmaf(-x, r, 1.0f), r);
+}
+__device__ __forceinline__ double reciprocal(double x) { return 1.0 / x; }
+
+// `root_v`: sqrt(v).
 template <typename T>
-__device__ __forceinline__ T update(T p, T m, T v, T decay, T step, T root, T eps) {
-  const T size = __builtin_elementwise_sqrt(v) * root + eps;
-  return p - (decay * p + step * m / size);
+__device__ __forceinline__ T update(T p, T m, T root_v, T decay, T step, T root, T eps) {
+  return p - (decay * p + step * m * reciprocal(root_v * root + eps));
+}
+
+// The correctly rounded root. Between 2^-96 and 2^96 (and of 0) by the coupled
+// iteration of Markstein (Computation of elementary functions on the IBM RISC
+// System/6000 processor, 1990) without the scaling that the ends of the type need:
+// eleven instructions in place of about eighteen.
+__device__ __forceinline__ float root_of(float v) {
+  const float y = __builtin_amdgcn_rsqf(v);
+  float g = v * y, h = 0.5f * y;
+  const float r = __builtin_fmaf(-h, g, 0.5f);
+  g = __builtin_fmaf(g, r, g);
+  h = __builtin_fmaf(h, r, h);
+  g = __builtin_fmaf(__builtin_fmaf(-g, g, v), h, g);
+  return v == 0.0f ? v : g;
+}
+
+// Roots of a lane's elements; all lanes of a wave take one way.
+__device__ __forceinline__ Pack<float, 4> roots(const Pack<float, 4>& v) {
+  bool plain = true;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) plain = plain && (v.v[j] == 0.0f || (v.v[j] > 0x1p-96f && v.v[j] < 0x1p96f));
+  Pack<float, 4> r;
+  if (__all(plain)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.v[j] = root_of(v.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.v[j] = __builtin_sqrtf(v.v[j]);
+  }
+  return r;
+}
+__device__ __forceinline__ Pack<double, 4> roots(const Pack<double, 4>& v) {
+  Pack<double, 4> r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r.v[j] = __builtin_sqrt(v.v[j]);
+  return r;
 }
 
 // ---- 8-bit shares ----------------------------------------------------------------
 
-// LOW: the lowest 16 codes are multiples of 2^-LOW. A share's float bits, cut
-// after 4 of the mantissa, number the codes of an octave and the octaves, from
-// the octave 2^(4 - LOW) on.
+// LOW: the lowest 16 codes are multiples of 2^-LOW; from the octave 2^(4 - LOW) on
+// each octave has 16 codes. A share plus 1.5 x 2^(octave + 19) is rounded to its
+// octave's step, 2^(octave - 4), and has the number of steps in its last bits.
 template <int LOW>
 __device__ __forceinline__ unsigned encode(float share) {
-  const unsigned bits = __float_as_uint(share);
-  const unsigned rounded = (bits + 0x3FFFF + (bits >> 19 & 1)) >> 19;
-  const unsigned normal = rounded - ((127 + 4 - LOW) * 16 - 16);
-  const unsigned even = unsigned(__builtin_rintf(share * float(1 << LOW)));
-  return share < 16.0f / float(1 << LOW) ? even : normal;
+  constexpr unsigned kLowest = (127 + 4 - LOW) << 23, kMagic = (19u << 23) + 0x400000u;
+  const unsigned octave = max(__float_as_uint(share) & 0x7F800000u, kLowest);
+  const unsigned steps = __float_as_uint(share + __uint_as_float(octave + kMagic));
+  return steps - octave + (octave >> 19) - (kMagic + (kLowest >> 19));
 }
 
+// A code's bits, put to the top of a float below its sign, are its share times
+// 2^(LOW - 130), with the float's own denormal numbers for the lowest 16.
 template <int LOW>
-__device__ __forceinline__ float decode(unsigned code) {
-  const float normal = __uint_as_float((code + ((127 + 4 - LOW) * 16 - 16)) << 19);
-  return code < 16 ? float(code) * (1.0f / float(1 << LOW)) : normal;
+__device__ __forceinline__ float decode(unsigned top_bits) {
+  constexpr unsigned kScale = (127 + 130 - LOW) << 23;
+  return __uint_as_float(top_bits) * __uint_as_float(kScale);
 }
 
 constexpr int kFirst = 10, kSecond = 18;
 
 __device__ __forceinline__ float decode_first(unsigned code, float top) {
-  const float m = decode<kFirst>(code & 127) * top;
-  return code & 128 ? -m : m;
+  return decode<kFirst>((code & 128) << 24 | (code & 127) << 19) * top;
 }
 
 __device__ __forceinline__ float decode_second(unsigned code, float top) {
-  const float u = decode<kSecond>(code) * top;
+  const float u = decode<kSecond>(code << 19) * top;
   return u * u;
 }
 
@@ -138,27 +187,47 @@ __device__ __forceinline__ float block_top(const Pack<float, 4>& v) {
   return top >= 0x7F800000u ? __builtin_nanf("") : __uint_as_float(top);
 }
 
-// Codes of four moments a lane of a block of 256, and the block's scales.
-__device__ __forceinline__ void encode_block(const Pack<float, 4>& m, const Pack<float, 4>& v, int64_t block,
-                                             const Moments<float>& to, int lane) {
-  Pack<float, 4> size, root;
+// Shares in `top`, each correctly rounded: two corrections of the product with the
+// reciprocal (Markstein, as above), or where that could leave the type, divisions.
+__device__ __forceinline__ Pack<float, 4> shares(const Pack<float, 4>& v, float top) {
+  Pack<float, 4> r;
+  if (top > 0x1p-60f && top < 0x1p60f) {
+    const float inverse = reciprocal(top);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    size.v[j] = __builtin_fabsf(m.v[j]);
-    root.v[j] = __builtin_sqrtf(v.v[j]);
+    for (int j = 0; j < 4; ++j) {
+      float q = v.v[j] * inverse;
+      q = __builtin_fmaf(__builtin_fmaf(-q, top, v.v[j]), inverse, q);
+      r.v[j] = __builtin_fmaf(__builtin_fmaf(-q, top, v.v[j]), inverse, q);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.v[j] = v.v[j] / top;
   }
+  return r;
+}
+
+// Codes of four moments a lane of a block of 256 (`root`: of the second), and the
+// block's scales.
+__device__ __forceinline__ void encode_block(const Pack<float, 4>& m, const Pack<float, 4>& root, int64_t block,
+                                             const Moments<float>& to, int lane) {
+  Pack<float, 4> size;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) size.v[j] = __builtin_fabsf(m.v[j]);
   const float top1 = block_top(size), top2 = block_top(root);
   uint32_t codes1 = 0, codes2 = 0;
+  // Comparisons that a NaN scale fails leave code 0, which stands for 0 times NaN.
+  if (top1 > 0) {
+    const Pack<float, 4> share = shares(size, top1);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    // Comparisons that a NaN scale fails leave code 0, which stands for 0 times NaN.
-    unsigned first = top1 > 0 ? encode<kFirst>(size.v[j] / top1) : 0;
-    unsigned second = top2 > 0 ? encode<kSecond>(root.v[j] / top2) : 0;
-    if (second == 0 && top2 > 0 && root.v[j] > 0) second = 1;
-    first |= __float_as_uint(m.v[j]) >> 24 & 128;
-    codes1 |= first << 8 * j;
-    codes2 |= second << 8 * j;
+    for (int j = 0; j < 4; ++j) codes1 |= encode<kFirst>(share.v[j]) << 8 * j;
   }
+  if (top2 > 0) {
+    const Pack<float, 4> share = shares(root, top2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) codes2 |= max(encode<kSecond>(share.v[j]), root.v[j] > 0 ? 1u : 0u) << 8 * j;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) codes1 |= (__float_as_uint(m.v[j]) >> 31) << (8 * j + 7);
   reinterpret_cast<uint32_t*>(to.codes1)[block * 64 + lane] = codes1;
   reinterpret_cast<uint32_t*>(to.codes2)[block * 64 + lane] = codes2;
   if (lane == 0) to.top1[block] = top1, to.top2[block] = top2;
@@ -215,12 +284,14 @@ __global__ __launch_bounds__(256) void step_kernel(Table<T> table, Moments<T> fr
   for (int j = 0; j < W; ++j) {
     m.v[j] = m.v[j] * beta1 + g.v[j] * rest1;
     v.v[j] = v.v[j] * beta2 + (g.v[j] * g.v[j]) * rest2;
-    out.v[j] = update(p.v[j], m.v[j], v.v[j], decay, step, root, eps);
   }
+  const Pack<T, W> root_v = roots(v);
+#pragma unroll
+  for (int j = 0; j < W; ++j) out.v[j] = update(p.v[j], m.v[j], root_v.v[j], decay, step, root, eps);
   store_pack<T, W>(params + place, out);
   if constexpr (sizeof(T) == 4) {
     if (to.codes1) {
-      encode_block(m, v, block, to, lane);
+      encode_block(m, root_v, block, to, lane);
       return;
     }
   }
@@ -240,7 +311,7 @@ __global__ __launch_bounds__(256) void load_kernel(Table<T> table, Moments<T> to
   const Pack<T, W> m = load_pack<T, W>(t.param + at, left >= W, left), v = load_pack<T, W>(t.grad + at, left >= W, left);
   if constexpr (sizeof(T) == 4) {
     if (to.codes1) {
-      encode_block(m, v, block, to, lane);
+      encode_block(m, roots(v), block, to, lane);
       return;
     }
   }

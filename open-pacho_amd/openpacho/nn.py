@@ -386,8 +386,8 @@ def adamw(params, grads, state, *, learning_rate=1e-3, betas=(0.9, 0.999), eps=1
     learning_rate = _number("learning_rate", learning_rate, 0)
     beta1, beta2 = (_number("betas", b, 0, 1) for b in betas)
     eps = _number("eps", eps)
-    if eps <= 0:
-        raise ValueError("eps must be positive")
+    if eps < np.finfo(dtype).tiny:
+        raise ValueError(f"eps must be positive, and at least {np.finfo(dtype).tiny} for {dtype}")
     if np.ndim(weight_decay):
         decays = [_number("weight_decay", d, 0) for d in weight_decay]
         if len(decays) != len(shapes):

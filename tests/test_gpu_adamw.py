@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import openpacho as p
-from test_nn_adamw import OPTIONS, SHAPES, bring, check_codes, check_first_step, check_resume, check_steps, make, put
+from test_nn_adamw import OPTIONS, SHAPES, bring, check_codes, check_ends, check_first_step, check_resume, check_steps, make, put
 
 pytestmark = pytest.mark.gpu
 
@@ -34,8 +34,26 @@ def test_first_step(hip, dtype):
     check_first_step(hip, dtype)
 
 
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_ends_of_the_type(hip, dtype):
+    check_ends(hip, dtype)
+
+
 def test_codes(hip):
     check_codes(hip)
+
+
+def test_codes_of_many_values(hip):
+    # Roots and shares are correctly rounded: as many codes as these agree with the host's to the last one.
+    rng = np.random.default_rng(9)
+    values = np.exp(rng.uniform(-40, 3, (4000, 1024))).astype(np.float32) * np.exp(rng.uniform(-30, 30, (4000, 1))).astype(np.float32)
+    first = np.where(rng.random(values.shape) < 0.5, values, -values).astype(np.float32)
+    params = put(hip, [values])
+    state = p.nn.adamw_state(params, state_bits=8, first=put(hip, [first]), second=params)
+    host = p.get_backend("numpy")
+    want = p.nn.adamw_state(put(host, [values]), state_bits=8, first=put(host, [first]), second=put(host, [values]))
+    np.testing.assert_array_equal(bring(state.first)[0], bring(want.first)[0])
+    np.testing.assert_array_equal(bring(state.second)[0], bring(want.second)[0])
 
 
 @pytest.mark.parametrize("bits", [None, 8])

@@ -94,6 +94,24 @@ def test_first_step(numpy_backend, dtype):
     check_first_step(numpy_backend, dtype)
 
 
+def check_ends(backend, dtype):
+    """Gradients whose squares leave the type, and none at all: finite parameters wherever the definition has them."""
+    big = np.sqrt(float(np.finfo(dtype).max)) * 10
+    given = np.array([1.0, 1.0, 1.0, 1.0, 1.0, 1.0], dtype)
+    grad = np.array([0.0, big, -big, 1.0, np.nan, 1e-30], dtype)
+    params = put(backend, [given])
+    new, state = p.nn.adamw(params, put(backend, [grad]), p.nn.adamw_state(params), learning_rate=0.5, weight_decay=0)
+    got, second = bring(new)[0], bring(state.second)[0]
+    # An infinite second moment moves nothing; no gradient moves nothing; eps bounds the step of a tiny one.
+    assert list(got[:3]) == [1, 1, 1] and np.isinf(second[1:3]).all() and np.isnan(got[4])
+    assert abs(got[3] - 0.5) < 1e-4 and abs(got[5] - 1) < 1e-6
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_ends_of_the_type(numpy_backend, dtype):
+    check_ends(numpy_backend, dtype)
+
+
 def check_codes(backend):
     """Every share that has a code, the middles between them, and blocks at the ends of the type."""
     m_grid, u_grid = training._grid(112, 10), training._grid(240, 18)
@@ -186,7 +204,7 @@ def test_refusals(numpy_backend):
         p.nn.adamw_state(params, steps=-1)
     with pytest.raises(ValueError, match="together"):
         p.nn.adamw_state(params, first=params)
-    for name, bad in [("learning_rate", -1), ("learning_rate", np.nan), ("betas", (1.0, 0.9)), ("betas", (0.9, -0.1)), ("eps", 0),
+    for name, bad in [("learning_rate", -1), ("learning_rate", np.nan), ("betas", (1.0, 0.9)), ("betas", (0.9, -0.1)), ("eps", 0), ("eps", 1e-39),
                       ("weight_decay", -1), ("weight_decay", [0.1]), ("weight_decay", [0.1, np.inf])]:  # fmt: skip
         with pytest.raises(ValueError, match=name):
             p.nn.adamw(params, params, state, **{name: bad})
