@@ -110,12 +110,13 @@ __device__ __forceinline__ T apply(T a, T b, T h) {
 }
 
 // R values of a column from its step t on; steps outside [0, end) hold `outside`.
-template <typename T, int R>
+// STREAM: past the caches.
+template <bool STREAM, typename T, int R>
 __device__ __forceinline__ void load_steps(const T* column, int64_t stride, int64_t t, int64_t end, T outside, T (&v)[R]) {
   if (t >= 0 && t + R <= end) {
     const T* p = column + t * stride;
 #pragma unroll
-    for (int i = 0; i < R; ++i) v[i] = p[i * stride];
+    for (int i = 0; i < R; ++i) v[i] = STREAM ? __builtin_nontemporal_load(p + i * stride) : p[i * stride];
   } else {
 #pragma unroll
     for (int i = 0; i < R; ++i) v[i] = t + i >= 0 && t + i < end ? column[(t + i) * stride] : outside;
@@ -336,8 +337,8 @@ struct ForwardLoads {
   // Steps past the end keep the state: their gate is +inf.
   template <bool RESETS>
   __device__ __forceinline__ void load(const T* xs, const T* gs, const uint8_t* rs, const Extents& e, int64_t t, int64_t end) {
-    load_steps<T, R>(xs, e.channels, t, end, T(0), x);
-    load_steps<T, R>(gs, e.gates, t, end, T(__builtin_huge_val()), gate);
+    load_steps<true>(xs, e.channels, t, end, T(0), x);
+    load_steps<true>(gs, e.gates, t, end, T(__builtin_huge_val()), gate);
     if (RESETS) resets = load_resets<R>(rs, t, end);
   }
 
@@ -455,13 +456,13 @@ struct BackwardLoads {
 
   // Steps before the row pass the gradient on: their gate is +inf and their
   // gradient 0. h is that of the step before.
-  template <bool RESETS>
+  template <bool RESETS, bool STREAM, bool SHARED>
   __device__ __forceinline__ void load(const T* xs, const T* gs, const T* hs, const T* ds, const uint8_t* rs, T before,
                                        const Extents& e, int64_t t) {
-    load_steps<T, R>(gs, e.gates, t, e.time, T(__builtin_huge_val()), gate);
-    load_steps<T, R>(ds, e.channels, t, e.time, T(0), grad);
-    load_steps<T, R>(xs, e.channels, t, e.time, T(0), x);
-    load_steps<T, R>(hs, e.channels, t - 1, e.time, before, h);
+    load_steps<STREAM && !SHARED>(gs, e.gates, t, e.time, T(__builtin_huge_val()), gate);
+    load_steps<STREAM>(ds, e.channels, t, e.time, T(0), grad);
+    load_steps<STREAM>(xs, e.channels, t, e.time, T(0), x);
+    load_steps<STREAM>(hs, e.channels, t - 1, e.time, before, h);
     if (RESETS) resets = load_resets<R>(rs, t, e.time);
   }
 
@@ -503,7 +504,7 @@ struct Backward {
 };
 
 // SHARED: gates that heads share.
-template <typename T, bool SHARED>
+template <typename T, bool SHARED, bool STREAM>
 struct BackwardColumns {
   const T *x, *gate, *h, *grad;
   const uint8_t* resets;
@@ -528,7 +529,12 @@ struct BackwardColumns {
 
   template <bool RESETS, int R>
   __device__ __forceinline__ void load(BackwardLoads<T, R>& to, const Extents& e, int64_t t) const {
-    to.template load<RESETS>(x, gate, h, grad, resets, before, e, t);
+    to.template load<RESETS, STREAM, SHARED>(x, gate, h, grad, resets, before, e, t);
+  }
+
+  __device__ __forceinline__ static void store(T* to, T v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+    else *to = v;
   }
 
   // The gradients of composed steps from t on; `shares`: LDS of this wave.
@@ -549,8 +555,8 @@ struct BackwardColumns {
       if (t >= 0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          out[i * e.channels] = now.x[i];
-          if (!SHARED) out_gate[i * e.gates] = now.h[i];
+          store(out + i * e.channels, now.x[i]);
+          if (!SHARED) store(out_gate + i * e.gates, now.h[i]);
         }
       } else {
 #pragma unroll
@@ -600,13 +606,13 @@ struct BackwardColumns {
 
 // Rows as in forward_kernel. Wave 0 takes the last R steps, wave 1 those before them:
 // a wave's first step is below zero at the start of the row.
-template <typename T, int R, int W, bool DOUBLE, bool RESETS, bool SHARED>
+template <typename T, int R, int W, bool DOUBLE, bool RESETS, bool SHARED, bool STREAM>
 __global__ __launch_bounds__(W * 64) void backward_kernel(Backward<T> f, Extents e) {
   __shared__ Left<T, W> left;
   __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];  // rows of a sum's lanes in banks of their own
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t group = by_die();
-  const BackwardColumns<T, SHARED> c(f, e, group, lane);
+  const BackwardColumns<T, SHARED, STREAM> c(f, e, group, lane);
   T carried = T(0);
   const int64_t t = e.time - int64_t(wave + 1) * R;
   BackwardLoads<T, R> loads[DOUBLE ? 2 : 1];
@@ -622,14 +628,14 @@ __global__ __launch_bounds__(W * 64) void backward_kernel(Backward<T> f, Extents
   if (c.dinitial && wave == 0 && c.valid) *c.dinitial = carried;
 }
 
-template <typename T, int R, int W, bool RESETS, bool SHARED>
+template <typename T, int R, int W, bool RESETS, bool SHARED, bool STREAM>
 __global__ __launch_bounds__(W * 64) void backward_chained_kernel(Backward<T> f, Extents e, Chain<T> chain) {
   __shared__ ChainLeft<T, W> left;
   __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = take_tile(chain.tickets, e);
   if (tile.number < 0) return;
-  const BackwardColumns<T, SHARED> c(f, e, tile.group, lane);
+  const BackwardColumns<T, SHARED, STREAM> c(f, e, tile.group, lane);
   const int64_t t = e.time - (tile.number * W + wave + 1) * R;
   BackwardLoads<T, R> now;
   c.template load<RESETS>(now, e, t);
@@ -742,7 +748,7 @@ void forward(hp_ctx* ctx, const Forward<T>& f, Extents e) {
   hp::check_launch("recurrence");
 }
 
-template <typename T, bool SHARED>
+template <typename T, bool SHARED, bool STREAM>
 void backward(hp_ctx* ctx, Backward<T> f, Extents e) {
   constexpr int R = Steps<T>::backward;
   hp::Scratch scratch(ctx);
@@ -753,13 +759,15 @@ void backward(hp_ctx* ctx, Backward<T> f, Extents e) {
   if (plan_chain(e, R)) {
     const unsigned grid = checked_grid(e.groups * e.tiles, 64 * kWaves);
     const Chain<T> chain = make_chain<T>(ctx, scratch, e);
-    const auto kernel = f.resets ? backward_chained_kernel<T, R, kWaves, true, SHARED> : backward_chained_kernel<T, R, kWaves, false, SHARED>;
+    const auto kernel = f.resets ? backward_chained_kernel<T, R, kWaves, true, SHARED, STREAM>
+                                 : backward_chained_kernel<T, R, kWaves, false, SHARED, STREAM>;
     kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
   } else {
     with_shape<R>(e.time, [&](auto steps, auto waves, auto twice) {
       constexpr int S = steps, W = waves;
       const unsigned grid = checked_grid(e.groups, 64 * W);
-      const auto kernel = f.resets ? backward_kernel<T, S, W, twice, true, SHARED> : backward_kernel<T, S, W, twice, false, SHARED>;
+      const auto kernel = f.resets ? backward_kernel<T, S, W, twice, true, SHARED, STREAM>
+                                   : backward_kernel<T, S, W, twice, false, SHARED, STREAM>;
       kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
     });
   }
@@ -808,8 +816,13 @@ int hp_gated_recurrence_grad(hp_ctx* ctx, int dtype, const void* grad, const voi
       const Backward<T> f{static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const T*>(gate),
                           static_cast<const T*>(h), static_cast<const T*>(initial), r, static_cast<T*>(dx),
                           static_cast<T*>(dgate), static_cast<T*>(dinitial)};
-      if (e.width > 1) backward<T, true>(ctx, f, e);
-      else backward<T, false>(ctx, f, e);
+      // Past the caches where steps are whole lines; else neighbouring groups meet in
+      // the lines that they share (float32, us: 8 x 4096 x 2048 274 against 292 through
+      // the caches, 2 x 8192 x 3001 298 against 255).
+      const bool stream = channels * int64_t(sizeof(T)) % 128 == 0;
+      const auto launch = e.width > 1 ? (stream ? backward<T, true, true> : backward<T, true, false>)
+                                      : (stream ? backward<T, false, true> : backward<T, false, false>);
+      launch(ctx, f, e);
     };
     if (dtype == HP_F32) run(float(0));
     else run(double(0));
