@@ -28,10 +28,15 @@
 // wait ends. A published word is valid by itself, without fences: memory is all
 // ones before, which no published value is. One workgroup that walks all tiles of
 // its channels with the next tile's loads in flight took 163 us forward and 327
-// backward for 8 x 4096 x 2048 float32 where chained tiles take 150 and 294 (5.4 and
-// 5.5 TB/s of 5.5 that reads and writes together reach here): its waves wait for
-// each other every tile. For 1 x 65536 x 1024, segments of time in two passes took
-// 278 and 448 us, chained tiles 174 and 331.
+// backward for 8 x 4096 x 2048 float32 where chained tiles took 150 and 294: its
+// waves wait for each other every tile. For 1 x 65536 x 1024, segments of time in two
+// passes took 278 and 448 us, chained tiles 174 and 331. Past the caches, as they are
+// now, tiles take 130 and 275 us, 6.2 and 5.9 TB/s, and 159 and 301.
+//
+// A head that has whole waves computes the sigmoid of a step once in the wave; its
+// gate's gradient is summed over the lanes through LDS. Rows that are no whole lines
+// cost most now: 65536 x 1000 in 8 heads of 125 channels, in waves of 63 and 62, takes
+// 321 us backward where 1024 channels take 242.
 //
 // Runs of 16 and 8 steps (forward, backward; half as many float64) fill 72 and 90
 // registers, so that three and two workgroups share a compute unit. Half as many
@@ -92,7 +97,7 @@ __device__ __forceinline__ Place head_place(const Extents& e, int64_t group, int
   const int slot = lane / e.piece, within = lane - slot * e.piece;
   const int64_t offset = (group % e.pieces) * e.piece + within;
   const bool valid = slot < e.pack && first + slot < e.heads && offset < e.width;
-  const int64_t head = valid ? first + slot : e.heads - 1;
+  const int64_t head = valid ? first + slot : first;
   const int64_t row = head / e.gates, gate = head - row * e.gates;
   return {row, gate * e.width + (valid ? offset : 0), gate, valid};
 }
@@ -329,31 +334,82 @@ __device__ __forceinline__ T through_chain(const Run<T>& run, ChainLeft<T, W>& l
 
 // ---- forward ---------------------------------------------------------------------
 
+// Where a lane's gates come from: kOwn: each channel has its own; kShared: heads
+// share them; kWave: one head has the whole wave.
+enum Gating { kOwn, kShared, kWave };
+
+// The gates of a run: raw ones, +inf (a step that keeps the state) outside [0, end),
+// which open() turns into sigmoids.
+template <typename T, int R, Gating G>
+struct Gates {
+  T v[R];
+
+  template <bool STREAM>
+  __device__ __forceinline__ void load(const T* gs, const Extents& e, int64_t t, int64_t end, int) {
+    load_steps<STREAM && G == kOwn>(gs, e.gates, t, end, T(__builtin_huge_val()), v);
+  }
+  __device__ __forceinline__ void open() {}
+  // a_i, once; then keep(i) has it and the result is 1 - a_i.
+  __device__ __forceinline__ T take(int i) {
+    T keep, take;
+    hpd::gates(v[i], keep, take);
+    v[i] = keep;
+    return take;
+  }
+  __device__ __forceinline__ T keep(int i) const { return v[i]; }
+};
+
+// Lane i has step i's: one load and one sigmoid a lane in place of R.
 template <typename T, int R>
+struct Gates<T, R, kWave> {
+  T own, taken;
+
+  template <bool STREAM>
+  __device__ __forceinline__ void load(const T* gs, const Extents& e, int64_t t, int64_t end, int lane) {
+    own = T(__builtin_huge_val());
+    if (lane < R && t + lane >= 0 && t + lane < end) own = gs[(t + lane) * e.gates];
+  }
+  __device__ __forceinline__ void open() {
+    const T raw = own;
+    hpd::gates(raw, own, taken);
+  }
+  __device__ __forceinline__ T take(int i) const { return of_lane(taken, i); }
+  __device__ __forceinline__ T keep(int i) const { return of_lane(own, i); }
+
+ private:
+  __device__ __forceinline__ static float of_lane(float v, int i) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));
+  }
+  __device__ __forceinline__ static double of_lane(double v, int i) {
+    const int64_t bits = __builtin_bit_cast(int64_t, v);
+    const uint32_t low = uint32_t(__builtin_amdgcn_readlane(int(bits), i)), high = uint32_t(__builtin_amdgcn_readlane(int(bits >> 32), i));
+    return __builtin_bit_cast(double, uint64_t(high) << 32 | low);
+  }
+};
+
+template <typename T, int R, Gating G>
 struct ForwardLoads {
-  T x[R], gate[R];
+  T x[R];
+  Gates<T, R, G> gates;
   unsigned resets = 0;
 
-  // Steps past the end keep the state: their gate is +inf.
   template <bool RESETS>
-  __device__ __forceinline__ void load(const T* xs, const T* gs, const uint8_t* rs, const Extents& e, int64_t t, int64_t end) {
-    load_steps<true>(xs, e.channels, t, end, T(0), x);
-    load_steps<true>(gs, e.gates, t, end, T(__builtin_huge_val()), gate);
-    if (RESETS) resets = load_resets<R>(rs, t, end);
+  __device__ __forceinline__ void load(const T* xs, const T* gs, const uint8_t* rs, const Extents& e, int64_t t, int lane) {
+    load_steps<true>(xs, e.channels, t, e.time, T(0), x);
+    gates.template load<true>(gs, e, t, e.time, lane);
+    if (RESETS) resets = load_resets<R>(rs, t, e.time);
   }
 
-  // x and gate become (1 - a) x and a; `run` goes on through the steps.
+  // x becomes (1 - a) x; `run` goes on through the steps.
   template <bool RESETS>
   __device__ __forceinline__ void compose(Run<T>& run) {
+    gates.open();
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      T keep, take;
-      hpd::gates(gate[i], keep, take);
-      gate[i] = keep;
-      x[i] *= take;
+      x[i] *= gates.take(i);
       const bool cut = RESETS && (resets >> i & 1);
-      run.b = (cut ? T(0) : keep * run.b) + x[i];
-      run.a *= keep;
+      run.b = (cut ? T(0) : gates.keep(i) * run.b) + x[i];
+      run.a *= gates.keep(i);
     }
     run.cut = run.cut || (RESETS && resets);
   }
@@ -368,7 +424,7 @@ struct Forward {
 };
 
 // A lane's columns of them.
-template <typename T>
+template <typename T, Gating G>
 struct ForwardColumns {
   const T *x, *gate;
   const uint8_t* resets;
@@ -376,7 +432,7 @@ struct ForwardColumns {
   bool valid;
 
   __device__ __forceinline__ ForwardColumns(const Forward<T>& f, const Extents& e, int64_t group, int lane) {
-    const Place at = flat_place(e, group, lane);
+    const Place at = G == kWave ? head_place(e, group, lane) : flat_place(e, group, lane);
     const int64_t column = at.row * e.time * e.channels + at.channel;
     x = f.x + column;
     h = f.h + column;
@@ -388,11 +444,11 @@ struct ForwardColumns {
 
   // The states of composed steps from t on.
   template <int R, bool RESETS>
-  __device__ __forceinline__ void finish(ForwardLoads<T, R>& now, const Extents& e, int64_t t, T value) const {
+  __device__ __forceinline__ void finish(ForwardLoads<T, R, G>& now, const Extents& e, int64_t t, T value) const {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const bool cut = RESETS && (now.resets >> i & 1);
-      now.x[i] = value = (cut ? T(0) : now.gate[i] * value) + now.x[i];
+      now.x[i] = value = (cut ? T(0) : now.gates.keep(i) * value) + now.x[i];
     }
     if (!valid) return;
     T* out = h + t * e.channels;
@@ -409,17 +465,17 @@ struct ForwardColumns {
 };
 
 // Rows of at most W x R steps, or of two times as many where DOUBLE.
-template <typename T, int R, int W, bool DOUBLE, bool RESETS>
+template <typename T, int R, int W, bool DOUBLE, bool RESETS, Gating G>
 __global__ __launch_bounds__(W * 64) void forward_kernel(Forward<T> f, Extents e) {
   __shared__ Left<T, W> left;
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const ForwardColumns<T> c(f, e, by_die(), lane);
+  const ForwardColumns<T, G> c(f, e, by_die(), lane);
   T state = c.first;
   constexpr int stride = W * R;
-  ForwardLoads<T, R> loads[DOUBLE ? 2 : 1];
+  ForwardLoads<T, R, G> loads[DOUBLE ? 2 : 1];
 #pragma unroll
   for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) {
-    loads[n].template load<RESETS>(c.x, c.gate, c.resets, e, n * stride + wave * R, e.time);
+    loads[n].template load<RESETS>(c.x, c.gate, c.resets, e, n * stride + wave * R, lane);
   }
 #pragma unroll
   for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) {
@@ -430,16 +486,16 @@ __global__ __launch_bounds__(W * 64) void forward_kernel(Forward<T> f, Extents e
   }
 }
 
-template <typename T, int R, int W, bool RESETS>
+template <typename T, int R, int W, bool RESETS, Gating G>
 __global__ __launch_bounds__(W * 64) void forward_chained_kernel(Forward<T> f, Extents e, Chain<T> chain) {
   __shared__ ChainLeft<T, W> left;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = take_tile(chain.tickets, e);
   if (tile.number < 0) return;
-  const ForwardColumns<T> c(f, e, tile.group, lane);
+  const ForwardColumns<T, G> c(f, e, tile.group, lane);
   const int64_t t = (tile.number * W + wave) * R;
-  ForwardLoads<T, R> now;
-  now.template load<RESETS>(c.x, c.gate, c.resets, e, t, e.time);
+  ForwardLoads<T, R, G> now;
+  now.template load<RESETS>(c.x, c.gate, c.resets, e, t, lane);
   Run<T> run{T(1), T(0), false};
   now.template compose<RESETS>(run);
   T after;
@@ -449,49 +505,38 @@ __global__ __launch_bounds__(W * 64) void forward_chained_kernel(Forward<T> f, E
 
 // ---- backward --------------------------------------------------------------------
 
-template <typename T, int R>
+template <typename T, int R, Gating G>
 struct BackwardLoads {
-  T x[R], gate[R], h[R], grad[R];
+  T x[R], h[R], grad[R];
+  Gates<T, R, G> gates;
   unsigned resets = 0;
 
   // Steps before the row pass the gradient on: their gate is +inf and their
   // gradient 0. h is that of the step before.
-  template <bool RESETS, bool STREAM, bool SHARED>
+  template <bool RESETS, bool STREAM>
   __device__ __forceinline__ void load(const T* xs, const T* gs, const T* hs, const T* ds, const uint8_t* rs, T before,
-                                       const Extents& e, int64_t t) {
-    load_steps<STREAM && !SHARED>(gs, e.gates, t, e.time, T(__builtin_huge_val()), gate);
+                                       const Extents& e, int64_t t, int lane) {
+    gates.template load<STREAM>(gs, e, t, e.time, lane);
     load_steps<STREAM>(ds, e.channels, t, e.time, T(0), grad);
     load_steps<STREAM>(xs, e.channels, t, e.time, T(0), x);
     load_steps<STREAM>(hs, e.channels, t - 1, e.time, before, h);
     if (RESETS) resets = load_resets<R>(rs, t, e.time);
   }
 
-  // gate becomes a, h - x (0 - x at a reset) stands in h and 1 - a in x; `run`
-  // goes on through the steps, from the last.
+  // h - x (0 - x at a reset) stands in h and 1 - a in x; `run` goes on through the
+  // steps, from the last.
   template <bool RESETS>
   __device__ __forceinline__ void compose(Run<T>& run) {
+    gates.open();
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
-      T keep, take;
-      hpd::gates(gate[i], keep, take);
-      gate[i] = keep;
       const bool cut = RESETS && (resets >> i & 1);
       h[i] = (cut ? T(0) : h[i]) - x[i];
-      x[i] = take;
-      run.b = cut ? T(0) : keep * (grad[i] + run.b);
-      run.a *= keep;
+      x[i] = gates.take(i);
+      run.b = cut ? T(0) : gates.keep(i) * (grad[i] + run.b);
+      run.a *= gates.keep(i);
     }
     run.cut = run.cut || (RESETS && resets);
-  }
-};
-
-// Lanes that share one of a wave's R x pack sums of gate gradients: a power of two.
-template <int R>
-struct SumLanes {
-  __device__ __forceinline__ static int of(int pack) {
-    int lanes = 1;
-    while (lanes * 2 * R * pack <= 64) lanes *= 2;
-    return lanes;
   }
 };
 
@@ -503,9 +548,9 @@ struct Backward {
   T *dx, *dgate, *dinitial;
 };
 
-// SHARED: gates that heads share.
-template <typename T, bool SHARED, bool STREAM>
+template <typename T, Gating G, bool STREAM>
 struct BackwardColumns {
+  static constexpr bool SHARED = G != kOwn;
   const T *x, *gate, *h, *grad;
   const uint8_t* resets;
   T *dx, *dgate, *dinitial, before;
@@ -528,8 +573,8 @@ struct BackwardColumns {
   }
 
   template <bool RESETS, int R>
-  __device__ __forceinline__ void load(BackwardLoads<T, R>& to, const Extents& e, int64_t t) const {
-    to.template load<RESETS, STREAM, SHARED>(x, gate, h, grad, resets, before, e, t);
+  __device__ __forceinline__ void load(BackwardLoads<T, R, G>& to, const Extents& e, int64_t t, int lane) const {
+    to.template load<RESETS, STREAM>(x, gate, h, grad, resets, before, e, t, lane);
   }
 
   __device__ __forceinline__ static void store(T* to, T v) {
@@ -539,14 +584,14 @@ struct BackwardColumns {
 
   // The gradients of composed steps from t on; `shares`: LDS of this wave.
   template <int R, bool RESETS>
-  __device__ __forceinline__ void finish(BackwardLoads<T, R>& now, const Extents& e, int64_t group, int64_t t, int lane,
+  __device__ __forceinline__ void finish(BackwardLoads<T, R, G>& now, const Extents& e, int64_t group, int64_t t, int lane,
                                          T (*shares)[65], T value) const {
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
       const bool cut = RESETS && (now.resets >> i & 1);
       const T slope = now.grad[i] + value;
-      value = cut ? T(0) : now.gate[i] * slope;
-      now.h[i] = slope * now.h[i] * (now.gate[i] * now.x[i]);
+      value = cut ? T(0) : now.gates.keep(i) * slope;
+      now.h[i] = slope * now.h[i] * (now.gates.keep(i) * now.x[i]);
       now.x[i] = slope * now.x[i];
     }
     T* out = dx + t * e.channels;
@@ -573,7 +618,7 @@ struct BackwardColumns {
 
   // One sum for each step and head of the wave, by neighbouring lanes.
   template <int R>
-  __device__ __forceinline__ void add_shares(const BackwardLoads<T, R>& now, const Extents& e, int64_t group, int64_t t,
+  __device__ __forceinline__ void add_shares(const BackwardLoads<T, R, G>& now, const Extents& e, int64_t group, int64_t t,
                                              int lane, T (*shares)[65]) const {
     // The wave's own rows of LDS: its stores are in order before its loads.
 #pragma unroll
@@ -606,18 +651,19 @@ struct BackwardColumns {
 
 // Rows as in forward_kernel. Wave 0 takes the last R steps, wave 1 those before them:
 // a wave's first step is below zero at the start of the row.
-template <typename T, int R, int W, bool DOUBLE, bool RESETS, bool SHARED, bool STREAM>
+template <typename T, int R, int W, bool DOUBLE, bool RESETS, Gating G, bool STREAM>
 __global__ __launch_bounds__(W * 64) void backward_kernel(Backward<T> f, Extents e) {
   __shared__ Left<T, W> left;
+  constexpr bool SHARED = G != kOwn;
   __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];  // rows of a sum's lanes in banks of their own
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t group = by_die();
-  const BackwardColumns<T, SHARED, STREAM> c(f, e, group, lane);
+  const BackwardColumns<T, G, STREAM> c(f, e, group, lane);
   T carried = T(0);
   const int64_t t = e.time - int64_t(wave + 1) * R;
-  BackwardLoads<T, R> loads[DOUBLE ? 2 : 1];
+  BackwardLoads<T, R, G> loads[DOUBLE ? 2 : 1];
 #pragma unroll
-  for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) c.template load<RESETS>(loads[n], e, t - n * W * R);
+  for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) c.template load<RESETS>(loads[n], e, t - n * W * R, lane);
 #pragma unroll
   for (int n = 0; n < (DOUBLE ? 2 : 1); ++n) {
     Run<T> run{T(1), T(0), false};
@@ -628,17 +674,18 @@ __global__ __launch_bounds__(W * 64) void backward_kernel(Backward<T> f, Extents
   if (c.dinitial && wave == 0 && c.valid) *c.dinitial = carried;
 }
 
-template <typename T, int R, int W, bool RESETS, bool SHARED, bool STREAM>
+template <typename T, int R, int W, bool RESETS, Gating G, bool STREAM>
 __global__ __launch_bounds__(W * 64) void backward_chained_kernel(Backward<T> f, Extents e, Chain<T> chain) {
   __shared__ ChainLeft<T, W> left;
+  constexpr bool SHARED = G != kOwn;
   __shared__ T shares[SHARED ? W : 1][SHARED ? R : 1][65];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = take_tile(chain.tickets, e);
   if (tile.number < 0) return;
-  const BackwardColumns<T, SHARED, STREAM> c(f, e, tile.group, lane);
+  const BackwardColumns<T, G, STREAM> c(f, e, tile.group, lane);
   const int64_t t = e.time - (tile.number * W + wave + 1) * R;
-  BackwardLoads<T, R> now;
-  c.template load<RESETS>(now, e, t);
+  BackwardLoads<T, R, G> now;
+  c.template load<RESETS>(now, e, t, lane);
   Run<T> run{T(1), T(0), false};
   now.template compose<RESETS>(run);
   T after;
@@ -727,47 +774,46 @@ Chain<T> make_chain(hp_ctx* ctx, hp::Scratch& scratch, const Extents& e) {
   return {reinterpret_cast<unsigned*>(memory), reinterpret_cast<Bits*>(memory + tickets), reinterpret_cast<Bits*>(memory + tickets + runs)};
 }
 
-template <typename T>
+template <typename T, Gating G>
 void forward(hp_ctx* ctx, const Forward<T>& f, Extents e) {
   constexpr int R = Steps<T>::forward;
   hp::Scratch scratch(ctx);
-  e.groups = hp::ceil_div(e.total, 64);
+  e.groups = G == kWave ? e.heads * e.pieces : hp::ceil_div(e.total, 64);
   if (plan_chain(e, R)) {
     const unsigned grid = checked_grid(e.groups * e.tiles, 64 * kWaves);
     const Chain<T> chain = make_chain<T>(ctx, scratch, e);
-    const auto kernel = f.resets ? forward_chained_kernel<T, R, kWaves, true> : forward_chained_kernel<T, R, kWaves, false>;
+    const auto kernel = f.resets ? forward_chained_kernel<T, R, kWaves, true, G> : forward_chained_kernel<T, R, kWaves, false, G>;
     kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
   } else {
     with_shape<R>(e.time, [&](auto steps, auto waves, auto twice) {
       constexpr int S = steps, W = waves;
       const unsigned grid = checked_grid(e.groups, 64 * W);
-      const auto kernel = f.resets ? forward_kernel<T, S, W, twice, true> : forward_kernel<T, S, W, twice, false>;
+      const auto kernel = f.resets ? forward_kernel<T, S, W, twice, true, G> : forward_kernel<T, S, W, twice, false, G>;
       kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
     });
   }
   hp::check_launch("recurrence");
 }
 
-template <typename T, bool SHARED, bool STREAM>
+template <typename T, Gating G, bool STREAM>
 void backward(hp_ctx* ctx, Backward<T> f, Extents e) {
   constexpr int R = Steps<T>::backward;
   hp::Scratch scratch(ctx);
-  e.groups = SHARED ? hp::ceil_div(e.heads, e.pack) * e.pieces : hp::ceil_div(e.total, 64);
+  e.groups = G == kOwn ? hp::ceil_div(e.total, 64) : hp::ceil_div(e.heads, e.pack) * e.pieces;
   T* const dgate = f.dgate;
   const int64_t count = e.heads * e.time;
   if (e.pieces > 1) f.dgate = scratch.take<T>(e.pieces * count);
   if (plan_chain(e, R)) {
     const unsigned grid = checked_grid(e.groups * e.tiles, 64 * kWaves);
     const Chain<T> chain = make_chain<T>(ctx, scratch, e);
-    const auto kernel = f.resets ? backward_chained_kernel<T, R, kWaves, true, SHARED, STREAM>
-                                 : backward_chained_kernel<T, R, kWaves, false, SHARED, STREAM>;
+    const auto kernel = f.resets ? backward_chained_kernel<T, R, kWaves, true, G, STREAM>
+                                 : backward_chained_kernel<T, R, kWaves, false, G, STREAM>;
     kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
   } else {
     with_shape<R>(e.time, [&](auto steps, auto waves, auto twice) {
       constexpr int S = steps, W = waves;
       const unsigned grid = checked_grid(e.groups, 64 * W);
-      const auto kernel = f.resets ? backward_kernel<T, S, W, twice, true, SHARED, STREAM>
-                                   : backward_kernel<T, S, W, twice, false, SHARED, STREAM>;
+      const auto kernel = f.resets ? backward_kernel<T, S, W, twice, true, G, STREAM> : backward_kernel<T, S, W, twice, false, G, STREAM>;
       kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
     });
   }
@@ -794,7 +840,13 @@ int hp_gated_recurrence(hp_ctx* ctx, int dtype, const void* x, const void* gate,
     const auto r = static_cast<const uint8_t*>(resets);
     const auto run = [&](auto zero) {
       using T = decltype(zero);
-      forward<T>(ctx, {static_cast<const T*>(x), static_cast<const T*>(gate), static_cast<const T*>(initial), r, static_cast<T*>(h)}, e);
+      const Forward<T> f{static_cast<const T*>(x), static_cast<const T*>(gate), static_cast<const T*>(initial), r, static_cast<T*>(h)};
+      // Heads of whole waves are laid out by waves, for one sigmoid a step (65536 x 1024
+      // float32 in 8 heads: 125 us, 131 with a sigmoid a lane; 65536 x 1000 in 8 heads,
+      // waves of 63: 157 and 148).
+      if (e.width == 1) forward<T, kOwn>(ctx, f, e);
+      else if (e.pack == 1 && e.piece == 64) forward<T, kWave>(ctx, f, e);
+      else forward<T, kShared>(ctx, f, e);
     };
     if (dtype == HP_F32) run(float(0));
     else run(double(0));
@@ -820,8 +872,9 @@ int hp_gated_recurrence_grad(hp_ctx* ctx, int dtype, const void* grad, const voi
       // the lines that they share (float32, us: 8 x 4096 x 2048 274 against 292 through
       // the caches, 2 x 8192 x 3001 298 against 255).
       const bool stream = channels * int64_t(sizeof(T)) % 128 == 0;
-      const auto launch = e.width > 1 ? (stream ? backward<T, true, true> : backward<T, true, false>)
-                                      : (stream ? backward<T, false, true> : backward<T, false, false>);
+      const auto launch = e.width == 1  ? (stream ? backward<T, kOwn, true> : backward<T, kOwn, false>)
+                          : e.pack == 1 ? (stream ? backward<T, kWave, true> : backward<T, kWave, false>)
+                                        : (stream ? backward<T, kShared, true> : backward<T, kShared, false>);
       launch(ctx, f, e);
     };
     if (dtype == HP_F32) run(float(0));
