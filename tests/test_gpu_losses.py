@@ -33,6 +33,34 @@ def test_policy_loss_of_many_rows(hip, rows, vocab, dtype):
     check_policy(hip, rows, vocab, dtype, seed=5)
 
 
+# Rows of which a team holds several at a time, and groups of them that the last rows do not fill.
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("rows,vocab", [(257, 1), (1000, 12), (511, 30), (2049, 60), (97, 100), (1003, 200), (338, 254), (85, 400), (41, 512)])
+def test_policy_loss_of_short_rows(hip, rows, vocab, dtype):
+    print(rows, vocab, dtype, flush=True)
+    check_policy(hip, rows, vocab, dtype, seed=rows)
+
+
+def test_more_short_rows_than_one_launch_has_teams(hip):
+    rows, vocab = 16384 * 16 + 37, 130
+    rng = np.random.default_rng(8)
+    z = p.random.default_rng(8, backend=hip).normal(0, 1, (rows, vocab), dtype=np.float32)
+    targets = rng.integers(0, vocab, rows)
+    mask = rng.random(rows) < 0.7
+    wide = p.asnumpy(z).astype(np.float64)
+    share = np.exp(wide)
+    share /= share.sum(1, keepdims=True)
+    at = np.arange(rows)
+    logs = np.where(mask, np.log(share[at, targets]), 0)
+    # An exponential, a sum of 130 and a logarithm: some 1e-6 of values up to 10.
+    np.testing.assert_allclose(p.asnumpy(p.nn.token_log_probs(z, targets, mask=mask)), logs, rtol=1e-6, atol=2e-6)
+    _, found, grad = p.nn.policy_loss_grad(z, targets, logs.astype(np.float32), np.ones(rows, np.float32), mask=mask, count=1.0)
+    np.testing.assert_allclose(p.asnumpy(found), logs, rtol=1e-6, atol=2e-6)
+    want = share * mask[:, None]
+    want[at, targets] -= mask
+    np.testing.assert_allclose(p.asnumpy(grad), want, rtol=2e-5, atol=1e-6)
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 @pytest.mark.parametrize("pairs,time,vocab", [(1, 1, 3), (3, 5, 7), (2, 300, 18), (5, 9, 1025), (2, 7, 9001), (1, 3, 70001), (40, 11, 2050)])
 def test_preference_loss(hip, pairs, time, vocab, dtype):
