@@ -101,13 +101,11 @@ struct Call {
   __device__ int64_t target(int64_t row) const {
     return wide_targets ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
   }
-  // The log-probability of the row's target, NaN outside the vocabulary. From
-  // here on a token's terms are differences in 64 bits: float32 would lose
-  // digits of the ratio and of a pair's margin.
-  __device__ double log_prob(int64_t row, int64_t y, T top, T total) const {
-    const T at = y >= 0 && y < vocab ? logits[row * vocab + y] : T(__builtin_nan(""));
-    return (double(at) - double(top)) - log_wide(total);
-  }
+  // NaN outside the vocabulary.
+  __device__ T logit(int64_t row, int64_t y) const { return y >= 0 && y < vocab ? logits[row * vocab + y] : T(__builtin_nan("")); }
+  // The log-probability of a target. From here on a token's terms are differences in
+  // 64 bits: float32 would lose digits of the ratio and of a pair's margin.
+  __device__ double log_prob(T logit, T top, T total) const { return (double(logit) - double(top)) - log_wide(total); }
   __device__ void keep(int64_t row, double value, T top, T total) const {
     log_probs[row] = T(value);
     if (exact) exact[row] = value;
@@ -123,12 +121,26 @@ struct Call {
   }
 };
 
+// What a row's token brings to the policy loss. Short rows read it and the target's
+// logit before their own logits (2^20 x 18: 54 us, after the statistics 59), others
+// where they need it: all else would wait for the target (8192 x 32000: 380 us, 355 so).
+template <typename T>
+struct Token {
+  T old = T(0), advantage = T(0), reference = T(0);
+
+  __device__ __forceinline__ void read(const Call<T>& c, int64_t row) {
+    old = c.old[row];
+    advantage = c.advantage(row);
+    if (c.reference) reference = c.reference[row];
+  }
+};
+
 // The policy loss of a token and its derivative by the log-probability.
 // expm1 keeps the KL term's digits where the two policies nearly agree.
 template <typename T>
-__device__ __forceinline__ void policy_token(const Call<T>& c, int64_t row, double log_prob, double& loss, double& slope) {
-  const double advantage = c.advantage(row);
-  const double ratio = exp_difference(T(0), log_prob - double(c.old[row]));
+__device__ __forceinline__ void policy_token(const Call<T>& c, const Token<T>& token, double log_prob, double& loss, double& slope) {
+  const double advantage = token.advantage;
+  const double ratio = exp_difference(T(0), log_prob - double(token.old));
   const double free = ratio * advantage;
   // Not fmin/fmax: a NaN ratio stays NaN.
   const double within = ratio < c.low ? c.low : ratio > c.high ? c.high : ratio;
@@ -137,7 +149,7 @@ __device__ __forceinline__ void policy_token(const Call<T>& c, int64_t row, doub
   loss = -(stopped ? held : free);
   slope = stopped ? 0.0 : -free;
   if (c.reference) {
-    const double apart = double(c.reference[row]) - log_prob;
+    const double apart = double(token.reference) - log_prob;
     const double grown = expm1_difference(T(0), apart);
     loss += c.kl * (grown - apart);
     slope -= c.kl * grown;
@@ -150,6 +162,13 @@ __device__ __forceinline__ T team_reduce(T v, Op op) {
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
   return v;
+}
+
+// A value that all lanes have, in scalar registers.
+__device__ __forceinline__ double of_wave(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t low = __builtin_amdgcn_readfirstlane(int(bits)), high = __builtin_amdgcn_readfirstlane(int(bits >> 32));
+  return __builtin_bit_cast(double, uint64_t(high) << 32 | low);
 }
 
 // (m, S) of a row from those of pieces in the lanes that have one.
@@ -420,7 +439,7 @@ __device__ __forceinline__ void leave_loss(const Call<T>& c, double sum, double 
 // At 16 vectors a lane, four waves per SIMD (128 registers) keep a second
 // workgroup's loads in flight while one waits at its barriers.
 template <typename T, int L, int K, bool LOSS>
-__global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? (L > 256 ? 4 : 3) : 1) void row_kernel(Call<T> c) {
+__global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L == 256 && K == 16 ? 3 : 4) void row_kernel(Call<T> c) {
   constexpr int kTeams = L > 256 ? 1 : 256 / L;
   using S = Share<T, L, K>;
   __shared__ Meet<T, S::kDeep> meet;
@@ -447,11 +466,13 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? (L >
     T tops[S::kDeep], top, total;
     share.statistics(length, lane, meet, turn, tops, top, total);
     turn ^= 1;
-    const double log_prob = c.log_prob(row, y, top, total);
+    const double log_prob = c.log_prob(c.logit(row, y), top, total);
     if (lane == 0) c.keep(row, log_prob, top, total);
     if constexpr (LOSS) {
+      Token<T> token;
+      token.read(c, row);
       double loss, slope;
-      policy_token(c, row, log_prob, loss, slope);
+      policy_token(c, token, log_prob, loss, slope);
       if (lane == 0) sum += loss;
       if (!out) continue;
       const T w = T(slope * factor), scale = -w * (T(1) / total);
@@ -466,22 +487,33 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 4 && K == 16 ? (L >
 // Rows that a team of L <= 64 lanes holds in K <= 2 vectors a lane (4 of doubles), B of
 // them at a time: more loads in flight, and lane b forms the terms of the token of row b,
 // so that a wave forms those of all its rows at once where every lane of a team would
-// form them again for each row. 2^20 x 18 with the gradient: 59 us, one row at a time
-// 85, two 72; 2^16 x 256: 42 and 56. With K = 4 the registers of a second row of
+// form them again for each row. 2^20 x 18 with the gradient: 54 us, one row at a time
+// 85; 2^18 x 200: 104 and 155. With K = 4 the registers of a second row of
 // floats cost more waves than its loads gain: 2^16 x 1000 takes 102 us so and 96 in
 // row_kernel; of doubles, whose terms weigh more, 2^16 x 400 takes 125 and 139.
 // LOSS: as for row_kernel.
 template <typename T, int L, int K, int B, bool LOSS>
-__global__ __launch_bounds__(256) void short_row_kernel(Call<T> c) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 4 : 1) void short_row_kernel(Call<T> c) {
   static_assert(B <= L && L <= 64, "a lane for each row of a team");
   constexpr int kTeams = 256 / L;
   using S = Share<T, L, K>;
   const int lane = threadIdx.x % L, team = threadIdx.x / L, first_lane = (threadIdx.x & 63) - lane;
   const int length = int(c.vocab);
-  const double factor = LOSS ? scale_of(c) : 1.0;
+  const double factor = LOSS ? of_wave(scale_of(c)) : 1.0;
   double sum = 0;
   __shared__ Meet<T, S::kDeep> meet;  // teams within a wave leave it alone
   for (int64_t base = int64_t(blockIdx.x) * (kTeams * B) + team; base < c.rows; base += int64_t(gridDim.x) * (kTeams * B)) {
+    const int64_t own = base + lane * kTeams;
+    const bool has = lane < B && own < c.rows, keeps = has && c.kept(own);
+    Token<T> token;
+    T logit = T(0);
+    int at = -1;
+    if (keeps) {
+      const int64_t y = c.target(own);
+      if (y >= 0 && y < c.vocab) at = int(y);
+      logit = c.logit(own, y);
+      if constexpr (LOSS) token.read(c, own);
+    }
     S share[B];
 #pragma unroll
     for (int b = 0; b < B; ++b) {
@@ -497,24 +529,18 @@ __global__ __launch_bounds__(256) void short_row_kernel(Call<T> c) {
       if (lane == b) top = row_top, total = row_total;
     }
     T w = T(0), scale = T(0);
-    int at = -1;
-    const int64_t own = base + lane * kTeams;
-    if (lane < B && own < c.rows) {
-      if (c.kept(own)) {
-        const int64_t y = c.target(own);
-        const double log_prob = c.log_prob(own, y, top, total);
-        c.keep(own, log_prob, top, total);
-        if constexpr (LOSS) {
-          double loss, slope;
-          policy_token(c, own, log_prob, loss, slope);
-          sum += loss;
-          w = T(slope * factor);
-          scale = -w * (T(1) / total);
-          at = y >= 0 && y < c.vocab ? int(y) : -1;
-        }
-      } else {
-        c.leave_out(own);
+    if (keeps) {
+      const double log_prob = c.log_prob(logit, top, total);
+      c.keep(own, log_prob, top, total);
+      if constexpr (LOSS) {
+        double loss, slope;
+        policy_token(c, token, log_prob, loss, slope);
+        sum += loss;
+        w = T(slope * factor);
+        scale = -w * (T(1) / total);
       }
+    } else if (has) {
+      c.leave_out(own);
     }
     if (!LOSS || !c.grad) continue;
 #pragma unroll
@@ -563,10 +589,14 @@ __global__ __launch_bounds__(kPieceThreads) void finish_kernel(Call<T> c, const 
   if (c.kept(row)) {
     T top, total;
     join_pieces(part_tops + row * pieces, part_totals + row * pieces, pieces, top, total);
-    const double log_prob = c.log_prob(row, c.target(row), top, total);
+    const double log_prob = c.log_prob(c.logit(row, c.target(row)), top, total);
     if (threadIdx.x == 0) c.keep(row, log_prob, top, total);
-    double slope;
-    if (c.old) policy_token(c, row, log_prob, loss, slope);
+    if (c.old) {
+      Token<T> token;
+      token.read(c, row);
+      double slope;
+      policy_token(c, token, log_prob, loss, slope);
+    }
   } else if (threadIdx.x == 0) {
     c.leave_out(row);
   }
@@ -616,10 +646,12 @@ __global__ __launch_bounds__(kPieceThreads) void policy_grad_kernel(Call<T> c, c
       T top, total;
       join_pieces(part_tops + row * pieces, part_totals + row * pieces, pieces, top, total);
       const int64_t y = c.target(row);
-      const double log_prob = c.log_prob(row, y, top, total);
+      const double log_prob = c.log_prob(c.logit(row, y), top, total);
       if (first && lane == 0) c.keep(row, log_prob, top, total);
+      Token<T> token;
+      token.read(c, row);
       double slope;
-      policy_token(c, row, log_prob, loss, slope);
+      policy_token(c, token, log_prob, loss, slope);
       const int at = y >= start && y < start + length ? int(y - start) : -1;
       const T w = T(slope * factor), scale = -w * (T(1) / total);
       share.each(length, lane, [&](T& v, int i, int) { v = hpd::exp_down(v - top) * scale + (i == at ? w : T(0)); });
@@ -770,8 +802,8 @@ int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   unsigned blocks = 0;
   if (teams_serve(c) && with_team<T>(c.vocab, [&](auto l, auto k) {
         constexpr int L = l, K = k, threads = L > 256 ? L : 256;
-        constexpr int wide = sizeof(T) == 8 ? 4 : 2;  // short_row_kernel
-        constexpr int B = L > 64 || K > wide ? 1 : K == 4 ? 2 : 4 / K;
+        constexpr int several = sizeof(T) == 8 ? 4 : 2;  // short_row_kernel
+        constexpr int B = L > 64 || K > several ? 1 : K == 4 ? 2 : 4 / K;
         constexpr bool both = L * K <= kPieceThreads * kPieceLoads;  // teams_serve()
         blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, threads / L * B), 16384));
         if (c.old) plan_losses(ctx, scratch, c, blocks, blocks);
