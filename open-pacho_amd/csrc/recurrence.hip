@@ -31,12 +31,15 @@
 // backward for 8 x 4096 x 2048 float32 where chained tiles took 150 and 294: its
 // waves wait for each other every tile. For 1 x 65536 x 1024, segments of time in two
 // passes took 278 and 448 us, chained tiles 174 and 331. Past the caches, as they are
-// now, tiles take 130 and 275 us, 6.2 and 5.9 TB/s, and 159 and 301.
+// now, tiles take 130 and 275 us, 6.2 and 5.9 TB/s, and 154 and 301.
 //
 // A head that has whole waves computes the sigmoid of a step once in the wave; its
 // gate's gradient is summed over the lanes through LDS. Rows that are no whole lines
 // cost most now: 65536 x 1000 in 8 heads of 125 channels, in waves of 63 and 62, takes
-// 321 us backward where 1024 channels take 242.
+// 308 us backward where 1024 channels take 237. Its dies read 1.29 times the arrays,
+// 1024 channels 1.04: each die has a head, whose lines the next one shares at both
+// ends in every step. Accesses past the caches make that worse (360 us), and tiles of
+// other dies' time would wait for workgroups that need not have started.
 //
 // Runs of 16 and 8 steps (forward, backward; half as many float64) fill 72 and 90
 // registers, so that three and two workgroups share a compute unit. Half as many
@@ -757,7 +760,10 @@ void with_shape(int64_t time, F&& f) {
 bool plan_chain(Extents& e, int steps) {
   e.tiles = hp::ceil_div(e.time, int64_t(kWaves) * steps);
   if (e.tiles < 3) return false;
-  e.span = e.groups >= 16 ? 16 : 64;
+  // Few groups are long in waiting from block to block: 65536 x 1000 in 8 heads, 16
+  // groups, takes 308 us backward in blocks of 64 and 321 of 16; with 256 groups,
+  // 8 x 4096 x 2048, the readings of a block's tiles weigh more, 281 and 274.
+  e.span = e.groups >= 32 ? 16 : 64;
   return true;
 }
 
