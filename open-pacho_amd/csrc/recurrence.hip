@@ -31,7 +31,7 @@
 // backward for 8 x 4096 x 2048 float32 where chained tiles took 150 and 294: its
 // waves wait for each other every tile. For 1 x 65536 x 1024, segments of time in two
 // passes took 278 and 448 us, chained tiles 174 and 331. Past the caches, as they are
-// now, tiles take 130 and 275 us, 6.2 and 5.9 TB/s, and 154 and 301.
+// now, tiles take 141 and 275 us, 5.7 and 5.9 TB/s, and 156 and 301.
 //
 // A head that has whole waves computes the sigmoid of a step once in the wave; its
 // gate's gradient is summed over the lanes through LDS. Rows that are no whole lines
@@ -426,8 +426,8 @@ struct Forward {
   T* h;
 };
 
-// A lane's columns of them.
-template <typename T, Gating G>
+// A lane's columns of them. STREAM: states are stored past the caches.
+template <typename T, Gating G, bool STREAM>
 struct ForwardColumns {
   const T *x, *gate;
   const uint8_t* resets;
@@ -457,7 +457,10 @@ struct ForwardColumns {
     T* out = h + t * e.channels;
     if (t + R <= e.time) {
 #pragma unroll
-      for (int i = 0; i < R; ++i) out[i * e.channels] = now.x[i];
+      for (int i = 0; i < R; ++i) {
+        if constexpr (STREAM) __builtin_nontemporal_store(now.x[i], out + i * e.channels);
+        else out[i * e.channels] = now.x[i];
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < R; ++i) {
@@ -468,11 +471,11 @@ struct ForwardColumns {
 };
 
 // Rows of at most W x R steps, or of two times as many where DOUBLE.
-template <typename T, int R, int W, bool DOUBLE, bool RESETS, Gating G>
+template <typename T, int R, int W, bool DOUBLE, bool RESETS, Gating G, bool STREAM>
 __global__ __launch_bounds__(W * 64) void forward_kernel(Forward<T> f, Extents e) {
   __shared__ Left<T, W> left;
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const ForwardColumns<T, G> c(f, e, by_die(), lane);
+  const ForwardColumns<T, G, STREAM> c(f, e, by_die(), lane);
   T state = c.first;
   constexpr int stride = W * R;
   ForwardLoads<T, R, G> loads[DOUBLE ? 2 : 1];
@@ -489,13 +492,13 @@ __global__ __launch_bounds__(W * 64) void forward_kernel(Forward<T> f, Extents e
   }
 }
 
-template <typename T, int R, int W, bool RESETS, Gating G>
+template <typename T, int R, int W, bool RESETS, Gating G, bool STREAM>
 __global__ __launch_bounds__(W * 64) void forward_chained_kernel(Forward<T> f, Extents e, Chain<T> chain) {
   __shared__ ChainLeft<T, W> left;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = take_tile(chain.tickets, e);
   if (tile.number < 0) return;
-  const ForwardColumns<T, G> c(f, e, tile.group, lane);
+  const ForwardColumns<T, G, STREAM> c(f, e, tile.group, lane);
   const int64_t t = (tile.number * W + wave) * R;
   ForwardLoads<T, R, G> now;
   now.template load<RESETS>(c.x, c.gate, c.resets, e, t, lane);
@@ -780,7 +783,7 @@ Chain<T> make_chain(hp_ctx* ctx, hp::Scratch& scratch, const Extents& e) {
   return {reinterpret_cast<unsigned*>(memory), reinterpret_cast<Bits*>(memory + tickets), reinterpret_cast<Bits*>(memory + tickets + runs)};
 }
 
-template <typename T, Gating G>
+template <typename T, Gating G, bool STREAM>
 void forward(hp_ctx* ctx, const Forward<T>& f, Extents e) {
   constexpr int R = Steps<T>::forward;
   hp::Scratch scratch(ctx);
@@ -788,13 +791,14 @@ void forward(hp_ctx* ctx, const Forward<T>& f, Extents e) {
   if (plan_chain(e, R)) {
     const unsigned grid = checked_grid(e.groups * e.tiles, 64 * kWaves);
     const Chain<T> chain = make_chain<T>(ctx, scratch, e);
-    const auto kernel = f.resets ? forward_chained_kernel<T, R, kWaves, true, G> : forward_chained_kernel<T, R, kWaves, false, G>;
+    const auto kernel = f.resets ? forward_chained_kernel<T, R, kWaves, true, G, STREAM>
+                                 : forward_chained_kernel<T, R, kWaves, false, G, STREAM>;
     kernel<<<grid, 64 * kWaves, 0, ctx->stream>>>(f, e, chain);
   } else {
     with_shape<R>(e.time, [&](auto steps, auto waves, auto twice) {
       constexpr int S = steps, W = waves;
       const unsigned grid = checked_grid(e.groups, 64 * W);
-      const auto kernel = f.resets ? forward_kernel<T, S, W, twice, true, G> : forward_kernel<T, S, W, twice, false, G>;
+      const auto kernel = f.resets ? forward_kernel<T, S, W, twice, true, G, STREAM> : forward_kernel<T, S, W, twice, false, G, STREAM>;
       kernel<<<grid, 64 * W, 0, ctx->stream>>>(f, e);
     });
   }
@@ -850,9 +854,15 @@ int hp_gated_recurrence(hp_ctx* ctx, int dtype, const void* x, const void* gate,
       // Heads of whole waves are laid out by waves, for one sigmoid a step (65536 x 1024
       // float32 in 8 heads: 125 us, 131 with a sigmoid a lane; 65536 x 1000 in 8 heads,
       // waves of 63: 157 and 148).
-      if (e.width == 1) forward<T, kOwn>(ctx, f, e);
-      else if (e.pack == 1 && e.piece == 64) forward<T, kWave>(ctx, f, e);
-      else forward<T, kShared>(ctx, f, e);
+      // States are stored past the caches where steps are whole lines and all of them are
+      // more than the last cache holds (16 x 4096 x 2048 float32: 259 us, 280 through it);
+      // fewer are left there for their reader (64 x 256 x 2048 into one block again and
+      // again: 76 us past the caches, 70).
+      const bool stream = channels * int64_t(sizeof(T)) % 128 == 0 && double(e.total) * double(time) * sizeof(T) > 256e6;
+      const auto launch = e.width == 1                      ? (stream ? forward<T, kOwn, true> : forward<T, kOwn, false>)
+                          : e.pack == 1 && e.piece == 64    ? (stream ? forward<T, kWave, true> : forward<T, kWave, false>)
+                                                            : (stream ? forward<T, kShared, true> : forward<T, kShared, false>);
+      launch(ctx, f, e);
     };
     if (dtype == HP_F32) run(float(0));
     else run(double(0));

@@ -31,8 +31,9 @@ def test_values_and_gradients(hip, sizes, state, resets, dtype):
     check(hip, sizes, dtype, state, resets)
 
 
-# Several blocks of tiles, of 16 (from 16 groups of channels on) and of 64.
-@pytest.mark.parametrize("sizes", [(1, 20000, 5, 5), (1, 5001, 130, 2), (2, 4099, 65, 65), (1, 2100, 1030, 1030), (3, 2049, 400, 4)])
+# Several blocks of tiles, of 16 (from 32 groups of channels on) and of 64.
+@pytest.mark.parametrize("sizes", [(1, 20000, 5, 5), (1, 5001, 130, 2), (2, 4099, 65, 65), (1, 2100, 1030, 1030), (3, 2049, 400, 4),
+                                   (2, 2100, 1030, 1030), (1, 2200, 2050, 1)])  # fmt: skip
 def test_long_rows(hip, sizes):
     print(sizes, flush=True)
     check(hip, sizes, np.float32, True, True)
@@ -78,6 +79,21 @@ def test_gates_at_their_ends(hip, dtype):
     with np.errstate(over="ignore"):
         want = training.sigmoid(-gate.astype(training.WIDE))
     near(dx, want, want, dtype)
+
+
+@pytest.mark.parametrize("sizes,dtype", [((9, 4100, 2048, 2048), np.float32), ((9, 4100, 2048, 4), np.float32), ((9, 4100, 2048, 256), np.float32),
+                                         ((4100, 20, 1024, 1024), np.float32), ((9, 2100, 2048, 2048), np.float64)])  # fmt: skip
+def test_more_states_than_the_last_cache_holds(hip, sizes, dtype):
+    # They are stored past it; fewer rows of the same are not, and have the same bits.
+    print(sizes, dtype, flush=True)
+    rows, time, channels, gates = sizes
+    rng = p.random.default_rng(1, backend=hip)
+    x, gate = rng.normal(0, 1, (rows, time, channels), dtype=dtype), rng.normal(2, 1, (rows, time, gates), dtype=dtype)
+    resets = np.random.default_rng(1).random((rows, time)) < 0.01
+    h = p.nn.gated_recurrence(x, gate, resets=resets)
+    for part in (slice(0, 2), slice(rows - 2, rows)):
+        fewer = p.nn.gated_recurrence(x[part], gate[part], resets=resets[part])
+        np.testing.assert_array_equal(p.asnumpy(h[part]), p.asnumpy(fewer))
 
 
 def test_repeated_calls_give_the_same_bits(hip):
