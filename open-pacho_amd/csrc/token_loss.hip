@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kPieceThreads = 256, kPieceLoads = 8;
 constexpr int64_t kFewPieces = 1024;
-constexpr int64_t kCountedBytes = int64_t(1) << 25;
+constexpr double kCountedBytes = 1 << 25;
 
 // Elements of a piece, of which the last one of a row may have fewer.
 __device__ __forceinline__ int piece_end(int64_t left, int piece) { return left < piece ? int(left) : piece; }
@@ -781,13 +781,16 @@ void final_loss(hp_ctx* ctx, const Call<T>& c, int64_t sums) {
 }
 
 // Prepares a launch of `blocks` workgroups that leave `sums` sums of losses. Few
-// sums are added by the last workgroup, and few workgroups count the mask
-// themselves, which saves a launch each.
+// sums are added by the last workgroup (up to 1024: the tickets of 4096 took 18 us more than
+// a launch). The mask is counted by every workgroup for itself where that
+// reads little, or little beside the logits (8192 masked rows of 32000 floats: 293 us,
+// with a launch for it 297; of 6000: 71 and 67).
 template <typename T>
 void plan_losses(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c, unsigned sums, unsigned blocks) {
   if (sums <= hp::kTicketPlaces) c.ticket = ctx->ticket;
   else c.sums = scratch.take<double>(sums);
-  if (!c.count_here || int64_t(blocks) * c.rows <= kCountedBytes) return;
+  const double counted = double(blocks) * double(c.rows), logits = double(c.rows) * double(c.vocab) * sizeof(T);
+  if (!c.count_here || counted <= kCountedBytes || counted * 8 <= logits) return;
   double* scale = scratch.take<double>(1);
   count_kernel<T><<<1, 1024, 0, ctx->stream>>>(c, scale);
   hp::check_launch("token count");
