@@ -578,29 +578,32 @@ __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __re
   }
 }
 
-// A workgroup per row: its pieces' statistics meet, and with them its token's
-// loss. As wide as policy_grad_kernel, so that both add the losses in one order.
-template <typename T>
+// The pieces' statistics of a row meet, and with them its token's terms. LOSS: the
+// policy loss, a workgroup per row, as wide as policy_grad_kernel, so that both add
+// the losses in one order; else a wave per row (8192 rows: 5.1 us, a workgroup each 7.0).
+template <typename T, bool LOSS>
 __global__ __launch_bounds__(kPieceThreads) void finish_kernel(Call<T> c, const T* __restrict__ part_tops,
                                                                const T* __restrict__ part_totals, int pieces) {
-  const double factor = c.old ? scale_of(c) : 1.0;
-  const int64_t row = blockIdx.x;
+  const double factor = LOSS ? scale_of(c) : 1.0;
+  const int64_t row = LOSS ? blockIdx.x : blockIdx.x * int64_t(kPieceThreads / 64) + (threadIdx.x >> 6);
+  const bool writes = (LOSS ? threadIdx.x : threadIdx.x & 63) == 0;
+  if (!LOSS && row >= c.rows) return;
   double loss = 0;
   if (c.kept(row)) {
     T top, total;
     join_pieces(part_tops + row * pieces, part_totals + row * pieces, pieces, top, total);
     const double log_prob = c.log_prob(c.logit(row, c.target(row)), top, total);
-    if (threadIdx.x == 0) c.keep(row, log_prob, top, total);
-    if (c.old) {
+    if (writes) c.keep(row, log_prob, top, total);
+    if constexpr (LOSS) {
       Token<T> token;
       token.read(c, row);
       double slope;
       policy_token(c, token, log_prob, loss, slope);
     }
-  } else if (threadIdx.x == 0) {
+  } else if (writes) {
     c.leave_out(row);
   }
-  if (c.old) leave_loss(c, loss, factor, blockIdx.x, gridDim.x);
+  if constexpr (LOSS) leave_loss(c, loss, factor, blockIdx.x, gridDim.x);
 }
 
 // The gradient of one piece of a row from the row's statistics and weight.
@@ -686,14 +689,16 @@ __global__ __launch_bounds__(1024) void loss_kernel(Call<T> c, int64_t n) {
 template <typename T>
 __global__ __launch_bounds__(256) void pair_kernel(Call<T> c, const T* __restrict__ reference, int64_t pairs, double beta,
                                                    double smoothing, T* __restrict__ sums_out) {
-  double ratio[2];
+  const int64_t rows[2] = {int64_t(blockIdx.x), pairs + blockIdx.x};
+  const double known[2] = {double(reference[rows[0]]), double(reference[rows[1]])};
+  double sums[2] = {0, 0}, ratio[2];
+  for (int64_t t = threadIdx.x; t < c.tokens; t += 256) {
+    for (int side = 0; side < 2; ++side) sums[side] += c.exact[rows[side] * c.tokens + t];
+  }
   for (int side = 0; side < 2; ++side) {
-    const int64_t at = side * pairs + blockIdx.x;
-    double sum = 0;
-    for (int64_t t = threadIdx.x; t < c.tokens; t += 256) sum += c.exact[at * c.tokens + t];
-    sum = workgroup_sum(sum);
-    if (threadIdx.x == 0) sums_out[at] = T(sum);
-    ratio[side] = sum - double(reference[at]);
+    const double sum = workgroup_sum(sums[side]);
+    if (threadIdx.x == 0) sums_out[rows[side]] = T(sum);
+    ratio[side] = sum - known[side];
   }
   const double margin = beta * (ratio[0] - ratio[1]);
   // -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)), with a NaN margin kept.
@@ -833,7 +838,8 @@ int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   stats<<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
   hp::check_launch("token statistics");
   if (done) policy_grad_kernel<T><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count, pieces.length);
-  else finish_kernel<T><<<blocks, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count);
+  else if (c.old) finish_kernel<T, true><<<blocks, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count);
+  else finish_kernel<T, false><<<hp::ceil_div(blocks, 4u), kPieceThreads, 0, ctx->stream>>>(c, tops, totals, pieces.count);
   hp::check_launch("token losses");
   return blocks;
 }
