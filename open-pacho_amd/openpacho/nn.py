@@ -23,6 +23,7 @@ from .backends import _DEFAULT
 from .exceptions import BackendMismatchError, UnsupportedDtypeError
 
 _FLOATS = (np.dtype("float32"), np.dtype("float64"))
+_TINY = {dtype: float(np.finfo(dtype).tiny) for dtype in _FLOATS}
 _INDICES = (np.dtype("int32"), np.dtype("int64"))
 _BOOL = np.dtype("bool")
 
@@ -385,10 +386,10 @@ def adamw(params, grads, state, *, learning_rate=1e-3, betas=(0.9, 0.999), eps=1
     _check_tensors(what, "grads", grads, backend, dtype, shapes)
     learning_rate = _number("learning_rate", learning_rate, 0)
     beta1, beta2 = (_number("betas", b, 0, 1) for b in betas)
-    eps = _number("eps", eps)
-    if eps < np.finfo(dtype).tiny:
-        raise ValueError(f"eps must be positive, and at least {np.finfo(dtype).tiny} for {dtype}")
-    if np.ndim(weight_decay):
+    eps = _number("eps", eps, 0)
+    if eps < _TINY[dtype]:
+        raise ValueError(f"eps must be positive, and at least {_TINY[dtype]} for {dtype}")
+    if type(weight_decay) is not float and np.ndim(weight_decay):
         decays = [_number("weight_decay", d, 0) for d in weight_decay]
         if len(decays) != len(shapes):
             raise ValueError(f"{what}: {len(decays)} values of weight_decay for {len(shapes)} tensors")
