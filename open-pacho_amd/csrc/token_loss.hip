@@ -7,9 +7,10 @@
 // so that a row needs its statistics (m, S), one scalar w that follows from
 // log p_y, and a pass that writes. Bound: HBM, each logit read once and each
 // gradient written once where a row can stay in registers meanwhile:
-//   - row_kernel, short_row_kernel: a team of L threads holds a whole row in K vectors of 16 bytes
-//     each and computes m and S from registers (the terms exp(z - m) replace the
-//     logits there), then the loss of its token and the gradient;
+//   - row_kernel, short_row_kernel: a team of L threads holds a whole row in K
+//     vectors of 16 bytes each and computes m and S from registers (the terms
+//     exp(z - m) replace the logits there), then the loss of its token and the
+//     gradient;
 //   - rows that no team holds, or so few of them that teams would leave the chip
 //     idle, are cut into pieces (stats_kernel), whose (m, S) meet per row
 //     (finish_kernel, policy_grad_kernel), and are read again for the gradient.
