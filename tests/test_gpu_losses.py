@@ -104,9 +104,10 @@ def test_forbidden_logits_at_the_ends_of_rows(hip, vocab):
     assert p.asnumpy(found[1])[2] == 0 and not grad[2].any()
 
 
-@pytest.mark.parametrize("rows,vocab", [(1030, 4097), (1500, 6000), (4200, 65), (1100, 66000), (40000, 9)])
+@pytest.mark.parametrize("rows,vocab", [(1030, 4097), (1500, 6000), (4200, 65), (1100, 66000), (40000, 9), (6000, 12500), (6000, 3000)])
 def test_more_sums_than_one_launch_adds(hip, rows, vocab):
-    # Losses of rows and workgroups beyond what the last workgroup adds, with and without a mask.
+    # Losses of rows and workgroups beyond what the last workgroup adds, with and without a mask,
+    # which every workgroup counts or (the last of these sizes) a launch of its own.
     rng = np.random.default_rng(rows)
     z = p.random.default_rng(3, backend=hip).normal(0, 1, (rows, vocab), dtype=np.float32)
     actions, advantages = rng.integers(0, vocab, rows), rng.standard_normal(rows).astype(np.float32)
