@@ -316,11 +316,12 @@ def _wrapped_list(storages, shapes, dtype, backend):
 
 def _check_tensors(what, name, values, backend, dtype, shapes):
     """Refuse what is not a list of arrays of this backend, dtype and these shapes."""
-    try:
-        if [v._shape for v in values if v._backend is backend and v._dtype is dtype] == shapes and type(values) in (list, tuple):
-            return
-    except (AttributeError, TypeError):
-        pass  # something in it is no array
+    if type(values) in (list, tuple) and len(values) == len(shapes):
+        try:  # of as many tensors none is left out where all shapes are found
+            if [v._shape for v in values if v._backend is backend and v._dtype is dtype] == shapes:
+                return
+        except AttributeError:
+            pass  # something in it is no array
     if not isinstance(values, (list, tuple)) or not all([isinstance(v, xp.ndarray) for v in values]):
         raise TypeError(f"{what}: {name} must be a list of arrays")
     for value in values:

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import openpacho as p
+from openpacho.backends import NumpyBackend
 from oracle import training
 
 OPTIONS = dict(learning_rate=3e-3, betas=(0.9, 0.99), eps=1e-8)
@@ -169,6 +170,40 @@ def check_resume(backend, bits):
 @pytest.mark.parametrize("bits", [None, 8])
 def test_resume(numpy_backend, bits):
     check_resume(numpy_backend, bits)
+
+
+def check_mixed_lists(backend):
+    """Lists that hold the state's tensors and others besides, which are of another dtype or backend, wherever these stand."""
+    other = NumpyBackend()
+
+    def tensor(size, dtype="float32", where=backend):
+        return p.zeros((size,), dtype=dtype, backend=where)
+
+    params = [tensor(3), tensor(2)]
+    state = p.nn.adamw_state(params)
+    for foreign, error in [(tensor(3, "float64"), p.UnsupportedDtypeError), (tensor(7, "float64"), p.UnsupportedDtypeError),
+                           (tensor(3, where=other), p.BackendMismatchError)]:  # fmt: skip
+        for at in range(3):
+            mixed = params[:at] + [foreign] + params[at:]
+            for bad in (mixed, tuple(mixed)):
+                with pytest.raises(error):
+                    p.nn.adamw(bad, params, state)
+                with pytest.raises(error):
+                    p.nn.adamw(params, bad, state)
+                with pytest.raises(error):
+                    p.nn.adamw_state(params, first=bad, second=params)
+                with pytest.raises(error):
+                    p.nn.adamw_state(params, first=params, second=bad)
+        for at in range(2):
+            mixed = params[:at] + [foreign] + params[at + 1 :]
+            with pytest.raises(error):
+                p.nn.adamw(params, mixed, state)
+    with pytest.raises(TypeError):
+        p.nn.adamw(params, [*params, None], state)
+
+
+def test_mixed_lists(numpy_backend):
+    check_mixed_lists(numpy_backend)
 
 
 def test_refusals(numpy_backend):
