@@ -705,7 +705,10 @@ __global__ __launch_bounds__(256) void pair_kernel(Call<T> c, const T* __restric
   // -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)), with a NaN margin kept.
   const double small = exp(-fabs(margin)), soft = log1p(small), large = 1.0 / (1.0 + small);
   const double yes = margin >= 0 ? large : small * large, no = margin >= 0 ? small * large : large;
-  const double loss = (1 - smoothing) * ((margin < 0 ? -margin : 0.0) + soft) + smoothing * ((margin > 0 ? margin : 0.0) + soft);
+  // A side of weight 0 is left out: where a response has probability 0 it is infinite.
+  const double won = smoothing < 1 ? (1 - smoothing) * ((margin < 0 ? -margin : 0.0) + soft) : 0.0;
+  const double lost = smoothing > 0 ? smoothing * ((margin > 0 ? margin : 0.0) + soft) : 0.0;
+  const double loss = won + lost;
   if (c.weights && threadIdx.x == 0) {
     const double slope = beta * (smoothing * yes - (1 - smoothing) * no) / double(pairs);
     c.weights[blockIdx.x] = T(slope);

@@ -117,7 +117,9 @@ def preference_loss(logits, targets, reference, mask, beta, smoothing, gradient)
         ratios = sums - _view(reference)
         margin = beta * (ratios[0] - ratios[1])
         soft = np.log1p(np.exp(-np.abs(margin)))
-        losses = (1 - smoothing) * (np.maximum(-margin, 0) + soft) + smoothing * (np.maximum(margin, 0) + soft)
+        # A side of weight 0 is left out: where a response has probability 0 it is infinite.
+        sides = [(1 - smoothing, -margin), (smoothing, margin)]
+        losses = sum(weight * (np.maximum(side, 0) + soft) for weight, side in sides if weight)
         yes, no = _gates(margin, 1)
         slope = beta * (smoothing * yes - (1 - smoothing) * no) / pairs
         loss = np.asarray(losses.sum(dtype=np.float64) / pairs, sums.dtype)

@@ -1,11 +1,18 @@
 """Operators of ``nn`` on the device at the ends of what they take."""
 
+import numpy as np
 import pytest
 
 from test_nn_adamw import check_mixed_lists
+from test_nn_losses import check_impossible_responses
 
 pytestmark = pytest.mark.gpu
 
 
 def test_mixed_lists(hip):
     check_mixed_lists(hip)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_impossible_responses(hip, dtype):
+    check_impossible_responses(hip, dtype)

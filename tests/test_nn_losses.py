@@ -172,6 +172,41 @@ def test_edges(numpy_backend, dtype):
     check_edges(numpy_backend, dtype)
 
 
+def check_impossible_responses(backend, dtype):
+    """A forbidden logit as a token of a response: its sum is -inf and the margin infinite; the loss is what its limit is."""
+    logits = np.array([[[[0, 1, 2]], [[0, 0, 0]]], [[[1, -np.inf, 0]], [[0, 1, 0]]]], dtype)
+    targets = np.array([[[2], [0]], [[1], [1]]])
+    reference = np.array([[-1, -1], [-2, -0.5]], dtype)
+    one = np.finfo(dtype).eps
+    other = 0.1 * ((-np.log(3) + 1) - (1 - np.log(2 + np.e) + 0.5))  # the second pair's margin
+    for swap in (False, True):
+        z, y, r = (a[::-1].copy() if swap else a for a in (logits, targets, reference))
+        sign = -1 if swap else 1
+        for smoothing in (0.0, 1.0, 0.25):
+            found = p.nn.preference_loss_grad(*put(backend, z, y, r), smoothing=smoothing)
+            alone = p.nn.preference_loss(*put(backend, z, y, r), smoothing=smoothing)
+            # The side that the impossible response loses costs nothing, the other all there is.
+            free = smoothing == (1.0 if swap else 0.0)
+            side = sign * other * (-1 if smoothing == 1 else 1)
+            want = np.log1p(np.exp(-side)) / 2 if free else np.inf
+            for loss in (found[0].item(), alone[0].item()):
+                # A margin and a logarithm near 1: some ten roundings.
+                assert abs(loss - want) <= 16 * one if free else loss == want
+            sums, grad = p.asnumpy(found[1]), p.asnumpy(found[2])
+            assert np.isneginf(sums).sum() == 1 and sums[0 if swap else 1, 0] == -np.inf
+            # The pair's slope at an infinite margin is beta / pairs times the weight of the side that it loses.
+            slope = 0.05 * (-(1 - smoothing) if swap else smoothing)
+            for side, weight in enumerate((slope, -slope)):
+                share = np.exp(z[side, 0, 0].astype(float))
+                want = weight * ((np.arange(3) == y[side, 0, 0]) - share / share.sum())
+                np.testing.assert_allclose(grad[side, 0, 0], want, rtol=16 * one, atol=one)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_impossible_responses(numpy_backend, dtype):
+    check_impossible_responses(numpy_backend, dtype)
+
+
 def test_ties_and_broadcast_advantages(numpy_backend):
     # At the ends of the clip the ratio's own side gives the gradient.
     logits = np.log(np.array([[0.5, 0.5]] * 2))
