@@ -152,7 +152,8 @@ __device__ __forceinline__ void policy_token(const Call<T>& c, const Token<T>& t
   if (c.reference) {
     const double apart = double(token.reference) - log_prob;
     const double grown = expm1_difference(T(0), apart);
-    loss += c.kl * (grown - apart);
+    // Infinite where the policy gives the token no probability; grown - apart would be NaN.
+    loss += c.kl * (grown == __builtin_huge_val() ? grown : grown - apart);
     slope -= c.kl * grown;
   }
 }

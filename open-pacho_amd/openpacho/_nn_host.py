@@ -102,7 +102,9 @@ def policy_loss(logits, actions, old, advantages, reference, mask, low, high, kl
         if reference is not None:
             apart = _view(reference) - log_probs
             grown = np.expm1(apart)
-            losses, slopes = losses + kl_weight * (grown - apart), slopes - kl_weight * grown
+            # Infinite where the policy gives the token no probability; grown - apart would be NaN.
+            excess = np.where(grown == np.inf, grown, grown - apart)
+            losses, slopes = losses + kl_weight * excess, slopes - kl_weight * grown
         if count is None:
             count = max(1, int(rows.kept.sum()))
         loss = np.asarray(np.where(rows.kept, losses, 0).sum(dtype=np.float64) / count, log_probs.dtype)

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from test_nn_adamw import check_mixed_lists
-from test_nn_losses import check_impossible_responses
+from test_nn_losses import check_impossible_responses, check_impossible_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -16,3 +16,10 @@ def test_mixed_lists(hip):
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 def test_impossible_responses(hip, dtype):
     check_impossible_responses(hip, dtype)
+
+
+# Short rows, rows of one workgroup, rows in pieces.
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("vocab", [2, 40, 3000, 70001])
+def test_impossible_tokens(hip, vocab, dtype):
+    check_impossible_tokens(hip, dtype, vocab)

@@ -207,6 +207,40 @@ def test_impossible_responses(numpy_backend, dtype):
     check_impossible_responses(numpy_backend, dtype)
 
 
+def check_impossible_tokens(backend, dtype, vocab):
+    """An action whose logit is -inf: ratio 0, and an infinite KL term where the reference gives it any probability."""
+    rng = np.random.default_rng(vocab)
+    logits = rng.standard_normal((3, vocab)).astype(dtype)
+    logits[1, 0] = -np.inf
+    actions, old = np.array([vocab - 1, 0, 0]), np.full(3, -1.5, dtype)
+    advantages, reference = np.array([0.5, -1, 2], dtype), np.array([-1, -2, -np.inf], dtype)
+
+    def call(**options):
+        found = p.nn.policy_loss_grad(*put(backend, logits, actions, old, advantages), count=1.0, **options)
+        assert p.nn.policy_loss(*put(backend, logits, actions, old, advantages), count=1.0, **options)[0].item() == found[0].item()
+        return [p.asnumpy(a) for a in found]
+
+    # Not a NaN: the sum over the tokens is that of its terms, the second of which is infinite.
+    loss, log_probs, grad = call(reference_log_probs=reference, kl_weight=0.1)
+    assert loss == np.inf and log_probs[1] == -np.inf
+    assert np.isfinite(grad[[0, 2]]).all() and not np.isfinite(grad[1, 0])
+    # The others' gradients are those that they have beside a possible one, and without the KL term the token's ratio is 0:
+    # its gradient is, and of its loss only the clipped side is left, 1 - 0.2 times the advantage.
+    kept = call(reference_log_probs=reference, kl_weight=0.1, mask=np.array([True, False, True]))
+    assert kept[0] == np.inf  # the last token's reference gives it no probability: exp(d) - d - 1 with d = -inf
+    np.testing.assert_array_equal(grad[[0, 2]], kept[2][[0, 2]])
+    plain, without = call(), call(mask=np.array([True, False, True]))
+    assert abs(plain[0] - without[0] - 0.8) <= 64 * np.finfo(dtype).eps * (1 + abs(without[0])) and not plain[2][1].any()
+    kept = call(reference_log_probs=reference, kl_weight=0.1, mask=np.array([True, False, False]))
+    assert np.isfinite(kept[0])
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("vocab", [2, 40])
+def test_impossible_tokens(numpy_backend, vocab, dtype):
+    check_impossible_tokens(numpy_backend, dtype, vocab)
+
+
 def test_ties_and_broadcast_advantages(numpy_backend):
     # At the ends of the clip the ratio's own side gives the gradient.
     logits = np.log(np.array([[0.5, 0.5]] * 2))
