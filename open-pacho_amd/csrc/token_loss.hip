@@ -66,8 +66,29 @@ __device__ __forceinline__ double log_wide(double x) { return log(x); }
 // float's precision loses no more than the rounding of the result.
 __device__ __forceinline__ double exp_difference(float, double x) { return expf(float(x)); }
 __device__ __forceinline__ double exp_difference(double, double x) { return exp(x); }
-__device__ __forceinline__ double expm1_difference(float, double x) { return expm1f(float(x)); }
+__device__ __forceinline__ double expm1_difference(float, double x) { return exp_difference(0.0f, x) - 1; }
 __device__ __forceinline__ double expm1_difference(double, double x) { return expm1(x); }
+
+// grown = exp(x) - 1 and excess = exp(x) - 1 - x of such a difference, both with a T's
+// digits. Near 0 the difference of x and grown would lose excess's, which is some
+// x^2 / 2 there: it is the series x^2/2 (1 + x/3 (1 + x/4 (...))), whose first term left
+// out is below 2^-27 of it for floats up to 2 and 2^-54 for doubles up to 1. Beyond, the
+// difference loses two bits at most.
+template <typename T>
+__device__ __forceinline__ void grow(double x, double& grown, double& excess) {
+  constexpr int kTerms = sizeof(T) == 4 ? 15 : 18;
+  if (fabs(x) < (sizeof(T) == 4 ? 2.0 : 1.0)) {
+    double rest = 1;
+#pragma unroll
+    for (int k = kTerms; k > 2; --k) rest = __builtin_fma(x * (1.0 / k), rest, 1.0);
+    excess = 0.5 * x * x * rest;
+    grown = x + excess;
+  } else {
+    grown = expm1_difference(T(0), x);
+    // Infinite where the policy gives a token no probability; grown - x would be NaN.
+    excess = grown == __builtin_huge_val() ? grown : grown - x;
+  }
+}
 
 // The values of one call; pointers that it does not have are null.
 template <typename T>
@@ -137,7 +158,6 @@ struct Token {
 };
 
 // The policy loss of a token and its derivative by the log-probability.
-// expm1 keeps the KL term's digits where the two policies nearly agree.
 template <typename T>
 __device__ __forceinline__ void policy_token(const Call<T>& c, const Token<T>& token, double log_prob, double& loss, double& slope) {
   const double advantage = token.advantage;
@@ -150,10 +170,9 @@ __device__ __forceinline__ void policy_token(const Call<T>& c, const Token<T>& t
   loss = -(stopped ? held : free);
   slope = stopped ? 0.0 : -free;
   if (c.reference) {
-    const double apart = double(token.reference) - log_prob;
-    const double grown = expm1_difference(T(0), apart);
-    // Infinite where the policy gives the token no probability; grown - apart would be NaN.
-    loss += c.kl * (grown == __builtin_huge_val() ? grown : grown - apart);
+    double grown, excess;
+    grow<T>(double(token.reference) - log_prob, grown, excess);
+    loss += c.kl * excess;
     slope -= c.kl * grown;
   }
 }

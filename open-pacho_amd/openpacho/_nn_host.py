@@ -91,6 +91,18 @@ def token_log_probs(logits, targets, mask):
     return _Rows(logits, targets, mask).log_probs.reshape(-1)
 
 
+def _grow(x):
+    """exp(x) - 1 and exp(x) - 1 - x in 64 bits. Near 0, where a difference would lose the digits of the second, its series."""
+    near = np.where(np.abs(x) < 1, x, 0)
+    rest = np.ones_like(near)
+    for k in range(18, 2, -1):  # x^2/2 (1 + x/3 (1 + x/4 (...)))
+        rest = 1 + near / k * rest
+    grown = np.expm1(x)
+    # Infinite where the policy gives a token no probability; grown - x would be NaN.
+    apart = np.where(grown == np.inf, grown, grown - x)
+    return grown, np.where(np.abs(x) < 1, near * near / 2 * rest, apart)
+
+
 def policy_loss(logits, actions, old, advantages, reference, mask, low, high, kl_weight, count, gradient):
     rows = _Rows(logits, actions, mask)
     log_probs, advantages = rows.log_probs, _view(advantages)
@@ -100,10 +112,7 @@ def policy_loss(logits, actions, old, advantages, reference, mask, low, high, kl
         held = np.minimum(np.maximum(ratio, 1 - low), 1 + high) * advantages
         losses, slopes = -np.minimum(free, held), np.where(free > held, 0, -free)
         if reference is not None:
-            apart = _view(reference) - log_probs
-            grown = np.expm1(apart)
-            # Infinite where the policy gives the token no probability; grown - apart would be NaN.
-            excess = np.where(grown == np.inf, grown, grown - apart)
+            grown, excess = _grow(_view(reference).astype(np.float64) - log_probs)
             losses, slopes = losses + kl_weight * excess, slopes - kl_weight * grown
         if count is None:
             count = max(1, int(rows.kept.sum()))

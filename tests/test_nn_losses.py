@@ -241,6 +241,28 @@ def test_impossible_tokens(numpy_backend, vocab, dtype):
     check_impossible_tokens(numpy_backend, dtype, vocab)
 
 
+def check_near_policies(backend, dtype):
+    """The KL term from policies that nearly agree to ones that are far apart, over a vocabulary of one: the log-probability
+    is 0, and d the reference's, both exactly."""
+    logits, zero = p.asarray(np.ones((1, 1), dtype), backend=backend), np.zeros(1, dtype)
+    for size in [*10.0 ** np.arange(-12, 0), 0.3, 0.999, 1.0, 1.001, 1.999, 2.0, 2.001, 3.7, 10.3, 40.7]:
+        for d in (dtype(size), dtype(-size)):
+            got = p.nn.policy_loss(logits, [0], zero, zero, reference_log_probs=[d], kl_weight=1.0)[0].item()
+            # The definition's series in extended precision, from its smallest term.
+            wide = training.WIDE(d)
+            terms = [wide * wide / 2]
+            while abs(terms[-1]) > 1e-25 * abs(terms[0]) or len(terms) < 2 * abs(d):
+                terms.append(terms[-1] * wide / (len(terms) + 2))
+            want = sum(sorted(terms, key=abs)) if abs(d) < 2 else np.exp(wide) - 1 - wide
+            # An exponential of 3 units of rounding, of which the subtractions leave 2.4 times as many; a rounding.
+            assert abs(got - want) <= 8 * np.finfo(dtype).eps / 2 * want, (d, got, want)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_near_policies(numpy_backend, dtype):
+    check_near_policies(numpy_backend, dtype)
+
+
 def test_ties_and_broadcast_advantages(numpy_backend):
     # At the ends of the clip the ratio's own side gives the gradient.
     logits = np.log(np.array([[0.5, 0.5]] * 2))
