@@ -62,9 +62,15 @@ __device__ __forceinline__ double log_wide(float x) {
   return double(exponent) * 0.6931471805599453 + double(logf(rest));
 }
 __device__ __forceinline__ double log_wide(double x) { return log(x); }
-// exp and exp - 1 of a difference of log-probabilities formed in 64 bits: a
-// float's precision loses no more than the rounding of the result.
-__device__ __forceinline__ double exp_difference(float, double x) { return expf(float(x)); }
+// exp and exp - 1 of a difference of log-probabilities formed in 64 bits, to a T's
+// precision: a float takes the exponential of x rounded to a float and puts what that
+// cuts off back to first order, exp(near + d) = exp(near) (1 + d). Without it the result
+// would be off by up to |x| / 2 units of rounding. exp(-inf) and results past the type
+// have nothing to put back.
+__device__ __forceinline__ double exp_difference(float, double x) {
+  const float near = float(x), r = expf(near);
+  return r < __builtin_huge_valf() && x > -128 ? double(r) + double(r) * (x - double(near)) : double(r);
+}
 __device__ __forceinline__ double exp_difference(double, double x) { return exp(x); }
 __device__ __forceinline__ double expm1_difference(float, double x) { return exp_difference(0.0f, x) - 1; }
 __device__ __forceinline__ double expm1_difference(double, double x) { return expm1(x); }

@@ -3,6 +3,8 @@
 import numpy as np
 import pytest
 
+import openpacho as p
+from oracle import training
 from test_nn_adamw import check_mixed_lists
 from test_nn_losses import check_impossible_responses, check_impossible_tokens, check_near_policies
 
@@ -28,3 +30,23 @@ def test_impossible_tokens(hip, vocab, dtype):
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 def test_near_policies(hip, dtype):
     check_near_policies(hip, dtype)
+
+
+def test_ratios_of_policies_that_are_far_apart(hip):
+    # Two equal logits: log-probabilities of -log 2, whose difference from `old` is no float.
+    log_prob, one = -np.log(training.WIDE(2)), np.float32(1)
+    unit = np.finfo(np.float32).eps / 2
+    logits, zero = p.asarray(np.zeros((1, 2), np.float32), backend=hip), np.zeros(1, np.float32)
+    rng = np.random.default_rng(0)
+    for other in np.concatenate([rng.uniform(-12, 12, 60), [-80, 80]]).astype(np.float32):
+        ratio = np.exp(log_prob - training.WIDE(other))
+        loss, _, grad = p.nn.policy_loss_grad(logits, [1], [other], [one], clip=(1.0, np.inf))
+        # An exponential (a unit in the last place, two of rounding), its correction and the result's rounding.
+        assert abs(loss.item() + ratio) <= 4 * unit * ratio, (other, loss.item(), ratio)
+        # Shares of exactly a half: the gradient is the ratio's half, both ways.
+        assert np.all(np.abs(p.asnumpy(grad)[0] - [ratio / 2, -ratio / 2]) <= 4 * unit * ratio / 2), other
+        apart = training.WIDE(other) - log_prob
+        excess = np.exp(apart) - 1 - apart
+        loss = p.nn.policy_loss(logits, [1], zero, zero, reference_log_probs=[other], kl_weight=1.0)[0].item()
+        # The exponential's, of which the subtractions leave 1.7 times as much, and the rounding.
+        assert abs(apart) < 0.5 or abs(loss - excess) <= 8 * unit * excess, (other, loss, excess)
