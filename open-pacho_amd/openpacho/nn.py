@@ -140,7 +140,8 @@ def gated_recurrence(x, gate, initial=None, *, resets=None):
     fewer: its last axis divides the channels into heads that share one.
     ``initial`` (..., channels) is the state before the first step, zero if not
     given. Where ``resets`` (..., time) is true the state before that step
-    counts as zero, whatever it holds. Returns every state, of x's shape.
+    counts as zero, whatever it holds; an infinite state stays so until then, and is
+    NaN from a gate of ``-inf`` on. Returns every state, of x's shape.
     """
     ops, x, gate, initial, resets, sizes = _recurrence_operands("gated_recurrence", x, gate, initial, resets)
     return ops.result(ops.backend.gated_recurrence(x, gate, initial, resets, *sizes), x._shape)

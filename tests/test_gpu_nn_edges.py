@@ -7,6 +7,7 @@ import openpacho as p
 from oracle import training
 from test_nn_adamw import check_mixed_lists
 from test_nn_losses import check_impossible_responses, check_impossible_tokens, check_near_policies
+from test_nn_recurrence import check_infinite_states
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,14 @@ def test_ratios_of_policies_that_are_far_apart(hip):
         loss = p.nn.policy_loss(logits, [1], zero, zero, reference_log_probs=[other], kl_weight=1.0)[0].item()
         # The exponential's, of which the subtractions leave 1.7 times as much, and the rounding.
         assert abs(apart) < 0.5 or abs(loss - excess) <= 8 * unit * excess, (other, loss, excess)
+
+
+# Rows of one wave, of four, of eight and of two runs of these; tiles in one block and in several of both
+# lengths, with heads of a channel, packed ones, and ones of whole waves.
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("resets", [True, False])
+@pytest.mark.parametrize("sizes", [(1, 1, 3, 3), (2, 4, 70, 70), (2, 15, 12, 6), (2, 50, 70, 35), (3, 120, 13, 13), (2, 250, 256, 4), (2, 1001, 130, 130),
+                                   (1, 3000, 256, 2), (1, 15000, 12, 4), (2, 2500, 1030, 1030)])  # fmt: skip
+def test_infinite_states(hip, sizes, resets, dtype):
+    print(sizes, resets, dtype, flush=True)
+    check_infinite_states(hip, sizes, dtype, resets)

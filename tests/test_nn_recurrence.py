@@ -55,6 +55,49 @@ def test_values_and_gradients(numpy_backend, sizes, state, resets, dtype):
     check(numpy_backend, sizes, dtype, state, resets)
 
 
+def agree(got, want, size, dtype):
+    """`near` wherever the definition has a number, and its infinities and NaN elsewhere."""
+    finite = np.isfinite(want)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    np.testing.assert_array_equal(got[np.isinf(want)], want[np.isinf(want)].astype(dtype))
+    near(got[finite], want[finite], size[finite], dtype)
+
+
+def check_infinite_states(backend, sizes, dtype, resets):
+    """An infinite state stays so for as long as no reset drops it, over gates whose product leaves the type;
+    past a gate of 0, or beside the other infinity, it is NaN. Gradients do so towards the start."""
+    batch, time, channels, gates = sizes
+    x, gate, initial, starts, d = make(sizes, dtype, 5, True, resets)
+    if resets:
+        starts[:] = np.random.default_rng(6).random((batch, time)) < 1.5 / time
+    width, middle = channels // gates, time // 2
+    given, given_d = x.copy(), d.copy()
+    initial[:, 0] = np.inf
+    for n, channel in enumerate(range(width, channels, width)):  # one of each further head
+        at = (n * 37) % time
+        given[:, at, channel], given_d[:, at, channel] = (-1) ** n * np.inf, (-1) ** n * np.inf
+        if n % 5 == 1:
+            gate[:, middle, channel // width] = -np.inf
+        if n % 5 == 2:
+            given[:, middle, channel], given_d[:, middle, channel] = -given[:, at, channel], -given_d[:, at, channel]
+    with np.errstate(invalid="ignore"):
+        want, size = training.recurrence(given, gate, initial, starts)
+        agree(p.asnumpy(p.nn.gated_recurrence(*put(backend, given, gate, initial), resets=put(backend, starts)[0])), want, size, dtype)
+        initial[:, 0] = 1
+        h = training.recurrence(x, gate, initial, starts)[0].astype(dtype)
+        values, bounds = training.recurrence_grad(given_d, x, gate, h, initial, starts)
+    found = p.nn.gated_recurrence_grad(*put(backend, given_d, x, gate, h, initial), resets=put(backend, starts)[0])
+    for got, want, size in zip(found, values, bounds):
+        agree(p.asnumpy(got), want, size, dtype)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("resets", [True, False])
+@pytest.mark.parametrize("sizes", [(1, 1, 3, 3), (2, 40, 12, 12), (2, 300, 12, 4)])
+def test_infinite_states(numpy_backend, sizes, resets, dtype):
+    check_infinite_states(numpy_backend, sizes, dtype, resets)
+
+
 def test_gradients_match_differences(numpy_backend):
     x, gate, initial, starts, d = make((2, 6, 4, 2), np.float64, 3)
 
