@@ -37,7 +37,7 @@ def _refuse_capture(what, backend):
 
 
 class _Operands:
-    """The arrays of one call: their backend, and their float dtype, which the first one gives."""
+    """The arrays of one call: their backend, and their float dtype, which the first one gives that is no host value."""
 
     __slots__ = ("what", "backend", "dtype")
 
@@ -47,7 +47,11 @@ class _Operands:
             if value is not None and isinstance(value, xp.ndarray) and value._backend is not self.backend:
                 raise BackendMismatchError("Arrays belong to different backends/devices; use to_backend()")
         _refuse_capture(what, self.backend)
-        self.dtype = lead._dtype if isinstance(lead, xp.ndarray) else np.asarray(lead).dtype
+        if isinstance(lead, xp.ndarray):
+            self.dtype = lead._dtype
+        else:
+            given = [v._dtype for v in others if isinstance(v, xp.ndarray) and v._dtype in _FLOATS]
+            self.dtype = given[0] if given else np.asarray(lead).dtype
         if self.dtype not in _FLOATS:
             raise UnsupportedDtypeError(f"{what} requires float32 or float64, got {self.dtype}")
 

@@ -137,6 +137,29 @@ def test_leading_axes_and_host_values(numpy_backend):
     np.testing.assert_array_equal(p.asnumpy(alone), flat[0])
 
 
+def test_the_first_operand_may_be_a_host_value(numpy_backend):
+    x, gate, initial, starts, d = make((2, 5, 4, 2), np.float32)
+    want = p.nn.gated_recurrence(*put(numpy_backend, x, gate, initial), resets=starts)
+    # Of the arrays' dtype, whatever the host's is.
+    for host in (x, x.astype(np.float64), x.tolist()):
+        got = p.nn.gated_recurrence(host, p.asarray(gate), initial, resets=p.asarray(starts))
+        assert got.dtype == np.float32
+        np.testing.assert_array_equal(p.asnumpy(got), p.asnumpy(want))
+        grads = p.nn.gated_recurrence_grad(p.asarray(d), host, gate.tolist(), want)
+        for one, two in zip(grads[:2], p.nn.gated_recurrence_grad(*put(numpy_backend, d, x, gate), want)):
+            np.testing.assert_array_equal(p.asnumpy(one), p.asnumpy(two))
+    step = p.nn.gated_recurrence_step(x[:, 0].astype(np.float64), gate[:, 0].tolist(), p.asarray(initial))
+    assert step.dtype == np.float32
+    # Without any array of floats the first operand gives the dtype; arrays of integers beside it do not.
+    assert p.nn.token_log_probs([[1.0, 2.0]], p.asarray([0])).dtype == np.float64
+    loss, _ = p.nn.policy_loss(np.zeros((1, 4)), [0], p.zeros((1,), dtype="float32"), [1.0])
+    assert loss.dtype == np.float32
+    with pytest.raises(p.UnsupportedDtypeError):
+        p.nn.token_log_probs([[1, 2]], p.asarray([0]))
+    with pytest.raises(p.UnsupportedDtypeError):
+        p.nn.gated_recurrence(x, p.zeros((2, 5, 2), dtype="float32"), p.zeros((2, 4), dtype="float64"))
+
+
 def test_refusals(numpy_backend):
     x, gate = p.zeros((2, 3, 4), dtype="float32"), p.zeros((2, 3, 4), dtype="float32")
     f = p.nn.gated_recurrence
