@@ -198,3 +198,82 @@ def test_refusals(numpy_backend):
         p.compile(lambda x, g: f(x, g))(x, gate)
     with pytest.raises(NotImplementedError, match="not captured"):
         p.fuse(lambda x, g: f(x, g))(x, gate)
+
+
+# ---- slow gates ------------------------------------------------------------------
+
+
+def make_slow(sizes, dtype, seed=0, resets=False):
+    """Channels that remember some tens to some thousands of steps, a few of them everything, with states that start large
+    in every third channel; resets every 3000 steps or so."""
+    batch, time, channels, gates = sizes
+    rng = np.random.default_rng(seed)
+    x, d = (rng.standard_normal((batch, time, channels)).astype(dtype) for _ in range(2))
+    gate = (rng.standard_normal((batch, time, gates)) + rng.uniform(4, 10, gates)).astype(dtype)
+    if gates > 2:
+        gate[:, :, gates // 2] = np.inf
+    initial = (rng.standard_normal((batch, channels)) * np.where(np.arange(channels) % 3, 1, 100)).astype(dtype)
+    starts = rng.random((batch, time)) < 1 / 3000 if resets else None
+    return x, gate, initial, starts, d
+
+
+def check_slow(backend, sizes, dtype, resets):
+    x, gate, initial, starts, d = make_slow(sizes, dtype, sum(sizes), resets)
+    xs, gs, first, rs, ds = put(backend, x, gate, initial, starts, d)
+    want, size = training.recurrence(x, gate, initial, starts)
+    h = p.nn.gated_recurrence(xs, gs, first, resets=rs)
+    near(p.asnumpy(h), want, size, dtype)
+    values, bounds = training.recurrence_grad(d, x, gate, p.asnumpy(h), initial, starts)
+    found = p.nn.gated_recurrence_grad(ds, xs, gs, h, first, resets=rs)
+    for got, want, size in zip(found, values, bounds):
+        near(p.asnumpy(got), want, size, dtype)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("resets", [False, True])
+def test_slow_gates(numpy_backend, resets, dtype):
+    check_slow(numpy_backend, (2, 700, 12, 4), dtype, resets)
+
+
+def mistakes(state, keep, tile, span):
+    """What the carried value before each tile would be off by in three mistakes, from the states (time, channels) and gates:
+    the second-last tile left out, the state before the block left out, the block's last tile left out of that state.
+    Yields (mistake, first step of the tile, error of the value before it)."""
+    for first in range(3 * tile, len(state), tile):
+        number = first // tile
+        inner = number % span
+        block = first - inner * tile  # its first step
+        if inner >= 2:
+            last = keep[first - tile : first].prod(0)
+            yield "tile", first, last * (state[first - 2 * tile - 1] - state[first - tile - 1])
+        if number >= span:
+            since = keep[block:first].prod(0)
+            yield "state", first, -since * state[block - 1]
+            yield "publish", first, since * (state[block - tile - 1] - state[block - 1])
+
+
+# Tiles of the device's kernels, forward and backward, in both types, and both lengths of a block.
+@pytest.mark.parametrize("dtype,forward,backward", [(np.float32, 128, 64), (np.float64, 64, 32)])
+@pytest.mark.parametrize("span,time", [(16, 2200), (64, 17000)])
+def test_slow_gates_show_what_tiles_pass_on(span, time, dtype, forward, backward):
+    # A tile that got a wrong value from those before it is off by more than test_slow_gates allows, at its first step already.
+    x, gate, initial, _, d = make_slow((1, time, 48, 48), dtype, span)
+    unit = 20 * np.finfo(dtype).eps / 2
+    h, size = training.recurrence(x, gate, initial)
+    keep, take = training.sigmoid(gate[0].astype(training.WIDE)), training.sigmoid(-gate[0].astype(training.WIDE))
+    seen = set()
+    for what, first, off in mistakes(h[0], keep, forward, span):
+        seen.add(what)
+        # A state that everything before the block has left does not show it in every channel; some do in every tile.
+        assert (np.abs(keep[first] * off) > unit * size[0, first]).sum() >= 2, (what, first)
+    (dx, _, _), (bound, _, _) = training.recurrence_grad(d, x, gate, h.astype(dtype), initial)
+    # The carried gradient m_t = a_t (g_t + m_{t+1}), in the kernels' order, from the last step.
+    carried = np.zeros_like(h[0])
+    value = np.zeros_like(h[0, 0])
+    for t in reversed(range(time)):
+        carried[time - 1 - t] = value = keep[t] * (d[0, t] + value)
+    for what, first, off in mistakes(carried, keep[::-1], backward, span):
+        seen.add(what + " of gradients")
+        t = time - 1 - first  # its dx is off by 1 - a times what is carried
+        assert (np.abs(take[t] * off) > unit * bound[0, t]).sum() >= 2, (what, first)
+    assert len(seen) == 6
