@@ -16,8 +16,9 @@
 //     (finish_kernel, policy_grad_kernel), and are read again for the gradient.
 //     The preference loss needs this second reading (grad_kernel) in any case: w
 //     depends on every token of both responses.
-// Sums over a row are float (double of doubles) in a tree; the loss sums are
-// double. Every order is fixed, so results repeat bit for bit.
+// Sums over a row are float (double of doubles) in a tree over lanes, a lane's
+// vectors one after the other, and a lane's pieces of a very long row in double; the
+// loss sums are double. Every order is fixed, so results repeat bit for bit.
 //
 // A row that the mask leaves out is not read. Pieces and teams pad with -inf,
 // which adds nothing to S; the reference of a piece that is all -inf is 0, so
@@ -208,19 +209,21 @@ __device__ __forceinline__ void join(bool has, T piece_top, T piece_total, T& to
   total = team_reduce<64>(part, [](T a, T b) { return a + b; });
 }
 
-// The same from memory, by every wave for itself; a lane's pieces join first.
+// The same from memory, by every wave for itself; a lane's pieces join first, one after
+// the other in 64 bits: a row of 2^31 floats has 4096 a lane.
 template <typename T>
 __device__ __forceinline__ void join_pieces(const T* tops, const T* totals, int pieces, T& top, T& total) {
   const int lane = threadIdx.x & 63;
   const T none = -T(__builtin_huge_val());
-  T own = lane < pieces ? tops[lane] : none, sum = lane < pieces ? totals[lane] : T(0);
+  T own = lane < pieces ? tops[lane] : none;
+  double sum = lane < pieces ? totals[lane] : T(0);
   for (int k = lane + 64; k < pieces; k += 64) {
     const T next = larger(own, tops[k]);
     if (own != none) sum *= hpd::exp_down(own - next);
-    sum += tops[k] == none ? totals[k] : totals[k] * hpd::exp_down(tops[k] - next);
+    sum += tops[k] == none ? double(totals[k]) : double(totals[k]) * hpd::exp_down(tops[k] - next);
     own = next;
   }
-  join(lane < pieces, own, sum, top, total);
+  join(lane < pieces, own, T(sum), top, total);
 }
 
 // What the waves of a workgroup leave for each other, for two rows in turn: of

@@ -62,3 +62,19 @@ def test_ratios_of_policies_that_are_far_apart(hip):
 def test_infinite_states(hip, sizes, resets, dtype):
     print(sizes, resets, dtype, flush=True)
     check_infinite_states(hip, sizes, dtype, resets)
+
+
+def test_one_row_of_many_equal_pieces(hip):
+    # 262143 pieces of 8192 logits with one sum, which a chain of additions would round the same way again and again.
+    pieces, rng = 262143, np.random.default_rng(1)
+    pattern = (rng.integers(-1024, 1024, 8192) / 256).astype(np.float32)
+    logits = p.zeros((pieces, 1), dtype=np.float32, backend=hip) + p.asarray(pattern, backend=hip)
+    logits = logits.reshape(1, -1)
+    total = np.log(training.WIDE(pieces)) + np.log(np.exp(pattern.astype(training.WIDE)).sum())
+    for target in (0, 8191, 2**30 + 70, pieces * 8192 - 1):
+        found = p.nn.token_log_probs(logits, [target]).item()
+        # Units of rounding: an exponential's 4, a piece's sum of 19 additions one after the other, 6 of the pieces' tree,
+        # and 25 of the result and its terms.
+        want = pattern[target % 8192] - total
+        assert abs(found - want) <= 64 * np.finfo(np.float32).eps / 2, (target, found, want)
+    hip.release_cached_memory()
