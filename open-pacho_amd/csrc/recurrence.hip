@@ -64,6 +64,7 @@ struct Steps<double> {
 };
 
 constexpr unsigned kDies = 8;  // of the chip, each with a cache of its own
+constexpr double kLastCache = 1 << 28;  // bytes of the cache that they share
 
 struct Extents {
   int64_t time;      // steps of a row
@@ -913,10 +914,11 @@ int hp_gated_recurrence(hp_ctx* ctx, int dtype, const void* x, const void* gate,
       // float32 in 8 heads: 125 us, 131 with a sigmoid a lane; 65536 x 1000 in 8 heads,
       // waves of 63: 157 and 148).
       // States are stored past the caches where steps are whole lines and all of them are
-      // more than the last cache holds (16 x 4096 x 2048 float32: 259 us, 280 through it);
-      // fewer are left there for their reader (64 x 256 x 2048 into one block again and
-      // again: 76 us past the caches, 70).
-      const bool stream = channels * int64_t(sizeof(T)) % 128 == 0 && double(e.total) * double(time) * sizeof(T) > 256e6;
+      // more than the last cache holds (16 x 4096 x 2048 float32: 264 us, 284 through it;
+      // with a product of 18 columns right after, 460 and 487). Fewer are left there for
+      // their reader: of 8 x 4096 x 2048, just what it holds, 141 us and 147, but with a sum
+      // or a product of 512 columns right after 186 and 170, 615 and 605.
+      const bool stream = channels * int64_t(sizeof(T)) % 128 == 0 && double(e.total) * double(time) * sizeof(T) > kLastCache;
       const auto launch = e.width == 1                      ? (stream ? forward<T, kOwn, true> : forward<T, kOwn, false>)
                           : e.pack == 1 && e.piece == 64    ? (stream ? forward<T, kWave, true> : forward<T, kWave, false>)
                                                             : (stream ? forward<T, kShared, true> : forward<T, kShared, false>);
@@ -942,10 +944,14 @@ int hp_gated_recurrence_grad(hp_ctx* ctx, int dtype, const void* grad, const voi
       const Backward<T> f{static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const T*>(gate),
                           static_cast<const T*>(h), static_cast<const T*>(initial), r, static_cast<T*>(dx),
                           static_cast<T*>(dgate), static_cast<T*>(dinitial)};
-      // Past the caches where steps are whole lines; else neighbouring groups meet in
-      // the lines that they share (float32, us: 8 x 4096 x 2048 274 against 292 through
-      // the caches, 2 x 8192 x 3001 298 against 255).
-      const bool stream = channels * int64_t(sizeof(T)) % 128 == 0;
+      // Past the caches where steps are whole lines and the call's arrays together are more
+      // than the last one holds (float32, us: 8 x 4096 x 2048 275 against 292 through the
+      // caches, 4 x 4096 x 2048 145 and 153, with sums over the gradients right after 367 and
+      // 377, 196 and 196; but 8 x 512 x 2048, 192 MiB in all, 44 and 38, 66 and 57). Without
+      // whole lines neighbouring groups meet in the lines that they share (2 x 8192 x 3001
+      // 298 against 255).
+      const double bytes = (4.0 * double(e.total) + 2.0 * double(e.heads)) * double(time) * sizeof(T);
+      const bool stream = channels * int64_t(sizeof(T)) % 128 == 0 && bytes > kLastCache;
       const auto launch = e.width == 1  ? (stream ? backward<T, kOwn, true> : backward<T, kOwn, false>)
                           : e.pack == 1 ? (stream ? backward<T, kWave, true> : backward<T, kWave, false>)
                                         : (stream ? backward<T, kShared, true> : backward<T, kShared, false>);
