@@ -26,8 +26,9 @@ __device__ __forceinline__ float inverse(float x) {
 }
 __device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
 
-// keep = sigmoid(g) and take = 1 - keep, each to full precision: one of them is
-// 1 / (1 + exp(-|g|)), the other exp(-|g|) times it. Of a NaN both are NaN.
+// keep = sigmoid(g) and take = 1 - keep, each to full precision where it is a normal
+// number: one of them is 1 / (1 + exp(-|g|)), the other exp(-|g|) times it. Of a float
+// past 87.3 the smaller one is 0. Of a NaN both are NaN.
 template <typename T>
 __device__ __forceinline__ void gates(T g, T& keep, T& take) {
   const T small = exp_down(-__builtin_elementwise_abs(g));

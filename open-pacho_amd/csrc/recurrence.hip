@@ -31,17 +31,22 @@
 // backward for 8 x 4096 x 2048 float32 where chained tiles took 150 and 294: its
 // waves wait for each other every tile. For 1 x 65536 x 1024, segments of time in two
 // passes took 278 and 448 us, chained tiles 174 and 331. Past the caches, as they are
-// now, tiles take 141 and 275 us, 5.7 and 5.9 TB/s, and 156 and 301.
+// now, tiles take 141 and 275 us, 5.7 and 5.9 TB/s, and 160 and 306 (forward just
+// this size goes through them, 147, for its reader's sake).
 //
 // A head that has whole waves computes the sigmoid of a step once in the wave; its
-// gate's gradient is summed over the lanes through LDS. Rows that are no whole lines
-// cost most now: 65536 x 1000 in 8 heads of 125 channels, in waves of 63 and 62, takes
-// 308 us backward where 1024 channels take 237. Its dies read 1.29 times the arrays,
-// 1024 channels 1.04: each die has a head, whose lines the next one shares at both
-// ends in every step. Accesses past the caches make that worse (360 us), and tiles of
-// other dies' time would wait for workgroups that need not have started.
+// gate's gradient is summed over the lanes through LDS. Shared gates are furthest from
+// the bytes' time: 65536 x 1024 in 8 heads takes 243 us backward where they take 177,
+// 4.4 TB/s, and 65536 x 1000 308 of 173. The sums over lanes make a quarter more vector
+// instructions than gates of their own have (85.7 million against 68.6, 57% of the
+// SIMDs' cycles against 42%) and twice the scalar ones, and with 16 groups a wave waits
+// 58% of its time (53%); which of these bounds it has not been separated. Rows that are
+// no whole lines add the rest: in waves of 63 and 62 channels dies read 1.29 times the
+// arrays, with 1024 channels 1.04, as each die has a head, whose lines the next one
+// shares at both ends in every step. Accesses past the caches make that worse (360 us),
+// and tiles of other dies' time would wait for workgroups that need not have started.
 //
-// Runs of 16 and 8 steps (forward, backward; half as many float64) fill 72 and 90
+// Runs of 16 and 8 steps (forward, backward; half as many float64) fill 78 and 96
 // registers, so that three and two workgroups share a compute unit. Half as many
 // steps take 2 to 25% longer, twice as many backward 4 to 8%, four waves 3 to 15%.
 #include <type_traits>
@@ -824,7 +829,9 @@ bool plan_chain(Extents& e, int steps) {
   if (e.tiles < 3) return false;
   // Few groups are long in waiting from block to block: 65536 x 1000 in 8 heads, 16
   // groups, takes 308 us backward in blocks of 64 and 321 of 16; with 256 groups,
-  // 8 x 4096 x 2048, the readings of a block's tiles weigh more, 281 and 274.
+  // 8 x 4096 x 2048, the readings of a block's tiles weigh more, 281 and 274. Between
+  // them nothing was measured. The order in which a row's tiles meet, and with it the
+  // rounding, so depends on the rows beside it.
   e.span = e.groups >= 32 ? 16 : 64;
   return true;
 }

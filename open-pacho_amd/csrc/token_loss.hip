@@ -286,7 +286,10 @@ struct Share {
     rest = -T(__builtin_huge_val());
   }
 
-  // Past the caches: the gradient is larger than they are, or read by other kernels.
+  // Past the caches at every size (float32 with the gradient, in parentheses with a sum
+  // over it right after, us, past and through the caches): 8192 x 32000 353 (512) and 392
+  // (529), 65536 x 1000 103 (144) and 102 (138), 16384 x 1000 31 (46) and 34 (48), 16448 x 18
+  // 15 (28) and 16 (31).
   __device__ __forceinline__ void store(T* row, int length, int lane) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -466,8 +469,10 @@ __device__ __forceinline__ void leave_loss(const Call<T>& c, double sum, double 
 
 // LOSS: the policy loss and, unless c.grad is null, its gradient; else the
 // statistics alone, which leave the logits in the caches for the gradient's pass.
-// At 16 vectors a lane, four waves per SIMD (128 registers) keep a second
-// workgroup's loads in flight while one waits at its barriers.
+// Floats in 8 vectors a lane and more leave room for four waves a SIMD (128 registers):
+// four workgroups of 256 threads and two of 512, one of which loads while the other
+// waits at its barriers; of 1024 threads it is one, which loads and then stores. 256
+// threads with 16 vectors each take three workgroups.
 template <typename T, int L, int K, bool LOSS>
 __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L == 256 && K == 16 ? 3 : 4) void row_kernel(Call<T> c) {
   constexpr int kTeams = L > 256 ? 1 : 256 / L;

@@ -145,7 +145,8 @@ def gated_recurrence(x, gate, initial=None, *, resets=None):
     ``initial`` (..., channels) is the state before the first step, zero if not
     given. Where ``resets`` (..., time) is true the state before that step
     counts as zero, whatever it holds; an infinite state stays so until then, and is
-    NaN from a gate of ``-inf`` on. Returns every state, of x's shape.
+    NaN past a gate whose sigmoid is 0. Returns every state, of x's shape. Equal calls
+    give equal bits; a row's rounding may differ beside more or fewer rows.
     """
     ops, x, gate, initial, resets, sizes = _recurrence_operands("gated_recurrence", x, gate, initial, resets)
     return ops.result(ops.backend.gated_recurrence(x, gate, initial, resets, *sizes), x._shape)
@@ -193,7 +194,8 @@ def token_log_probs(logits, targets, *, mask=None):
     """``log softmax(logits)`` over the last axis at the integer ``targets``; zero where ``mask`` is false.
 
     Rows that the mask leaves out are not read, and their targets may be
-    anything. Another target outside the vocabulary gives NaN.
+    anything. Another target outside the vocabulary gives NaN. Equal calls give
+    equal bits; a long row's rounding may differ beside more or fewer rows.
     """
     ops, logits, tokens = _logits_operands("token_log_probs", logits, targets, mask)
     targets = ops.array("targets", targets, tokens, _INDICES)
