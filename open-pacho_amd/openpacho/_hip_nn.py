@@ -73,6 +73,8 @@ def _broadcast(backend, array, whole):
     if whole and array._shape == whole[:-1] + (1,):  # one for each row, the usual one
         return array._data, max(1, whole[-1]), max(1, array.size)
     found = _period(array._shape, whole)
+    if found is None and not prod(whole):
+        found = 1, 1  # nothing is read
     if found is None:
         strides = [prod(array._shape[axis + 1 :]) if d != 1 else 0 for axis, d in enumerate(array._shape)]
         return backend.gather(array, whole, 0, (0,) * (len(whole) - len(strides)) + tuple(strides)), 1, prod(whole)

@@ -78,3 +78,11 @@ def test_one_row_of_many_equal_pieces(hip):
         want = pattern[target % 8192] - total
         assert abs(found - want) <= 64 * np.finfo(np.float32).eps / 2, (target, found, want)
     hip.release_cached_memory()
+
+
+def test_advantages_broadcast_to_no_tokens(hip):
+    for whole, shape in [((3, 0, 5), (3, 1, 5)), ((2, 3, 0), (2, 1, 1)), ((0, 3, 4), (1, 3, 1)), ((0, 3, 6), (0, 1, 6)), ((2, 0, 3, 4), (2, 1, 3, 1)),
+                         ((2, 0), ()), ((3, 4, 0), (4, 1))]:  # fmt: skip
+        logits, advantages = (p.zeros(s, dtype=np.float32, backend=hip) for s in (whole + (6,), shape))
+        found = p.nn.policy_loss_grad(logits, np.zeros(whole, np.int64), np.zeros(whole, np.float32), advantages)
+        assert found[0].item() == 0 and found[1].shape == whole and found[2].shape == whole + (6,)
