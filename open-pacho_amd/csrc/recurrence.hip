@@ -126,8 +126,8 @@ __device__ __forceinline__ T apply(T a, T b, T h) {
 // An infinite state passes steps whose gates' product is too small for the type, and is
 // NaN past a gate of 0. Runs and tiles tell the two apart: a product that has become 0 of
 // gates above 0 is kept as -0. apply() makes NaN of both; where a NaN turns up the values
-// are formed again by apply_all(). (8 x 4096 x 2048 float32: forward 139.1 us without any
-// of this and 139.4, backward 273 and 275-278; 1 x 65536 x 1024 in 8 heads 120.6 and 121.9,
+// are formed again by apply_all(). (8 x 4096 x 2048 float32: forward, past the caches,
+// 139.1 us without any of this and 139.4, backward 273 and 275-278; 1 x 65536 x 1024 in 8 heads 120.6 and 121.9,
 // 243.6 and 244.4. Products and states told apart in every step of the way: 143 and 292,
 // 129 and 263.)
 template <typename T>
