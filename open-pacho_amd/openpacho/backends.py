@@ -141,6 +141,13 @@ class NumpyBackend:
     token_log_probs = staticmethod(_nn_host.token_log_probs)
     policy_loss = staticmethod(_nn_host.policy_loss)
     preference_loss = staticmethod(_nn_host.preference_loss)
+    causal_conv = staticmethod(_nn_host.causal_conv)
+    causal_conv_grad = staticmethod(_nn_host.causal_conv_grad)
+    selective_scan = staticmethod(_nn_host.selective_scan)
+    selective_scan_grad = staticmethod(_nn_host.selective_scan_grad)
+    residual_norm = staticmethod(_nn_host.residual_norm)
+    residual_norm_grad = staticmethod(_nn_host.residual_norm_grad)
+    distillation_loss = staticmethod(_nn_host.distillation_loss)
     adamw_load = staticmethod(_nn_host.adamw_load)
     adamw_moments = staticmethod(_nn_host.adamw_moments)
     adamw_step = staticmethod(_nn_host.adamw_step)

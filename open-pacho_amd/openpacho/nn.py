@@ -1,4 +1,4 @@
-"""Operators of model training: a gated recurrence, losses from logits, AdamW.
+"""Operators of model training: recurrences over time, residual norms, losses from logits, AdamW.
 
 Each works on resident arrays of one backend, float32 or float64 throughout,
 and returns new arrays; gradients are functions of their own, since arrays
@@ -15,6 +15,7 @@ these operators: call them between compiled functions.
 import math
 import operator
 from math import prod
+from typing import NamedTuple
 
 import numpy as np
 
@@ -110,6 +111,13 @@ def _number(what, value, least=None, below=None, infinite=False):
     return value
 
 
+def _positive(what, value):
+    value = _number(what, value)
+    if value <= 0:
+        raise ValueError(f"{what} must be positive")
+    return value
+
+
 # ---- gated recurrence ----------------------------------------------------------
 
 
@@ -179,6 +187,270 @@ def gated_recurrence_grad(grad, x, gate, h, initial=None, *, resets=None):
     return ops.result(dx, x._shape), ops.result(d_gate, gate._shape), first
 
 
+# ---- causal convolution ----------------------------------------------------------
+
+_MOST_TAPS = 8
+_ACTIVATIONS = {None: 0, "silu": 1}
+
+
+def _conv_weights(ops, channels, weight, bias, activation):
+    what = ops.what
+    weight = ops.array("weight", weight)
+    if len(weight._shape) != 2 or weight._shape[0] != channels:
+        raise ValueError(f"{what}: weight must have shape ({channels}, taps), got {weight.shape}")
+    taps = weight._shape[1]
+    if not 1 <= taps <= _MOST_TAPS:
+        raise ValueError(f"{what}: weight must have 1 to {_MOST_TAPS} taps, got {taps}")
+    if activation is not None and activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be None or 'silu', got {activation!r}")
+    return weight, ops.optional("bias", bias, (channels,)), taps, _ACTIVATIONS[activation]
+
+
+def _sequence_operands(what, x, resets, lengths, *others):
+    ops = _Operands(what, x, resets, lengths, *others)
+    x = ops.array("x", x)
+    if len(x._shape) < 2:
+        raise ValueError(f"{what}: x must have axes (..., time, channels), got {x.shape}")
+    lead, (time, channels) = x._shape[:-2], x._shape[-2:]
+    resets = ops.optional("resets", resets, lead + (time,), (_BOOL,))
+    lengths = ops.optional("lengths", lengths, lead, _INDICES)
+    return ops, x, resets, lengths, lead, (prod(lead), time, channels)
+
+
+def _conv_operands(what, x, weight, bias, initial, resets, lengths, activation, *others):
+    ops, x, resets, lengths, lead, sizes = _sequence_operands(what, x, resets, lengths, weight, bias, initial, *others)
+    weight, bias, taps, activation = _conv_weights(ops, sizes[2], weight, bias, activation)
+    window = lead + (taps - 1, sizes[2])
+    initial = ops.optional("initial", initial, window)
+    return ops, x, weight, bias, initial, resets, lengths, window, sizes + (taps, activation)
+
+
+def causal_conv(x, weight, bias=None, initial=None, *, resets=None, lengths=None, activation=None):
+    """A short convolution of each channel over time: (y, last inputs).
+
+    ``y_t = f(bias + sum_k weight[:, k] x_{t - taps + 1 + k})`` of x (..., time,
+    channels) with ``weight`` (channels, taps), of 1 to 8 taps; ``f`` is the
+    identity or, with ``activation="silu"``, v sigmoid(v). ``initial`` (...,
+    taps - 1, channels) are the inputs before the first step, zero if not given.
+    Where ``resets`` (..., time) is true, that step and later ones see the inputs
+    before it as zero. Rows end after ``lengths`` (...) steps (all of them if not
+    given, and at most): what is behind is not read and y is zero there. The
+    last inputs (..., taps - 1, channels), as a later step would see them, are
+    the ``initial`` of a call that goes on.
+    """
+    what = "causal_conv"
+    ops, x, weight, bias, initial, resets, lengths, window, sizes = _conv_operands(
+        what, x, weight, bias, initial, resets, lengths, activation
+    )
+    y, last = ops.backend.causal_conv(x, weight, bias, initial, resets, lengths, *sizes)
+    return ops.result(y, x._shape), ops.result(last, window)
+
+
+def causal_conv_step(x, weight, state, bias=None, *, activation=None):
+    """One token: (y, last inputs) of x (..., channels) after the inputs ``state`` (..., taps - 1, channels)."""
+    what = "causal_conv_step"
+    ops = _Operands(what, x, weight, state, bias)
+    x = ops.array("x", x)
+    if not x._shape:
+        raise ValueError(f"{what}: x must have axes (..., channels), got {x.shape}")
+    lead, channels = x._shape[:-1], x._shape[-1]
+    weight, bias, taps, activation = _conv_weights(ops, channels, weight, bias, activation)
+    state = ops.array("state", state, lead + (taps - 1, channels))
+    y, last = ops.backend.causal_conv(x, weight, bias, state, None, None, prod(lead), 1, channels, taps, activation)
+    return ops.result(y, x._shape), ops.result(last, state._shape)
+
+
+def causal_conv_grad(grad, x, weight, bias=None, initial=None, *, resets=None, lengths=None, activation=None):
+    """Gradients (x, weight, bias, initial) of ``causal_conv`` whose y has the gradient ``grad``.
+
+    Those of ``bias`` and ``initial`` are None where they are not given. The
+    last inputs' own gradient is not part of it. Equal calls give equal bits.
+    """
+    what = "causal_conv_grad"
+    ops, x, weight, bias, initial, resets, lengths, window, sizes = _conv_operands(
+        what, x, weight, bias, initial, resets, lengths, activation, grad
+    )
+    grad = ops.array("grad", grad, x._shape)
+    dx, d_weight, d_bias, d_initial = ops.backend.causal_conv_grad(grad, x, weight, bias, initial, resets, lengths, *sizes)
+    return (
+        ops.result(dx, x._shape),
+        ops.result(d_weight, weight._shape),
+        None if bias is None else ops.result(d_bias, bias._shape),
+        None if initial is None else ops.result(d_initial, window),
+    )
+
+
+# ---- selective scan ----------------------------------------------------------------
+
+_MOST_STATES = 256
+
+
+def _scan_parameters(ops, channels, a_log, skip, delta_bias):
+    a_log = ops.array("a_log", a_log)
+    if len(a_log._shape) != 2 or a_log._shape[0] != channels:
+        raise ValueError(f"{ops.what}: a_log must have shape ({channels}, states), got {a_log.shape}")
+    states = a_log._shape[1]
+    if not 1 <= states <= _MOST_STATES:
+        raise ValueError(f"{ops.what}: a_log must have 1 to {_MOST_STATES} states, got {states}")
+    return a_log, ops.optional("skip", skip, (channels,)), ops.optional("delta_bias", delta_bias, (channels,)), states
+
+
+def _projections(ops, steps, channels, states, b, c):
+    b = ops.array("b", b)
+    if len(b._shape) != len(steps) + 2 or b._shape[:-2] != steps or b._shape[-1] != states:
+        raise ValueError(f"{ops.what}: b must have shape {steps} and axes (groups, {states}), got {b.shape}")
+    groups = b._shape[-2]
+    if channels % groups if groups else channels:
+        raise ValueError(f"{ops.what}: {groups} groups do not divide {channels} channels")
+    if groups and not channels:
+        raise ValueError(f"{ops.what}: {groups} groups without channels")
+    return b, ops.array("c", c, b._shape), groups
+
+
+def _scan_operands(what, x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths, *others):
+    ops, x, resets, lengths, lead, sizes = _sequence_operands(
+        what, x, resets, lengths, delta, a_log, b, c, skip, gate, initial, delta_bias, *others
+    )
+    delta = ops.array("delta", delta, x._shape)
+    a_log, skip, delta_bias, states = _scan_parameters(ops, sizes[2], a_log, skip, delta_bias)
+    b, c, groups = _projections(ops, x._shape[:-1], sizes[2], states, b, c)
+    gate = ops.optional("gate", gate, x._shape)
+    whole = lead + (sizes[2], states)
+    initial = ops.optional("initial", initial, whole)
+    return ops, (x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths), whole, sizes + (groups, states)
+
+
+def selective_scan(x, delta, a_log, b, c, skip=None, gate=None, initial=None, *, delta_bias=None, resets=None, lengths=None):
+    """A state space recurrence whose steps the inputs select: (y, last states).
+
+    With ``dt = softplus(delta + delta_bias)`` each channel has ``states`` states
+    ``h_t = exp(-dt exp(a_log)) h_{t-1} + dt x_t b_t`` and
+    ``y_t = (sum c_t h_t + skip x_t) gate_t sigmoid(gate_t)``, without the last
+    factor if ``gate`` is not given. Shapes: x, delta, gate (..., time, channels);
+    a_log (channels, states), of 1 to 256 states; b, c (..., time, groups, states),
+    whose groups divide the channels; skip, delta_bias (channels,); ``initial``
+    (..., channels, states), the states before the first step, zero if not
+    given. Where ``resets`` (..., time) is true the states before that step count
+    as zero, whatever they hold. Rows end after ``lengths`` (...) steps (all of
+    them if not given, and at most): what is behind is not read, y is zero there
+    and the last states (..., channels, states) are those of the row's last step.
+    Equal calls give equal bits; a row's rounding may differ beside more or fewer rows.
+    """
+    ops, given, whole, sizes = _scan_operands("selective_scan", x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths)
+    y, last = ops.backend.selective_scan(*given, *sizes)
+    return ops.result(y, given[0]._shape), ops.result(last, whole)
+
+
+def selective_scan_step(x, delta, a_log, b, c, state, skip=None, gate=None, *, delta_bias=None):
+    """One token: (y, new states) of x, delta, gate (..., channels) and b, c (..., groups, states), from ``state``."""
+    what = "selective_scan_step"
+    ops = _Operands(what, x, delta, a_log, b, c, state, skip, gate, delta_bias)
+    x = ops.array("x", x)
+    if not x._shape:
+        raise ValueError(f"{what}: x must have axes (..., channels), got {x.shape}")
+    lead, channels = x._shape[:-1], x._shape[-1]
+    delta = ops.array("delta", delta, x._shape)
+    a_log, skip, delta_bias, states = _scan_parameters(ops, channels, a_log, skip, delta_bias)
+    b, c, groups = _projections(ops, lead, channels, states, b, c)
+    gate = ops.optional("gate", gate, x._shape)
+    state = ops.array("state", state, lead + (channels, states))
+    y, last = ops.backend.selective_scan(
+        x, delta, a_log, b, c, skip, gate, state, delta_bias, None, None, prod(lead), 1, channels, groups, states
+    )
+    return ops.result(y, x._shape), ops.result(last, state._shape)
+
+
+class ScanGrads(NamedTuple):
+    """Gradients of ``selective_scan``; None for what is not given."""
+
+    x: object
+    delta: object
+    a_log: object
+    b: object
+    c: object
+    skip: object
+    gate: object
+    delta_bias: object
+    initial: object
+
+
+def selective_scan_grad(grad, x, delta, a_log, b, c, skip=None, gate=None, initial=None, *, delta_bias=None, resets=None, lengths=None, grad_state=None):
+    """Gradients (a ``ScanGrads``) of ``selective_scan`` whose y has the gradient ``grad`` and whose last
+    states have ``grad_state`` (zero if not given).
+
+    b and c get the sums over their group's channels, a_log, skip and
+    delta_bias those over all steps. Equal calls give equal bits.
+    """
+    what = "selective_scan_grad"
+    ops, given, whole, sizes = _scan_operands(
+        what, x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths, grad, grad_state
+    )
+    grad, grad_state = ops.array("grad", grad, given[0]._shape), ops.optional("grad_state", grad_state, whole)
+    found = ops.backend.selective_scan_grad(grad, grad_state, *given, *sizes)
+    like = given[:7] + (given[8], given[7])
+    return ScanGrads(*(None if array is None else ops.result(data, array._shape) for data, array in zip(found, like)))
+
+
+# ---- residual stream and norms -------------------------------------------------------
+
+
+def _norm_operands(what, x, stream, weight, post_weight, gate, scale, eps, *others):
+    ops = _Operands(what, x, stream, weight, post_weight, gate, *others)
+    x = ops.array("x", x)
+    if not x._shape or not x._shape[-1]:
+        raise ValueError(f"{what}: x must have axes (..., channels), none of it empty, got {x.shape}")
+    lead, channels = x._shape[:-1], x._shape[-1]
+    weight = ops.array("weight", weight, (channels,))
+    post_weight = ops.optional("post_weight", post_weight, (channels,))
+    divide = 1
+    if gate is not None:
+        gate = ops.array("gate", gate)
+        # Leading axes as x has them, then ones: a factor for `divide` neighbouring rows.
+        whole = (1,) * (len(x._shape) - len(gate._shape)) + gate._shape
+        kept = max((i + 1 for i, d in enumerate(whole[:-1]) if d != 1), default=0)
+        if whole != lead[:kept] + (1,) * (len(lead) - kept) + (channels,):
+            raise ValueError(f"{what}: gate must have x's channels, and x's leading axes up to one and 1 after it, got {gate.shape} for {x.shape}")
+        divide = prod(lead[kept:])
+    scale, eps = _number("scale", scale), _number("eps", eps, 0)
+    if eps < _TINY[ops.dtype]:
+        raise ValueError(f"eps must be positive, and at least {_TINY[ops.dtype]} for {ops.dtype}")
+    return ops, x, weight, post_weight, gate, (prod(lead), channels, divide, scale, eps)
+
+
+def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale=1.0, eps=1e-6):
+    """The residual stream after a block, and the next block's normed input: (stream, normed).
+
+    With ``rms(v) = v / sqrt(mean(v v) + eps)`` over the last axis, for x, the
+    block's output, and the stream before it:
+    ``stream = residual + scale gate rms(x) post_weight`` and
+    ``normed = rms(stream) weight``. Without ``post_weight`` x itself takes the
+    place of rms(x) post_weight; without ``gate`` it is one. ``gate`` has the
+    channels, and any number of x's leading axes followed by axes of 1: one
+    factor for each token and channel, each sequence and channel, or each channel.
+    """
+    what = "residual_norm"
+    ops, x, weight, post_weight, gate, sizes = _norm_operands(what, x, residual, weight, post_weight, gate, scale, eps)
+    residual = ops.array("residual", residual, x._shape)
+    stream, normed = ops.backend.residual_norm(x, residual, weight, post_weight, gate, *sizes)
+    return ops.result(stream, x._shape), ops.result(normed, x._shape)
+
+
+def residual_norm_grad(grad_stream, grad_normed, x, stream, weight, *, post_weight=None, gate=None, scale=1.0, eps=1e-6):
+    """Gradients (x, residual, weight, post_weight, gate) of ``residual_norm``, whose ``stream`` it found.
+
+    ``grad_stream`` and ``grad_normed`` are the gradients of its two results.
+    What is not given has None. Equal calls give equal bits.
+    """
+    what = "residual_norm_grad"
+    ops, x, weight, post_weight, gate, sizes = _norm_operands(
+        what, x, stream, weight, post_weight, gate, scale, eps, grad_stream, grad_normed
+    )
+    stream = ops.array("stream", stream, x._shape)
+    grad_stream, grad_normed = ops.array("grad_stream", grad_stream, x._shape), ops.array("grad_normed", grad_normed, x._shape)
+    found = ops.backend.residual_norm_grad(grad_stream, grad_normed, x, stream, weight, post_weight, gate, *sizes)
+    like = (x, x, weight, post_weight, gate)
+    return tuple(None if array is None else ops.result(data, array._shape) for data, array in zip(found, like))
+
 # ---- losses from logits ----------------------------------------------------------
 
 
@@ -216,9 +488,7 @@ def _policy(what, gradient, logits, actions, old_log_probs, advantages, referenc
     if kl_weight and reference is None:
         raise ValueError(f"{what}: kl_weight needs reference_log_probs")
     if count is not None:
-        count = _number("count", count)
-        if count <= 0:
-            raise ValueError("count must be positive")
+        count = _positive("count", count)
     loss, log_probs, d_logits = ops.backend.policy_loss(
         logits, actions, old_log_probs, advantages, reference if kl_weight else None, mask, low, high, kl_weight, count, gradient
     )
@@ -279,6 +549,52 @@ def preference_loss_grad(logits, targets, reference_log_probs, *, mask=None, bet
     """``preference_loss`` and its gradient: (loss, responses' log-probabilities, gradient of the logits)."""
     return _preference("preference_loss_grad", True, logits, targets, reference_log_probs, mask, beta, smoothing)
 
+
+_MOST_LISTED = 1024
+
+
+def _distillation(what, gradient, logits, indices, teacher_logits, teacher_rest, mask, temperature, count):
+    ops, logits, tokens = _logits_operands(what, logits, indices, teacher_logits, teacher_rest, mask)
+    indices = ops.array("indices", indices, dtypes=_INDICES)
+    if not indices._shape or indices._shape[:-1] != tokens or not 1 <= indices._shape[-1] <= _MOST_LISTED:
+        raise ValueError(f"{what}: indices must have shape {tokens} and an axis of 1 to {_MOST_LISTED} entries, got {indices.shape}")
+    teacher_logits = ops.array("teacher_logits", teacher_logits, indices._shape)
+    teacher_rest = ops.optional("teacher_rest", teacher_rest, tokens)
+    mask = ops.optional("mask", mask, tokens, (_BOOL,))
+    temperature = _positive("temperature", temperature)
+    if temperature < _TINY[ops.dtype] or 1 / temperature < _TINY[ops.dtype]:
+        raise ValueError(f"temperature is out of range: {temperature}")
+    if count is not None:
+        count = _positive("count", count)
+    loss, losses, d_logits = ops.backend.distillation_loss(
+        logits, indices, teacher_logits, teacher_rest, mask, temperature, count, gradient
+    )
+    found = ops.result(loss, ()), ops.result(losses, tokens)
+    return found + (ops.result(d_logits, logits.shape),) if gradient else found
+
+
+def distillation_loss(logits, indices, teacher_logits, teacher_rest=None, *, mask=None, temperature=1.0, count=None):
+    """Divergence of the logits' softmax from a teacher known by its largest logits: (loss, losses of the tokens).
+
+    ``teacher_logits`` (..., entries) stand at the vocabulary's ``indices`` (...,
+    entries), 1 to 1024 of them. Both sides are divided by ``temperature``. The
+    teacher's distribution p is the softmax of its list, q that of all logits,
+    and a token's loss is ``sum p (log p - log q)`` over the list. With
+    ``teacher_rest`` (...), the log-sum-exp of the teacher's other logits over the
+    temperature, p has the rest of the vocabulary as one more class, whose q is
+    the sum over all logits that the list does not name. An entry of -inf is
+    none, and its index may be anything; another index outside the vocabulary
+    gives NaN; an index that stands twice is two entries of the sum. The loss is
+    the sum over the tokens that ``mask`` keeps, divided by their number or by
+    ``count``; zero where it keeps none. Masked rows are not read and have
+    losses of zero. Equal calls give equal bits.
+    """
+    return _distillation("distillation_loss", False, logits, indices, teacher_logits, teacher_rest, mask, temperature, count)
+
+
+def distillation_loss_grad(logits, indices, teacher_logits, teacher_rest=None, *, mask=None, temperature=1.0, count=None):
+    """``distillation_loss`` and its gradient: (loss, losses of the tokens, gradient of the logits)."""
+    return _distillation("distillation_loss_grad", True, logits, indices, teacher_logits, teacher_rest, mask, temperature, count)
 
 # ---- AdamW ---------------------------------------------------------------------
 
