@@ -294,6 +294,19 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
                        const void* reference, const void* mask, void* loss, void* sums, void* grad, int64_t pairs,
                        int64_t time, int64_t vocab, double beta, double smoothing);
 
+/* Divergence of rows x vocab logits from a teacher that is known by `entries` (1
+ * to 1024) logits of each row, which stand at `indices` (rows, entries; index_dtype
+ * HP_I32 or HP_I64): sum p (log p - log q), where q is the softmax of the logits
+ * over the temperature and p that of the list's, to which `teacher_rest` (rows;
+ * NULL: none) adds a class for all logits that the list does not name, by its
+ * logit over the temperature. An entry of -inf is none; another index outside
+ * the vocabulary gives NaN. Writes the 0-d loss, a sum over the rows that `mask`
+ * keeps divided by `count`, or by their number (at least 1) if count is 0, the
+ * rows' losses (0 for rows left out) and unless NULL the gradient of the logits. */
+int hp_distillation_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, const void* indices, const void* teacher,
+                         const void* teacher_rest, const void* mask, void* loss, void* losses, void* grad, int64_t rows,
+                         int64_t vocab, int64_t entries, double temperature, double count);
+
 /* AdamW over `count` tensors of sizes[i] elements, float32 or float64. The
  * state holds both moments in the tensors' type (bits 0) or in 8 bits with a
  * float32 scale for every 256 elements of a tensor (bits 8, float32 tensors):

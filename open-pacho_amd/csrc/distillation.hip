@@ -1,0 +1,440 @@
+// Divergence of rows of logits from a teacher that is known by its largest logits,
+// and its gradient.
+//
+//   q_j = exp((z_j - m) / T) / S,  S = sum_j exp((z_j - m) / T)
+//   p_e = softmax over the list's t_e / T (and the rest's logit, if there is one)
+//   loss = sum_e p_e (log p_e - log q_{i(e)}) + p_r (log p_r - log (R / S))
+//   T dloss/dz_j = q_j - sum_{i(e) = j} p_e            where the list names j
+//                = q_j - p_r exp((z_j - m) / T) / R    elsewhere (p_r = 0 without a rest)
+//
+// with R the sum S without the terms that the list names. R is formed as a sum of its
+// own, not as a difference: where the list holds nearly all of q the rest would lose
+// its digits. Which logits are named stands in a bit for each of a row, in LDS; a vector's
+// bits are one read. Bound: HBM, each logit read once and each gradient written
+// once, as for the losses of token_loss.hip, whose teams and pieces of rows it shares.
+//
+// The list is the work of one wave, or of a team within one: its softmax, its bits and
+// its terms of the loss, each entry's logit read again. The named places of the
+// gradient are written once more, after a barrier, as p_e has no place in the registers
+// that hold a row. An index that stands twice is found by the bit that it finds set;
+// then every entry adds up the entries of its index.
+#include "token_rows.h"
+
+namespace {
+
+template <typename T>
+struct Call : LossCall<T> {
+  const void* indices;
+  int wide_indices;  // int64, else int32
+  int entries;       // of a row's list
+  const T *teacher, *teacher_rest;
+  T* losses;
+  double inverse;  // of the temperature
+
+  __device__ __forceinline__ int64_t index(int64_t row, int entry) const {
+    const int64_t at = row * entries + entry;
+    return wide_indices ? static_cast<const int64_t*>(indices)[at] : static_cast<const int32_t*>(indices)[at];
+  }
+  __device__ __forceinline__ double logit(int64_t row, int entry) const { return double(teacher[row * entries + entry]) * inverse; }
+  __device__ __forceinline__ auto scaled() const {
+    const T by = T(inverse);
+    return [by](T x) { return x * by; };
+  }
+};
+
+// Bits of the logits that a list names, those from `start` on.
+struct Bits {
+  static constexpr bool some = true;
+  unsigned* words;
+
+  // For the vector at i, which is a multiple of its width.
+  __device__ __forceinline__ unsigned bits(int i) const { return words[i >> 5] >> (i & 31); }
+  __device__ __forceinline__ bool one(int i) const { return words[i >> 5] >> (i & 31) & 1; }
+};
+
+// The team's stores to LDS and memory before are seen by its loads after.
+__device__ __forceinline__ void team_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// A row's list, by L <= 64 neighbouring lanes.
+template <typename T, int L>
+struct List {
+  double top, log_total;  // of the teacher's logits
+  T inverse, rest;        // 1 / their sum of exponentials, and the rest's p
+  T spoiled;              // 0, or NaN where an entry stands outside the vocabulary
+  bool repeats;           // an index stands twice
+
+  __device__ __forceinline__ T share(double logit) const { return hpd::exp_down(T(logit - top)) * inverse; }
+
+  __device__ __forceinline__ void read(const Call<T>& c, int64_t row, int lane) {
+    const double none = -__builtin_huge_val(), other = c.teacher_rest ? double(c.teacher_rest[row]) : none;
+    double most = other;
+    for (int e = lane; e < c.entries; e += L) most = larger(most, c.logit(row, e));
+    top = team_reduce<L>(most, [](double a, double b) { return larger(a, b); });
+    T sum = lane == 0 ? hpd::exp_down(T(other - top)) : T(0);
+    bool outside = false;
+    for (int e = lane; e < c.entries; e += L) {
+      const double logit = c.logit(row, e);
+      const int64_t i = c.index(row, e);
+      sum += hpd::exp_down(T(logit - top));
+      outside = outside || (logit != none && (i < 0 || i >= c.vocab));
+    }
+    sum = team_reduce<L>(sum, [](T a, T b) { return a + b; });
+    outside = team_reduce<L>(int(outside), [](int a, int b) { return a | b; });
+    inverse = T(1) / sum;
+    log_total = log_wide(sum);
+    rest = c.teacher_rest ? share(other) : T(0);
+    spoiled = outside || sum != sum ? T(__builtin_nan("")) : T(0);
+  }
+
+  // f(entry, its index) for every entry of the lane that names one of [start, start + length).
+  template <typename F>
+  __device__ __forceinline__ static void each(const Call<T>& c, int64_t row, int lane, int64_t start, int64_t length, F&& f) {
+    for (int e = lane; e < c.entries; e += L) {
+      const int64_t i = c.index(row, e);
+      if (i >= start && i < start + length && i < c.vocab && c.logit(row, e) != -__builtin_huge_val()) f(e, i);
+    }
+  }
+
+  __device__ __forceinline__ void set(const Call<T>& c, Bits bits, int64_t row, int lane, int64_t start, int64_t length) {
+    bool again = false;
+    each(c, row, lane, start, length, [&](int, int64_t i) {
+      const unsigned at = unsigned(i - start), bit = 1u << (at & 31);
+      again = again || (atomicOr(&bits.words[at >> 5], bit) & bit);
+    });
+    repeats = team_reduce<L>(int(again), [](int a, int b) { return a | b; });
+  }
+  __device__ __forceinline__ static void clear(const Call<T>& c, Bits bits, int64_t row, int lane, int64_t start, int64_t length) {
+    each(c, row, lane, start, length, [&](int, int64_t i) { bits.words[(i - start) >> 5] = 0; });
+  }
+
+  // The row's loss from the statistics of its logits, for every lane of the team.
+  __device__ __forceinline__ double loss(const Call<T>& c, int64_t row, int lane, T row_top, T total, T unlisted) const {
+    const double log_row = log_wide(total);
+    double sum = 0;
+    each(c, row, lane, 0, c.vocab, [&](int e, int64_t i) {
+      const double logit = c.logit(row, e);
+      const T p = share(logit);
+      const double log_q = (double(c.logits[row * c.vocab + i]) - double(row_top)) * c.inverse - log_row;
+      if (p != T(0)) sum += double(p) * ((logit - top - log_total) - log_q);
+    });
+    if (lane == 0 && rest != T(0)) {
+      sum += double(rest) * ((double(c.teacher_rest[row]) - top - log_total) - (log_wide(unlisted) - log_row));
+    }
+    sum = team_reduce<L>(sum, [](double a, double b) { return a + b; });
+    return sum + double(spoiled) + (total == total ? 0.0 : double(total));
+  }
+
+  // The gradient at the named places of [start, start + length), whose other terms are
+  // stored already: (q - p) weight.
+  __device__ __forceinline__ void correct(const Call<T>& c, int64_t row, int lane, int64_t start, int64_t length, T row_top, T row_inverse,
+                                          T weight) const {
+    const auto scaled = c.scaled();
+    each(c, row, lane, start, length, [&](int e, int64_t i) {
+      T p = T(0);
+      if (repeats) {
+        for (int k = 0; k < c.entries; ++k) {
+          if (c.index(row, k) == i) p += share(c.logit(row, k));
+        }
+      } else {
+        p = share(c.logit(row, e));
+      }
+      const T q = hpd::exp_down(scaled(c.logits[row * c.vocab + i] - row_top)) * row_inverse;
+      c.grad[row * c.vocab + i] = (q - p) * weight;
+    });
+  }
+};
+
+// What a gradient's value exp((z - m) / T) is multiplied by where the list does not name it.
+template <typename T>
+__device__ __forceinline__ T unlisted_factor(T row_inverse, T rest, T unlisted) {
+  return row_inverse - (rest == T(0) || unlisted == T(0) ? T(0) : rest / unlisted);
+}
+
+// REST: the rest of the teacher's mass is a class of its own.
+template <typename T, int L, int K, bool REST>
+__global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L == 256 && K == 16 ? 3 : 4) void row_kernel(Call<T> c) {
+  constexpr int kTeams = L > 256 ? 1 : 256 / L, kLanes = L < 64 ? L : 64;  // lanes that work on the list
+  using S = Share<T, L, K>;
+  constexpr int kWords = (L * K * S::W + 31) / 32;
+  __shared__ Meet<T, S::kDeep, REST ? 2 : 1> meet;
+  __shared__ unsigned words[kTeams][kWords];
+  __shared__ T told[2];  // by the wave of the list: rest, spoiled
+  const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : threadIdx.x / L;
+  const bool lists = L <= 64 || threadIdx.x < 64;
+  const int length = int(c.vocab);
+  const auto scaled = c.scaled();
+  const Bits bits{words[team]};
+  for (int i = threadIdx.x; i < kTeams * kWords; i += blockDim.x) words[0][i] = 0;
+  __syncthreads();
+  const double factor = scale_of(c);
+  double sum = 0;
+  int turn = 0;
+  // Teams of several waves are alone in their workgroup, as in token_loss.hip.
+  for (int64_t row = int64_t(blockIdx.x) * kTeams + team; row < c.rows; row += int64_t(gridDim.x) * kTeams) {
+    T* out = c.grad ? c.grad + row * c.vocab : nullptr;
+    S share;
+    if (!c.kept(row)) {
+      if (lane == 0) c.losses[row] = T(0);
+      if (out) {
+        share.each(length, lane, [](T& v, int, int) { v = T(0); });
+        share.store(out, length, lane);
+      }
+      continue;
+    }
+    share.template load<true>(c.logits + row * c.vocab, length, lane);
+    List<T, kLanes> list{};
+    if (lists) {
+      list.read(c, row, lane);
+      list.set(c, bits, row, lane, 0, length);
+      if constexpr (L > 64) {
+        if (lane == 0) told[0] = list.rest, told[1] = list.spoiled;
+      } else {
+        team_fence();
+      }
+    }
+    T tops[S::kDeep], top, total, unlisted = T(0);
+    if constexpr (REST) share.statistics(length, lane, meet, turn, tops, top, total, scaled, bits, unlisted);
+    else share.statistics(length, lane, meet, turn, tops, top, total, scaled, NoNames(), unlisted);
+    turn ^= 1;
+    const T inverse = T(1) / total;
+    if (out) {
+      const T rest = L > 64 ? told[0] : list.rest, weight = T(factor * c.inverse) + (L > 64 ? told[1] : list.spoiled);
+      const T inner = inverse * weight, outer = REST ? unlisted_factor(inverse, rest, unlisted) * weight : inner;
+      if constexpr (REST) {
+        share.each_named(length, lane, bits, [&](T& v, bool named, int d) { v = v * S::part(tops[d], top, scaled) * (named ? inner : outer); });
+      } else {
+        share.each(length, lane, [&](T& v, int, int d) { v = v * (S::part(tops[d], top, scaled) * inner); });
+      }
+      share.store(out, length, lane);
+      if constexpr (L > 64) __syncthreads();
+      else team_fence();
+      if (lists) list.correct(c, row, lane, 0, length, top, inverse, weight);
+    }
+    if (lists) {
+      const double loss = list.loss(c, row, lane, top, total, unlisted);
+      if (lane == 0) c.losses[row] = T(loss), sum += loss;
+      list.clear(c, bits, row, lane, 0, length);
+      if constexpr (L <= 64) team_fence();
+    }
+  }
+  leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
+}
+
+// Statistics of one piece of a row: parts[row * pieces + piece].
+template <typename T, bool REST>
+__global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __restrict__ part_tops, T* __restrict__ part_totals,
+                                                              T* __restrict__ part_seconds, int pieces, int piece) {
+  using S = Share<T, kPieceThreads, kPieceLoads>;
+  __shared__ Meet<T, 1, REST ? 2 : 1> meet;
+  __shared__ unsigned words[REST ? kPieceThreads * kPieceLoads * S::W / 32 : 1];
+  const auto scaled = c.scaled();
+  const Bits bits{words};
+  if constexpr (REST) {
+    for (unsigned i = threadIdx.x; i < sizeof(words) / 4; i += kPieceThreads) words[i] = 0;
+    __syncthreads();
+  }
+  int turn = 0;
+  for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
+    const int64_t row = part / pieces;
+    if (!c.kept(row)) continue;
+    const int64_t start = (part - row * pieces) * piece;
+    const int length = piece_end(c.vocab - start, piece);
+    T tops[1], top, total, second;
+    S share;
+    share.template load<true>(c.logits + row * c.vocab + start, length, threadIdx.x);
+    List<T, 64> list;
+    if constexpr (REST) {
+      // Seen by all at the first of the statistics' barriers, and read before the second.
+      if (threadIdx.x < 64) list.set(c, bits, row, threadIdx.x, start, length);
+      share.statistics(length, threadIdx.x, meet, turn, tops, top, total, scaled, bits, second);
+      if (threadIdx.x < 64) list.clear(c, bits, row, threadIdx.x, start, length);
+    } else {
+      share.statistics(length, threadIdx.x, meet, turn, tops, top, total, scaled, NoNames(), second);
+    }
+    turn ^= 1;
+    if (threadIdx.x == 0) {
+      part_tops[part] = top, part_totals[part] = total;
+      if constexpr (REST) part_seconds[part] = second;
+    }
+  }
+}
+
+// What a row's pieces add up to, by every wave for itself; a lane's pieces join first,
+// one after the other in 64 bits (join_pieces, with two sums).
+template <typename T, bool REST, typename Scale>
+__device__ __forceinline__ void join_row(const T* tops, const T* totals, const T* seconds, int pieces, Scale scaled, T& top, T& total, T& second) {
+  const int lane = threadIdx.x & 63;
+  const T none = -T(__builtin_huge_val());
+  const bool has = lane < pieces;
+  T own = has ? tops[lane] : none;
+  double sum = has ? totals[lane] : T(0), other = REST && has ? seconds[lane] : T(0);
+  for (int k = lane + 64; k < pieces; k += 64) {
+    const T next = larger(own, tops[k]);
+    const double before = own == none ? 1.0 : double(hpd::exp_down(scaled(own - next)));
+    const double here = tops[k] == none ? 1.0 : double(hpd::exp_down(scaled(tops[k] - next)));
+    sum = sum * before + double(totals[k]) * here;
+    if constexpr (REST) other = other * before + double(seconds[k]) * here;
+    own = next;
+  }
+  join(has, own, T(sum), top, total, scaled);
+  T again;
+  if constexpr (REST) join(has, own, T(other), again, second, scaled);
+}
+
+// The rows' losses from their pieces, a workgroup each, as wide as piece_grad_kernel, so
+// that both add the losses in one order.
+template <typename T, bool REST>
+__global__ __launch_bounds__(kPieceThreads) void finish_kernel(Call<T> c, const T* __restrict__ part_tops, const T* __restrict__ part_totals,
+                                                               const T* __restrict__ part_seconds, int pieces) {
+  const double factor = scale_of(c);
+  const int64_t row = blockIdx.x;
+  double loss = 0;
+  if (threadIdx.x < 64) {
+    if (c.kept(row)) {
+      T top, total, unlisted = T(0);
+      join_row<T, REST>(part_tops + row * pieces, part_totals + row * pieces, part_seconds + row * pieces, pieces, c.scaled(), top, total, unlisted);
+      List<T, 64> list;
+      list.read(c, row, threadIdx.x);
+      loss = list.loss(c, row, threadIdx.x, top, total, unlisted);
+    }
+    if (threadIdx.x == 0) c.losses[row] = T(loss);
+  }
+  leave_loss(c, loss, factor, blockIdx.x, gridDim.x);
+}
+
+// The gradient of one piece of a row from the statistics of its pieces, which every
+// workgroup joins for itself; that of the first piece leaves the row's loss.
+template <typename T, bool REST>
+__global__ __launch_bounds__(kPieceThreads) void piece_grad_kernel(Call<T> c, const T* __restrict__ part_tops, const T* __restrict__ part_totals,
+                                                                   const T* __restrict__ part_seconds, int pieces, int piece) {
+  using S = Share<T, kPieceThreads, kPieceLoads>;
+  __shared__ unsigned words[kPieceThreads * kPieceLoads * S::W / 32];
+  __shared__ T told[2];
+  const int lane = threadIdx.x;
+  const auto scaled = c.scaled();
+  const Bits bits{words};
+  for (unsigned i = threadIdx.x; i < sizeof(words) / 4; i += kPieceThreads) words[i] = 0;
+  __syncthreads();
+  const double factor = scale_of(c);
+  for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
+    const int64_t row = part / pieces;
+    const bool first = part == row * pieces;
+    const int64_t start = (part - row * pieces) * piece;
+    const int length = piece_end(c.vocab - start, piece);
+    T* out = c.grad + row * c.vocab + start;
+    double loss = 0;
+    S share;
+    if (c.kept(row)) {
+      share.template load<true>(c.logits + row * c.vocab + start, length, lane);
+      List<T, 64> list{};
+      if (lane < 64) {
+        list.read(c, row, lane);
+        list.set(c, bits, row, lane, start, length);
+        if (lane == 0) told[0] = list.rest, told[1] = list.spoiled;
+      }
+      T top, total, unlisted = T(0);
+      join_row<T, REST>(part_tops + row * pieces, part_totals + row * pieces, part_seconds + row * pieces, pieces, scaled, top, total, unlisted);
+      __syncthreads();
+      const T inverse = T(1) / total, weight = T(factor * c.inverse) + told[1];
+      const T inner = inverse * weight, outer = REST ? unlisted_factor(inverse, told[0], unlisted) * weight : inner;
+      share.each_named(length, lane, bits, [&](T& v, bool named, int) { v = hpd::exp_down(scaled(v - top)) * (!REST || named ? inner : outer); });
+      share.store(out, length, lane);
+      __syncthreads();
+      if (lane < 64) {
+        list.correct(c, row, lane, start, length, top, inverse, weight);
+        list.clear(c, bits, row, lane, start, length);
+        if (first) loss = list.loss(c, row, lane, top, total, unlisted);
+      }
+    } else {
+      share.each(length, lane, [](T& v, int, int) { v = T(0); });
+      share.store(out, length, lane);
+    }
+    if (first) {
+      if (lane == 0) c.losses[row] = T(loss);
+      leave_loss(c, loss, factor, unsigned(row), unsigned(c.rows));
+    }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------
+
+// Whether a call takes teams: as the losses of token_loss.hip do.
+template <typename T>
+bool teams_serve(const Call<T>& c) {
+  if (c.vocab <= kPieceThreads * kPieceLoads * Vec<T>::width) return true;
+  return c.grad && teams_hold<T>(c.rows, c.vocab);
+}
+
+// Returns how many sums of losses there are.
+template <typename T, bool REST>
+int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
+  unsigned blocks = 0;
+  if (teams_serve(c) && with_team<T>(c.vocab, [&](auto l, auto k) {
+        constexpr int L = l, K = k, threads = L > 256 ? L : 256;
+        blocks = unsigned(std::min<int64_t>(hp::ceil_div(c.rows, threads / L), 16384));
+        plan_losses(ctx, scratch, c, blocks, blocks);
+        row_kernel<T, L, K, REST><<<blocks, threads, 0, ctx->stream>>>(c);
+        hp::check_launch("distillation rows");
+      })) {
+    return blocks;
+  }
+  const Pieces<T> pieces(c.rows, c.vocab);
+  const int64_t parts = c.rows * pieces.count;
+  T *tops = scratch.take<T>(parts), *totals = scratch.take<T>(parts), *seconds = scratch.take<T>(REST ? parts : 1);
+  const unsigned grid = loop_grid(parts);
+  hp::require(c.rows <= hp::kMaxGrid, "too many long rows for one launch");
+  blocks = unsigned(c.rows);
+  plan_losses(ctx, scratch, c, blocks, c.grad ? grid : blocks);
+  stats_kernel<T, REST><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, seconds, pieces.count, pieces.length);
+  hp::check_launch("distillation statistics");
+  if (c.grad) piece_grad_kernel<T, REST><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, seconds, pieces.count, pieces.length);
+  else finish_kernel<T, REST><<<blocks, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, seconds, pieces.count);
+  hp::check_launch("distillation losses");
+  return blocks;
+}
+
+}  // namespace
+
+extern "C" {
+
+int hp_distillation_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logits, const void* indices, const void* teacher,
+                         const void* teacher_rest, const void* mask, void* loss, void* losses, void* grad, int64_t rows,
+                         int64_t vocab, int64_t entries, double temperature, double count) {
+  return hp::guarded([&] {
+    hp::enter(ctx);
+    hp::require(dtype == HP_F32 || dtype == HP_F64, "logits must be float32 or float64");
+    hp::require(index_dtype == HP_I32 || index_dtype == HP_I64, "indices must be int32 or int64");
+    hp::require(rows >= 0 && vocab > 0 && entries > 0 && entries <= 1024, "extents out of range");
+    hp::require(temperature > 0 && temperature < __builtin_huge_val() && 1 / temperature < __builtin_huge_val(), "temperature out of range");
+    hp::require(loss && (rows == 0 || (logits && indices && teacher && losses)), "null pointer");
+    by_type(dtype, [&](auto zero) {
+      using T = decltype(zero);
+      hp::Scratch scratch(ctx);
+      Call<T> c{};
+      c.logits = static_cast<const T*>(logits);
+      c.mask = static_cast<const uint8_t*>(mask);
+      c.rows = rows;
+      c.vocab = vocab;
+      c.grad = static_cast<T*>(grad);
+      c.loss = static_cast<T*>(loss);
+      c.indices = indices;
+      c.wide_indices = index_dtype == HP_I64;
+      c.entries = int(entries);
+      c.teacher = static_cast<const T*>(teacher);
+      c.teacher_rest = static_cast<const T*>(teacher_rest);
+      c.losses = static_cast<T*>(losses);
+      c.inverse = 1 / temperature;
+      if (count > 0) c.scale_value = 1 / count;
+      else if (!mask) c.scale_value = 1.0 / double(std::max<int64_t>(rows, 1));
+      else c.count_here = rows > 0;
+      int64_t sums = 0;
+      if (rows) sums = teacher_rest ? rows_pass<T, true>(ctx, scratch, c) : rows_pass<T, false>(ctx, scratch, c);
+      final_loss(ctx, c, sums);
+    });
+  });
+}
+
+}  // extern "C"

@@ -104,6 +104,18 @@ def preference_loss(backend, logits, targets, reference, mask, beta, smoothing, 
     return loss, sums, grad
 
 
+def distillation_loss(backend, logits, indices, teacher, rest, mask, temperature, count, gradient):
+    tokens = indices._shape[:-1]
+    loss, losses = backend.empty((), logits._dtype), backend.empty(tokens, logits._dtype)
+    grad = backend.empty(logits._shape, logits._dtype) if gradient else None
+    _run(
+        backend, "hp_distillation_loss", *_codes(logits, indices), logits._data.ptr, indices._data.ptr, teacher._data.ptr,
+        _ptr(rest), _ptr(mask), loss.ptr, losses.ptr, None if grad is None else grad.ptr, prod(tokens), logits._shape[-1],
+        indices._shape[-1], temperature, count or 0.0,
+    )
+    return loss, losses, grad
+
+
 # ---- AdamW ---------------------------------------------------------------------
 
 
