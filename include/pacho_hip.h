@@ -294,6 +294,22 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
                        const void* reference, const void* mask, void* loss, void* sums, void* grad, int64_t pairs,
                        int64_t time, int64_t vocab, double beta, double smoothing);
 
+/* With rms(v) = v / sqrt(mean(v v) + eps) over rows of `channels`:
+ * stream = residual + scale gate rms(x) post_weight, normed = rms(stream) weight.
+ * post_weight NULL: x in place of rms(x) post_weight; gate NULL: one. Row r has
+ * row r / divide of the gate, and `divide` divides the rows. float32 or float64. */
+int hp_residual_norm(hp_ctx* ctx, int dtype, const void* x, const void* residual, const void* weight, const void* post_weight,
+                     const void* gate, void* stream, void* normed, int64_t rows, int64_t channels, int64_t divide, double scale,
+                     double eps);
+
+/* Its gradients of x, residual (d), weight, post_weight and gate (the last two
+ * where given), from those of both results and the stream. `gates`: rows of the
+ * gate, which also stand without rows of x. */
+int hp_residual_norm_grad(hp_ctx* ctx, int dtype, const void* grad_stream, const void* grad_normed, const void* x, const void* stream,
+                          const void* weight, const void* post_weight, const void* gate, void* dx, void* d, void* dweight,
+                          void* dpost, void* dgate, int64_t rows, int64_t channels, int64_t divide, int64_t gates, double scale,
+                          double eps);
+
 /* Divergence of rows x vocab logits from a teacher that is known by `entries` (1
  * to 1024) logits of each row, which stand at `indices` (rows, entries; index_dtype
  * HP_I32 or HP_I64): sum p (log p - log q), where q is the softmax of the logits

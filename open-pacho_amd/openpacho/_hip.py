@@ -697,6 +697,8 @@ class HIPBackend:
     token_log_probs = _hip_nn.token_log_probs
     policy_loss = _hip_nn.policy_loss
     preference_loss = _hip_nn.preference_loss
+    residual_norm = _hip_nn.residual_norm
+    residual_norm_grad = _hip_nn.residual_norm_grad
     distillation_loss = _hip_nn.distillation_loss
     adamw_load = _hip_nn.adamw_load
     adamw_moments = _hip_nn.adamw_moments

@@ -40,6 +40,25 @@ def gated_recurrence_grad(backend, grad, x, gate, h, initial, resets, batch, tim
     return dx, d_gate, d_initial
 
 
+def residual_norm(backend, x, residual, weight, post_weight, gate, rows, channels, divide, scale, eps):
+    stream, normed = backend.empty(x._shape, x._dtype), backend.empty(x._shape, x._dtype)
+    _run(
+        backend, "hp_residual_norm", lib_.DTYPE_CODES[x._dtype], x._data.ptr, residual._data.ptr, weight._data.ptr,
+        _ptr(post_weight), _ptr(gate), stream.ptr, normed.ptr, rows, channels, divide, scale, eps,
+    )
+    return stream, normed
+
+
+def residual_norm_grad(backend, grad_stream, grad_normed, x, stream, weight, post_weight, gate, rows, channels, divide, scale, eps):
+    found = [None if array is None else backend.empty(array._shape, x._dtype) for array in (x, x, weight, post_weight, gate)]
+    _run(
+        backend, "hp_residual_norm_grad", lib_.DTYPE_CODES[x._dtype], grad_stream._data.ptr, grad_normed._data.ptr, x._data.ptr,
+        stream._data.ptr, weight._data.ptr, _ptr(post_weight), _ptr(gate), *(None if data is None else data.ptr for data in found),
+        rows, channels, divide, 0 if gate is None else gate.size // channels, scale, eps,
+    )
+    return found
+
+
 def _codes(logits, targets):
     return lib_.DTYPE_CODES[logits._dtype], lib_.DTYPE_CODES[targets._dtype]
 
