@@ -294,6 +294,24 @@ int hp_preference_loss(hp_ctx* ctx, int dtype, int index_dtype, const void* logi
                        const void* reference, const void* mask, void* loss, void* sums, void* grad, int64_t pairs,
                        int64_t time, int64_t vocab, double beta, double smoothing);
 
+/* A causal convolution of 1 to 8 taps of each channel of x (batch, time, channels):
+ * y_t = f(bias + sum_k weight[:, k] x_{t - taps + 1 + k}) with weight (channels, taps)
+ * and f the identity (activation 0) or v sigmoid(v) (1). `initial` (batch, taps - 1,
+ * channels) are the inputs before the first step (NULL: zero); a step where the
+ * bool `resets` (batch, time; NULL: nowhere) is set, and later ones, see the inputs
+ * before it as zero. Rows have lengths[row] steps (index_dtype HP_I32 or HP_I64;
+ * NULL: `time`), at least 0 and at most `time`; y is 0 behind them. `last` (batch,
+ * taps - 1, channels): the inputs as a step behind the row would see them. */
+int hp_causal_conv(hp_ctx* ctx, int dtype, int index_dtype, const void* x, const void* weight, const void* bias, const void* initial,
+                   const void* resets, const void* lengths, void* y, void* last, int64_t batch, int64_t time, int64_t channels,
+                   int64_t taps, int activation);
+
+/* Its gradients of x, weight, bias and initial (the last two unless NULL) from
+ * that of y. */
+int hp_causal_conv_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* grad, const void* x, const void* weight, const void* bias,
+                        const void* initial, const void* resets, const void* lengths, void* dx, void* dweight, void* dbias,
+                        void* dinitial, int64_t batch, int64_t time, int64_t channels, int64_t taps, int activation);
+
 /* With rms(v) = v / sqrt(mean(v v) + eps) over rows of `channels`:
  * stream = residual + scale gate rms(x) post_weight, normed = rms(stream) weight.
  * post_weight NULL: x in place of rms(x) post_weight; gate NULL: one. Row r has

@@ -20,7 +20,7 @@
 // group that it sees a part of: at most two, as groups are neighbouring rows too.
 #include <type_traits>
 
-#include "common.h"
+#include "sequence.h"
 
 namespace {
 
@@ -357,38 +357,11 @@ __global__ __launch_bounds__(kLong) void long_backward_kernel(Norm<T> c) {
 
 // ---- sums of workers -----------------------------------------------------------------
 
-// out[i] = the sum of parts[w * stride + i] over w from low to high, in a fixed order:
-// 64 columns a workgroup, waves on every sixteenth part.
-template <typename T>
-__device__ __forceinline__ void add_parts(const T* parts, int64_t stride, int64_t low, int64_t high, int64_t column, int64_t columns, T* out) {
-  __shared__ T meet[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const bool valid = column + lane < columns;
-  T sum[4] = {};
-  if (valid) {
-    int64_t w = low + wave;
-    for (; w + 48 < high; w += 64) {
-      T v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = parts[(w + 16 * k) * stride + column + lane];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) sum[k] += v[k];
-    }
-    for (; w < high; w += 16) sum[0] += parts[w * stride + column + lane];
-  }
-  meet[wave][lane] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-  __syncthreads();
-  if (wave == 0 && valid) {
-    T total = meet[0][lane];
-    for (int k = 1; k < 16; ++k) total += meet[k][lane];
-    out[column + lane] = total;
-  }
-}
-
 template <typename T>
 __global__ __launch_bounds__(1024) void sums_kernel(const T* weight_sums, T* dweight, const T* post_sums, T* dpost, int64_t workers, int64_t channels) {
   const T* parts = blockIdx.y == 0 ? weight_sums : post_sums;
-  add_parts(parts, channels, 0, workers, int64_t(blockIdx.x) * 64, channels, blockIdx.y == 0 ? dweight : dpost);
+  T* out = blockIdx.y == 0 ? dweight : dpost;
+  hpd::add_parts(parts, channels, 0, workers, int64_t(blockIdx.x) * 64, channels, [&](int64_t i, T sum) { out[i] = sum; });
 }
 
 // Groups that more than one worker has a part of: the first of them may leave it in
@@ -399,11 +372,8 @@ __global__ __launch_bounds__(1024) void gate_sums_kernel(Norm<T> c, int64_t bloc
   const int64_t low = group * c.divide / c.each, high = ((group + 1) * c.divide - 1) / c.each;
   if (low == high) return;
   T* out = c.dgate + group * c.channels;
-  // Counted in places of two a worker: from the first worker's place on, by twos, with that one moved.
-  const int64_t start = gate_slot(low, group, c.divide, c.each);
-  add_parts(c.gate_sums, 2 * c.channels, low + 1, high + 1, column, c.channels, out);
-  const int lane = threadIdx.x & 63;
-  if (threadIdx.x < 64 && column + lane < c.channels) out[column + lane] += c.gate_sums[start * c.channels + column + lane];
+  const T* start = c.gate_sums + gate_slot(low, group, c.divide, c.each) * c.channels;
+  hpd::add_parts(c.gate_sums, 2 * c.channels, low + 1, high + 1, column, c.channels, [&](int64_t i, T sum) { out[i] = start[i] + sum; });
 }
 
 template <typename T>

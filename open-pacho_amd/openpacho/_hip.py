@@ -697,6 +697,8 @@ class HIPBackend:
     token_log_probs = _hip_nn.token_log_probs
     policy_loss = _hip_nn.policy_loss
     preference_loss = _hip_nn.preference_loss
+    causal_conv = _hip_nn.causal_conv
+    causal_conv_grad = _hip_nn.causal_conv_grad
     residual_norm = _hip_nn.residual_norm
     residual_norm_grad = _hip_nn.residual_norm_grad
     distillation_loss = _hip_nn.distillation_loss

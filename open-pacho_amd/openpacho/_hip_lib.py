@@ -69,6 +69,8 @@ PROTOTYPES = {
     "hp_token_log_probs": [_ptr, _i32, _i32] + [_ptr] * 4 + [_i64] * 2,
     "hp_policy_loss": [_ptr, _i32, _i32] + [_ptr] * 4 + [_i64] * 2 + [_ptr] * 5 + [_i64] * 2 + [ctypes.c_double] * 4,
     "hp_preference_loss": [_ptr, _i32, _i32] + [_ptr] * 7 + [_i64] * 3 + [ctypes.c_double] * 2,
+    "hp_causal_conv": [_ptr, _i32, _i32] + [_ptr] * 8 + [_i64] * 4 + [_i32],
+    "hp_causal_conv_grad": [_ptr, _i32, _i32] + [_ptr] * 11 + [_i64] * 4 + [_i32],
     "hp_residual_norm": [_ptr, _i32] + [_ptr] * 7 + [_i64] * 3 + [ctypes.c_double] * 2,
     "hp_residual_norm_grad": [_ptr, _i32] + [_ptr] * 12 + [_i64] * 4 + [ctypes.c_double] * 2,
     "hp_distillation_loss": [_ptr, _i32, _i32] + [_ptr] * 8 + [_i64] * 3 + [ctypes.c_double] * 2,

@@ -5,7 +5,11 @@ operand that is not given."""
 import ctypes
 from math import prod
 
+import numpy as np
+
 from . import _hip_lib as lib_
+
+_INT64 = np.dtype("int64")
 
 
 def _ptr(array):
@@ -38,6 +42,29 @@ def gated_recurrence_grad(backend, grad, x, gate, h, initial, resets, batch, tim
         batch, time, channels, gates,
     )
     return dx, d_gate, d_initial
+
+
+def _lengths_code(lengths):
+    return lib_.DTYPE_CODES[_INT64 if lengths is None else lengths._dtype]
+
+
+def causal_conv(backend, x, weight, bias, initial, resets, lengths, batch, time, channels, taps, activation):
+    y, last = backend.empty(x._shape, x._dtype), backend.empty((batch, taps - 1, channels), x._dtype)
+    _run(
+        backend, "hp_causal_conv", lib_.DTYPE_CODES[x._dtype], _lengths_code(lengths), x._data.ptr, weight._data.ptr, _ptr(bias),
+        _ptr(initial), _ptr(resets), _ptr(lengths), y.ptr, last.ptr, batch, time, channels, taps, activation,
+    )
+    return y, last
+
+
+def causal_conv_grad(backend, grad, x, weight, bias, initial, resets, lengths, batch, time, channels, taps, activation):
+    found = [None if array is None else backend.empty(array._shape, x._dtype) for array in (x, weight, bias, initial)]
+    _run(
+        backend, "hp_causal_conv_grad", lib_.DTYPE_CODES[x._dtype], _lengths_code(lengths), grad._data.ptr, x._data.ptr,
+        weight._data.ptr, _ptr(bias), _ptr(initial), _ptr(resets), _ptr(lengths), *(None if data is None else data.ptr for data in found),
+        batch, time, channels, taps, activation,
+    )
+    return found
 
 
 def residual_norm(backend, x, residual, weight, post_weight, gate, rows, channels, divide, scale, eps):
