@@ -312,6 +312,31 @@ int hp_causal_conv_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* gra
                         const void* initial, const void* resets, const void* lengths, void* dx, void* dweight, void* dbias,
                         void* dinitial, int64_t batch, int64_t time, int64_t channels, int64_t taps, int activation);
 
+/* A selective state space scan of x (batch, time, channels): with
+ * dt = softplus(delta + delta_bias) each channel's 1 to 256 states are
+ * h_t = exp(-dt exp(a_log)) h_{t-1} + dt x_t b_t, and
+ * y_t = (sum c_t h_t + skip x_t) gate_t sigmoid(gate_t), without the last factor if
+ * gate is NULL. delta and gate as x; a_log (channels, states); b, c (batch, time,
+ * groups, states), whose groups divide the channels; skip, delta_bias (channels) or
+ * NULL: zero; `initial` (batch, channels, states) or NULL: zero. Where the bool
+ * `resets` (batch, time; NULL: nowhere) is set h_{t-1} counts as zero. Rows have
+ * lengths[row] steps (index_dtype HP_I32 or HP_I64; NULL: `time`), at least 0 and
+ * at most `time`; y is 0 behind them. `last` (batch, channels, states): the
+ * states after a row's last step. */
+int hp_selective_scan(hp_ctx* ctx, int dtype, int index_dtype, const void* x, const void* delta, const void* a_log, const void* b,
+                      const void* c, const void* skip, const void* gate, const void* initial, const void* delta_bias,
+                      const void* resets, const void* lengths, void* y, void* last, int64_t batch, int64_t time, int64_t channels,
+                      int64_t groups, int64_t states);
+
+/* Its gradients (those of skip, gate, delta_bias and initial where they are
+ * given; dskip and ddelta_bias also unless NULL) from those of y and, unless
+ * NULL, of the last states. */
+int hp_selective_scan_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* grad, const void* grad_state, const void* x,
+                           const void* delta, const void* a_log, const void* b, const void* c, const void* skip, const void* gate,
+                           const void* initial, const void* delta_bias, const void* resets, const void* lengths, void* dx,
+                           void* ddelta, void* da_log, void* db, void* dc, void* dskip, void* dgate, void* ddelta_bias,
+                           void* dinitial, int64_t batch, int64_t time, int64_t channels, int64_t groups, int64_t states);
+
 /* With rms(v) = v / sqrt(mean(v v) + eps) over rows of `channels`:
  * stream = residual + scale gate rms(x) post_weight, normed = rms(stream) weight.
  * post_weight NULL: x in place of rms(x) post_weight; gate NULL: one. Row r has

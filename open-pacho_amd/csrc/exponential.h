@@ -1,4 +1,4 @@
-// exp of arguments up to zero, as softmax terms and gates need it.
+// exp of arguments up to zero, as softmax terms and gates need it, and what is made of it.
 #pragma once
 
 #include "common.h"
@@ -19,7 +19,7 @@ __device__ __forceinline__ float exp_down(float x) {
 }
 __device__ __forceinline__ double exp_down(double x) { return exp(x); }
 
-// 1 / x for x in [1, 2]: the hardware's estimate (1 ulp) and a Newton step.
+// 1 / x for x in [1, 3]: the hardware's estimate (1 ulp) and a Newton step.
 __device__ __forceinline__ float inverse(float x) {
   const float r = __builtin_amdgcn_rcpf(x);
   return __builtin_fmaf(r, __builtin_fmaf(-x, r, 1.0f), r);
@@ -35,6 +35,23 @@ __device__ __forceinline__ void gates(T g, T& keep, T& take) {
   const T large = inverse(T(1) + small);
   keep = g >= T(0) ? large : small * large;
   take = g >= T(0) ? small * large : large;
+}
+
+// log(1 + exp(v)) to full relative precision: max(v, 0) + log(1 + e) with e = exp(-|v|),
+// log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3, by its series; the first term left
+// out is below 2^-26 of it.
+__device__ __forceinline__ float softplus(float v) {
+  const float e = exp_down(-__builtin_elementwise_abs(v));
+  const float s = e * inverse(2.0f + e), p = s * s;
+  float r = 1.0f / 13;
+#pragma unroll
+  for (int k = 11; k > 0; k -= 2) r = __builtin_fmaf(r, p, 1.0f / k);
+  const float tail = 2.0f * s * r;
+  return v > 0.0f ? v + tail : v <= 0.0f ? tail : v;
+}
+__device__ __forceinline__ double softplus(double v) {
+  const double tail = log1p(exp(-__builtin_elementwise_abs(v)));
+  return v > 0 ? v + tail : v <= 0 ? tail : v;
 }
 
 }  // namespace hpd

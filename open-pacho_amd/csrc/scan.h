@@ -1,0 +1,188 @@
+// The selective scan: what its forward and backward kernels share.
+//
+//   dt = softplus(delta + bias),  r_n = exp(a_log_n)
+//   h_t,n = exp(-dt r_n) h_{t-1},n + dt x_t b_t,n,  y_t = (sum_n c_t,n h_t,n + skip x_t) silu(gate_t)
+//
+// A lane owns a channel, a wave kStates of its states, a workgroup all states of up to 64
+// channels that share b and c. So b and c are the same in a whole wave and come by scalar
+// loads, an exponential, two products and two fused multiply-adds make a state's step, and
+// only the sums over states meet in LDS, once for a tile of kSteps steps: each wave has
+// some of the tile's steps as its own, whose dt and dt x it leaves for all waves before
+// they walk the tile, and whose sums it adds up afterwards.
+//
+// Where a call has few channels the steps of a row are cut into parts with workgroups of
+// their own. A part from zero states ends in states E; from states h it ends in E + D h,
+// D = exp(-r sum dt): each part needs the sum of its dt and its E from a launch before,
+// which reads everything once more.
+#pragma once
+
+#include <type_traits>
+
+#include "exponential.h"
+#include "sequence.h"
+
+namespace hpd {
+
+constexpr int kStates = 4;  // of a wave
+
+// The arrays of a call; pointers that it does not have are null.
+template <typename T>
+struct Scan {
+  const T *x, *delta, *a_log, *skip, *gate, *initial, *delta_bias;
+  T *y, *last;
+  Rows rows;
+  int64_t batch, channels, groups;
+  int64_t width;   // channels of a group
+  int64_t pieces;  // of a group's channels, 64 each
+  int64_t states;  // of a channel
+  int64_t padded;  // of a step and group in b and c: states, up to a multiple of kStates
+  int64_t first;   // state of this launch, which takes kStates for each wave
+  bool starts, ends;  // the first and the last launch over the states
+  int64_t parts;   // of a row's steps
+  int64_t steps;   // of a part, a multiple of the tile
+  // (parts, batch, channels): sums of dt; (parts, batch, states of a launch, channels): states that parts end in.
+  T *spans, *ended;
+  // Backward, (tiles, batch, states of a launch, channels): states before each tile, from the
+  // part's zero states where there are several; (tiles, batch, channels): sums of dt from the
+  // part's start; (parts, batch, states of a launch, channels): what a part passes back.
+  T *before, *since, *passed;
+  const T *grad, *grad_state;
+};
+
+// The same memory as constants, which uniform addresses read by scalar loads.
+template <typename T>
+using Constant = const __attribute__((address_space(4))) T*;
+
+template <typename T>
+struct Quad {
+  typedef T type __attribute__((ext_vector_type(kStates), aligned(sizeof(T))));
+};
+
+// exp(dt rate) of rates that are -r, for floats -r log2 e: the rounding of the product is off
+// by 2^-24 of an exponent whose power is at most 0.37 of its inverse, so by half a unit of 1.
+__device__ __forceinline__ float decay(float dt, float rate) { return __builtin_amdgcn_exp2f(dt * rate); }
+__device__ __forceinline__ double decay(double dt, double rate) { return exp(dt * rate); }
+__device__ __forceinline__ float rate_of(float a_log) { return -(expf(a_log) * 0x1.715476p+0f); }
+__device__ __forceinline__ double rate_of(double a_log) { return -exp(a_log); }
+// A state passes parts however small the product of its decays is: infinite ones stay so.
+template <typename T>
+__device__ __forceinline__ T passed_decay(T span, T rate) {
+  const T least = sizeof(T) == 4 ? T(0x1p-126f) : T(0x1p-1022);
+  const T found = decay(span, rate);
+  return found < least ? least : found;
+}
+
+// What a workgroup and its lanes work on.
+template <typename T, int NW>
+struct Place {
+  int lane, wave;
+  int64_t row, group, piece, part, channel, first, end, length;  // steps [first, end) of a row of `length`
+  int64_t state;     // the wave's first, within the channel
+  int64_t slot;      // the wave's first, within the launch
+  bool valid;
+
+  __device__ __forceinline__ explicit Place(const Scan<T>& c) {
+    lane = threadIdx.x & 63;
+    wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t block = by_die();
+    part = block % c.parts, block /= c.parts;
+    piece = block % c.pieces, block /= c.pieces;
+    group = block % c.groups;
+    row = block / c.groups;
+    const int64_t within = piece * 64 + lane;
+    valid = within < c.width;
+    channel = group * c.width + (valid ? within : c.width - 1);  // lanes behind it load what the last one does
+    length = c.rows.end(row);
+    first = part * c.steps;
+    end = first + c.steps < length ? first + c.steps : length;
+    slot = wave * kStates;
+    state = c.first + slot;
+  }
+  __device__ __forceinline__ int64_t at(const Scan<T>& c, int64_t t) const { return (row * c.rows.time + t) * c.channels + channel; }
+  // Of (..., batch, states of a launch, channels).
+  __device__ __forceinline__ int64_t state_at(const Scan<T>& c, int64_t lead, int s) const {
+    return ((lead * c.batch + row) * (NW * kStates) + slot + s) * c.channels + channel;
+  }
+  // b or c of the wave's states at step t.
+  __device__ __forceinline__ typename Quad<T>::type projected(const Scan<T>& c, const T* array, int64_t t) const {
+    using Q = typename Quad<T>::type;
+    return *(Constant<Q>)(array + ((row * c.rows.time + t) * c.groups + group) * c.padded + state);
+  }
+  // Values of the wave's states in an array (batch, channels, states), zero for those that pad.
+  __device__ __forceinline__ void read(const Scan<T>& c, const T* array, int64_t lead, T (&to)[kStates]) const {
+    const T* from = array + (lead * c.channels + channel) * c.states + state;
+    if (state + kStates <= c.states) {
+      const auto v = *reinterpret_cast<const typename Quad<T>::type*>(from);
+#pragma unroll
+      for (int s = 0; s < kStates; ++s) to[s] = v[s];
+    } else {
+#pragma unroll
+      for (int s = 0; s < kStates; ++s) to[s] = state + s < c.states ? from[s] : T(0);
+    }
+  }
+  __device__ __forceinline__ void write(const Scan<T>& c, T* array, int64_t lead, const T (&from)[kStates]) const {
+    if (!valid) return;
+    T* to = array + (lead * c.channels + channel) * c.states + state;
+#pragma unroll
+    for (int s = 0; s < kStates; ++s) {
+      if (state + s < c.states) to[s] = from[s];
+    }
+  }
+  // The states before the part, from its predecessors' sums and ends.
+  __device__ __forceinline__ void arrive(const Scan<T>& c, const T (&rate)[kStates], T (&h)[kStates]) const {
+#pragma unroll
+    for (int s = 0; s < kStates; ++s) h[s] = T(0);
+    if (c.initial) read(c, c.initial, row, h);
+    for (int64_t p = 0; p < part; ++p) {
+      const T span = c.spans[(p * c.batch + row) * c.channels + channel];
+#pragma unroll
+      for (int s = 0; s < kStates; ++s) {
+        const T end = c.ended[state_at(c, p, s)];
+        h[s] = span < T(0) ? end : __builtin_elementwise_fma(passed_decay(span, rate[s]), h[s], end);
+      }
+    }
+  }
+};
+
+// The sum of dt of a part in which a reset cuts off what came before: below zero.
+template <typename T>
+__device__ __forceinline__ T cut_span() {
+  return T(-1);
+}
+
+// dt of a raw step.
+template <typename T>
+__device__ __forceinline__ T step_of(T delta, T bias) {
+  return softplus(delta + bias);
+}
+
+}  // namespace hpd
+
+namespace hp {
+
+// Whether waves of a launch over `states` number 1, 2, 4, ... up to `most`.
+inline int scan_waves(int64_t states, int most) {
+  int waves = 1;
+  while (waves < most && int64_t(waves) * hpd::kStates < states) waves *= 2;
+  return waves;
+}
+
+void scan_check(int dtype, int index_dtype, int64_t batch, int64_t time, int64_t channels, int64_t groups, int64_t states);
+// b or c (steps, states) with zeros up to `padded` states, or as they are where there are so many.
+template <typename T>
+const T* scan_padded(hp_ctx* ctx, Scratch& scratch, const T* array, int64_t steps, int64_t states, int64_t padded);
+template <typename T>
+void scan_fill(hp_ctx* ctx, T* to, const T* from, int64_t n);
+
+// Parts of rows: one, or as many as make enough workgroups.
+template <typename T>
+void scan_plan(hpd::Scan<T>& c, int64_t tile) {
+  const int64_t blocks = c.batch * c.groups * c.pieces, tiles = ceil_div(c.rows.time, tile);
+  c.parts = 1;
+  if (blocks <= 128) c.parts = std::min<int64_t>(std::min<int64_t>(ceil_div(512, blocks), 64), std::max<int64_t>(1, tiles / 4));
+  c.steps = ceil_div(tiles, c.parts) * tile;
+  c.parts = ceil_div(c.rows.time, c.steps);
+  require(blocks * c.parts <= kMaxThreads / 1024, "too many channels for one launch");
+}
+
+}  // namespace hp

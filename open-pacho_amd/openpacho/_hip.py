@@ -699,6 +699,8 @@ class HIPBackend:
     preference_loss = _hip_nn.preference_loss
     causal_conv = _hip_nn.causal_conv
     causal_conv_grad = _hip_nn.causal_conv_grad
+    selective_scan = _hip_nn.selective_scan
+    selective_scan_grad = _hip_nn.selective_scan_grad
     residual_norm = _hip_nn.residual_norm
     residual_norm_grad = _hip_nn.residual_norm_grad
     distillation_loss = _hip_nn.distillation_loss

@@ -71,6 +71,8 @@ PROTOTYPES = {
     "hp_preference_loss": [_ptr, _i32, _i32] + [_ptr] * 7 + [_i64] * 3 + [ctypes.c_double] * 2,
     "hp_causal_conv": [_ptr, _i32, _i32] + [_ptr] * 8 + [_i64] * 4 + [_i32],
     "hp_causal_conv_grad": [_ptr, _i32, _i32] + [_ptr] * 11 + [_i64] * 4 + [_i32],
+    "hp_selective_scan": [_ptr, _i32, _i32] + [_ptr] * 13 + [_i64] * 5,
+    "hp_selective_scan_grad": [_ptr, _i32, _i32] + [_ptr] * 22 + [_i64] * 5,
     "hp_residual_norm": [_ptr, _i32] + [_ptr] * 7 + [_i64] * 3 + [ctypes.c_double] * 2,
     "hp_residual_norm_grad": [_ptr, _i32] + [_ptr] * 12 + [_i64] * 4 + [ctypes.c_double] * 2,
     "hp_distillation_loss": [_ptr, _i32, _i32] + [_ptr] * 8 + [_i64] * 3 + [ctypes.c_double] * 2,

@@ -67,6 +67,29 @@ def causal_conv_grad(backend, grad, x, weight, bias, initial, resets, lengths, b
     return found
 
 
+def selective_scan(backend, x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths, batch, time, channels, groups, states):
+    y, last = backend.empty(x._shape, x._dtype), backend.empty((batch, channels, states), x._dtype)
+    given = (x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths)
+    _run(
+        backend, "hp_selective_scan", lib_.DTYPE_CODES[x._dtype], _lengths_code(lengths), *(_ptr(array) for array in given), y.ptr,
+        last.ptr, batch, time, channels, groups, states,
+    )
+    return y, last
+
+
+def selective_scan_grad(
+    backend, grad, grad_state, x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths, batch, time, channels, groups, states
+):
+    given = (grad, grad_state, x, delta, a_log, b, c, skip, gate, initial, delta_bias, resets, lengths)
+    like = (x, delta, a_log, b, c, skip, gate, delta_bias, initial)
+    found = [None if array is None else backend.empty(array._shape, x._dtype) for array in like]
+    _run(
+        backend, "hp_selective_scan_grad", lib_.DTYPE_CODES[x._dtype], _lengths_code(lengths), *(_ptr(array) for array in given),
+        *(None if data is None else data.ptr for data in found), batch, time, channels, groups, states,
+    )
+    return found
+
+
 def residual_norm(backend, x, residual, weight, post_weight, gate, rows, channels, divide, scale, eps):
     stream, normed = backend.empty(x._shape, x._dtype), backend.empty(x._shape, x._dtype)
     _run(
