@@ -4,11 +4,15 @@
 //   h_t,n = exp(-dt r_n) h_{t-1},n + dt x_t b_t,n,  y_t = (sum_n c_t,n h_t,n + skip x_t) silu(gate_t)
 //
 // A lane owns a channel, a wave kStates of its states, a workgroup all states of up to 64
-// channels that share b and c. So b and c are the same in a whole wave and come by scalar
-// loads, an exponential, two products and two fused multiply-adds make a state's step, and
-// only the sums over states meet in LDS, once for a tile of kSteps steps: each wave has
-// some of the tile's steps as its own, whose dt and dt x it leaves for all waves before
-// they walk the tile, and whose sums it adds up afterwards.
+// channels that share b and c. So b and c are the same in a whole wave: a register holds
+// those of four steps in the lanes of each row of 16, and an instruction that multiplies by
+// one of them takes it from its lane on the way (a row broadcast). An exponential, two
+// products and two fused multiply-adds make a state's step. (Scalar loads of b and c in
+// each step, whose waits no other work covers, took 1458 us where this takes 282, 8 x 2048 x
+// 2048 float32 with 16 states.) Only the sums over states meet in LDS, once for a tile of
+// steps: each wave has some of the tile's steps as its own, whose dt and dt x it leaves for
+// all waves before they walk the tile, and whose sums it adds up afterwards. Steps of a
+// tile behind the row's end have dt, x, b and c of zero and change nothing.
 //
 // Where a call has few channels the steps of a row are cut into parts with workgroups of
 // their own. A part from zero states ends in states E; from states h it ends in E + D h,
@@ -48,10 +52,6 @@ struct Scan {
   T *before, *since, *passed;
   const T *grad, *grad_state;
 };
-
-// The same memory as constants, which uniform addresses read by scalar loads.
-template <typename T>
-using Constant = const __attribute__((address_space(4))) T*;
 
 template <typename T>
 struct Quad {
@@ -99,14 +99,13 @@ struct Place {
     state = c.first + slot;
   }
   __device__ __forceinline__ int64_t at(const Scan<T>& c, int64_t t) const { return (row * c.rows.time + t) * c.channels + channel; }
+  // Of x's shape, at a step < end: a scalar address and the lane's offset.
+  __device__ __forceinline__ T get(const Scan<T>& c, const T* array, int64_t t) const {
+    return (array + (row * c.rows.time + t) * c.channels)[unsigned(channel)];
+  }
   // Of (..., batch, states of a launch, channels).
   __device__ __forceinline__ int64_t state_at(const Scan<T>& c, int64_t lead, int s) const {
     return ((lead * c.batch + row) * (NW * kStates) + slot + s) * c.channels + channel;
-  }
-  // b or c of the wave's states at step t.
-  __device__ __forceinline__ typename Quad<T>::type projected(const Scan<T>& c, const T* array, int64_t t) const {
-    using Q = typename Quad<T>::type;
-    return *(Constant<Q>)(array + ((row * c.rows.time + t) * c.groups + group) * c.padded + state);
   }
   // Values of the wave's states in an array (batch, channels, states), zero for those that pad.
   __device__ __forceinline__ void read(const Scan<T>& c, const T* array, int64_t lead, T (&to)[kStates]) const {
@@ -141,6 +140,57 @@ struct Place {
         h[s] = span < T(0) ? end : __builtin_elementwise_fma(passed_decay(span, rate[s]), h[s], end);
       }
     }
+  }
+};
+
+// f(std::integral_constant<int, i>) for i from 0 to N - 1.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void for_each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    for_each<N, I + 1>(f);
+  }
+}
+
+// The value that lane I of each row of 16 lanes has.
+template <int I>
+__device__ __forceinline__ float of_row(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + I, 0xF, 0xF, true));
+}
+template <int I>
+__device__ __forceinline__ double of_row(double v) {
+  struct Words {
+    int low, high;
+  } w = __builtin_bit_cast(Words, v);
+  w.low = __builtin_amdgcn_update_dpp(0, w.low, 0x150 + I, 0xF, 0xF, true);
+  w.high = __builtin_amdgcn_update_dpp(0, w.high, 0x150 + I, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, w);
+}
+
+// b or c of the wave's states in the L steps of a tile.
+template <typename T, int L>
+struct Projections {
+  T v[L / 4];
+
+  // Those of steps behind the end are what the last one's are, until keep() clears them.
+  template <int NW>
+  __device__ __forceinline__ void load(const Scan<T>& c, const Place<T, NW>& at, const T* array, int64_t t) {
+    const T* from = array + ((at.row * c.rows.time + t) * c.groups + at.group) * c.padded + at.state;
+    const unsigned stride = unsigned(c.groups * c.padded), left = at.end - t < L ? unsigned(at.end - t) : unsigned(L);
+#pragma unroll
+    for (int q = 0; q < L / 4; ++q) {
+      const unsigned i = 4 * q + (at.lane >> 2 & 3);
+      v[q] = from[(i < left ? i : left - 1) * stride + (at.lane & 3)];
+    }
+  }
+  __device__ __forceinline__ void keep(int lane, int count) {
+#pragma unroll
+    for (int q = 0; q < L / 4; ++q) v[q] = 4 * q + (lane >> 2 & 3) < count ? v[q] : T(0);
+  }
+  // Of step I and state S.
+  template <int I, int S>
+  __device__ __forceinline__ T get() const {
+    return of_row<(I % 4) * 4 + S>(v[I / 4]);
   }
 };
 
@@ -183,6 +233,7 @@ void scan_plan(hpd::Scan<T>& c, int64_t tile) {
   c.steps = ceil_div(tiles, c.parts) * tile;
   c.parts = ceil_div(c.rows.time, c.steps);
   require(blocks * c.parts <= kMaxThreads / 1024, "too many channels for one launch");
+  require(c.channels <= INT32_MAX / 8 && c.groups * c.padded <= INT32_MAX / 128, "too many channels or groups");
 }
 
 }  // namespace hp

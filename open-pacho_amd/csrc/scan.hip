@@ -29,58 +29,55 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
   }
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0), skip = c.skip ? c.skip[at.channel] : T(0);
   T x[kOwn], delta[kOwn], gate[kOwn], span = T(0);
+  Projections<T, kSteps> next_b, next_c;
   bool cut = false;
   const auto load = [&](int64_t t) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const bool inside = t + own + i < at.end;
-      const int64_t from = at.at(c, t + own + i);
-      x[i] = inside ? c.x[from] : T(0);
-      delta[i] = inside ? c.delta[from] : T(0);
-      if (!SUMMARY) gate[i] = inside && c.gate ? c.gate[from] : T(0);
+      const int64_t step = t + own + i < at.end ? t + own + i : at.end - 1;
+      x[i] = at.get(c, c.x, step);
+      delta[i] = at.get(c, c.delta, step);
+      if (!SUMMARY && c.gate) gate[i] = at.get(c, c.gate, step);
     }
+    next_b.load(c, at, b_, t);
+    if (!SUMMARY) next_c.load(c, at, c_, t);
   };
-  load(at.first);
+  if (at.first < at.end) load(at.first);
   for (int64_t t = at.first; t < at.end; t += kSteps) {
+    const int count = at.end - t < kSteps ? int(at.end - t) : kSteps;
     T now_x[kOwn], now_gate[kOwn];
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const T dt = t + own + i < at.end ? step_of(delta[i], bias) : T(0);
-      shared_dt[own + i][lane] = dt;
-      shared_u[own + i][lane] = dt * x[i];
+      const bool inside = own + i < count;
+      const T dt = step_of(delta[i], bias);
+      shared_dt[own + i][lane] = inside ? dt : T(0);
+      shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
       now_x[i] = x[i];
       if (!SUMMARY) now_gate[i] = gate[i];
     }
+    Projections<T, kSteps> bs = next_b, cs = next_c;
+    bs.keep(lane, count);
+    if (!SUMMARY) cs.keep(lane, count);
     __syncthreads();
-    load(t + kSteps);
-    const int count = at.end - t < kSteps ? int(at.end - t) : kSteps;
+    if (t + kSteps < at.end) load(t + kSteps);
     const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<kSteps>(at.row, t, at.end)) : 0;
-    const auto step = [&](int i) {
+    for_each<kSteps>([&](auto step) {
+      constexpr int i = step;
       const T dt = shared_dt[i][lane], u = shared_u[i][lane];
-      const auto bs = at.projected(c, b_, t + i);
       if (RESETS && (starts >> i & 1)) {
 #pragma unroll
         for (int s = 0; s < kStates; ++s) h[s] = T(0);
         cut = true;
       }
       T y = T(0);
-#pragma unroll
-      for (int s = 0; s < kStates; ++s) h[s] = __builtin_elementwise_fma(decay(dt, rate[s]), h[s], u * bs[s]);
+      for_each<kStates>([&](auto state) {
+        constexpr int s = state;
+        h[s] = __builtin_elementwise_fma(decay(dt, rate[s]), h[s], u * bs.template get<i, s>());
+        if constexpr (!SUMMARY) y = __builtin_elementwise_fma(cs.template get<i, s>(), h[s], y);
+      });
       if constexpr (SUMMARY) span += dt;
-      else {
-        const auto cs = at.projected(c, c_, t + i);
-#pragma unroll
-        for (int s = 0; s < kStates; ++s) y = __builtin_elementwise_fma(cs[s], h[s], y);
-        sums[at.wave][i][lane] = y;
-      }
-    };
-    if (count == kSteps) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) step(i);
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < count; ++i) step(i);
-    }
+      else sums[at.wave][i][lane] = y;
+    });
     __syncthreads();
     if constexpr (!SUMMARY) {
 #pragma unroll

@@ -43,76 +43,75 @@ __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_,
   for (int s = 0; s < kStates; ++s) rate[s] = rate_of(rate[s]), h[s] = back[s] = T(0), through[s] = T(1);
   if (!SPLIT && c.initial) at.read(c, c.initial, at.row, h);
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0);
-  T x[kOwn], delta[kOwn], g[kOwn];
+  T x[kOwn], delta[kOwn], grad[kOwn], gate[kOwn];
+  Projections<T, L> next_b, next_c;
   bool cut = false;
   const auto load = [&](int64_t t) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const bool inside = t + own + i < at.end;
-      const int64_t from = at.at(c, t + own + i);
-      x[i] = inside ? c.x[from] : T(0);
-      delta[i] = inside ? c.delta[from] : T(0);
+      const int64_t step = t + own + i < at.end ? t + own + i : at.end - 1;
+      x[i] = at.get(c, c.x, step);
+      delta[i] = at.get(c, c.delta, step);
       if constexpr (SPLIT) {
-        g[i] = inside ? c.grad[from] : T(0);
-        if (inside && c.gate) {
-          T keep, rest;
-          const T gate = c.gate[from];
-          gates(gate, keep, rest);
-          g[i] *= gate * keep;
-        }
+        grad[i] = at.get(c, c.grad, step);
+        if (c.gate) gate[i] = at.get(c, c.gate, step);
       }
     }
+    next_b.load(c, at, b_, t);
+    if (SPLIT) next_c.load(c, at, c_, t);
   };
-  load(at.first);
+  if (at.first < at.end) load(at.first);
   for (int64_t t = at.first; t < at.end; t += L) {
+    const int count = at.end - t < L ? int(at.end - t) : L;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const T dt = t + own + i < at.end ? step_of(delta[i], bias) : T(0);
-      shared_dt[own + i][lane] = dt;
-      shared_u[own + i][lane] = dt * x[i];
-      if constexpr (SPLIT) shared_g[own + i][lane] = g[i];
+      const bool inside = own + i < count;
+      const T dt = step_of(delta[i], bias);
+      shared_dt[own + i][lane] = inside ? dt : T(0);
+      shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
+      if constexpr (SPLIT) {
+        T g = grad[i];
+        if (c.gate) {
+          T keep, rest;
+          gates(gate[i], keep, rest);
+          g *= gate[i] * keep;
+        }
+        shared_g[own + i][lane] = inside ? g : T(0);
+      }
     }
+    Projections<T, L> bs = next_b, cs = next_c;
+    bs.keep(lane, count);
+    if (SPLIT) cs.keep(lane, count);
     __syncthreads();
-    load(t + L);
+    if (t + L < at.end) load(t + L);
     const int64_t tile = t / L;
     if (at.valid) {
 #pragma unroll
       for (int s = 0; s < kStates; ++s) c.before[at.state_at(c, tile, s)] = h[s];
       if (SPLIT && at.wave == 0) c.since[(tile * c.batch + at.row) * c.channels + at.channel] = cut ? cut_span<T>() : span;
     }
-    const int count = at.end - t < L ? int(at.end - t) : L;
     const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<L>(at.row, t, at.end)) : 0;
-    const auto step = [&](int i) {
+    for_each<L>([&](auto step) {
+      constexpr int i = step;
       const T dt = shared_dt[i][lane], u = shared_u[i][lane];
-      const auto bs = at.projected(c, b_, t + i);
-      T keep[kStates];
-#pragma unroll
-      for (int s = 0; s < kStates; ++s) keep[s] = decay(dt, rate[s]);
+      T g = SPLIT ? shared_g[SPLIT ? i : 0][lane] : T(0);
       if (RESETS && (starts >> i & 1)) {
 #pragma unroll
         for (int s = 0; s < kStates; ++s) h[s] = through[s] = T(0);
         cut = true;
       }
-#pragma unroll
-      for (int s = 0; s < kStates; ++s) h[s] = __builtin_elementwise_fma(keep[s], h[s], u * bs[s]);
-      if constexpr (SPLIT) {
-        const auto cs = at.projected(c, c_, t + i);
-        const T gt = shared_g[i][lane];
-        span += dt;
-#pragma unroll
-        for (int s = 0; s < kStates; ++s) {
-          through[s] *= keep[s];
-          back[s] = __builtin_elementwise_fma(through[s], cut ? T(0) : cs[s] * gt, back[s]);
+      if (RESETS && cut) g = T(0);
+      for_each<kStates>([&](auto state) {
+        constexpr int s = state;
+        const T keep = decay(dt, rate[s]);
+        h[s] = __builtin_elementwise_fma(keep, h[s], u * bs.template get<i, s>());
+        if constexpr (SPLIT) {
+          through[s] *= keep;
+          back[s] = __builtin_elementwise_fma(through[s], cs.template get<i, s>() * g, back[s]);
         }
-      }
-    };
-    if (count == L) {
-#pragma unroll
-      for (int i = 0; i < L; ++i) step(i);
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < count; ++i) step(i);
-    }
+      });
+      if constexpr (SPLIT) span += dt;
+    });
     __syncthreads();
   }
   if constexpr (SPLIT) {
@@ -247,33 +246,38 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
   }
   const int64_t tiles = at.end > at.first ? (at.end - at.first + L - 1) / L : 0;
   T x[kOwn], delta[kOwn], gate[kOwn], grad[kOwn];
+  Projections<T, L> bs, cs;
   const auto load = [&](int64_t t) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const bool inside = t >= at.first && t + own + i < at.end;
-      const int64_t from = at.at(c, t + own + i);
-      x[i] = inside ? c.x[from] : T(0);
-      delta[i] = inside ? c.delta[from] : T(0);
-      gate[i] = inside && c.gate ? c.gate[from] : T(0);
-      grad[i] = inside ? c.grad[from] : T(0);
+      const int64_t step = t + own + i < at.end ? t + own + i : at.end - 1;
+      x[i] = at.get(c, c.x, step);
+      delta[i] = at.get(c, c.delta, step);
+      grad[i] = at.get(c, c.grad, step);
+      if (c.gate) gate[i] = at.get(c, c.gate, step);
     }
+    bs.load(c, at, b_, t);
+    cs.load(c, at, c_, t);
   };
   for (int64_t n = tiles - 1; n >= 0; --n) {
     const int64_t t = at.first + n * L;
+    const int count = at.end - t < L ? int(at.end - t) : L;
     load(t);
+    bs.keep(lane, count);
+    cs.keep(lane, count);
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const bool inside = at.valid && t + own + i < at.end;
-      const T dt = inside ? step_of(delta[i], bias) : T(0);
-      T g = inside ? grad[i] : T(0);
-      if (inside && c.gate) {
+      const bool inside = at.valid && own + i < count;
+      const T dt = step_of(delta[i], bias);
+      T g = grad[i];
+      if (c.gate) {
         T keep, rest;
         gates(gate[i], keep, rest);
         g *= gate[i] * keep;
       }
-      shared_dt[own + i][lane] = dt;
+      shared_dt[own + i][lane] = inside ? dt : T(0);
       shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
-      shared_g[own + i][lane] = g;
+      shared_g[own + i][lane] = inside ? g : T(0);
     }
     T start[kStates];
     const int64_t tile = t / L;
@@ -287,53 +291,47 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
       }
     }
     __syncthreads();
-    const int count = at.end - t < L ? int(at.end - t) : L;
     const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<L>(at.row, t, at.end)) : 0;
-    const auto walk = [&](auto whole) {
-      // Steps behind the end have dt, u and g of zero and take b and c of zero: they change nothing.
-      const auto projected = [&](const T* array, int i) {
-        auto v = at.projected(c, array, t + (whole || i < count ? i : count - 1));
-        if (!whole && i >= count) v = T(0);
-        return v;
-      };
+    {
       T h[L][kStates], keep[L][kStates];
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
+      for_each<L>([&](auto step) {
+        constexpr int i = step;
         const T dt = shared_dt[i][lane], u = shared_u[i][lane];
-        const auto bs = projected(b_, i);
         const bool cut = RESETS && (starts >> i & 1);
-#pragma unroll
-        for (int s = 0; s < kStates; ++s) {
+        for_each<kStates>([&](auto state) {
+          constexpr int s = state;
           keep[i][s] = decay(dt, rate[s]);
-          const T before = i ? h[i - 1][s] : start[s];
-          h[i][s] = __builtin_elementwise_fma(keep[i][s], cut ? T(0) : before, u * bs[s]);
-        }
-      }
+          T before = start[s];
+          if constexpr (i > 0) before = h[i - 1][s];
+          h[i][s] = __builtin_elementwise_fma(keep[i][s], cut ? T(0) : before, u * bs.template get<i, s>());
+        });
+      });
       T rows_b[L], rows_c[L];
-#pragma unroll
-      for (int i = L - 1; i >= 0; --i) {
+      for_each<L>([&](auto step) {
+        constexpr int i = L - 1 - step;
         const T dt = shared_dt[i][lane], u = shared_u[i][lane], g = shared_g[i][lane];
-        const auto bs = projected(b_, i), cs = projected(c_, i);
         const bool cut = RESETS && (starts >> i & 1);
         T along = T(0), decays = T(0), y = T(0), to_b[kStates], to_c[kStates];
-#pragma unroll
-        for (int s = 0; s < kStates; ++s) {
-          const T m = __builtin_elementwise_fma(cs[s], g, e[s]);
+        for_each<kStates>([&](auto state) {
+          constexpr int s = state;
+          const T m = __builtin_elementwise_fma(cs.template get<i, s>(), g, e[s]);
           to_c[s] = g * h[i][s];
           to_b[s] = u * m;
-          along = __builtin_elementwise_fma(m, bs[s], along);
-          y = __builtin_elementwise_fma(cs[s], h[i][s], y);
+          along = __builtin_elementwise_fma(bs.template get<i, s>(), m, along);
+          y = __builtin_elementwise_fma(cs.template get<i, s>(), h[i][s], y);
           e[s] = cut ? T(0) : keep[i][s] * m;
-          const T before = i ? h[i - 1][s] : start[s], share = cut ? T(0) : e[s] * before;
+          T before = start[s];
+          if constexpr (i > 0) before = h[i - 1][s];
+          const T share = cut ? T(0) : e[s] * before;
           decays = __builtin_elementwise_fma(share, slow[s], decays);
           da[s] = __builtin_elementwise_fma(share, dt, da[s]);
-        }
+        });
         sums_b[at.wave][i][lane] = along;
         sums_a[at.wave][i][lane] = decays;
         if (c.gate) sums_y[at.wave][i][lane] = y;
         rows_b[i] = fold_rows<4>(fold_rows<5>(to_b[0], to_b[1]), fold_rows<5>(to_b[2], to_b[3]));
         rows_c[i] = fold_rows<4>(fold_rows<5>(to_c[0], to_c[1]), fold_rows<5>(to_c[2], to_c[3]));
-      }
+      });
       const T all_b = fold_steps<T, L>(rows_b, lane), all_c = fold_steps<T, L>(rows_c, lane);
       const int i = step_of_lane<L>(lane), s = (lane >> 5 & 1) | (lane >> 4 & 1) << 1;
       if (i < count && (L == 16 || !(lane & 1))) {
@@ -342,9 +340,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
         o.db[to] = all_b;
         o.dc[to] = all_c;
       }
-    };
-    if (count == L) walk(std::true_type{});
-    else walk(std::false_type{});
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
