@@ -37,20 +37,22 @@ __device__ __forceinline__ void gates(T g, T& keep, T& take) {
   take = g >= T(0) ? small * large : large;
 }
 
-// log(1 + exp(v)) to full relative precision: max(v, 0) + log(1 + e) with e = exp(-|v|),
-// log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3, by its series; the first term left
-// out is below 2^-26 of it.
-__device__ __forceinline__ float softplus(float v) {
+// log(1 + exp(v)) and its derivative sigmoid(v), to full relative precision:
+// max(v, 0) + log(1 + e) with e = exp(-|v|), log(1 + e) = 2 artanh(t), t = e / (2 + e) <= 1/3,
+// by its series; the first term left out is below 2^-26 of it.
+__device__ __forceinline__ float softplus(float v, float& slope) {
   const float e = exp_down(-__builtin_elementwise_abs(v));
-  const float s = e * inverse(2.0f + e), p = s * s;
+  const float t = e * inverse(2.0f + e), p = t * t, large = inverse(1.0f + e);
   float r = 1.0f / 13;
 #pragma unroll
   for (int k = 11; k > 0; k -= 2) r = __builtin_fmaf(r, p, 1.0f / k);
-  const float tail = 2.0f * s * r;
+  const float tail = 2.0f * t * r;
+  slope = v >= 0.0f ? large : e * large;
   return v > 0.0f ? v + tail : v <= 0.0f ? tail : v;
 }
-__device__ __forceinline__ double softplus(double v) {
-  const double tail = log1p(exp(-__builtin_elementwise_abs(v)));
+__device__ __forceinline__ double softplus(double v, double& slope) {
+  const double e = exp(-__builtin_elementwise_abs(v)), tail = log1p(e), large = 1.0 / (1.0 + e);
+  slope = v >= 0 ? large : e * large;
   return v > 0 ? v + tail : v <= 0 ? tail : v;
 }
 

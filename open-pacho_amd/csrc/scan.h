@@ -3,7 +3,7 @@
 //   dt = softplus(delta + bias),  r_n = exp(a_log_n)
 //   h_t,n = exp(-dt r_n) h_{t-1},n + dt x_t b_t,n,  y_t = (sum_n c_t,n h_t,n + skip x_t) silu(gate_t)
 //
-// A lane owns a channel, a wave kStates of its states, a workgroup all states of up to 64
+// A lane owns a channel, a wave S (2 or 4) of its states, a workgroup all states of up to 64
 // channels that share b and c. So b and c are the same in a whole wave: a register holds
 // those of four steps in the lanes of each row of 16, and an instruction that multiplies by
 // one of them takes it from its lane on the way (a row broadcast). An exponential, two
@@ -27,8 +27,6 @@
 
 namespace hpd {
 
-constexpr int kStates = 4;  // of a wave
-
 // The arrays of a call; pointers that it does not have are null.
 template <typename T>
 struct Scan {
@@ -39,8 +37,8 @@ struct Scan {
   int64_t width;   // channels of a group
   int64_t pieces;  // of a group's channels, 64 each
   int64_t states;  // of a channel
-  int64_t padded;  // of a step and group in b and c: states, up to a multiple of kStates
-  int64_t first;   // state of this launch, which takes kStates for each wave
+  int64_t padded;  // of a step and group in b and c: states, up to whole launches
+  int64_t first;   // state of this launch, which takes S for each wave
   bool starts, ends;  // the first and the last launch over the states
   int64_t parts;   // of a row's steps
   int64_t steps;   // of a part, a multiple of the tile
@@ -53,9 +51,9 @@ struct Scan {
   const T *grad, *grad_state;
 };
 
-template <typename T>
-struct Quad {
-  typedef T type __attribute__((ext_vector_type(kStates), aligned(sizeof(T))));
+template <typename T, int S>
+struct Several {
+  typedef T type __attribute__((ext_vector_type(S), aligned(sizeof(T))));
 };
 
 // exp(dt rate) of rates that are -r, for floats -r log2 e: the rounding of the product is off
@@ -73,7 +71,7 @@ __device__ __forceinline__ T passed_decay(T span, T rate) {
 }
 
 // What a workgroup and its lanes work on.
-template <typename T, int NW>
+template <typename T, int NW, int S>
 struct Place {
   int lane, wave;
   int64_t row, group, piece, part, channel, first, end, length;  // steps [first, end) of a row of `length`
@@ -95,7 +93,7 @@ struct Place {
     length = c.rows.end(row);
     first = part * c.steps;
     end = first + c.steps < length ? first + c.steps : length;
-    slot = wave * kStates;
+    slot = wave * S;
     state = c.first + slot;
   }
   __device__ __forceinline__ int64_t at(const Scan<T>& c, int64_t t) const { return (row * c.rows.time + t) * c.channels + channel; }
@@ -105,37 +103,37 @@ struct Place {
   }
   // Of (..., batch, states of a launch, channels).
   __device__ __forceinline__ int64_t state_at(const Scan<T>& c, int64_t lead, int s) const {
-    return ((lead * c.batch + row) * (NW * kStates) + slot + s) * c.channels + channel;
+    return ((lead * c.batch + row) * (NW * S) + slot + s) * c.channels + channel;
   }
   // Values of the wave's states in an array (batch, channels, states), zero for those that pad.
-  __device__ __forceinline__ void read(const Scan<T>& c, const T* array, int64_t lead, T (&to)[kStates]) const {
+  __device__ __forceinline__ void read(const Scan<T>& c, const T* array, int64_t lead, T (&to)[S]) const {
     const T* from = array + (lead * c.channels + channel) * c.states + state;
-    if (state + kStates <= c.states) {
-      const auto v = *reinterpret_cast<const typename Quad<T>::type*>(from);
+    if (state + S <= c.states) {
+      const auto v = *reinterpret_cast<const typename Several<T, S>::type*>(from);
 #pragma unroll
-      for (int s = 0; s < kStates; ++s) to[s] = v[s];
+      for (int s = 0; s < S; ++s) to[s] = v[s];
     } else {
 #pragma unroll
-      for (int s = 0; s < kStates; ++s) to[s] = state + s < c.states ? from[s] : T(0);
+      for (int s = 0; s < S; ++s) to[s] = state + s < c.states ? from[s] : T(0);
     }
   }
-  __device__ __forceinline__ void write(const Scan<T>& c, T* array, int64_t lead, const T (&from)[kStates]) const {
+  __device__ __forceinline__ void write(const Scan<T>& c, T* array, int64_t lead, const T (&from)[S]) const {
     if (!valid) return;
     T* to = array + (lead * c.channels + channel) * c.states + state;
 #pragma unroll
-    for (int s = 0; s < kStates; ++s) {
+    for (int s = 0; s < S; ++s) {
       if (state + s < c.states) to[s] = from[s];
     }
   }
   // The states before the part, from its predecessors' sums and ends.
-  __device__ __forceinline__ void arrive(const Scan<T>& c, const T (&rate)[kStates], T (&h)[kStates]) const {
+  __device__ __forceinline__ void arrive(const Scan<T>& c, const T (&rate)[S], T (&h)[S]) const {
 #pragma unroll
-    for (int s = 0; s < kStates; ++s) h[s] = T(0);
+    for (int s = 0; s < S; ++s) h[s] = T(0);
     if (c.initial) read(c, c.initial, row, h);
     for (int64_t p = 0; p < part; ++p) {
       const T span = c.spans[(p * c.batch + row) * c.channels + channel];
 #pragma unroll
-      for (int s = 0; s < kStates; ++s) {
+      for (int s = 0; s < S; ++s) {
         const T end = c.ended[state_at(c, p, s)];
         h[s] = span < T(0) ? end : __builtin_elementwise_fma(passed_decay(span, rate[s]), h[s], end);
       }
@@ -167,30 +165,36 @@ __device__ __forceinline__ double of_row(double v) {
   return __builtin_bit_cast(double, w);
 }
 
-// b or c of the wave's states in the L steps of a tile.
-template <typename T, int L>
+// b or c of the wave's states in the L steps of a tile: 16 / S steps a register.
+template <typename T, int L, int S>
 struct Projections {
-  T v[L / 4];
+  static constexpr int kSteps = 16 / S;
+  T v[L / kSteps];
 
   // Those of steps behind the end are what the last one's are, until keep() clears them.
   template <int NW>
-  __device__ __forceinline__ void load(const Scan<T>& c, const Place<T, NW>& at, const T* array, int64_t t) {
+  __device__ __forceinline__ void load(const Scan<T>& c, const Place<T, NW, S>& at, const T* array, int64_t t) {
     const T* from = array + ((at.row * c.rows.time + t) * c.groups + at.group) * c.padded + at.state;
     const unsigned stride = unsigned(c.groups * c.padded), left = at.end - t < L ? unsigned(at.end - t) : unsigned(L);
 #pragma unroll
-    for (int q = 0; q < L / 4; ++q) {
-      const unsigned i = 4 * q + (at.lane >> 2 & 3);
-      v[q] = from[(i < left ? i : left - 1) * stride + (at.lane & 3)];
+    for (int q = 0; q < L / kSteps; ++q) {
+      const unsigned i = q * kSteps + (at.lane & 15) / S;
+      v[q] = from[(i < left ? i : left - 1) * stride + at.lane % S];
     }
   }
   __device__ __forceinline__ void keep(int lane, int count) {
 #pragma unroll
-    for (int q = 0; q < L / 4; ++q) v[q] = 4 * q + (lane >> 2 & 3) < count ? v[q] : T(0);
+    for (int q = 0; q < L / kSteps; ++q) v[q] = q * kSteps + (lane & 15) / S < count ? v[q] : T(0);
   }
-  // Of step I and state S.
-  template <int I, int S>
+  // What was taken from lanes before is taken again after this, in place of staying in registers.
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int q = 0; q < L / kSteps; ++q) asm("" : "+v"(v[q]));
+  }
+  // Of step I and state J.
+  template <int I, int J>
   __device__ __forceinline__ T get() const {
-    return of_row<(I % 4) * 4 + S>(v[I / 4]);
+    return of_row<I % kSteps * S + J>(v[I / kSteps]);
   }
 };
 
@@ -200,20 +204,14 @@ __device__ __forceinline__ T cut_span() {
   return T(-1);
 }
 
-// dt of a raw step.
-template <typename T>
-__device__ __forceinline__ T step_of(T delta, T bias) {
-  return softplus(delta + bias);
-}
-
 }  // namespace hpd
 
 namespace hp {
 
-// Whether waves of a launch over `states` number 1, 2, 4, ... up to `most`.
-inline int scan_waves(int64_t states, int most) {
+// Waves of a launch with `each` states a wave: 1, 2, 4, ... up to `most`.
+inline int scan_waves(int64_t states, int each, int most) {
   int waves = 1;
-  while (waves < most && int64_t(waves) * hpd::kStates < states) waves *= 2;
+  while (waves < most && int64_t(waves) * each < states) waves *= 2;
   return waves;
 }
 
@@ -223,6 +221,13 @@ template <typename T>
 const T* scan_padded(hp_ctx* ctx, Scratch& scratch, const T* array, int64_t steps, int64_t states, int64_t padded);
 template <typename T>
 void scan_fill(hp_ctx* ctx, T* to, const T* from, int64_t n);
+
+// States of a wave: two where four would leave SIMDs with one wave, whose waits nothing covers.
+template <typename T>
+int scan_states(const hpd::Scan<T>& c) {
+  const int64_t waves = c.batch * c.groups * c.pieces * c.parts * ceil_div(c.states, 4);
+  return c.states > 2 && c.states <= 16 && waves < 2048 ? 2 : 4;
+}
 
 // Parts of rows: one, or as many as make enough workgroups.
 template <typename T>

@@ -9,27 +9,27 @@ namespace {
 constexpr int kSteps = 16;  // of a tile
 
 // SUMMARY: a part's sum of dt and the states that it ends in from zero ones, in place of y.
-template <typename T, int NW, bool RESETS, bool SUMMARY>
+template <typename T, int NW, int S, bool RESETS, bool SUMMARY>
 __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_, const T* c_) {
   constexpr int kOwn = kSteps / NW;  // steps of a tile that a wave prepares and finishes
   __shared__ T shared_dt[kSteps][64], shared_u[kSteps][64];
   __shared__ T sums[SUMMARY ? 1 : NW][SUMMARY ? 1 : kSteps][64];
-  const Place<T, NW> at(c);
+  const Place<T, NW, S> at(c);
   if (SUMMARY && at.part == c.parts - 1) return;
   const int lane = at.lane, own = at.wave * kOwn;
-  T rate[kStates], h[kStates];
+  T rate[S], h[S];
   at.read(c, c.a_log, 0, rate);
 #pragma unroll
-  for (int s = 0; s < kStates; ++s) rate[s] = rate_of(rate[s]);
+  for (int s = 0; s < S; ++s) rate[s] = rate_of(rate[s]);
   if constexpr (SUMMARY) {
 #pragma unroll
-    for (int s = 0; s < kStates; ++s) h[s] = T(0);
+    for (int s = 0; s < S; ++s) h[s] = T(0);
   } else {
     at.arrive(c, rate, h);
   }
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0), skip = c.skip ? c.skip[at.channel] : T(0);
   T x[kOwn], delta[kOwn], gate[kOwn], span = T(0);
-  Projections<T, kSteps> next_b, next_c;
+  Projections<T, kSteps, S> next_b, next_c;
   bool cut = false;
   const auto load = [&](int64_t t) {
 #pragma unroll
@@ -49,35 +49,37 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const bool inside = own + i < count;
-      const T dt = step_of(delta[i], bias);
+      T slope;
+      const T dt = softplus(delta[i] + bias, slope);
       shared_dt[own + i][lane] = inside ? dt : T(0);
       shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
       now_x[i] = x[i];
       if (!SUMMARY) now_gate[i] = gate[i];
     }
-    Projections<T, kSteps> bs = next_b, cs = next_c;
+    Projections<T, kSteps, S> bs = next_b, cs = next_c;
     bs.keep(lane, count);
     if (!SUMMARY) cs.keep(lane, count);
     __syncthreads();
     if (t + kSteps < at.end) load(t + kSteps);
     const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<kSteps>(at.row, t, at.end)) : 0;
-    for_each<kSteps>([&](auto step) {
-      constexpr int i = step;
-      const T dt = shared_dt[i][lane], u = shared_u[i][lane];
-      if (RESETS && (starts >> i & 1)) {
-#pragma unroll
-        for (int s = 0; s < kStates; ++s) h[s] = T(0);
-        cut = true;
-      }
-      T y = T(0);
-      for_each<kStates>([&](auto state) {
-        constexpr int s = state;
-        h[s] = __builtin_elementwise_fma(decay(dt, rate[s]), h[s], u * bs.template get<i, s>());
-        if constexpr (!SUMMARY) y = __builtin_elementwise_fma(cs.template get<i, s>(), h[s], y);
+    // Tiles without a reset, nearly all of them, do without its selects.
+    const auto walk = [&](auto resets) {
+      for_each<kSteps>([&](auto step) {
+        constexpr int i = step;
+        const T dt = shared_dt[i][lane], u = shared_u[i][lane];
+        T y = T(0);
+        for_each<S>([&](auto state) {
+          constexpr int s = state;
+          if (resets) h[s] = starts >> i & 1 ? T(0) : h[s];
+          h[s] = __builtin_elementwise_fma(decay(dt, rate[s]), h[s], u * bs.template get<i, s>());
+          if constexpr (!SUMMARY) y = __builtin_elementwise_fma(cs.template get<i, s>(), h[s], y);
+        });
+        if constexpr (SUMMARY) span += dt;
+        else sums[at.wave][i][lane] = y;
       });
-      if constexpr (SUMMARY) span += dt;
-      else sums[at.wave][i][lane] = y;
-    });
+    };
+    if (RESETS && starts) walk(std::true_type{}), cut = true;
+    else walk(std::false_type{});
     __syncthreads();
     if constexpr (!SUMMARY) {
 #pragma unroll
@@ -104,7 +106,7 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
     if (!at.valid) return;
     if (at.wave == 0) c.spans[(at.part * c.batch + at.row) * c.channels + at.channel] = cut ? cut_span<T>() : span;
 #pragma unroll
-    for (int s = 0; s < kStates; ++s) c.ended[at.state_at(c, at.part, s)] = h[s];
+    for (int s = 0; s < S; ++s) c.ended[at.state_at(c, at.part, s)] = h[s];
   } else {
     // Behind the row's end, by every wave for its own steps.
     const int64_t stop = at.first + c.steps < c.rows.time ? at.first + c.steps : c.rows.time;
@@ -131,11 +133,17 @@ __global__ __launch_bounds__(256) void fill_kernel(T* to, const T* from, int64_t
 }
 
 template <typename T, bool SUMMARY>
-void launch(hp_ctx* ctx, const Scan<T>& c, const T* b, const T* cs, int waves) {
+void launch(hp_ctx* ctx, const Scan<T>& c, const T* b, const T* cs, int each, int waves) {
   const unsigned blocks = unsigned(c.batch * c.groups * c.pieces * c.parts);
   const auto run = [&](auto nw) {
-    const auto kernel = c.rows.resets ? forward_kernel<T, nw, true, SUMMARY> : forward_kernel<T, nw, false, SUMMARY>;
-    kernel<<<blocks, nw * 64, 0, ctx->stream>>>(c, b, cs);
+    const auto with = [&](auto states) {
+      const auto kernel = c.rows.resets ? forward_kernel<T, nw, states, true, SUMMARY> : forward_kernel<T, nw, states, false, SUMMARY>;
+      kernel<<<blocks, nw * 64, 0, ctx->stream>>>(c, b, cs);
+    };
+    if constexpr (nw >= 2 && nw <= 8) {
+      if (each == 2) return with(std::integral_constant<int, 2>{});
+    }
+    with(std::integral_constant<int, 4>{});
   };
   switch (waves) {
     case 1: run(std::integral_constant<int, 1>{}); break;
@@ -203,20 +211,20 @@ int hp_selective_scan(hp_ctx* ctx, int dtype, int index_dtype, const void* x, co
       s.rows = {static_cast<const uint8_t*>(resets), lengths, index_dtype == HP_I64, time};
       s.batch = batch, s.channels = channels, s.groups = groups, s.states = states;
       s.width = channels / groups, s.pieces = hp::ceil_div(s.width, 64);
-      const int waves = hp::scan_waves(states, 16);
-      s.padded = hp::ceil_div(states, waves * kStates) * waves * kStates;
+      hp::scan_plan(s, kSteps);
+      const int each = hp::scan_states(s), waves = hp::scan_waves(states, each, 16), width = waves * each;
+      s.padded = hp::ceil_div(states, width) * width;
       const T *bs = hp::scan_padded(ctx, scratch, in(b), batch * time * groups, states, s.padded);
       const T *cs = hp::scan_padded(ctx, scratch, in(c), batch * time * groups, states, s.padded);
-      hp::scan_plan(s, kSteps);
       if (s.parts > 1) {
         s.spans = scratch.take<T>(s.parts * batch * channels);
-        s.ended = scratch.take<T>(s.parts * batch * waves * kStates * channels);
+        s.ended = scratch.take<T>(s.parts * batch * width * channels);
       }
-      for (s.first = 0; s.first < states; s.first += waves * kStates) {
+      for (s.first = 0; s.first < states; s.first += width) {
         s.starts = s.first == 0;
-        s.ends = s.first + waves * kStates >= states;
-        if (s.parts > 1) launch<T, true>(ctx, s, bs, cs, waves);
-        launch<T, false>(ctx, s, bs, cs, waves);
+        s.ends = s.first + width >= states;
+        if (s.parts > 1) launch<T, true>(ctx, s, bs, cs, each, waves);
+        launch<T, false>(ctx, s, bs, cs, each, waves);
       }
     };
     if (dtype == HP_F32) run(float(0));

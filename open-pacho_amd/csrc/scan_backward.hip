@@ -26,25 +26,26 @@ using namespace hpd;
 namespace {
 
 // Steps of a tile, and waves of a launch, for the registers that a tile's states and decays take.
-template <typename T>
-constexpr int kTile = sizeof(T) == 4 ? 16 : 8;
+template <typename T, int NW, int S>
+constexpr int kTile = sizeof(T) == 4 ? (S == 4 && NW == 8 ? 8 : 16) : NW == 1 ? 4 : 8;
 template <typename T>
 constexpr int kMostWaves = sizeof(T) == 4 ? 8 : 4;
+constexpr int kLongestTile = 16;
 
-template <typename T, int NW, bool RESETS, bool SPLIT>
+template <typename T, int NW, int S, bool RESETS, bool SPLIT>
 __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_, const T* c_) {
-  constexpr int L = kTile<T>, kOwn = L / NW;
+  constexpr int L = kTile<T, NW, S>, kOwn = L / NW;
   __shared__ T shared_dt[L][64], shared_u[L][64], shared_g[SPLIT ? L : 1][64];
-  const Place<T, NW> at(c);
+  const Place<T, NW, S> at(c);
   const int lane = at.lane, own = at.wave * kOwn;
-  T rate[kStates], h[kStates], through[kStates], back[kStates], span = T(0);
+  T rate[S], h[S], through[S], back[S], span = T(0);
   at.read(c, c.a_log, 0, rate);
 #pragma unroll
-  for (int s = 0; s < kStates; ++s) rate[s] = rate_of(rate[s]), h[s] = back[s] = T(0), through[s] = T(1);
+  for (int s = 0; s < S; ++s) rate[s] = rate_of(rate[s]), h[s] = back[s] = T(0), through[s] = T(1);
   if (!SPLIT && c.initial) at.read(c, c.initial, at.row, h);
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0);
   T x[kOwn], delta[kOwn], grad[kOwn], gate[kOwn];
-  Projections<T, L> next_b, next_c;
+  Projections<T, L, S> next_b, next_c;
   bool cut = false;
   const auto load = [&](int64_t t) {
 #pragma unroll
@@ -66,7 +67,8 @@ __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_,
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const bool inside = own + i < count;
-      const T dt = step_of(delta[i], bias);
+      T slope;
+      const T dt = softplus(delta[i] + bias, slope);
       shared_dt[own + i][lane] = inside ? dt : T(0);
       shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
       if constexpr (SPLIT) {
@@ -79,7 +81,7 @@ __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_,
         shared_g[own + i][lane] = inside ? g : T(0);
       }
     }
-    Projections<T, L> bs = next_b, cs = next_c;
+    Projections<T, L, S> bs = next_b, cs = next_c;
     bs.keep(lane, count);
     if (SPLIT) cs.keep(lane, count);
     __syncthreads();
@@ -87,38 +89,43 @@ __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_,
     const int64_t tile = t / L;
     if (at.valid) {
 #pragma unroll
-      for (int s = 0; s < kStates; ++s) c.before[at.state_at(c, tile, s)] = h[s];
+      for (int s = 0; s < S; ++s) c.before[at.state_at(c, tile, s)] = h[s];
       if (SPLIT && at.wave == 0) c.since[(tile * c.batch + at.row) * c.channels + at.channel] = cut ? cut_span<T>() : span;
     }
     const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<L>(at.row, t, at.end)) : 0;
-    for_each<L>([&](auto step) {
-      constexpr int i = step;
-      const T dt = shared_dt[i][lane], u = shared_u[i][lane];
-      T g = SPLIT ? shared_g[SPLIT ? i : 0][lane] : T(0);
-      if (RESETS && (starts >> i & 1)) {
-#pragma unroll
-        for (int s = 0; s < kStates; ++s) h[s] = through[s] = T(0);
-        cut = true;
-      }
-      if (RESETS && cut) g = T(0);
-      for_each<kStates>([&](auto state) {
-        constexpr int s = state;
-        const T keep = decay(dt, rate[s]);
-        h[s] = __builtin_elementwise_fma(keep, h[s], u * bs.template get<i, s>());
+    // Tiles without a reset, nearly all of them, do without its selects.
+    const auto walk = [&](auto resets) {
+      for_each<L>([&](auto step) {
+        constexpr int i = step;
+        const bool start = resets && (starts >> i & 1);
+        const T dt = shared_dt[i][lane], u = shared_u[i][lane];
+        T g = T(0);
         if constexpr (SPLIT) {
-          through[s] *= keep;
-          back[s] = __builtin_elementwise_fma(through[s], cs.template get<i, s>() * g, back[s]);
+          cut = cut || start;
+          g = RESETS && cut ? T(0) : shared_g[i][lane];
+          span += dt;
         }
+        for_each<S>([&](auto state) {
+          constexpr int s = state;
+          const T keep = decay(dt, rate[s]);
+          if (resets) h[s] = start ? T(0) : h[s];
+          h[s] = __builtin_elementwise_fma(keep, h[s], u * bs.template get<i, s>());
+          if constexpr (SPLIT) {
+            through[s] *= keep;
+            back[s] = __builtin_elementwise_fma(through[s], cs.template get<i, s>() * g, back[s]);
+          }
+        });
       });
-      if constexpr (SPLIT) span += dt;
-    });
+    };
+    if (RESETS && starts) walk(std::true_type{});
+    else walk(std::false_type{});
     __syncthreads();
   }
   if constexpr (SPLIT) {
     if (!at.valid) return;
     if (at.wave == 0) c.spans[(at.part * c.batch + at.row) * c.channels + at.channel] = cut ? cut_span<T>() : span;
 #pragma unroll
-    for (int s = 0; s < kStates; ++s) {
+    for (int s = 0; s < S; ++s) {
       c.ended[at.state_at(c, at.part, s)] = h[s];
       c.passed[at.state_at(c, at.part, s)] = back[s];
     }
@@ -179,52 +186,87 @@ __device__ __forceinline__ T fold_pair(T a, T b, bool bit) {
   return (bit ? b : a) + from_across<MASK>(bit ? a : b);
 }
 
-// Of a value for each of L steps the sums over a row of 16 lanes: lane i has step
-// step_of_lane(i). Pairs meet across 8, 7, 3 and 1 lanes, which reaches all 16.
-template <typename T, int L>
-__device__ __forceinline__ T fold_steps(const T (&v)[L], int lane) {
-  T a[L / 2];
+// Of N values (4, 8 or 16) the sums over a row of 16 lanes: lane i has value number_of_lane(i).
+// Pairs meet across 8, 7, 3 and 1 lanes, which reaches all 16.
+template <typename T, int N>
+__device__ __forceinline__ T fold_row(const T (&v)[N], int lane) {
+  T a[N / 2];
 #pragma unroll
-  for (int k = 0; k < L / 2; ++k) a[k] = fold_pair<8>(v[2 * k], v[2 * k + 1], lane & 8);
-  T b[L / 4];
+  for (int k = 0; k < N / 2; ++k) a[k] = fold_pair<8>(v[2 * k], v[2 * k + 1], lane & 8);
+  T b[N / 4];
 #pragma unroll
-  for (int k = 0; k < L / 4; ++k) b[k] = fold_pair<7>(a[2 * k], a[2 * k + 1], lane & 4);
-  T d[L / 8];
+  for (int k = 0; k < N / 4; ++k) b[k] = fold_pair<7>(a[2 * k], a[2 * k + 1], lane & 4);
+  T d[N < 8 ? 1 : N / 8];
+  if constexpr (N >= 8) {
 #pragma unroll
-  for (int k = 0; k < L / 8; ++k) d[k] = fold_pair<3>(b[2 * k], b[2 * k + 1], lane & 2);
-  if constexpr (L == 16) return fold_pair<1>(d[0], d[1], lane & 1);
+    for (int k = 0; k < N / 8; ++k) d[k] = fold_pair<3>(b[2 * k], b[2 * k + 1], lane & 2);
+  } else {
+    d[0] = b[0] + from_across<3>(b[0]);
+  }
+  if constexpr (N == 16) return fold_pair<1>(d[0], d[1], lane & 1);
   else return d[0] + from_across<1>(d[0]);
 }
-template <int L>
+template <int N>
+__device__ __forceinline__ int number_of_lane(int lane) {
+  return (lane >> 3 & 1) | (lane >> 2 & 1) << 1 | (N >= 8 ? (lane >> 1 & 1) << 2 : 0) | (N == 16 ? (lane & 1) << 3 : 0);
+}
+
+// Of S values for each of L steps the sums over all lanes: lane i has that of step
+// step_of_lane(i) and state state_of_lane(i).
+template <int S, typename T>
+__device__ __forceinline__ T fold_states(const T (&v)[S]) {
+  if constexpr (S == 4) return fold_rows<4>(fold_rows<5>(v[0], v[1]), fold_rows<5>(v[2], v[3]));
+  else return fold_rows<5>(v[0], v[1]);
+}
+template <int S, typename T, int L>
+__device__ __forceinline__ T fold_steps(const T (&v)[L], int lane) {
+  if constexpr (S == 4) return fold_row<T, L>(v, lane);
+  else {
+    T pairs[L / 2];
+#pragma unroll
+    for (int k = 0; k < L / 2; ++k) pairs[k] = fold_rows<4>(v[2 * k], v[2 * k + 1]);
+    return fold_row<T, L / 2>(pairs, lane);
+  }
+}
+template <int S, int L>
 __device__ __forceinline__ int step_of_lane(int lane) {
-  return (lane >> 3 & 1) | (lane >> 2 & 1) << 1 | (lane >> 1 & 1) << 2 | (L == 16 ? (lane & 1) << 3 : 0);
+  return S == 4 ? number_of_lane<L>(lane) : (lane >> 4 & 1) | number_of_lane<L / 2>(lane) << 1;
+}
+template <int S>
+__device__ __forceinline__ int state_of_lane(int lane) {
+  return (lane >> 5 & 1) | (S == 4 ? (lane >> 4 & 1) << 1 : 0);
+}
+// Of the lanes that have the same sum, the one that leaves it.
+template <int S, int L>
+__device__ __forceinline__ bool leaves(int lane) {
+  return lane % (64 / (S * L)) == 0;
 }
 
 // ---- backward ------------------------------------------------------------------------
 
-template <typename T, int NW, bool RESETS>
+template <typename T, int NW, int S, bool RESETS>
 __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o, const T* b_, const T* c_) {
-  constexpr int L = kTile<T>, kOwn = L / NW;
+  constexpr int L = kTile<T, NW, S>, kOwn = L / NW;
   __shared__ T shared_dt[L][64], shared_u[L][64], shared_g[L][64];
   __shared__ T sums_b[NW][L][64], sums_a[NW][L][64], sums_y[NW][L][64];
-  const Place<T, NW> at(c);
+  const Place<T, NW, S> at(c);
   const int lane = at.lane, own = at.wave * kOwn;
-  T rate[kStates], slow[kStates], e[kStates], da[kStates];
+  T rate[S], slow[S], e[S], da[S];
   at.read(c, c.a_log, 0, slow);
 #pragma unroll
-  for (int s = 0; s < kStates; ++s) {
+  for (int s = 0; s < S; ++s) {
     rate[s] = rate_of(slow[s]);
     slow[s] = sizeof(T) == 4 ? -T(expf(float(slow[s]))) : rate[s];
     e[s] = da[s] = T(0);
   }
-  T arrived[kStates];
+  T arrived[S] = {};
   if (c.parts > 1) {
     at.arrive(c, rate, arrived);
     if (c.grad_state) at.read(c, c.grad_state, at.row, e);
     for (int64_t p = c.parts - 1; p > at.part; --p) {
       const T span = c.spans[(p * c.batch + at.row) * c.channels + at.channel];
 #pragma unroll
-      for (int s = 0; s < kStates; ++s) {
+      for (int s = 0; s < S; ++s) {
         const T back = c.passed[at.state_at(c, p, s)];
         e[s] = span < T(0) ? back : __builtin_elementwise_fma(passed_decay(span, rate[s]), e[s], back);
       }
@@ -233,7 +275,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
     at.read(c, c.grad_state, at.row, e);
   }
 #pragma unroll
-  for (int s = 0; s < kStates; ++s) e[s] = at.valid ? e[s] : T(0);  // other lanes add nothing to db and dc
+  for (int s = 0; s < S; ++s) e[s] = at.valid ? e[s] : T(0);  // other lanes add nothing to db and dc
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0), skip = c.skip ? c.skip[at.channel] : T(0);
   T dskip = T(0), dbias = T(0);
   // Behind the row's end, by every wave for its own steps.
@@ -245,60 +287,65 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
     if (c.gate) o.dgate[to] = T(0);
   }
   const int64_t tiles = at.end > at.first ? (at.end - at.first + L - 1) / L : 0;
-  T x[kOwn], delta[kOwn], gate[kOwn], grad[kOwn];
-  Projections<T, L> bs, cs;
+  T next_x[kOwn], delta[kOwn], gate[kOwn], grad[kOwn], before[S], since = cut_span<T>();
+  Projections<T, L, S> next_b, next_c;
   const auto load = [&](int64_t t) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int64_t step = t + own + i < at.end ? t + own + i : at.end - 1;
-      x[i] = at.get(c, c.x, step);
+      next_x[i] = at.get(c, c.x, step);
       delta[i] = at.get(c, c.delta, step);
       grad[i] = at.get(c, c.grad, step);
       if (c.gate) gate[i] = at.get(c, c.gate, step);
     }
-    bs.load(c, at, b_, t);
-    cs.load(c, at, c_, t);
+    next_b.load(c, at, b_, t);
+    next_c.load(c, at, c_, t);
+    const int64_t tile = t / L;
+#pragma unroll
+    for (int s = 0; s < S; ++s) before[s] = c.before[at.state_at(c, tile, s)];
+    if (c.parts > 1) since = c.since[(tile * c.batch + at.row) * c.channels + at.channel];
   };
+  if (tiles) load(at.first + (tiles - 1) * L);
   for (int64_t n = tiles - 1; n >= 0; --n) {
     const int64_t t = at.first + n * L;
     const int count = at.end - t < L ? int(at.end - t) : L;
-    load(t);
-    bs.keep(lane, count);
-    cs.keep(lane, count);
+    T x[kOwn], slope[kOwn], passes[kOwn];  // of the wave's own steps; slopes of dt, and of y by the gate times dy
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const bool inside = at.valid && own + i < count;
-      const T dt = step_of(delta[i], bias);
+      x[i] = next_x[i];
+      const T dt = softplus(delta[i] + bias, slope[i]);
       T g = grad[i];
       if (c.gate) {
         T keep, rest;
         gates(gate[i], keep, rest);
+        passes[i] = g * (keep * (T(1) + gate[i] * rest));
         g *= gate[i] * keep;
       }
       shared_dt[own + i][lane] = inside ? dt : T(0);
       shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
       shared_g[own + i][lane] = inside ? g : T(0);
     }
-    T start[kStates];
-    const int64_t tile = t / L;
+    T start[S];
 #pragma unroll
-    for (int s = 0; s < kStates; ++s) start[s] = at.valid ? c.before[at.state_at(c, tile, s)] : T(0);
-    if (c.parts > 1 && at.valid) {
-      const T span = c.since[(tile * c.batch + at.row) * c.channels + at.channel];
-      if (span >= T(0)) {
-#pragma unroll
-        for (int s = 0; s < kStates; ++s) start[s] = __builtin_elementwise_fma(passed_decay(span, rate[s]), arrived[s], start[s]);
-      }
+    for (int s = 0; s < S; ++s) {
+      start[s] = before[s];
+      if (since >= T(0)) start[s] = __builtin_elementwise_fma(passed_decay(since, rate[s]), arrived[s], start[s]);
+      if (!at.valid) start[s] = T(0);
     }
+    Projections<T, L, S> bs = next_b, cs = next_c;
+    bs.keep(lane, count);
+    cs.keep(lane, count);
     __syncthreads();
+    if (n > 0) load(t - L);
     const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<L>(at.row, t, at.end)) : 0;
-    {
-      T h[L][kStates], keep[L][kStates];
+    const auto walk = [&](auto resets) {
+      T h[L][S], keep[L][S];
       for_each<L>([&](auto step) {
         constexpr int i = step;
         const T dt = shared_dt[i][lane], u = shared_u[i][lane];
-        const bool cut = RESETS && (starts >> i & 1);
-        for_each<kStates>([&](auto state) {
+        const bool cut = resets && (starts >> i & 1);
+        for_each<S>([&](auto state) {
           constexpr int s = state;
           keep[i][s] = decay(dt, rate[s]);
           T before = start[s];
@@ -306,13 +353,14 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
           h[i][s] = __builtin_elementwise_fma(keep[i][s], cut ? T(0) : before, u * bs.template get<i, s>());
         });
       });
+      bs.renew();
       T rows_b[L], rows_c[L];
       for_each<L>([&](auto step) {
         constexpr int i = L - 1 - step;
         const T dt = shared_dt[i][lane], u = shared_u[i][lane], g = shared_g[i][lane];
-        const bool cut = RESETS && (starts >> i & 1);
-        T along = T(0), decays = T(0), y = T(0), to_b[kStates], to_c[kStates];
-        for_each<kStates>([&](auto state) {
+        const bool cut = resets && (starts >> i & 1);
+        T along = T(0), decays = T(0), y = T(0), to_b[S], to_c[S];
+        for_each<S>([&](auto state) {
           constexpr int s = state;
           const T m = __builtin_elementwise_fma(cs.template get<i, s>(), g, e[s]);
           to_c[s] = g * h[i][s];
@@ -329,18 +377,20 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
         sums_b[at.wave][i][lane] = along;
         sums_a[at.wave][i][lane] = decays;
         if (c.gate) sums_y[at.wave][i][lane] = y;
-        rows_b[i] = fold_rows<4>(fold_rows<5>(to_b[0], to_b[1]), fold_rows<5>(to_b[2], to_b[3]));
-        rows_c[i] = fold_rows<4>(fold_rows<5>(to_c[0], to_c[1]), fold_rows<5>(to_c[2], to_c[3]));
+        rows_b[i] = fold_states<S>(to_b);
+        rows_c[i] = fold_states<S>(to_c);
       });
-      const T all_b = fold_steps<T, L>(rows_b, lane), all_c = fold_steps<T, L>(rows_c, lane);
-      const int i = step_of_lane<L>(lane), s = (lane >> 5 & 1) | (lane >> 4 & 1) << 1;
-      if (i < count && (L == 16 || !(lane & 1))) {
+      const T all_b = fold_steps<S>(rows_b, lane), all_c = fold_steps<S>(rows_c, lane);
+      const int i = step_of_lane<S, L>(lane), s = state_of_lane<S>(lane);
+      if (i < count && leaves<S, L>(lane)) {
         const int64_t line = (at.row * c.rows.time + t + i) * c.groups + at.group, lines = c.batch * c.rows.time * c.groups;
-        const int64_t to = (at.piece * lines + line) * (NW * kStates) + at.slot + s;
+        const int64_t to = (at.piece * lines + line) * (NW * S) + at.slot + s;
         o.db[to] = all_b;
         o.dc[to] = all_c;
       }
-    }
+    };
+    if (RESETS && starts) walk(std::true_type{});
+    else walk(std::false_type{});
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
@@ -358,9 +408,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
       if (!c.starts) dx += o.dx[to], ddt += o.ddelta[to];
       else if (c.skip) dx = __builtin_elementwise_fma(skip, g, dx);
       if (c.ends) {
-        T keep, rest;
-        gates(delta[i] + bias, keep, rest);
-        ddt *= keep;
+        ddt *= slope[i];
         dbias += ddt;
         if (c.skip) dskip = __builtin_elementwise_fma(g, x[i], dskip);
       }
@@ -370,9 +418,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
         if (!c.starts) y += o.dgate[to];
         if (c.ends) {
           if (c.skip) y = __builtin_elementwise_fma(skip, x[i], y);
-          T keep, rest;
-          gates(gate[i], keep, rest);
-          y = grad[i] * y * (keep * (T(1) + gate[i] * rest));
+          y *= passes[i];
         }
         o.dgate[to] = y;
       }
@@ -381,7 +427,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
   const int64_t line = at.row * c.parts + at.part;
   if (at.valid) {
 #pragma unroll
-    for (int s = 0; s < kStates; ++s) o.da[(line * (NW * kStates) + at.slot + s) * c.channels + at.channel] = da[s] * slow[s];
+    for (int s = 0; s < S; ++s) o.da[(line * (NW * S) + at.slot + s) * c.channels + at.channel] = da[s] * slow[s];
     if (o.dinitial && at.part == 0) at.write(c, o.dinitial, at.row, e);
   }
   if (!c.ends) return;
@@ -464,15 +510,14 @@ int hp_selective_scan_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* 
       s.rows = {static_cast<const uint8_t*>(resets), lengths, index_dtype == HP_I64, time};
       s.batch = batch, s.channels = channels, s.groups = groups, s.states = states;
       s.width = channels / groups, s.pieces = hp::ceil_div(s.width, 64);
-      const int waves = hp::scan_waves(states, kMostWaves<T>), width = waves * kStates;
+            hp::scan_plan(s, kLongestTile);
+      // Doubles of two states in eight waves would not fit into their registers.
+      const int each = sizeof(T) == 4 ? hp::scan_states(s) : 4, waves = hp::scan_waves(states, each, kMostWaves<T>), width = waves * each;
       s.padded = hp::ceil_div(states, width) * width;
       const T *bs = hp::scan_padded(ctx, scratch, in(b), batch * time * groups, states, s.padded);
       const T *cs = hp::scan_padded(ctx, scratch, in(c), batch * time * groups, states, s.padded);
-      hp::scan_plan(s, kTile<T>);
-      const int64_t tiles = hp::ceil_div(time, int64_t(kTile<T>)), lines = batch * time * groups, rows = batch * s.parts;
-      s.before = scratch.take<T>(tiles * batch * width * channels);
+      const int64_t lines = batch * time * groups, rows = batch * s.parts;
       if (s.parts > 1) {
-        s.since = scratch.take<T>(tiles * batch * channels);
         s.spans = scratch.take<T>(rows * channels);
         s.ended = scratch.take<T>(rows * width * channels);
         s.passed = scratch.take<T>(rows * width * channels);
@@ -487,21 +532,34 @@ int hp_selective_scan_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* 
       for (s.first = 0; s.first < states; s.first += width) {
         s.starts = s.first == 0;
         s.ends = s.first + width >= states;
-        const auto launch = [&](auto nw) {
-          constexpr int NW = nw;
-          const auto first = s.parts > 1 ? (resets ? before_kernel<T, NW, true, true> : before_kernel<T, NW, false, true>)
-                                         : (resets ? before_kernel<T, NW, true, false> : before_kernel<T, NW, false, false>);
+        const auto launch = [&](auto nw, auto of) {
+          constexpr int NW = nw, S = of;
+          if (s.starts) {
+            const int64_t tiles = hp::ceil_div(time, int64_t(kTile<T, NW, S>));
+            s.before = scratch.take<T>(tiles * batch * width * channels);
+            if (s.parts > 1) s.since = scratch.take<T>(tiles * batch * channels);
+          }
+          const auto first = s.parts > 1 ? (resets ? before_kernel<T, NW, S, true, true> : before_kernel<T, NW, S, false, true>)
+                                         : (resets ? before_kernel<T, NW, S, true, false> : before_kernel<T, NW, S, false, false>);
           first<<<blocks, NW * 64, 0, ctx->stream>>>(s, bs, cs);
           hp::check_launch("scan states");
-          const auto second = resets ? backward_kernel<T, NW, true> : backward_kernel<T, NW, false>;
+          const auto second = resets ? backward_kernel<T, NW, S, true> : backward_kernel<T, NW, S, false>;
           second<<<blocks, NW * 64, 0, ctx->stream>>>(s, o, bs, cs);
           hp::check_launch("scan gradient");
         };
-        switch (waves) {
-          case 1: launch(std::integral_constant<int, 1>{}); break;
-          case 2: launch(std::integral_constant<int, 2>{}); break;
-          case 4: launch(std::integral_constant<int, 4>{}); break;
-          default: launch(std::integral_constant<int, kMostWaves<T>>{}); break;
+        using Two = std::integral_constant<int, 2>;
+        using Four = std::integral_constant<int, 4>;
+        using Eight = std::integral_constant<int, 8>;
+        if constexpr (sizeof(T) == 4) {
+          if (each == 2 && waves == 2) launch(Two{}, Two{});
+          else if (each == 2 && waves == 4) launch(Four{}, Two{});
+          else if (each == 2) launch(Eight{}, Two{});
+          else if (waves == 8) launch(Eight{}, Four{});
+        }
+        if (each == 4) {
+          if (waves == 1) launch(std::integral_constant<int, 1>{}, Four{});
+          else if (waves == 2) launch(Two{}, Four{});
+          else if (waves == 4) launch(Four{}, Four{});
         }
         projections_kernel<T><<<unsigned(std::min<int64_t>(hp::ceil_div(lines * width, 256), 8192)), 256, 0, ctx->stream>>>(s, o, width, out(db), out(dc));
         hp::check_launch("scan projections");
