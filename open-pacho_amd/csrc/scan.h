@@ -3,7 +3,7 @@
 //   dt = softplus(delta + bias),  r_n = exp(a_log_n)
 //   h_t,n = exp(-dt r_n) h_{t-1},n + dt x_t b_t,n,  y_t = (sum_n c_t,n h_t,n + skip x_t) silu(gate_t)
 //
-// A lane owns a channel, a wave S (2 or 4) of its states, a workgroup all states of up to 64
+// A lane owns a channel, a wave S (2, or 4 of many) of its states, a workgroup all states of up to 64
 // channels that share b and c. So b and c are the same in a whole wave: a register holds
 // those of four steps in the lanes of each row of 16, and an instruction that multiplies by
 // one of them takes it from its lane on the way (a row broadcast). An exponential, two
@@ -33,15 +33,16 @@ struct Scan {
   const T *x, *delta, *a_log, *skip, *gate, *initial, *delta_bias;
   T *y, *last;
   Rows rows;
-  int64_t batch, channels, groups;
-  int64_t width;   // channels of a group
-  int64_t pieces;  // of a group's channels, 64 each
-  int64_t states;  // of a channel
-  int64_t padded;  // of a step and group in b and c: states, up to whole launches
-  int64_t first;   // state of this launch, which takes S for each wave
-  bool starts, ends;  // the first and the last launch over the states
-  int64_t parts;   // of a row's steps
-  int64_t steps;   // of a part, a multiple of the tile
+  // 32 bits: products of them are formed in 64.
+  int batch, time, channels, groups;
+  int width;    // channels of a group
+  int pieces;   // of a group's channels, 64 each
+  int states;   // of a channel
+  int padded;   // of a step and group in b and c: states, up to whole launches
+  int first;    // state of this launch, which takes S for each wave
+  int starts, ends;  // the first and the last launch over the states
+  int parts;    // of a row's steps
+  int steps;    // of a part, a multiple of the tile
   // (parts, batch, channels): sums of dt; (parts, batch, states of a launch, channels): states that parts end in.
   T *spans, *ended;
   // Backward, (tiles, batch, states of a launch, channels): states before each tile, from the
@@ -74,40 +75,48 @@ __device__ __forceinline__ T passed_decay(T span, T rate) {
 template <typename T, int NW, int S>
 struct Place {
   int lane, wave;
-  int64_t row, group, piece, part, channel, first, end, length;  // steps [first, end) of a row of `length`
-  int64_t state;     // the wave's first, within the channel
-  int64_t slot;      // the wave's first, within the launch
+  int row, group, piece, part;
+  int first, end, length;  // steps [first, end) of a row of `length`
+  int slot, state;         // the wave's first state, within the launch and the channel
+  unsigned channel;
   bool valid;
 
   __device__ __forceinline__ explicit Place(const Scan<T>& c) {
     lane = threadIdx.x & 63;
     wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int64_t block = by_die();
+    int block = int(by_die());
     part = block % c.parts, block /= c.parts;
     piece = block % c.pieces, block /= c.pieces;
     group = block % c.groups;
     row = block / c.groups;
-    const int64_t within = piece * 64 + lane;
+    const int within = piece * 64 + lane;
     valid = within < c.width;
-    channel = group * c.width + (valid ? within : c.width - 1);  // lanes behind it load what the last one does
-    length = c.rows.end(row);
+    channel = unsigned(group * c.width + (valid ? within : c.width - 1));  // lanes behind it load what the last one does
+    length = int(c.rows.end(row));
     first = part * c.steps;
-    end = first + c.steps < length ? first + c.steps : length;
+    end = length - first < c.steps ? length : first + c.steps;
     slot = wave * S;
     state = c.first + slot;
   }
-  __device__ __forceinline__ int64_t at(const Scan<T>& c, int64_t t) const { return (row * c.rows.time + t) * c.channels + channel; }
-  // Of x's shape, at a step < end: a scalar address and the lane's offset.
-  __device__ __forceinline__ T get(const Scan<T>& c, const T* array, int64_t t) const {
-    return (array + (row * c.rows.time + t) * c.channels)[unsigned(channel)];
+  // Of x's shape: a scalar address of step t and this lane's places in steps after it.
+  template <typename P>
+  __device__ __forceinline__ P* line(const Scan<T>& c, P* array, int t) const {
+    return array + (int64_t(row) * c.time + t) * c.channels;
   }
-  // Of (..., batch, states of a launch, channels).
-  __device__ __forceinline__ int64_t state_at(const Scan<T>& c, int64_t lead, int s) const {
-    return ((lead * c.batch + row) * (NW * S) + slot + s) * c.channels + channel;
+  __device__ __forceinline__ unsigned place(const Scan<T>& c, int i) const { return unsigned(i * c.channels) + channel; }
+  // Of (..., batch, states of a launch, channels): a scalar address of the wave's state s.
+  template <typename P>
+  __device__ __forceinline__ P* state_line(const Scan<T>& c, P* array, int lead, int s) const {
+    return array + ((int64_t(lead) * c.batch + row) * (NW * S) + slot + s) * c.channels;
+  }
+  // Of (..., batch, channels).
+  template <typename P>
+  __device__ __forceinline__ P* row_line(const Scan<T>& c, P* array, int lead) const {
+    return array + (int64_t(lead) * c.batch + row) * c.channels;
   }
   // Values of the wave's states in an array (batch, channels, states), zero for those that pad.
-  __device__ __forceinline__ void read(const Scan<T>& c, const T* array, int64_t lead, T (&to)[S]) const {
-    const T* from = array + (lead * c.channels + channel) * c.states + state;
+  __device__ __forceinline__ void read(const Scan<T>& c, const T* array, int lead, T (&to)[S]) const {
+    const T* from = array + (int64_t(lead) * c.channels + channel) * c.states + state;
     if (state + S <= c.states) {
       const auto v = *reinterpret_cast<const typename Several<T, S>::type*>(from);
 #pragma unroll
@@ -117,9 +126,9 @@ struct Place {
       for (int s = 0; s < S; ++s) to[s] = state + s < c.states ? from[s] : T(0);
     }
   }
-  __device__ __forceinline__ void write(const Scan<T>& c, T* array, int64_t lead, const T (&from)[S]) const {
+  __device__ __forceinline__ void write(const Scan<T>& c, T* array, int lead, const T (&from)[S]) const {
     if (!valid) return;
-    T* to = array + (lead * c.channels + channel) * c.states + state;
+    T* to = array + (int64_t(lead) * c.channels + channel) * c.states + state;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       if (state + s < c.states) to[s] = from[s];
@@ -130,11 +139,11 @@ struct Place {
 #pragma unroll
     for (int s = 0; s < S; ++s) h[s] = T(0);
     if (c.initial) read(c, c.initial, row, h);
-    for (int64_t p = 0; p < part; ++p) {
-      const T span = c.spans[(p * c.batch + row) * c.channels + channel];
+    for (int p = 0; p < part; ++p) {
+      const T span = row_line(c, c.spans, p)[channel];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const T end = c.ended[state_at(c, p, s)];
+        const T end = state_line(c, c.ended, p, s)[channel];
         h[s] = span < T(0) ? end : __builtin_elementwise_fma(passed_decay(span, rate[s]), h[s], end);
       }
     }
@@ -171,15 +180,15 @@ struct Projections {
   static constexpr int kSteps = 16 / S;
   T v[L / kSteps];
 
-  // Those of steps behind the end are what the last one's are, until keep() clears them.
+  // Of the tile at t < end; those of steps behind the end are what the last one's are, until keep() clears them.
   template <int NW>
-  __device__ __forceinline__ void load(const Scan<T>& c, const Place<T, NW, S>& at, const T* array, int64_t t) {
-    const T* from = array + ((at.row * c.rows.time + t) * c.groups + at.group) * c.padded + at.state;
-    const unsigned stride = unsigned(c.groups * c.padded), left = at.end - t < L ? unsigned(at.end - t) : unsigned(L);
+  __device__ __forceinline__ void load(const Scan<T>& c, const Place<T, NW, S>& at, const T* array, int t) {
+    const T* from = array + ((int64_t(at.row) * c.time + t) * c.groups + at.group) * c.padded + at.state;
+    const unsigned stride = unsigned(c.groups * c.padded), last = unsigned(at.end - 1 - t);
 #pragma unroll
     for (int q = 0; q < L / kSteps; ++q) {
       const unsigned i = q * kSteps + (at.lane & 15) / S;
-      v[q] = from[(i < left ? i : left - 1) * stride + at.lane % S];
+      v[q] = from[(i < last ? i : last) * stride + at.lane % S];
     }
   }
   __device__ __forceinline__ void keep(int lane, int count) {
@@ -208,9 +217,9 @@ __device__ __forceinline__ T cut_span() {
 
 namespace hp {
 
-// Waves of a launch with `each` states a wave: 1, 2, 4, ... up to `most`.
+// Waves of a launch with `each` states a wave: 2, 4, ... up to `most`.
 inline int scan_waves(int64_t states, int each, int most) {
-  int waves = 1;
+  int waves = 2;
   while (waves < most && int64_t(waves) * each < states) waves *= 2;
   return waves;
 }
@@ -222,23 +231,24 @@ const T* scan_padded(hp_ctx* ctx, Scratch& scratch, const T* array, int64_t step
 template <typename T>
 void scan_fill(hp_ctx* ctx, T* to, const T* from, int64_t n);
 
-// States of a wave: two where four would leave SIMDs with one wave, whose waits nothing covers.
-template <typename T>
-int scan_states(const hpd::Scan<T>& c) {
-  const int64_t waves = c.batch * c.groups * c.pieces * c.parts * ceil_div(c.states, 4);
-  return c.states > 2 && c.states <= 16 && waves < 2048 ? 2 : 4;
-}
-
 // Parts of rows: one, or as many as make enough workgroups.
 template <typename T>
-void scan_plan(hpd::Scan<T>& c, int64_t tile) {
-  const int64_t blocks = c.batch * c.groups * c.pieces, tiles = ceil_div(c.rows.time, tile);
-  c.parts = 1;
-  if (blocks <= 128) c.parts = std::min<int64_t>(std::min<int64_t>(ceil_div(512, blocks), 64), std::max<int64_t>(1, tiles / 4));
-  c.steps = ceil_div(tiles, c.parts) * tile;
-  c.parts = ceil_div(c.rows.time, c.steps);
+void scan_plan(hpd::Scan<T>& c, int tile) {
+  const int64_t blocks = int64_t(c.batch) * c.groups * c.pieces, tiles = ceil_div(c.time, tile);
+  int64_t parts = 1;
+  if (blocks <= 128) parts = std::min<int64_t>(std::min<int64_t>(ceil_div(512, blocks), 64), std::max<int64_t>(1, tiles / 4));
+  c.steps = int(ceil_div(tiles, parts)) * tile;
+  c.parts = int(ceil_div(c.time, c.steps));
   require(blocks * c.parts <= kMaxThreads / 1024, "too many channels for one launch");
-  require(c.channels <= INT32_MAX / 8 && c.groups * c.padded <= INT32_MAX / 128, "too many channels or groups");
+}
+
+// Sizes that fit what the kernels form in 32 bits.
+template <typename T>
+void scan_sizes(hpd::Scan<T>& c, int64_t batch, int64_t time, int64_t channels, int64_t groups, int64_t states, int width) {
+  const int64_t padded = ceil_div(states, width) * width;
+  require(batch <= INT32_MAX && time <= INT32_MAX - 128 && channels <= INT32_MAX / 32 && groups * padded <= INT32_MAX / 32, "extents out of range");
+  c.batch = int(batch), c.time = int(time), c.channels = int(channels), c.groups = int(groups), c.states = int(states);
+  c.width = c.channels / c.groups, c.pieces = int(ceil_div(c.width, 64)), c.padded = int(padded);
 }
 
 }  // namespace hp

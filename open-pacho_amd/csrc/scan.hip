@@ -6,13 +6,18 @@ using namespace hpd;
 
 namespace {
 
-constexpr int kSteps = 16;  // of a tile
+// Steps of a tile, tiles that are loaded ahead (an even number), and states and waves of a
+// launch, for the registers that they take.
+template <typename T>
+constexpr int kTile = sizeof(T) == 4 ? 16 : 8;
+template <typename T, int NW>
+constexpr int kTiles = sizeof(T) == 4 && NW > 2 && NW < 16 ? 4 : 2;
 
 // SUMMARY: a part's sum of dt and the states that it ends in from zero ones, in place of y.
 template <typename T, int NW, int S, bool RESETS, bool SUMMARY>
 __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_, const T* c_) {
-  constexpr int kOwn = kSteps / NW;  // steps of a tile that a wave prepares and finishes
-  __shared__ T shared_dt[kSteps][64], shared_u[kSteps][64];
+  constexpr int kSteps = kTile<T>, kAhead = kTiles<T, NW>, kOwn = kSteps / NW;  // steps of a tile that a wave prepares and finishes
+  __shared__ T shared_dt[2][kSteps][64], shared_u[2][kSteps][64];
   __shared__ T sums[SUMMARY ? 1 : NW][SUMMARY ? 1 : kSteps][64];
   const Place<T, NW, S> at(c);
   if (SUMMARY && at.part == c.parts - 1) return;
@@ -28,93 +33,130 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
     at.arrive(c, rate, h);
   }
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0), skip = c.skip ? c.skip[at.channel] : T(0);
-  T x[kOwn], delta[kOwn], gate[kOwn], span = T(0);
-  Projections<T, kSteps, S> next_b, next_c;
+  T span = T(0);
   bool cut = false;
-  const auto load = [&](int64_t t) {
+  const T* const gates_or_x = c.gate ? c.gate : c.x;
+  // Loads of the tiles ahead: a tile is too short to cover the memory's latency. They are
+  // issued without a branch, behind the end too, where they repeat the last step's: a wait
+  // for the oldest counts the loads issued since, as many as there are on every way.
+  struct Ahead {
+    T x[kOwn], delta[kOwn], gate[kOwn];
+    Projections<T, kSteps, S> b, c;
+    unsigned resets;
+  } ahead[kAhead];
+  const auto load = [&](Ahead& to, int t) __attribute__((always_inline)) {
+    t = t < at.end ? t : at.end - 1;
+    const T *x = at.line(c, c.x, t), *delta = at.line(c, c.delta, t), *gate = at.line(c, gates_or_x, t);
+    const int last = at.end - 1 - t;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int64_t step = t + own + i < at.end ? t + own + i : at.end - 1;
-      x[i] = at.get(c, c.x, step);
-      delta[i] = at.get(c, c.delta, step);
-      if (!SUMMARY && c.gate) gate[i] = at.get(c, c.gate, step);
+      const unsigned from = at.place(c, own + i < last ? own + i : last);
+      to.x[i] = x[from];
+      to.delta[i] = delta[from];
+      if (!SUMMARY) to.gate[i] = gate[from];
     }
-    next_b.load(c, at, b_, t);
-    if (!SUMMARY) next_c.load(c, at, c_, t);
+    to.b.load(c, at, b_, t);
+    if (!SUMMARY) to.c.load(c, at, c_, t);
+    if (RESETS) to.resets = c.rows.byte(at.row, t, at.end, lane);
   };
-  if (at.first < at.end) load(at.first);
-  for (int64_t t = at.first; t < at.end; t += kSteps) {
-    const int count = at.end - t < kSteps ? int(at.end - t) : kSteps;
-    T now_x[kOwn], now_gate[kOwn];
+  // Leaves dt and dt x of the wave's own steps of a tile.
+  const auto prepare = [&](const Ahead& from, int t, int turn) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const bool inside = own + i < count;
+      const bool inside = t + own + i < at.end;
       T slope;
-      const T dt = softplus(delta[i] + bias, slope);
-      shared_dt[own + i][lane] = inside ? dt : T(0);
-      shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
-      now_x[i] = x[i];
-      if (!SUMMARY) now_gate[i] = gate[i];
+      const T dt = softplus(from.delta[i] + bias, slope);
+      shared_dt[turn][own + i][lane] = inside ? dt : T(0);
+      shared_u[turn][own + i][lane] = inside ? dt * from.x[i] : T(0);
     }
-    Projections<T, kSteps, S> bs = next_b, cs = next_c;
+  };
+  if (at.first < at.end) {
+    for_each<kAhead>([&](auto k) __attribute__((always_inline)) { load(ahead[k], at.first + k * kSteps); });
+    prepare(ahead[0], at.first, 0);
+  }
+  __syncthreads();
+  // Tile t, whose loads stand in `now` and those of the next one in `next`.
+  const auto tile = [&](Ahead& now, const Ahead& next, int t, int turn) __attribute__((always_inline)) {
+    const int count = at.end - t < kSteps ? (at.end > t ? at.end - t : 0) : kSteps;
+    T x[kOwn], gate[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) x[i] = now.x[i], gate[i] = now.gate[i];
+    Projections<T, kSteps, S> bs = now.b, cs = now.c;
     bs.keep(lane, count);
     if (!SUMMARY) cs.keep(lane, count);
-    __syncthreads();
-    if (t + kSteps < at.end) load(t + kSteps);
-    const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<kSteps>(at.row, t, at.end)) : 0;
+    const unsigned starts = RESETS ? unsigned(__ballot(now.resets != 0 && lane < count)) : 0;
+    load(now, t + kAhead * kSteps);
+    prepare(next, t + kSteps, turn ^ 1);  // of no use behind the last tile
+    // All of the tile's at once: the compiler would wait for those of each step in turn.
+    T dts[kSteps], us[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) dts[i] = shared_dt[turn][i][lane], us[i] = shared_u[turn][i][lane];
+    __builtin_amdgcn_sched_barrier(0);
     // Tiles without a reset, nearly all of them, do without its selects.
-    const auto walk = [&](auto resets) {
+    const auto walk = [&](auto resets) __attribute__((always_inline)) {
       for_each<kSteps>([&](auto step) {
         constexpr int i = step;
-        const T dt = shared_dt[i][lane], u = shared_u[i][lane];
+        const T dt = dts[i], u = us[i];
         T y = T(0);
         for_each<S>([&](auto state) {
           constexpr int s = state;
           if (resets) h[s] = starts >> i & 1 ? T(0) : h[s];
           h[s] = __builtin_elementwise_fma(decay(dt, rate[s]), h[s], u * bs.template get<i, s>());
-          if constexpr (!SUMMARY) y = __builtin_elementwise_fma(cs.template get<i, s>(), h[s], y);
+          // A product takes the broadcast on the way, a fused one would not.
+          if constexpr (!SUMMARY) {
+            const T part = cs.template get<i, s>() * h[s];
+            y = s ? y + part : part;
+          }
         });
         if constexpr (SUMMARY) span += dt;
         else sums[at.wave][i][lane] = y;
       });
     };
-    if (RESETS && starts) walk(std::true_type{}), cut = true;
-    else walk(std::false_type{});
+    cut = cut || starts;
+    if constexpr (RESETS && NW == 16) walk(std::true_type{});  // two of them would take too many registers
+    else if (RESETS && starts) walk(std::true_type{});
+    else if (count) walk(std::false_type{});  // (the branch also keeps the tiles' registers apart)
     __syncthreads();
     if constexpr (!SUMMARY) {
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
-        if (t + own + i >= at.end) break;
+        if (own + i >= count) break;
         T y = sums[0][own + i][lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w) y += sums[w][own + i][lane];
-        T* to = c.y + at.at(c, t + own + i);
+        T* to = at.line(c, c.y, t) + at.place(c, own + i);
         if (!c.starts) y += *to;
         if (c.ends) {
-          if (c.skip) y = __builtin_elementwise_fma(skip, now_x[i], y);
+          if (c.skip) y = __builtin_elementwise_fma(skip, x[i], y);
           if (c.gate) {
             T keep, rest;
-            gates(now_gate[i], keep, rest);
-            y *= now_gate[i] * keep;
+            gates(gate[i], keep, rest);
+            y *= gate[i] * keep;
           }
         }
         if (at.valid) *to = y;
       }
+      __syncthreads();
     }
+  };
+  for (int t = at.first; t < at.end; t += kAhead * kSteps) {
+    for_each<kAhead>([&](auto k) __attribute__((always_inline)) {
+      tile(ahead[k], ahead[(k + 1) % kAhead], t + k * kSteps, k & 1);  // behind the end it changes nothing
+    });
   }
   if constexpr (SUMMARY) {
     if (!at.valid) return;
-    if (at.wave == 0) c.spans[(at.part * c.batch + at.row) * c.channels + at.channel] = cut ? cut_span<T>() : span;
+    if (at.wave == 0) at.row_line(c, c.spans, at.part)[at.channel] = cut ? cut_span<T>() : span;
 #pragma unroll
-    for (int s = 0; s < S; ++s) c.ended[at.state_at(c, at.part, s)] = h[s];
+    for (int s = 0; s < S; ++s) at.state_line(c, c.ended, at.part, s)[at.channel] = h[s];
   } else {
     // Behind the row's end, by every wave for its own steps.
-    const int64_t stop = at.first + c.steps < c.rows.time ? at.first + c.steps : c.rows.time;
-    for (int64_t t = (at.end > at.first ? at.end : at.first) + at.wave; t < stop; t += NW) {
-      if (at.valid) c.y[at.at(c, t)] = T(0);
+    const int stop = c.time - at.first < c.steps ? c.time : at.first + c.steps;
+    for (int t = (at.end > at.first ? at.end : at.first) + at.wave; t < stop; t += NW) {
+      if (at.valid) at.line(c, c.y, t)[at.channel] = T(0);
     }
     // The part that has the row's last step, or of a row without steps the first.
-    const bool last = at.length > at.first ? at.length <= at.first + c.steps : at.length == 0 && at.part == 0;
+    const bool last = at.length > at.first ? at.length - at.first <= c.steps : at.length == 0 && at.part == 0;
     if (last) at.write(c, c.last, at.row, h);
   }
 }
@@ -132,26 +174,16 @@ __global__ __launch_bounds__(256) void fill_kernel(T* to, const T* from, int64_t
   for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) to[i] = from ? from[i] : T(0);
 }
 
-template <typename T, bool SUMMARY>
-void launch(hp_ctx* ctx, const Scan<T>& c, const T* b, const T* cs, int each, int waves) {
-  const unsigned blocks = unsigned(c.batch * c.groups * c.pieces * c.parts);
-  const auto run = [&](auto nw) {
-    const auto with = [&](auto states) {
-      const auto kernel = c.rows.resets ? forward_kernel<T, nw, states, true, SUMMARY> : forward_kernel<T, nw, states, false, SUMMARY>;
-      kernel<<<blocks, nw * 64, 0, ctx->stream>>>(c, b, cs);
-    };
-    if constexpr (nw >= 2 && nw <= 8) {
-      if (each == 2) return with(std::integral_constant<int, 2>{});
-    }
-    with(std::integral_constant<int, 4>{});
-  };
-  switch (waves) {
-    case 1: run(std::integral_constant<int, 1>{}); break;
-    case 2: run(std::integral_constant<int, 2>{}); break;
-    case 4: run(std::integral_constant<int, 4>{}); break;
-    case 8: run(std::integral_constant<int, 8>{}); break;
-    default: run(std::integral_constant<int, 16>{}); break;
+template <typename T, int NW, int S>
+void launch(hp_ctx* ctx, const Scan<T>& c, const T* b, const T* cs) {
+  const unsigned blocks = unsigned(c.batch) * unsigned(c.groups) * unsigned(c.pieces) * unsigned(c.parts);
+  if (c.parts > 1) {
+    const auto kernel = c.rows.resets ? forward_kernel<T, NW, S, true, true> : forward_kernel<T, NW, S, false, true>;
+    kernel<<<blocks, NW * 64, 0, ctx->stream>>>(c, b, cs);
+    hp::check_launch("scan summary");
   }
+  const auto kernel = c.rows.resets ? forward_kernel<T, NW, S, true, false> : forward_kernel<T, NW, S, false, false>;
+  kernel<<<blocks, NW * 64, 0, ctx->stream>>>(c, b, cs);
   hp::check_launch("scan");
 }
 
@@ -209,11 +241,11 @@ int hp_selective_scan(hp_ctx* ctx, int dtype, int index_dtype, const void* x, co
       s.x = in(x), s.delta = in(delta), s.a_log = in(a_log), s.skip = in(skip), s.gate = in(gate), s.initial = in(initial), s.delta_bias = in(delta_bias);
       s.y = static_cast<T*>(y), s.last = static_cast<T*>(last);
       s.rows = {static_cast<const uint8_t*>(resets), lengths, index_dtype == HP_I64, time};
-      s.batch = batch, s.channels = channels, s.groups = groups, s.states = states;
-      s.width = channels / groups, s.pieces = hp::ceil_div(s.width, 64);
-      hp::scan_plan(s, kSteps);
-      const int each = hp::scan_states(s), waves = hp::scan_waves(states, each, 16), width = waves * each;
-      s.padded = hp::ceil_div(states, width) * width;
+      // Two states a wave, which leaves several waves a SIMD to cover each other's waits; four of many states.
+      const bool many = sizeof(T) == 4 && states > 16;
+      const int each = many ? 4 : 2, waves = hp::scan_waves(states, each, many ? 16 : 8), width = waves * each;
+      hp::scan_sizes(s, batch, time, channels, groups, states, width);
+      hp::scan_plan(s, kTile<T>);
       const T *bs = hp::scan_padded(ctx, scratch, in(b), batch * time * groups, states, s.padded);
       const T *cs = hp::scan_padded(ctx, scratch, in(c), batch * time * groups, states, s.padded);
       if (s.parts > 1) {
@@ -223,8 +255,15 @@ int hp_selective_scan(hp_ctx* ctx, int dtype, int index_dtype, const void* x, co
       for (s.first = 0; s.first < states; s.first += width) {
         s.starts = s.first == 0;
         s.ends = s.first + width >= states;
-        if (s.parts > 1) launch<T, true>(ctx, s, bs, cs, each, waves);
-        launch<T, false>(ctx, s, bs, cs, each, waves);
+        if (!many) {
+          if (waves == 2) launch<T, 2, 2>(ctx, s, bs, cs);
+          else if (waves == 4) launch<T, 4, 2>(ctx, s, bs, cs);
+          else launch<T, 8, 2>(ctx, s, bs, cs);
+        }
+        if constexpr (sizeof(T) == 4) {
+          if (many && waves == 8) launch<T, 8, 4>(ctx, s, bs, cs);
+          else if (many) launch<T, 16, 4>(ctx, s, bs, cs);
+        }
       }
     };
     if (dtype == HP_F32) run(float(0));

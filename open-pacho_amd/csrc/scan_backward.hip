@@ -14,8 +14,8 @@
 //
 // Sums over channels (db, dc): every lane has a value for each step and state of a tile. Pairs
 // of registers are folded into one whose halves, quarters, ... belong to one of the two each,
-// until a register holds a sum in each lane: two instructions a value where a sum over 64 lanes
-// by itself takes six times two. Workgroups leave these, and their sums over steps, as parts.
+// until a register holds a sum in each lane: three instructions a value where a sum over 64
+// lanes by itself takes six times two. Workgroups leave these, and their sums over steps, as parts.
 //
 // Where rows are cut into parts, the first launch also forms what a part passes back from
 // nothing, sum_t D_t c_t g_t with D_t the product of the decays up to t.
@@ -25,17 +25,24 @@ using namespace hpd;
 
 namespace {
 
-// Steps of a tile, and waves of a launch, for the registers that a tile's states and decays take.
-template <typename T, int NW, int S>
-constexpr int kTile = sizeof(T) == 4 ? (S == 4 && NW == 8 ? 8 : 16) : NW == 1 ? 4 : 8;
+// Exponentials of doubles, small programs, one after the other: side by side they would take all registers.
 template <typename T>
-constexpr int kMostWaves = sizeof(T) == 4 ? 8 : 4;
+__device__ __forceinline__ void apart() {
+  if constexpr (sizeof(T) == 8) __builtin_amdgcn_sched_barrier(0);
+}
+
+// Steps of a tile, for the registers that its states and decays take.
+template <typename T, int NW, int S>
+constexpr int kTile = sizeof(T) == 8 || S == 4 || NW == 2 ? 8 : 16;
 constexpr int kLongestTile = 16;
+// Tiles that the first launch loads ahead, an even number.
+template <typename T, int NW>
+constexpr int kTiles = sizeof(T) == 4 && NW > 2 ? 4 : 2;
 
 template <typename T, int NW, int S, bool RESETS, bool SPLIT>
 __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_, const T* c_) {
-  constexpr int L = kTile<T, NW, S>, kOwn = L / NW;
-  __shared__ T shared_dt[L][64], shared_u[L][64], shared_g[SPLIT ? L : 1][64];
+  constexpr int L = kTile<T, NW, S>, kOwn = L / NW, kAhead = kTiles<T, NW>;
+  __shared__ T shared_dt[2][L][64], shared_u[2][L][64], shared_g[2][SPLIT ? L : 1][64];
   const Place<T, NW, S> at(c);
   const int lane = at.lane, own = at.wave * kOwn;
   T rate[S], h[S], through[S], back[S], span = T(0);
@@ -44,65 +51,89 @@ __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_,
   for (int s = 0; s < S; ++s) rate[s] = rate_of(rate[s]), h[s] = back[s] = T(0), through[s] = T(1);
   if (!SPLIT && c.initial) at.read(c, c.initial, at.row, h);
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0);
-  T x[kOwn], delta[kOwn], grad[kOwn], gate[kOwn];
-  Projections<T, L, S> next_b, next_c;
   bool cut = false;
-  const auto load = [&](int64_t t) {
+  const T* const gates_or_x = c.gate ? c.gate : c.x;
+  // Loads of the tiles ahead: a tile is too short to cover the memory's latency. They are
+  // issued without a branch, behind the end too, where they repeat the last step's: a wait
+  // for the oldest counts the loads issued since, as many as there are on every way.
+  struct Ahead {
+    T x[kOwn], delta[kOwn], grad[kOwn], gate[kOwn];
+    Projections<T, L, S> b, c;
+    unsigned resets;
+  } ahead[kAhead];
+  const auto load = [&](Ahead& to, int t) __attribute__((always_inline)) {
+    t = t < at.end ? t : at.end - 1;
+    const T *x = at.line(c, c.x, t), *delta = at.line(c, c.delta, t);
+    const int last = at.end - 1 - t;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int64_t step = t + own + i < at.end ? t + own + i : at.end - 1;
-      x[i] = at.get(c, c.x, step);
-      delta[i] = at.get(c, c.delta, step);
+      const unsigned from = at.place(c, own + i < last ? own + i : last);
+      to.x[i] = x[from];
+      to.delta[i] = delta[from];
       if constexpr (SPLIT) {
-        grad[i] = at.get(c, c.grad, step);
-        if (c.gate) gate[i] = at.get(c, c.gate, step);
+        to.grad[i] = at.line(c, c.grad, t)[from];
+        to.gate[i] = at.line(c, gates_or_x, t)[from];
       }
     }
-    next_b.load(c, at, b_, t);
-    if (SPLIT) next_c.load(c, at, c_, t);
+    to.b.load(c, at, b_, t);
+    if (SPLIT) to.c.load(c, at, c_, t);
+    if (RESETS) to.resets = c.rows.byte(at.row, t, at.end, lane);
   };
-  if (at.first < at.end) load(at.first);
-  for (int64_t t = at.first; t < at.end; t += L) {
-    const int count = at.end - t < L ? int(at.end - t) : L;
+  // Leaves dt, dt x and g of the wave's own steps of a tile.
+  const auto prepare = [&](const Ahead& from, int t, int turn) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const bool inside = own + i < count;
+      const bool inside = t + own + i < at.end;
       T slope;
-      const T dt = softplus(delta[i] + bias, slope);
-      shared_dt[own + i][lane] = inside ? dt : T(0);
-      shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
+      const T dt = softplus(from.delta[i] + bias, slope);
+      shared_dt[turn][own + i][lane] = inside ? dt : T(0);
+      shared_u[turn][own + i][lane] = inside ? dt * from.x[i] : T(0);
       if constexpr (SPLIT) {
-        T g = grad[i];
-        if (c.gate) {
-          T keep, rest;
-          gates(gate[i], keep, rest);
-          g *= gate[i] * keep;
-        }
-        shared_g[own + i][lane] = inside ? g : T(0);
+        T g = from.grad[i], keep, rest;
+        gates(from.gate[i], keep, rest);
+        g *= c.gate ? from.gate[i] * keep : T(1);
+        shared_g[turn][own + i][lane] = inside ? g : T(0);
       }
     }
-    Projections<T, L, S> bs = next_b, cs = next_c;
+  };
+  if (at.first < at.end) {
+    for_each<kAhead>([&](auto k) __attribute__((always_inline)) { load(ahead[k], at.first + k * L); });
+    prepare(ahead[0], at.first, 0);
+  }
+  __syncthreads();
+  // Tile t, whose loads stand in `now` and those of the next one in `next`.
+  const auto tile = [&](Ahead& now, const Ahead& next, int t, int turn) __attribute__((always_inline)) {
+    const int count = at.end - t < L ? (at.end > t ? at.end - t : 0) : L;
+    Projections<T, L, S> bs = now.b, cs = now.c;
     bs.keep(lane, count);
     if (SPLIT) cs.keep(lane, count);
-    __syncthreads();
-    if (t + L < at.end) load(t + L);
-    const int64_t tile = t / L;
-    if (at.valid) {
+    const unsigned starts = RESETS ? unsigned(__ballot(now.resets != 0 && lane < count)) : 0;
+    load(now, t + kAhead * L);
+    const int number = t / L;
+    if (at.valid && count) {
 #pragma unroll
-      for (int s = 0; s < S; ++s) c.before[at.state_at(c, tile, s)] = h[s];
-      if (SPLIT && at.wave == 0) c.since[(tile * c.batch + at.row) * c.channels + at.channel] = cut ? cut_span<T>() : span;
+      for (int s = 0; s < S; ++s) at.state_line(c, c.before, number, s)[at.channel] = h[s];
+      if (SPLIT && at.wave == 0) at.row_line(c, c.since, number)[at.channel] = cut ? cut_span<T>() : span;
     }
-    const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<L>(at.row, t, at.end)) : 0;
+    prepare(next, t + L, turn ^ 1);  // of no use behind the last tile
+    // All of the tile's at once: the compiler would wait for those of each step in turn.
+    T dts[L], us[L], gs[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      dts[i] = shared_dt[turn][i][lane], us[i] = shared_u[turn][i][lane];
+      if constexpr (SPLIT) gs[i] = shared_g[turn][i][lane];
+    }
+    __builtin_amdgcn_sched_barrier(0);
     // Tiles without a reset, nearly all of them, do without its selects.
-    const auto walk = [&](auto resets) {
+    const auto walk = [&](auto resets) __attribute__((always_inline)) {
       for_each<L>([&](auto step) {
         constexpr int i = step;
         const bool start = resets && (starts >> i & 1);
-        const T dt = shared_dt[i][lane], u = shared_u[i][lane];
+        const T dt = dts[i], u = us[i];
         T g = T(0);
         if constexpr (SPLIT) {
           cut = cut || start;
-          g = RESETS && cut ? T(0) : shared_g[i][lane];
+          g = RESETS && cut ? T(0) : gs[i];
           span += dt;
         }
         for_each<S>([&](auto state) {
@@ -118,16 +149,21 @@ __global__ __launch_bounds__(NW * 64) void before_kernel(Scan<T> c, const T* b_,
       });
     };
     if (RESETS && starts) walk(std::true_type{});
-    else walk(std::false_type{});
+    else if (count) walk(std::false_type{});  // (the branch also keeps the tiles' registers apart)
     __syncthreads();
+  };
+  for (int t = at.first; t < at.end; t += kAhead * L) {
+    for_each<kAhead>([&](auto k) __attribute__((always_inline)) {
+      tile(ahead[k], ahead[(k + 1) % kAhead], t + k * L, k & 1);  // behind the end it changes nothing
+    });
   }
   if constexpr (SPLIT) {
     if (!at.valid) return;
-    if (at.wave == 0) c.spans[(at.part * c.batch + at.row) * c.channels + at.channel] = cut ? cut_span<T>() : span;
+    if (at.wave == 0) at.row_line(c, c.spans, at.part)[at.channel] = cut ? cut_span<T>() : span;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      c.ended[at.state_at(c, at.part, s)] = h[s];
-      c.passed[at.state_at(c, at.part, s)] = back[s];
+      at.state_line(c, c.ended, at.part, s)[at.channel] = h[s];
+      at.state_line(c, c.passed, at.part, s)[at.channel] = back[s];
     }
   }
 }
@@ -186,60 +222,42 @@ __device__ __forceinline__ T fold_pair(T a, T b, bool bit) {
   return (bit ? b : a) + from_across<MASK>(bit ? a : b);
 }
 
-// Of N values (4, 8 or 16) the sums over a row of 16 lanes: lane i has value number_of_lane(i).
-// Pairs meet across 8, 7, 3 and 1 lanes, which reaches all 16.
-template <typename T, int N>
-__device__ __forceinline__ T fold_row(const T (&v)[N], int lane) {
-  T a[N / 2];
+// Of values for each of S states and L steps (8 or 16) the sums over each row of 16 lanes,
+// and of the rows, whose pairs the lanes' halves share, over pairs: lane i has the sum of step
+// step_of_lane(i) and state state_of_lane(i). Within a row pairs of steps meet across 8, 7,
+// 3 and 1 lanes, which reaches all 16: an addition that takes its operand from another
+// lane costs no more than any other, where an exchange of rows takes 12 cycles or more.
+template <typename T, int S, int L>
+__device__ __forceinline__ T fold(const T (&pairs)[S][L / 2], int lane) {
+  T of_state[S];
 #pragma unroll
-  for (int k = 0; k < N / 2; ++k) a[k] = fold_pair<8>(v[2 * k], v[2 * k + 1], lane & 8);
-  T b[N / 4];
+  for (int s = 0; s < S; ++s) {
+    T a[L / 4], b[L / 8];
 #pragma unroll
-  for (int k = 0; k < N / 4; ++k) b[k] = fold_pair<7>(a[2 * k], a[2 * k + 1], lane & 4);
-  T d[N < 8 ? 1 : N / 8];
-  if constexpr (N >= 8) {
+    for (int k = 0; k < L / 4; ++k) a[k] = fold_pair<7>(pairs[s][2 * k], pairs[s][2 * k + 1], lane & 4);
 #pragma unroll
-    for (int k = 0; k < N / 8; ++k) d[k] = fold_pair<3>(b[2 * k], b[2 * k + 1], lane & 2);
-  } else {
-    d[0] = b[0] + from_across<3>(b[0]);
+    for (int k = 0; k < L / 8; ++k) b[k] = fold_pair<3>(a[2 * k], a[2 * k + 1], lane & 2);
+    if constexpr (L == 16) of_state[s] = fold_pair<1>(b[0], b[1], lane & 1);
+    else of_state[s] = b[0];
   }
-  if constexpr (N == 16) return fold_pair<1>(d[0], d[1], lane & 1);
-  else return d[0] + from_across<1>(d[0]);
-}
-template <int N>
-__device__ __forceinline__ int number_of_lane(int lane) {
-  return (lane >> 3 & 1) | (lane >> 2 & 1) << 1 | (N >= 8 ? (lane >> 1 & 1) << 2 : 0) | (N == 16 ? (lane & 1) << 3 : 0);
-}
-
-// Of S values for each of L steps the sums over all lanes: lane i has that of step
-// step_of_lane(i) and state state_of_lane(i).
-template <int S, typename T>
-__device__ __forceinline__ T fold_states(const T (&v)[S]) {
-  if constexpr (S == 4) return fold_rows<4>(fold_rows<5>(v[0], v[1]), fold_rows<5>(v[2], v[3]));
-  else return fold_rows<5>(v[0], v[1]);
-}
-template <int S, typename T, int L>
-__device__ __forceinline__ T fold_steps(const T (&v)[L], int lane) {
-  if constexpr (S == 4) return fold_row<T, L>(v, lane);
-  else {
-    T pairs[L / 2];
+  if constexpr (L == 8) {
+    if constexpr (S == 4) {
+      of_state[0] = fold_pair<1>(of_state[0], of_state[1], lane & 1);
+      of_state[1] = fold_pair<1>(of_state[2], of_state[3], lane & 1);
+    } else {
 #pragma unroll
-    for (int k = 0; k < L / 2; ++k) pairs[k] = fold_rows<4>(v[2 * k], v[2 * k + 1]);
-    return fold_row<T, L / 2>(pairs, lane);
+      for (int s = 0; s < S; ++s) of_state[s] += from_across<1>(of_state[s]);
+    }
   }
+  return fold_rows<5>(of_state[0], of_state[1]);
 }
-template <int S, int L>
+template <int L>
 __device__ __forceinline__ int step_of_lane(int lane) {
-  return S == 4 ? number_of_lane<L>(lane) : (lane >> 4 & 1) | number_of_lane<L / 2>(lane) << 1;
+  return (lane >> 3 & 1) | (lane >> 2 & 1) << 1 | (lane >> 1 & 1) << 2 | (L == 16 ? (lane & 1) << 3 : 0);
 }
 template <int S>
 __device__ __forceinline__ int state_of_lane(int lane) {
-  return (lane >> 5 & 1) | (S == 4 ? (lane >> 4 & 1) << 1 : 0);
-}
-// Of the lanes that have the same sum, the one that leaves it.
-template <int S, int L>
-__device__ __forceinline__ bool leaves(int lane) {
-  return lane % (64 / (S * L)) == 0;
+  return S == 4 ? (lane & 1) | (lane >> 5 & 1) << 1 : lane >> 5 & 1;
 }
 
 // ---- backward ------------------------------------------------------------------------
@@ -247,7 +265,7 @@ __device__ __forceinline__ bool leaves(int lane) {
 template <typename T, int NW, int S, bool RESETS>
 __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o, const T* b_, const T* c_) {
   constexpr int L = kTile<T, NW, S>, kOwn = L / NW;
-  __shared__ T shared_dt[L][64], shared_u[L][64], shared_g[L][64];
+  __shared__ T shared_dt[2][L][64], shared_u[2][L][64], shared_g[2][L][64];
   __shared__ T sums_b[NW][L][64], sums_a[NW][L][64], sums_y[NW][L][64];
   const Place<T, NW, S> at(c);
   const int lane = at.lane, own = at.wave * kOwn;
@@ -263,11 +281,11 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
   if (c.parts > 1) {
     at.arrive(c, rate, arrived);
     if (c.grad_state) at.read(c, c.grad_state, at.row, e);
-    for (int64_t p = c.parts - 1; p > at.part; --p) {
-      const T span = c.spans[(p * c.batch + at.row) * c.channels + at.channel];
+    for (int p = c.parts - 1; p > at.part; --p) {
+      const T span = at.row_line(c, c.spans, p)[at.channel];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const T back = c.passed[at.state_at(c, p, s)];
+        const T back = at.state_line(c, c.passed, p, s)[at.channel];
         e[s] = span < T(0) ? back : __builtin_elementwise_fma(passed_decay(span, rate[s]), e[s], back);
       }
     }
@@ -279,71 +297,109 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
   const T bias = c.delta_bias ? c.delta_bias[at.channel] : T(0), skip = c.skip ? c.skip[at.channel] : T(0);
   T dskip = T(0), dbias = T(0);
   // Behind the row's end, by every wave for its own steps.
-  const int64_t stop = at.first + c.steps < c.rows.time ? at.first + c.steps : c.rows.time;
-  for (int64_t t = (at.end > at.first ? at.end : at.first) + at.wave; t < stop; t += NW) {
-    const int64_t to = at.at(c, t);
+  const int stop = c.time - at.first < c.steps ? c.time : at.first + c.steps;
+  for (int t = (at.end > at.first ? at.end : at.first) + at.wave; t < stop; t += NW) {
     if (!at.valid) continue;
-    o.dx[to] = o.ddelta[to] = T(0);
-    if (c.gate) o.dgate[to] = T(0);
+    at.line(c, o.dx, t)[at.channel] = at.line(c, o.ddelta, t)[at.channel] = T(0);
+    if (c.gate) at.line(c, o.dgate, t)[at.channel] = T(0);
   }
-  const int64_t tiles = at.end > at.first ? (at.end - at.first + L - 1) / L : 0;
-  T next_x[kOwn], delta[kOwn], gate[kOwn], grad[kOwn], before[S], since = cut_span<T>();
-  Projections<T, L, S> next_b, next_c;
-  const auto load = [&](int64_t t) {
+  const int tiles = at.end > at.first ? (at.end - at.first + L - 1) / L : 0;
+  const T* const gates_or_x = c.gate ? c.gate : c.x;
+  struct Ahead {
+    T x[kOwn], delta[kOwn], gate[kOwn], grad[kOwn], before[S], since;
+    Projections<T, L, S> b, c;
+    unsigned resets;
+  } ahead;
+  const auto load = [&](int t) __attribute__((always_inline)) {
+    t = t < at.first ? at.first : t;
+    const int tile = t / L, last = at.end - 1 - t;
+    ahead.since = c.parts > 1 ? at.row_line(c, c.since, tile)[at.channel] : cut_span<T>();
+    const T *x = at.line(c, c.x, t), *delta = at.line(c, c.delta, t), *grad = at.line(c, c.grad, t), *gate = at.line(c, gates_or_x, t);
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int64_t step = t + own + i < at.end ? t + own + i : at.end - 1;
-      next_x[i] = at.get(c, c.x, step);
-      delta[i] = at.get(c, c.delta, step);
-      grad[i] = at.get(c, c.grad, step);
-      if (c.gate) gate[i] = at.get(c, c.gate, step);
+      const unsigned from = at.place(c, own + i < last ? own + i : last);
+      ahead.x[i] = x[from];
+      ahead.delta[i] = delta[from];
+      ahead.grad[i] = grad[from];
+      ahead.gate[i] = gate[from];
     }
-    next_b.load(c, at, b_, t);
-    next_c.load(c, at, c_, t);
-    const int64_t tile = t / L;
+    ahead.b.load(c, at, b_, t);
+    ahead.c.load(c, at, c_, t);
 #pragma unroll
-    for (int s = 0; s < S; ++s) before[s] = c.before[at.state_at(c, tile, s)];
-    if (c.parts > 1) since = c.since[(tile * c.batch + at.row) * c.channels + at.channel];
+    for (int s = 0; s < S; ++s) ahead.before[s] = at.state_line(c, c.before, tile, s)[at.channel];
+    if (RESETS) ahead.resets = c.rows.byte(at.row, t, at.end, lane);
   };
-  if (tiles) load(at.first + (tiles - 1) * L);
-  for (int64_t n = tiles - 1; n >= 0; --n) {
-    const int64_t t = at.first + n * L;
-    const int count = at.end - t < L ? int(at.end - t) : L;
-    T x[kOwn], slope[kOwn], passes[kOwn];  // of the wave's own steps; slopes of dt, and of y by the gate times dy
+  // What a tile needs besides shared_*: of the wave's own steps x and the slopes of dt, and of y by the gate times dy.
+  struct Ready {
+    T x[kOwn], slope[kOwn], passes[kOwn], start[S];
+    Projections<T, L, S> b, c;
+    unsigned starts;
+  };
+  const auto prepare = [&](int t, int turn) __attribute__((always_inline)) {
+    const int count = at.end - t < L ? at.end - t : L;
+    Ready r;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const bool inside = at.valid && own + i < count;
-      x[i] = next_x[i];
-      const T dt = softplus(delta[i] + bias, slope[i]);
-      T g = grad[i];
-      if (c.gate) {
-        T keep, rest;
-        gates(gate[i], keep, rest);
-        passes[i] = g * (keep * (T(1) + gate[i] * rest));
-        g *= gate[i] * keep;
-      }
-      shared_dt[own + i][lane] = inside ? dt : T(0);
-      shared_u[own + i][lane] = inside ? dt * x[i] : T(0);
-      shared_g[own + i][lane] = inside ? g : T(0);
+      r.x[i] = ahead.x[i];
+      const T dt = softplus(ahead.delta[i] + bias, r.slope[i]);
+      T keep, rest;
+      gates(ahead.gate[i], keep, rest);
+      r.passes[i] = ahead.grad[i] * (keep * (T(1) + ahead.gate[i] * rest));
+      const T g = c.gate ? ahead.grad[i] * (ahead.gate[i] * keep) : ahead.grad[i];
+      shared_dt[turn][own + i][lane] = inside ? dt : T(0);
+      shared_u[turn][own + i][lane] = inside ? dt * ahead.x[i] : T(0);
+      shared_g[turn][own + i][lane] = inside ? g : T(0);
+      apart<T>();
     }
-    T start[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      start[s] = before[s];
-      if (since >= T(0)) start[s] = __builtin_elementwise_fma(passed_decay(since, rate[s]), arrived[s], start[s]);
-      if (!at.valid) start[s] = T(0);
+      r.start[s] = ahead.before[s];
+      if (c.parts > 1) r.start[s] = ahead.since < T(0) ? r.start[s] : __builtin_elementwise_fma(passed_decay(ahead.since, rate[s]), arrived[s], r.start[s]);
+      if (!at.valid) r.start[s] = T(0);
     }
-    Projections<T, L, S> bs = next_b, cs = next_c;
-    bs.keep(lane, count);
-    cs.keep(lane, count);
-    __syncthreads();
-    if (n > 0) load(t - L);
-    const unsigned starts = RESETS ? __builtin_amdgcn_readfirstlane(c.rows.template starts<L>(at.row, t, at.end)) : 0;
-    const auto walk = [&](auto resets) {
+    r.b = ahead.b, r.c = ahead.c;
+    r.b.keep(lane, count);
+    r.c.keep(lane, count);
+    r.starts = RESETS ? unsigned(__ballot(ahead.resets != 0 && lane < count)) : 0;
+    return r;
+  };
+  Ready next{};
+  if (tiles) {
+    load(at.first + (tiles - 1) * L);
+    next = prepare(at.first + (tiles - 1) * L, 0);
+    load(at.first + (tiles - 2) * L);
+  }
+  __syncthreads();
+  int turn = 0;
+  for (int n = tiles - 1; n >= 0; --n, turn ^= 1) {
+    const int t = at.first + n * L;
+    const int count = at.end - t < L ? at.end - t : L;
+    Ready now = next;
+    auto &bs = now.b, &cs = now.c;
+    const auto& start = now.start;
+    const unsigned starts = now.starts;
+    // The tile before it, beside this one's work: its loads are there, and, half way through the walk, so are the
+    // stores of the tile behind it. (Doubles at once, while the walk does not have the registers yet.) Before the
+    // first tile there is none, and nothing reads what this leaves.
+    const auto prepare_next = [&]() __attribute__((always_inline)) {
+      next = prepare(t - L < at.first ? at.first : t - L, turn ^ 1);
+      load(t - 2 * L);
+    };
+    if constexpr (sizeof(T) == 8) prepare_next();
+    // Read for some steps at a time, and again on the way back: all of them would take registers from the states.
+    constexpr int kSome = sizeof(T) == 4 ? 8 : 2;
+    T dts[L], us[L], gs[L];
+    const auto walk = [&](auto resets) __attribute__((always_inline)) {
       T h[L][S], keep[L][S];
       for_each<L>([&](auto step) {
         constexpr int i = step;
-        const T dt = shared_dt[i][lane], u = shared_u[i][lane];
+        if constexpr (i % kSome == 0) {
+#pragma unroll
+          for (int k = i; k < i + kSome; ++k) dts[k] = shared_dt[turn][k][lane], us[k] = shared_u[turn][k][lane];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const T dt = dts[i], u = us[i];
         const bool cut = resets && (starts >> i & 1);
         for_each<S>([&](auto state) {
           constexpr int s = state;
@@ -352,12 +408,19 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
           if constexpr (i > 0) before = h[i - 1][s];
           h[i][s] = __builtin_elementwise_fma(keep[i][s], cut ? T(0) : before, u * bs.template get<i, s>());
         });
+        apart<T>();
       });
+      if constexpr (sizeof(T) == 4) prepare_next();
       bs.renew();
-      T rows_b[L], rows_c[L];
+      T pairs_b[S][L / 2], pairs_c[S][L / 2], last_b[S], last_c[S];
       for_each<L>([&](auto step) {
         constexpr int i = L - 1 - step;
-        const T dt = shared_dt[i][lane], u = shared_u[i][lane], g = shared_g[i][lane];
+        if constexpr (step % kSome == 0) {
+#pragma unroll
+          for (int k = i; k > i - kSome; --k) dts[k] = shared_dt[turn][k][lane], us[k] = shared_u[turn][k][lane], gs[k] = shared_g[turn][k][lane];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const T dt = dts[i], u = us[i], g = gs[i];
         const bool cut = resets && (starts >> i & 1);
         T along = T(0), decays = T(0), y = T(0), to_b[S], to_c[S];
         for_each<S>([&](auto state) {
@@ -365,7 +428,8 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
           const T m = __builtin_elementwise_fma(cs.template get<i, s>(), g, e[s]);
           to_c[s] = g * h[i][s];
           to_b[s] = u * m;
-          along = __builtin_elementwise_fma(bs.template get<i, s>(), m, along);
+          const T part = bs.template get<i, s>() * m;  // takes the broadcast on the way
+          along = s ? along + part : part;
           y = __builtin_elementwise_fma(cs.template get<i, s>(), h[i][s], y);
           e[s] = cut ? T(0) : keep[i][s] * m;
           T before = start[s];
@@ -377,20 +441,25 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
         sums_b[at.wave][i][lane] = along;
         sums_a[at.wave][i][lane] = decays;
         if (c.gate) sums_y[at.wave][i][lane] = y;
-        rows_b[i] = fold_states<S>(to_b);
-        rows_c[i] = fold_states<S>(to_c);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          if constexpr (i % 2) {
+            last_b[s] = to_b[s], last_c[s] = to_c[s];
+          } else {
+            pairs_b[s][i / 2] = fold_pair<8>(to_b[s], last_b[s], lane & 8);
+            pairs_c[s][i / 2] = fold_pair<8>(to_c[s], last_c[s], lane & 8);
+          }
+        }
       });
-      const T all_b = fold_steps<S>(rows_b, lane), all_c = fold_steps<S>(rows_c, lane);
-      const int i = step_of_lane<S, L>(lane), s = state_of_lane<S>(lane);
-      if (i < count && leaves<S, L>(lane)) {
-        const int64_t line = (at.row * c.rows.time + t + i) * c.groups + at.group, lines = c.batch * c.rows.time * c.groups;
-        const int64_t to = (at.piece * lines + line) * (NW * S) + at.slot + s;
-        o.db[to] = all_b;
-        o.dc[to] = all_c;
+      // Rows of lanes with bit 4 get the sums of dc.
+      const T all = fold_rows<4>(fold<T, S, L>(pairs_b, lane), fold<T, S, L>(pairs_c, lane));
+      const int i = step_of_lane<L>(lane), s = state_of_lane<S>(lane);
+      if (i < count && (S * L == 32 || !(lane & 1))) {
+        const int64_t step = (int64_t(at.piece) * c.batch + at.row) * c.time + t, to = (step * c.groups + at.group) * (NW * S) + at.slot;
+        ((lane & 16 ? o.dc : o.db) + to)[unsigned(i * c.groups) * (NW * S) + s] = all;
       }
     };
-    if (RESETS && starts) walk(std::true_type{});
-    else walk(std::false_type{});
+    walk(std::integral_constant<bool, RESETS>{});
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
@@ -402,37 +471,39 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
         decays += sums_a[w][own + i][lane];
         if (c.gate) y += sums_y[w][own + i][lane];
       }
-      const int64_t to = at.at(c, t + own + i);
-      const T dt = shared_dt[own + i][lane], g = shared_g[own + i][lane];
-      T dx = along * dt, ddt = __builtin_elementwise_fma(along, x[i], decays);
-      if (!c.starts) dx += o.dx[to], ddt += o.ddelta[to];
+      const unsigned to = at.place(c, own + i);
+      T *to_x = at.line(c, o.dx, t) + to, *to_delta = at.line(c, o.ddelta, t) + to;
+      const T dt = shared_dt[turn][own + i][lane], g = shared_g[turn][own + i][lane];
+      T dx = along * dt, ddt = __builtin_elementwise_fma(along, now.x[i], decays);
+      if (!c.starts) dx += *to_x, ddt += *to_delta;
       else if (c.skip) dx = __builtin_elementwise_fma(skip, g, dx);
       if (c.ends) {
-        ddt *= slope[i];
+        ddt *= now.slope[i];
         dbias += ddt;
-        if (c.skip) dskip = __builtin_elementwise_fma(g, x[i], dskip);
+        if (c.skip) dskip = __builtin_elementwise_fma(g, now.x[i], dskip);
       }
-      o.dx[to] = dx;
-      o.ddelta[to] = ddt;
+      *to_x = dx;
+      *to_delta = ddt;
       if (c.gate) {
-        if (!c.starts) y += o.dgate[to];
+        T* to_gate = at.line(c, o.dgate, t) + to;
+        if (!c.starts) y += *to_gate;
         if (c.ends) {
-          if (c.skip) y = __builtin_elementwise_fma(skip, x[i], y);
-          y *= passes[i];
+          if (c.skip) y = __builtin_elementwise_fma(skip, now.x[i], y);
+          y *= now.passes[i];
         }
-        o.dgate[to] = y;
+        *to_gate = y;
       }
     }
+    __syncthreads();
   }
-  const int64_t line = at.row * c.parts + at.part;
+  const int64_t line = int64_t(at.row) * c.parts + at.part;
   if (at.valid) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) o.da[(line * (NW * S) + at.slot + s) * c.channels + at.channel] = da[s] * slow[s];
+    for (int s = 0; s < S; ++s) (o.da + (line * (NW * S) + at.slot + s) * c.channels)[at.channel] = da[s] * slow[s];
     if (o.dinitial && at.part == 0) at.write(c, o.dinitial, at.row, e);
   }
   if (!c.ends) return;
   // The waves' sums over their own steps.
-  __syncthreads();
   sums_a[at.wave][0][lane] = dskip;
   sums_b[at.wave][0][lane] = dbias;
   __syncthreads();
@@ -446,14 +517,14 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
 // db and dc (batch, time, groups, states) from the pieces' parts; zero behind the rows' ends.
 template <typename T>
 __global__ __launch_bounds__(256) void projections_kernel(Scan<T> c, Grads<T> o, int width, T* db, T* dc) {
-  const int64_t lines = c.batch * c.rows.time * c.groups, n = lines * width;
+  const int64_t lines = int64_t(c.batch) * c.time * c.groups, n = lines * width;
   for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
     const int64_t line = i / width, s = i - line * width + c.first;
     if (s >= c.states) continue;
-    const int64_t step = line / c.groups, row = step / c.rows.time;
+    const int64_t step = line / c.groups, row = step / c.time;
     T b = T(0), d = T(0);
-    if (step - row * c.rows.time < c.rows.end(row)) {
-      for (int64_t p = 0; p < c.pieces; ++p) b += o.db[p * n + i], d += o.dc[p * n + i];
+    if (step - row * c.time < c.rows.end(row)) {
+      for (int p = 0; p < c.pieces; ++p) b += o.db[p * n + i], d += o.dc[p * n + i];
     }
     db[line * c.states + s] = b;
     dc[line * c.states + s] = d;
@@ -462,8 +533,8 @@ __global__ __launch_bounds__(256) void projections_kernel(Scan<T> c, Grads<T> o,
 
 template <typename T>
 __global__ __launch_bounds__(1024) void decays_kernel(Scan<T> c, const T* parts, int width, T* da) {
-  const int64_t columns = width * c.channels;
-  add_parts(parts, columns, 0, c.batch * c.parts, int64_t(blockIdx.x) * 64, columns, [&](int64_t q, T sum) {
+  const int64_t columns = int64_t(width) * c.channels;
+  add_parts(parts, columns, 0, int64_t(c.batch) * c.parts, int64_t(blockIdx.x) * 64, columns, [&](int64_t q, T sum) {
     const int64_t s = q / c.channels, channel = q - s * c.channels;
     if (c.first + s < c.states) da[channel * c.states + c.first + s] = sum;
   });
@@ -473,7 +544,7 @@ template <typename T>
 __global__ __launch_bounds__(1024) void channels_kernel(Scan<T> c, const T* skips, T* dskip, const T* biases, T* dbias) {
   T* to = blockIdx.y ? dbias : dskip;
   if (!to) return;
-  add_parts(blockIdx.y ? biases : skips, c.channels, 0, c.batch * c.parts, int64_t(blockIdx.x) * 64, c.channels, [&](int64_t q, T sum) { to[q] = sum; });
+  add_parts(blockIdx.y ? biases : skips, c.channels, 0, int64_t(c.batch) * c.parts, int64_t(blockIdx.x) * 64, c.channels, [&](int64_t q, T sum) { to[q] = sum; });
 }
 
 }  // namespace
@@ -508,12 +579,12 @@ int hp_selective_scan_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* 
       s.x = in(x), s.delta = in(delta), s.a_log = in(a_log), s.skip = in(skip), s.gate = in(gate), s.initial = in(initial), s.delta_bias = in(delta_bias);
       s.grad = in(grad), s.grad_state = in(grad_state);
       s.rows = {static_cast<const uint8_t*>(resets), lengths, index_dtype == HP_I64, time};
-      s.batch = batch, s.channels = channels, s.groups = groups, s.states = states;
-      s.width = channels / groups, s.pieces = hp::ceil_div(s.width, 64);
-            hp::scan_plan(s, kLongestTile);
-      // Doubles of two states in eight waves would not fit into their registers.
-      const int each = sizeof(T) == 4 ? hp::scan_states(s) : 4, waves = hp::scan_waves(states, each, kMostWaves<T>), width = waves * each;
-      s.padded = hp::ceil_div(states, width) * width;
+      // As forward; four states a wave would not leave as many waves their registers for more than 32. Doubles
+      // take twice the registers: four waves of two states leave each what it needs, for few states too.
+      const bool many = sizeof(T) == 4 && states > 16;
+      const int each = many ? 4 : 2, waves = sizeof(T) == 4 ? hp::scan_waves(states, each, 8) : 4, width = waves * each;
+      hp::scan_sizes(s, batch, time, channels, groups, states, width);
+      hp::scan_plan(s, kLongestTile);
       const T *bs = hp::scan_padded(ctx, scratch, in(b), batch * time * groups, states, s.padded);
       const T *cs = hp::scan_padded(ctx, scratch, in(c), batch * time * groups, states, s.padded);
       const int64_t lines = batch * time * groups, rows = batch * s.parts;
@@ -528,7 +599,7 @@ int hp_selective_scan_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* 
       o.da = scratch.take<T>(rows * width * channels);
       o.dskip = scratch.take<T>(rows * channels), o.dbias = scratch.take<T>(rows * channels);
       const unsigned blocks = unsigned(batch * groups * s.pieces * s.parts);
-      hp::require(hp::ceil_div(width * channels, int64_t(64)) <= hp::kMaxThreads / 1024, "too many channels for one launch");
+      hp::require(hp::ceil_div(int64_t(width) * channels, int64_t(64)) <= hp::kMaxThreads / 1024, "too many channels for one launch");
       for (s.first = 0; s.first < states; s.first += width) {
         s.starts = s.first == 0;
         s.ends = s.first + width >= states;
@@ -551,16 +622,11 @@ int hp_selective_scan_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* 
         using Four = std::integral_constant<int, 4>;
         using Eight = std::integral_constant<int, 8>;
         if constexpr (sizeof(T) == 4) {
-          if (each == 2 && waves == 2) launch(Two{}, Two{});
-          else if (each == 2 && waves == 4) launch(Four{}, Two{});
-          else if (each == 2) launch(Eight{}, Two{});
-          else if (waves == 8) launch(Eight{}, Four{});
+          if (many) launch(Eight{}, Four{});
+          else if (waves == 8) launch(Eight{}, Two{});
+          else if (waves == 2) launch(Two{}, Two{});
         }
-        if (each == 4) {
-          if (waves == 1) launch(std::integral_constant<int, 1>{}, Four{});
-          else if (waves == 2) launch(Two{}, Four{});
-          else if (waves == 4) launch(Four{}, Four{});
-        }
+        if (waves == 4) launch(Four{}, Two{});
         projections_kernel<T><<<unsigned(std::min<int64_t>(hp::ceil_div(lines * width, 256), 8192)), 256, 0, ctx->stream>>>(s, o, width, out(db), out(dc));
         hp::check_launch("scan projections");
         decays_kernel<T><<<unsigned(hp::ceil_div(width * channels, int64_t(64))), 1024, 0, ctx->stream>>>(s, o.da, width, out(da_log));

@@ -26,6 +26,10 @@ struct Rows {
     const int64_t n = wide ? static_cast<const int64_t*>(lengths)[row] : static_cast<const int32_t*>(lengths)[row];
     return n < 0 ? 0 : n < time ? n : time;
   }
+  // Lane i's byte of the resets from t on, of the last step < end for lanes behind it; for a later ballot().
+  __device__ __forceinline__ unsigned byte(int64_t row, int64_t t, int64_t end, int lane) const {
+    return resets[row * time + (t + lane < end ? t + lane : end - 1)];
+  }
   // Bit i: a reset at step t + i < end.
   template <int N>
   __device__ __forceinline__ unsigned starts(int64_t row, int64_t t, int64_t end) const {
