@@ -219,7 +219,21 @@ __device__ __forceinline__ T from_across(T v) {
 // Lanes without `bit` get a's sums over pairs of lanes, those with it b's.
 template <int MASK, typename T>
 __device__ __forceinline__ T fold_pair(T a, T b, bool bit) {
-  return (bit ? b : a) + from_across<MASK>(bit ? a : b);
+  if constexpr (sizeof(T) == 4 && (MASK == 8 || MASK == 7)) {
+    // Two additions that write the lanes of one kind each, in place of two selects and one;
+    // what they read may be as new as the wait for it; selects or another fold read what they leave.
+    T sum;
+    if constexpr (MASK == 8) {
+      asm("s_nop 1\n\tv_add_f32_dpp %0, %1, %1 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+          "v_add_f32_dpp %0, %2, %2 row_ror:8 row_mask:0xf bank_mask:0xc" : "=&v"(sum) : "v"(a), "v"(b));
+    } else {
+      asm("s_nop 1\n\tv_add_f32_dpp %0, %1, %1 row_half_mirror row_mask:0xf bank_mask:0x5\n\t"
+          "v_add_f32_dpp %0, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xa" : "=&v"(sum) : "v"(a), "v"(b));
+    }
+    return sum;
+  } else {
+    return (bit ? b : a) + from_across<MASK>(bit ? a : b);
+  }
 }
 
 // Of values for each of S states and L steps (8 or 16) the sums over each row of 16 lanes,
@@ -440,7 +454,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
         });
         sums_b[at.wave][i][lane] = along;
         sums_a[at.wave][i][lane] = decays;
-        if (c.gate) sums_y[at.wave][i][lane] = y;
+        sums_y[at.wave][i][lane] = y;  // without gates too: a branch in every step would keep the steps' work apart
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           if constexpr (i % 2) {
@@ -459,7 +473,8 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
         ((lane & 16 ? o.dc : o.db) + to)[unsigned(i * c.groups) * (NW * S) + s] = all;
       }
     };
-    walk(std::integral_constant<bool, RESETS>{});
+    if (RESETS && now.starts) walk(std::true_type{});  // few tiles have one
+    else walk(std::false_type{});
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
@@ -469,7 +484,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
       for (int w = 0; w < NW; ++w) {
         along += sums_b[w][own + i][lane];
         decays += sums_a[w][own + i][lane];
-        if (c.gate) y += sums_y[w][own + i][lane];
+        y += sums_y[w][own + i][lane];
       }
       const unsigned to = at.place(c, own + i);
       T *to_x = at.line(c, o.dx, t) + to, *to_delta = at.line(c, o.ddelta, t) + to;
