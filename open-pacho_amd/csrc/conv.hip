@@ -194,23 +194,30 @@ __global__ __launch_bounds__(256) void backward_kernel(Conv<T> c) {
   V dweight[K], dbias = V::of(T(0));
 #pragma unroll
   for (int k = 0; k < K; ++k) open[k] = dweight[k] = V::of(T(0));
+  // Loads of the next steps, without a branch: those behind the row's end repeat its last step's, which nothing uses.
+  const uint8_t* const marks = c.rows.resets ? c.rows.resets : reinterpret_cast<const uint8_t*>(c.x);
+  V next_x[U], next_d[U];
+  unsigned next_marks[U];
+  const auto load = [&](int64_t t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t from = t + i < run.end ? t + i : run.end - 1;
+      next_x[i] = V::load(run.at(c, c.x, from));
+      next_d[i] = V::load(run.at(c, c.grad, from));
+      next_marks[i] = marks[run.row * c.rows.time + from];
+    }
+  };
+  if (run.end > 0) load(run.first);
   // Through the steps behind the run that see its last ones.
   for (int64_t t = run.first; t < stop + K - 1; t += U) {
     V x[U], d[U];
-    const unsigned starts = c.rows.template starts<U>(run.row, t, run.end);
-    if (t + U <= run.end) {
+    unsigned starts = 0;
 #pragma unroll
-      for (int i = 0; i < U; ++i) x[i] = V::load(run.at(c, c.x, t + i));
-#pragma unroll
-      for (int i = 0; i < U; ++i) d[i] = V::load(run.at(c, c.grad, t + i));
-    } else {
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const bool inside = t + i < run.end;
-        x[i] = inside ? V::load(run.at(c, c.x, t + i)) : V::of(T(0));
-        d[i] = inside ? V::load(run.at(c, c.grad, t + i)) : V::of(T(0));
-      }
+    for (int i = 0; i < U; ++i) {
+      x[i] = next_x[i], d[i] = next_d[i];
+      if (c.rows.resets && next_marks[i] && t + i < run.end) starts |= 1u << i;
     }
+    if (run.end > 0) load(t + U);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int64_t now = t + i;

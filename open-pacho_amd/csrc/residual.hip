@@ -183,27 +183,40 @@ __device__ __forceinline__ int64_t gate_slot(int64_t worker, int64_t group, int6
   return 2 * worker + (group * divide > worker * each ? 1 : 0);
 }
 
+// Backward's waves a SIMD, for the registers of K vectors of each array and sum.
+template <int K, bool ALL>
+constexpr int kWaves = K > 2 ? 2 : K == 2 && ALL ? 3 : 4;
+
 // GATE: 0 none, 1 one for each row, 2 shared by rows.
 template <typename T, int L, int K, bool POST, int GATE>
-__global__ __launch_bounds__(L > 256 ? L : 256) void backward_kernel(Norm<T> c) {
+__global__ __launch_bounds__(L > 256 ? L : 256, (kWaves<K, (POST && GATE == 2)>)) void backward_kernel(Norm<T> c) {
   constexpr int kTeams = L > 256 ? 1 : 256 / L;
   using P = Part<T, L, K>;
   constexpr int N = POST ? 3 : 2;
   __shared__ T meet[N][16], meet_one[1][16];
-  const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : threadIdx.x / L;
+  const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : threadIdx.x / L;
   const unsigned length = unsigned(c.channels);
   const int64_t worker = int64_t(blockIdx.x) * kTeams + team, first = worker * c.each;
   if (first >= c.rows) return;  // whole teams; those of several waves are whole workgroups
   const int64_t end = first + c.each < c.rows ? first + c.each : c.rows;
   P weight_sum, post_sum, gate_sum;
   weight_sum.clear(), post_sum.clear(), gate_sum.clear();
+  P x, u, d, dn, next_x, next_u, next_d, next_dn;
+  const auto load = [&](int64_t row) __attribute__((always_inline)) {
+    const int64_t start = row * c.channels;
+    next_u.load(c.given + start, length, lane);
+    next_dn.load(c.grad_normed + start, length, lane);
+    next_x.load(c.x + start, length, lane);
+    next_d.load(c.grad_stream + start, length, lane);
+  };
+  constexpr bool kAhead = K == 1;  // a row ahead where there are registers for it
+  if (kAhead) load(first);
   for (int64_t row = first; row < end; ++row) {
     const int64_t start = row * c.channels;
-    P x, u, d, dn, other;
-    u.load(c.given + start, length, lane);
-    dn.load(c.grad_normed + start, length, lane);
-    x.load(c.x + start, length, lane);
-    d.load(c.grad_stream + start, length, lane);
+    if (!kAhead) load(row);
+    x = next_x, u = next_u, d = next_d, dn = next_dn;
+    if (kAhead) load(row + 1 < end ? row + 1 : row);
+    P other;
     other.load(c.weight, length, lane);
     T sums[N] = {};
     P::each([&](int k, int j) {
@@ -431,19 +444,24 @@ void backward(hp_ctx* ctx, Norm<T> c, T* dweight, T* dpost) {
   int64_t workers = 0;
   const auto launch = [&](auto l, auto k, auto shared) {
     constexpr int L = l, K = k, threads = L > 256 ? L : 256, teams = threads / L;
-    workers = plan(int64_t(1280) * teams);
     const auto run = [&](auto gate) {
-      const auto kernel = c.post ? backward_kernel<T, L, K, true, gate> : backward_kernel<T, L, K, false, gate>;
-      kernel<<<unsigned(hp::ceil_div(workers, teams)), threads, 0, ctx->stream>>>(c);
+      const auto go = [&](auto post) {
+        // As many as run at once: a second round would be a short one.
+        workers = plan(int64_t(256) * (4 * kWaves<K, post && gate == 2> * 64 / threads) * teams);
+        backward_kernel<T, L, K, post, gate><<<unsigned(hp::ceil_div(workers, teams)), threads, 0, ctx->stream>>>(c);
+      };
+      if (c.post) go(std::true_type{});
+      else go(std::false_type{});
     };
     if constexpr (shared) run(std::integral_constant<int, 2>{});
     else if (c.gate) run(std::integral_constant<int, 1>{});
     else run(std::integral_constant<int, 0>{});
   };
   const bool held = with_team<T>(c.channels, [&](auto l, auto k) {
-    // The third sum of 1024 threads would not fit into their registers: 512, with twice as many vectors.
-    constexpr bool half = l == 1024;
-    if (c.gate && c.divide > 1) launch(std::integral_constant<int, half ? 512 : l>{}, std::integral_constant<int, half ? 2 * k : k>{}, std::true_type{});
+    // A third sum leaves teams of several waves half the vectors a lane, so that two or more of them run beside
+    // each other, and the largest, which cannot grow, twice as many.
+    constexpr int many = l == 1024 ? 512 : l >= 256 && k == 2 ? 2 * l : l, of = l == 1024 ? 2 * k : l >= 256 && k == 2 ? 1 : k;
+    if (c.gate && c.divide > 1) launch(std::integral_constant<int, many>{}, std::integral_constant<int, of>{}, std::true_type{});
     else launch(l, k, std::false_type{});
   });
   if (!held) {

@@ -33,7 +33,7 @@ __device__ __forceinline__ void apart() {
 
 // Steps of a tile, for the registers that its states and decays take.
 template <typename T, int NW, int S>
-constexpr int kTile = sizeof(T) == 8 || S == 4 || NW == 2 ? 8 : 16;
+constexpr int kTile = sizeof(T) == 4 && S == 2 && NW == 8 ? 16 : 8;
 constexpr int kLongestTile = 16;
 // Tiles that the first launch loads ahead, an even number.
 template <typename T, int NW>
