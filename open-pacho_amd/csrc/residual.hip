@@ -20,6 +20,7 @@
 // group that it sees a part of: at most two, as groups are neighbouring rows too.
 #include <type_traits>
 
+#include "lanes.h"
 #include "sequence.h"
 
 namespace {
@@ -111,10 +112,7 @@ struct Part {
 template <int L, int N, typename T>
 __device__ __forceinline__ void team_sums(T (&v)[N], T (*meet)[N][16]) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-#pragma unroll
-    for (int o = (L < 64 ? L : 64) / 2; o > 0; o >>= 1) v[n] += __shfl_xor(v[n], o, 64);
-  }
+  for (int n = 0; n < N; ++n) v[n] = hpd::lane_sum<(L < 64 ? L : 64)>(v[n]);
   if constexpr (L > 64) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
@@ -124,9 +122,7 @@ __device__ __forceinline__ void team_sums(T (&v)[N], T (*meet)[N][16]) {
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < N; ++n) {  // lanes read a wave's each: all of them in one lane would take its registers
-      v[n] = (*meet)[n][threadIdx.x % (L / 64)];
-#pragma unroll
-      for (int o = L / 128; o > 0; o >>= 1) v[n] += __shfl_xor(v[n], o, 64);
+      v[n] = hpd::lane_sum<L / 64>((*meet)[n][threadIdx.x % (L / 64)]);
     }
   }
 }
@@ -209,6 +205,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, (kWaves<K, (POST && GATE == 2)>)
     next_x.load(c.x + start, length, lane);
     next_d.load(c.grad_stream + start, length, lane);
   };
+  int64_t group = GATE == 2 ? first / c.divide : 0, next = (group + 1) * c.divide;  // a shared gate's and its end
   constexpr bool kAhead = K == 1;  // a row ahead where there are registers for it
   if (kAhead) load(first);
   for (int64_t row = first; row < end; ++row) {
@@ -238,7 +235,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, (kWaves<K, (POST && GATE == 2)>)
     T inner = T(1);
     if constexpr (POST) inner = inverse_rms(c, sums[N - 1]);
     P gate;
-    if constexpr (GATE != 0) gate.load(c.gate + row / c.divide * c.channels, length, lane);
+    if constexpr (GATE != 0) gate.load(GATE == 1 ? c.gate + start : c.gate + group * c.channels, length, lane);
     if constexpr (POST) other.load(c.post, length, lane);
     T sum[1] = {};
     P::each([&](int k, int j) {
@@ -268,11 +265,11 @@ __global__ __launch_bounds__(L > 256 ? L : 256, (kWaves<K, (POST && GATE == 2)>)
     }
     dn.store(c.dx + start, length, lane);
     if constexpr (GATE == 2) {
-      const int64_t group = row / c.divide, next = (group + 1) * c.divide;
       if (row + 1 == end || row + 1 == next) {
         const bool whole = group * c.divide >= first && next <= end;
         gate_sum.store(whole ? c.dgate + group * c.channels : c.gate_sums + gate_slot(worker, group, c.divide, c.each) * c.channels, length, lane);
         gate_sum.clear();
+        if (row + 1 == next) ++group, next += c.divide;
       }
     }
   }

@@ -18,7 +18,9 @@ template <typename T, int NW, int S, bool RESETS, bool SUMMARY>
 __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_, const T* c_) {
   constexpr int kSteps = kTile<T>, kAhead = kTiles<T, NW>, kOwn = kSteps / NW;  // steps of a tile that a wave prepares and finishes
   __shared__ T shared_dt[2][kSteps][64], shared_u[2][kSteps][64];
-  __shared__ T sums[SUMMARY ? 1 : NW][SUMMARY ? 1 : kSteps][64];
+  // Two sets of sums where LDS has room: the waves then meet once a tile, not again behind its sums.
+  constexpr int kSets = NW <= 8 ? 2 : 1;
+  __shared__ T sums[SUMMARY ? 1 : kSets][SUMMARY ? 1 : NW][SUMMARY ? 1 : kSteps][64];
   const Place<T, NW, S> at(c);
   if (SUMMARY && at.part == c.parts - 1) return;
   const int lane = at.lane, own = at.wave * kOwn;
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
           }
         });
         if constexpr (SUMMARY) span += dt;
-        else sums[at.wave][i][lane] = y;
+        else sums[turn % kSets][at.wave][i][lane] = y;
       });
     };
     cut = cut || starts;
@@ -121,9 +123,9 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
         if (own + i >= count) break;
-        T y = sums[0][own + i][lane];
+        T y = sums[turn % kSets][0][own + i][lane];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) y += sums[w][own + i][lane];
+        for (int w = 1; w < NW; ++w) y += sums[turn % kSets][w][own + i][lane];
         T* to = at.line(c, c.y, t) + at.place(c, own + i);
         if (!c.starts) y += *to;
         if (c.ends) {
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
         }
         if (at.valid) *to = y;
       }
-      __syncthreads();
+      if (kSets == 1) __syncthreads();
     }
   };
   for (int t = at.first; t < at.end; t += kAhead * kSteps) {

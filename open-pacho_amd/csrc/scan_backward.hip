@@ -19,6 +19,7 @@
 //
 // Where rows are cut into parts, the first launch also forms what a part passes back from
 // nothing, sum_t D_t c_t g_t with D_t the product of the decays up to t.
+#include "lanes.h"
 #include "scan.h"
 
 using namespace hpd;
@@ -179,43 +180,6 @@ struct Grads {
 
 // ---- folding of registers ------------------------------------------------------------
 
-// Exchanges halves (BIT 5) or odd and even rows of 16 lanes (BIT 4) between a and b.
-template <int BIT>
-__device__ __forceinline__ void swap_lanes(uint32_t& a, uint32_t& b) {
-  if constexpr (BIT == 5) {
-    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = r[0], b = r[1];
-  } else {
-    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = r[0], b = r[1];
-  }
-}
-// Lane i: the value of lane i ^ 8 (8), i ^ 7 (7), i ^ 3 (3) or i ^ 1 (1).
-template <int MASK>
-__device__ __forceinline__ uint32_t across(uint32_t v) {
-  constexpr int kind = MASK == 8 ? 0x128 /* row_ror:8 */ : MASK == 7 ? 0x141 /* row_half_mirror */ : MASK == 3 ? 0x1B /* quad_perm 3 2 1 0 */ : 0xB1 /* 1 0 3 2 */;
-  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), kind, 0xF, 0xF, true));
-}
-
-template <typename T>
-struct Words {
-  uint32_t w[sizeof(T) / 4];
-};
-
-template <int BIT, typename T>
-__device__ __forceinline__ T fold_rows(T a, T b) {
-  auto x = __builtin_bit_cast(Words<T>, a), y = __builtin_bit_cast(Words<T>, b);
-#pragma unroll
-  for (unsigned k = 0; k < sizeof(T) / 4; ++k) swap_lanes<BIT>(x.w[k], y.w[k]);
-  return __builtin_bit_cast(T, x) + __builtin_bit_cast(T, y);
-}
-template <int MASK, typename T>
-__device__ __forceinline__ T from_across(T v) {
-  auto x = __builtin_bit_cast(Words<T>, v);
-#pragma unroll
-  for (unsigned k = 0; k < sizeof(T) / 4; ++k) x.w[k] = across<MASK>(x.w[k]);
-  return __builtin_bit_cast(T, x);
-}
 // Lanes without `bit` get a's sums over pairs of lanes, those with it b's.
 template <int MASK, typename T>
 __device__ __forceinline__ T fold_pair(T a, T b, bool bit) {
