@@ -184,7 +184,6 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
       }
       continue;
     }
-    share.template load<true>(c.logits + row * c.vocab, length, lane);
     List<T, kLanes> list{};
     if (lists) {
       list.read(c, row, lane);
@@ -195,6 +194,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
         team_fence();
       }
     }
+    share.template load<true>(c.logits + row * c.vocab, length, lane);
     T tops[S::kDeep], top, total, unlisted = T(0);
     if constexpr (REST) share.statistics(length, lane, meet, turn, tops, top, total, scaled, bits, unlisted);
     else share.statistics(length, lane, meet, turn, tops, top, total, scaled, NoNames(), unlisted);
@@ -204,7 +204,11 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
       const T rest = L > 64 ? told[0] : list.rest, weight = T(factor * c.inverse) + (L > 64 ? told[1] : list.spoiled);
       const T inner = inverse * weight, outer = REST ? unlisted_factor(inverse, rest, unlisted) * weight : inner;
       if constexpr (REST) {
-        share.each_named(length, lane, bits, [&](T& v, bool named, int d) { v = v * S::part(tops[d], top, scaled) * (named ? inner : outer); });
+        // Named ones carry a sign: -0 too, and NaN stays NaN.
+        share.each(length, lane, [&](T& v, int, int d) {
+          const T value = S::part(tops[d], top, scaled) * v;
+          v = __builtin_signbit(v) ? -value * inner : value * outer;
+        });
       } else {
         share.each(length, lane, [&](T& v, int, int d) { v = v * (S::part(tops[d], top, scaled) * inner); });
       }

@@ -233,7 +233,7 @@ struct Share {
   }
 
   // The values become exp(scaled(z - tops[d])), and `second` their sum without the
-  // values that `names` has: names.bits(i) has a bit for each value of the vector at i.
+  // values that `names` has, which become -exp(): names.bits(i) has a bit for each value of the vector at i.
   template <typename Scale, typename Names>
   __device__ __forceinline__ void statistics(int length, int lane, Meet<T, kDeep, Names::some ? 2 : 1>& meet, int turn, T (&tops)[kDeep], T& top, T& total,
                                              Scale scaled, Names names, T& second) {
@@ -258,7 +258,11 @@ struct Share {
       T sum = T(0), other = T(0);
       if (d == last) {
         sum = rest = hpd::exp_down(scaled(rest - reference));
-        if constexpr (Names::some) other = rest_index(length, lane) < length && names.one(rest_index(length, lane)) ? T(0) : rest;
+        if constexpr (Names::some) {
+          const bool named = rest_index(length, lane) < length && names.one(rest_index(length, lane));
+          other = named ? T(0) : rest;
+          rest = named ? -rest : rest;
+        }
       }
       T s[W] = {}, o[W] = {};
 #pragma unroll
@@ -269,8 +273,12 @@ struct Share {
         for (int j = 0; j < W; ++j) {
           z[k][j] = hpd::exp_down(scaled(z[k][j] - reference));
           s[j] += z[k][j];
-          if constexpr (Names::some) o[j] += bits >> j & 1 ? T(0) : z[k][j];
+          if constexpr (Names::some) {
+            o[j] += bits >> j & 1 ? T(0) : z[k][j];
+            z[k][j] = bits >> j & 1 ? -z[k][j] : z[k][j];
+          }
         }
+        if constexpr (Names::some) asm volatile("" ::: "memory");  // the bits of all vectors at once would take registers from the values
       }
 #pragma unroll
       for (int j = 0; j < W; ++j) sum += s[j];
