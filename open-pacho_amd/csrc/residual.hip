@@ -49,6 +49,7 @@ struct Norm {
   int64_t rows, channels, divide;  // rows that share a gate
   int64_t each;                    // rows of a worker
   T scale, eps, mean;              // mean: 1 / channels
+  bool past;                       // backward: a call's arrays do not fit into the last cache
 };
 
 // A lane's part of a row: K vectors, L lanes apart. A vector that would pass the row's
@@ -81,7 +82,7 @@ struct Part {
       }
     }
   }
-  __device__ __forceinline__ void store(T* row, unsigned length, int lane) const {
+  __device__ __forceinline__ void store(T* row, unsigned length, int lane, bool past = false) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (at(k, lane) >= length) continue;
@@ -91,7 +92,7 @@ struct Part {
 #pragma unroll
         for (int j = 0; j < W; ++j) to[j] = v[k][j];
       }
-      *reinterpret_cast<V*>(row + start(k, length, lane)) = to;
+      hpd::put(reinterpret_cast<V*>(row + start(k, length, lane)), to, past);
     }
   }
   // f(k, j) for every value.
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, (kWaves<K, (POST && GATE == 2)>)
       weight_sum.v[k][j] += dn.v[k][j] * unit;
       d.v[k][j] += outer * (dn.v[k][j] * other.v[k][j] - unit * along);
     });
-    d.store(c.d + start, length, lane);
+    d.store(c.d + start, length, lane, c.past);
     // From here on u holds the unit of x, or x itself, and dn the gradient of what the gate multiplies.
     T inner = T(1);
     if constexpr (POST) inner = inverse_rms(c, sums[N - 1]);
@@ -257,13 +258,13 @@ __global__ __launch_bounds__(L > 256 ? L : 256, (kWaves<K, (POST && GATE == 2)>)
       }
       dn.v[k][j] = e;
     });
-    if constexpr (GATE == 1) gate.store(c.dgate + start, length, lane);
+    if constexpr (GATE == 1) gate.store(c.dgate + start, length, lane, c.past);
     if constexpr (POST) {
       team_sums<L>(sum, &meet_one);
       const T shared = sum[0] * c.mean;
       P::each([&](int k, int j) { dn.v[k][j] = inner * (dn.v[k][j] - x.v[k][j] * shared); });
     }
-    dn.store(c.dx + start, length, lane);
+    dn.store(c.dx + start, length, lane, c.past);
     if constexpr (GATE == 2) {
       if (row + 1 == end || row + 1 == next) {
         const bool whole = group * c.divide >= first && next <= end;
@@ -428,6 +429,9 @@ void forward(hp_ctx* ctx, const Norm<T>& c) {
 template <typename T>
 void backward(hp_ctx* ctx, Norm<T> c, T* dweight, T* dpost) {
   hp::Scratch scratch(ctx);
+  // Six arrays, of which the caches would hold none to its next reader: 430 us -> 424 of 8 x 4096 x 2048 float32, and of
+  // rows that are no whole lines 87 -> 72 (3 x 1367 x 1537 float64).
+  c.past = c.rows * c.channels * int64_t(6 * sizeof(T)) > hp::kLastCache;
   const int64_t groups = c.gate ? c.rows / c.divide : 0;
   const auto plan = [&](int64_t most) {
     // Some rows a worker, so that the sums weigh little beside the rows, unless the chip would idle.
@@ -455,11 +459,18 @@ void backward(hp_ctx* ctx, Norm<T> c, T* dweight, T* dpost) {
     else run(std::integral_constant<int, 0>{});
   };
   const bool held = with_team<T>(c.channels, [&](auto l, auto k) {
-    // A third sum leaves teams of several waves half the vectors a lane, so that two or more of them run beside
-    // each other, and the largest, which cannot grow, twice as many.
-    constexpr int many = l == 1024 ? 512 : l >= 256 && k == 2 ? 2 * l : l, of = l == 1024 ? 2 * k : l >= 256 && k == 2 ? 1 : k;
-    if (c.gate && c.divide > 1) launch(std::integral_constant<int, many>{}, std::integral_constant<int, of>{}, std::true_type{});
-    else launch(l, k, std::false_type{});
+    // Teams of several waves with one vector a lane: next rows have registers. The largest cannot grow, and the third
+    // sum of shared gates does not fit its threads.
+    if constexpr (l == 1024) {
+      if (c.gate && c.divide > 1) launch(std::integral_constant<int, 512>{}, std::integral_constant<int, 2 * k>{}, std::true_type{});
+      else launch(l, k, std::false_type{});
+    } else {
+      constexpr int split = l >= 256 ? k : 1;
+      const std::integral_constant<int, split * l> many;
+      const std::integral_constant<int, k / split> of;
+      if (c.gate && c.divide > 1) launch(many, of, std::true_type{});
+      else launch(many, of, std::false_type{});
+    }
   });
   if (!held) {
     workers = plan(1024);

@@ -13,6 +13,18 @@ __device__ __forceinline__ int64_t by_die() {
   return int64_t(die) * least + (die < more ? die : more) + blockIdx.x / kDies;
 }
 
+// Stores `value`; with `past` the caches keep no place for it.
+template <typename V>
+__device__ __forceinline__ void put(V* at, V value, bool past) {
+  if (past) {
+    asm volatile("");  // else the compiler joins the two stores into a plain one, and without the other from behind
+    __builtin_nontemporal_store(value, at);
+    asm volatile("");
+  } else {
+    *at = value;
+  }
+}
+
 // Where rows begin anew and end; pointers that a call does not have are null.
 struct Rows {
   const uint8_t* resets;  // (rows, time)
@@ -86,3 +98,9 @@ __device__ __forceinline__ void add_parts(const T* parts, int64_t stride, int64_
 }
 
 }  // namespace hpd
+
+namespace hp {
+
+constexpr int64_t kLastCache = int64_t(256) << 20;  // bytes
+
+}  // namespace hp
