@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256) void forward_kernel(Conv<T> c) {
 template <typename T, int W, int K>
 __global__ __launch_bounds__(256) void backward_kernel(Conv<T> c) {
   using V = Value<T, W>;
-  constexpr int U = 4;
+  constexpr int U = K > 6 ? 2 : 4;  // steps ahead, for the registers beside the taps'
   Run<T, W, K> run(c);
   if (!run.valid) return;
   const int64_t stop = run.first + c.steps < c.rows.time ? run.first + c.steps : c.rows.time;

@@ -1,4 +1,5 @@
-"""Operators of model training: recurrences over time, residual norms, losses from logits, AdamW.
+"""Operators of model training and serving: recurrences, convolutions and scans over time, residual norms,
+losses from logits, AdamW.
 
 Each works on resident arrays of one backend, float32 or float64 throughout,
 and returns new arrays; gradients are functions of their own, since arrays
@@ -10,6 +11,13 @@ these operators: call them between compiled functions.
     loss, log_probs, d_logits = nn.policy_loss_grad(logits, actions, old, advantages, mask=mask)
     dx, d_gate, d_initial = nn.gated_recurrence_grad(d_h, x, gate, h, initial, resets=starts)
     params, state = nn.adamw(params, grads, state, learning_rate=3e-4)
+
+    u, inputs = nn.causal_conv(x, weight, bias, activation="silu", resets=starts, lengths=lengths)
+    y, states = nn.selective_scan(u, delta, a_log, b, c, skip, gate, delta_bias=bias, resets=starts, lengths=lengths)
+    stream, normed = nn.residual_norm(y @ w_out, stream, weight)
+    loss, losses, d_logits = nn.distillation_loss_grad(logits, indices, teacher_logits, teacher_rest, mask=mask)
+    d = nn.selective_scan_grad(d_y, u, delta, a_log, b, c, skip, gate, delta_bias=bias, resets=starts, lengths=lengths)
+    y, states = nn.selective_scan_step(u, delta, a_log, b, c, states, skip, gate, delta_bias=bias)  # one token
 """
 
 import math
