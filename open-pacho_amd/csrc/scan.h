@@ -6,10 +6,11 @@
 // A lane owns a channel, a wave S (2, or 4 of many) of its states, a workgroup all states of up to 64
 // channels that share b and c. So b and c are the same in a whole wave: a register holds
 // those of four steps in the lanes of each row of 16, and an instruction that multiplies by
-// one of them takes it from its lane on the way (a row broadcast). An exponential, two
-// products and two fused multiply-adds make a state's step. (Scalar loads of b and c in
-// each step, whose waits no other work covers, took 1458 us where this takes 282, 8 x 2048 x
-// 2048 float32 with 16 states.) Only the sums over states meet in LDS, once for a tile of
+// one of them takes it from its lane on the way (a row broadcast). Bound: vector issue. An
+// exponential, two products and two fused multiply-adds make a state's step: 213 us for 8 x 2048 x
+// 2048 float32 with 16 states, whose bytes would take 89. (Scalar loads of b and c in
+// each step, whose waits no other work covers, took 1458.) Two states a wave leave enough
+// waves; from 17 states on (33 forward in 16 waves) four save the steps' common work. Only the sums over states meet in LDS, once for a tile of
 // steps: each wave has some of the tile's steps as its own, whose dt and dt x it leaves for
 // all waves before they walk the tile, and whose sums it adds up afterwards. Steps of a
 // tile behind the row's end have dt, x, b and c of zero and change nothing.

@@ -14,8 +14,11 @@
 //
 // Sums over channels (db, dc): every lane has a value for each step and state of a tile. Pairs
 // of registers are folded into one whose halves, quarters, ... belong to one of the two each,
-// until a register holds a sum in each lane: three instructions a value where a sum over 64
-// lanes by itself takes six times two. Workgroups leave these, and their sums over steps, as parts.
+// until a register holds a sum in each lane: two or three instructions a value where a sum over
+// 64 lanes by itself takes six times two. Workgroups leave these, and their sums over steps, as parts.
+//
+// Bound: vector issue, 29 instructions a state and step. 8 x 2048 x 2048 float32 with 16 states: 175 us
+// for the first launch, 630-660 for the second, 20 for db and dc, where the call's bytes would take 155.
 //
 // Where rows are cut into parts, the first launch also forms what a part passes back from
 // nothing, sum_t D_t c_t g_t with D_t the product of the decays up to t.
@@ -32,7 +35,8 @@ __device__ __forceinline__ void apart() {
   if constexpr (sizeof(T) == 8) __builtin_amdgcn_sched_barrier(0);
 }
 
-// Steps of a tile, for the registers that its states and decays take.
+// Steps of a tile, for the registers that its states and decays take: of 16, float32 with four waves or
+// more states would need accumulation registers, which leaves them a wave a SIMD.
 template <typename T, int NW, int S>
 constexpr int kTile = sizeof(T) == 4 && S == 2 && NW == 8 ? 16 : 8;
 constexpr int kLongestTile = 16;
