@@ -13,10 +13,12 @@ constexpr int kTile = sizeof(T) == 4 ? 16 : 8;
 template <typename T, int NW>
 constexpr int kTiles = sizeof(T) == 4 && NW > 2 && NW < 16 ? 4 : 2;
 
-// SUMMARY: a part's sum of dt and the states that it ends in from zero ones, in place of y.
-template <typename T, int NW, int S, bool RESETS, bool SUMMARY>
+// SUMMARY: a part's sum of dt and the states that it ends in from zero ones, in place of y. ONE: rows of one tile, single
+// tokens among them, without the loads, barriers and waits of those ahead: 8.1 us in place of 13 for 16 tokens of 2048
+// channels with 16 states.
+template <typename T, int NW, int S, bool RESETS, bool SUMMARY, bool ONE = false>
 __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_, const T* c_) {
-  constexpr int kSteps = kTile<T>, kAhead = kTiles<T, NW>, kOwn = kSteps / NW;  // steps of a tile that a wave prepares and finishes
+  constexpr int kSteps = kTile<T>, kAhead = ONE ? 1 : kTiles<T, NW>, kOwn = kSteps / NW;  // steps of a tile that a wave prepares and finishes
   __shared__ T shared_dt[2][kSteps][64], shared_u[2][kSteps][64];
   // Two sets of sums where LDS has room: the waves then meet once a tile, not again behind its sums.
   constexpr int kSets = NW <= 8 ? 2 : 1;
@@ -87,8 +89,10 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Scan<T> c, const T* b_
     bs.keep(lane, count);
     if (!SUMMARY) cs.keep(lane, count);
     const unsigned starts = RESETS ? unsigned(__ballot(now.resets != 0 && lane < count)) : 0;
-    load(now, t + kAhead * kSteps);
-    prepare(next, t + kSteps, turn ^ 1);  // of no use behind the last tile
+    if constexpr (!ONE) {
+      load(now, t + kAhead * kSteps);
+      prepare(next, t + kSteps, turn ^ 1);  // of no use behind the last tile
+    }
     // All of the tile's at once: the compiler would wait for those of each step in turn.
     T dts[kSteps], us[kSteps];
 #pragma unroll
@@ -184,7 +188,8 @@ void launch(hp_ctx* ctx, const Scan<T>& c, const T* b, const T* cs) {
     kernel<<<blocks, NW * 64, 0, ctx->stream>>>(c, b, cs);
     hp::check_launch("scan summary");
   }
-  const auto kernel = c.rows.resets ? forward_kernel<T, NW, S, true, false> : forward_kernel<T, NW, S, false, false>;
+  const bool one = c.time <= kTile<T> && !c.rows.resets;
+  const auto kernel = c.rows.resets ? forward_kernel<T, NW, S, true, false> : one ? forward_kernel<T, NW, S, false, false, true> : forward_kernel<T, NW, S, false, false>;
   kernel<<<blocks, NW * 64, 0, ctx->stream>>>(c, b, cs);
   hp::check_launch("scan");
 }
