@@ -106,7 +106,8 @@ struct List {
     bool again = false;
     each(c, row, lane, start, length, [&](int, int64_t i) {
       const unsigned at = unsigned(i - start), bit = 1u << (at & 31);
-      again = again || (atomicOr(&bits.words[at >> 5], bit) & bit);
+      const unsigned before = atomicOr(&bits.words[at >> 5], bit);  // after a repeat too: it names the entry
+      again = again || (before & bit);
     });
     repeats = team_reduce<L>(int(again), [](int a, int b) { return a | b; });
   }
