@@ -9,7 +9,10 @@
 //
 // with R the sum S without the terms that the list names. R is formed as a sum of its
 // own, not as a difference: where the list holds nearly all of q the rest would lose
-// its digits. Which logits are named stands in a bit for each of a row, in LDS; a vector's
+// its digits. Where the list holds all that the type has of q, R is formed again, relative to the largest
+// logit m' that it does not name (Share::apart): log R = (m' - m) / T + log R', and
+// exp((z_j - m') / T) / R' takes its place in the gradient. Such rows are read again, and
+// their gradient is stored twice: 8192 x 32000 with 64 entries takes 332 us where no row is so and 1001 where all are. Which logits are named stands in a bit for each of a row, in LDS; a vector's
 // bits are one read, and where a team holds the row the only one: named exponentials carry
 // a sign from there on. (A second read for the gradient, and the bits of all vectors at
 // once, took the values' registers: 451 us in place of 361.) Bound: HBM, each logit read once
@@ -116,7 +119,8 @@ struct List {
   }
 
   // The row's loss from the statistics of its logits, for every lane of the team.
-  __device__ __forceinline__ double loss(const Call<T>& c, int64_t row, int lane, T row_top, T total, T unlisted) const {
+  // `unlisted` is relative to `rest_top`.
+  __device__ __forceinline__ double loss(const Call<T>& c, int64_t row, int lane, T row_top, T total, T rest_top, T unlisted) const {
     const double log_row = log_wide(total);
     double sum = 0;
     each(c, row, lane, 0, c.vocab, [&](int e, int64_t i) {
@@ -126,7 +130,8 @@ struct List {
       if (p != T(0)) sum += double(p) * ((logit - top - log_total) - log_q);
     });
     if (lane == 0 && rest != T(0)) {
-      sum += double(rest) * ((double(c.teacher_rest[row]) - top - log_total) - (log_wide(unlisted) - log_row));
+      const double log_q = (double(rest_top) - double(row_top)) * c.inverse + log_wide(unlisted) - log_row;
+      sum += double(rest) * ((double(c.teacher_rest[row]) - top - log_total) - log_q);
     }
     sum = team_reduce<L>(sum, [](double a, double b) { return a + b; });
     return sum + double(spoiled) + (total == total ? 0.0 : double(total));
@@ -158,6 +163,21 @@ __device__ __forceinline__ T unlisted_factor(T row_inverse, T rest, T unlisted) 
   return row_inverse - (rest == T(0) || unlisted == T(0) ? T(0) : rest / unlisted);
 }
 
+// The gradient at the places of [start, start + length) that are not named, for a rest that
+// is relative to its own largest logit; `by`: the rest's p over its sum.
+template <int L, typename T>
+__device__ __forceinline__ void correct_rest(const Call<T>& c, Bits bits, int64_t row, int lane, int64_t start, int length, T row_top, T row_inverse, T rest_top,
+                                             T by, T weight) {
+  const auto scaled = c.scaled();
+  const T* logits = c.logits + row * c.vocab + start;
+  T* out = c.grad + row * c.vocab + start;
+  asm volatile("" : "+v"(lane));
+  for (int i = lane; i < length; i += L) {
+    const T z = logits[i];
+    if (!bits.one(i)) out[i] = (hpd::exp_down(scaled(z - row_top)) * row_inverse - hpd::exp_down(scaled(z - rest_top)) * by) * weight;
+  }
+}
+
 // REST: the rest of the teacher's mass is a class of its own.
 template <typename T, int L, int K, bool REST>
 __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L == 256 && K == 16 ? 3 : 4) void row_kernel(Call<T> c) {
@@ -166,7 +186,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
   constexpr int kWords = (L * K * S::W + 31) / 32;
   __shared__ Meet<T, S::kDeep, REST ? 2 : 1> meet;
   __shared__ unsigned words[kTeams][kWords];
-  __shared__ T told[2];  // by the wave of the list: rest, spoiled
+  __shared__ T told[2][2];  // by the wave of the list, for two rows in turn: rest, spoiled
   const int lane = kTeams == 1 ? int(threadIdx.x) : threadIdx.x % L, team = kTeams == 1 ? 0 : threadIdx.x / L;
   const bool lists = L <= 64 || threadIdx.x < 64;
   const int length = int(c.vocab);
@@ -194,7 +214,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
       list.read(c, row, lane);
       list.set(c, bits, row, lane, 0, length);
       if constexpr (L > 64) {
-        if (lane == 0) told[0] = list.rest, told[1] = list.spoiled;
+        if (lane == 0) told[turn][0] = list.rest, told[turn][1] = list.spoiled;
       } else {
         team_fence();
       }
@@ -203,11 +223,11 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
     T tops[S::kDeep], top, total, unlisted = T(0);
     if constexpr (REST) share.statistics(length, lane, meet, turn, tops, top, total, scaled, bits, unlisted);
     else share.statistics(length, lane, meet, turn, tops, top, total, scaled, NoNames(), unlisted);
-    turn ^= 1;
-    const T inverse = T(1) / total;
+    const T inverse = T(1) / total, rest = L > 64 ? told[turn][0] : list.rest;
+    const bool apart = REST && rest != T(0) && unlisted < kLeastSecond<T>;
+    const T weight = T(factor * c.inverse) + (L > 64 ? told[turn][1] : list.spoiled);
     if (out) {
-      const T rest = L > 64 ? told[0] : list.rest, weight = T(factor * c.inverse) + (L > 64 ? told[1] : list.spoiled);
-      const T inner = inverse * weight, outer = REST ? unlisted_factor(inverse, rest, unlisted) * weight : inner;
+      const T inner = inverse * weight, outer = REST && !apart ? unlisted_factor(inverse, rest, unlisted) * weight : inner;
       if constexpr (REST) {
         // Named ones carry a sign: -0 too, and NaN stays NaN.
         share.each(length, lane, [&](T& v, int, int d) {
@@ -220,10 +240,19 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
       share.store(out, length, lane);
       if constexpr (L > 64) __syncthreads();
       else team_fence();
-      if (lists) list.correct(c, row, lane, 0, length, top, inverse, weight);
     }
+    T rest_top = top;
+    if constexpr (REST) {
+      if (apart) {  // here, where the row's registers are free
+        S::apart(c.logits + row * c.vocab, length, lane, meet, turn, scaled, bits, rest_top, unlisted);
+        if (out && unlisted != T(0)) correct_rest<L>(c, bits, row, lane, 0, length, top, inverse, rest_top, rest / unlisted, weight);
+        if constexpr (L > 64) __syncthreads();  // before the list's bits are cleared
+      }
+    }
+    if (out && lists) list.correct(c, row, lane, 0, length, top, inverse, weight);
+    turn ^= 1;
     if (lists) {
-      const double loss = list.loss(c, row, lane, top, total, unlisted);
+      const double loss = list.loss(c, row, lane, top, total, rest_top, unlisted);
       if (lane == 0) c.losses[row] = T(loss), sum += loss;
       list.clear(c, bits, row, lane, 0, length);
       if constexpr (L <= 64) team_fence();
@@ -232,10 +261,16 @@ __global__ __launch_bounds__(L > 256 ? L : 256, sizeof(T) == 8 || K < 8 ? 1 : L 
   leave_loss(c, workgroup_sum(sum), factor, blockIdx.x, gridDim.x);
 }
 
-// Statistics of one piece of a row: parts[row * pieces + piece].
+// Statistics of pieces of rows, number row * pieces + piece.
+template <typename T>
+struct Statistics {
+  T *tops, *totals, *seconds;
+  T *rest_tops, *rests;  // the second sum relative to the largest of its own logits where it is small (Share::apart)
+  int pieces, length;    // of a row, of a piece
+};
+
 template <typename T, bool REST>
-__global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __restrict__ part_tops, T* __restrict__ part_totals,
-                                                              T* __restrict__ part_seconds, int pieces, int piece) {
+__global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, Statistics<T> parts) {
   using S = Share<T, kPieceThreads, kPieceLoads>;
   __shared__ Meet<T, 1, REST ? 2 : 1> meet;
   __shared__ unsigned words[REST ? kPieceThreads * kPieceLoads * S::W / 32 : 1];
@@ -246,27 +281,30 @@ __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __re
     __syncthreads();
   }
   int turn = 0;
-  for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
-    const int64_t row = part / pieces;
+  for (int64_t part = blockIdx.x; part < c.rows * parts.pieces; part += gridDim.x) {
+    const int64_t row = part / parts.pieces;
     if (!c.kept(row)) continue;
-    const int64_t start = (part - row * pieces) * piece;
-    const int length = piece_end(c.vocab - start, piece);
-    T tops[1], top, total, second;
+    const int64_t start = (part - row * parts.pieces) * parts.length;
+    const int length = piece_end(c.vocab - start, parts.length);
+    const T* logits = c.logits + row * c.vocab + start;
+    T tops[1], top, total, second, rest_top, rest;
     S share;
-    share.template load<true>(c.logits + row * c.vocab + start, length, threadIdx.x);
+    share.template load<true>(logits, length, threadIdx.x);
     List<T, 64> list;
     if constexpr (REST) {
       // Seen by all at the first of the statistics' barriers, and read before the second.
       if (threadIdx.x < 64) list.set(c, bits, row, threadIdx.x, start, length);
       share.statistics(length, threadIdx.x, meet, turn, tops, top, total, scaled, bits, second);
+      rest_top = top, rest = second;
+      if (second < kLeastSecond<T>) share.apart(logits, length, threadIdx.x, meet, turn, scaled, bits, rest_top, rest);
       if (threadIdx.x < 64) list.clear(c, bits, row, threadIdx.x, start, length);
     } else {
       share.statistics(length, threadIdx.x, meet, turn, tops, top, total, scaled, NoNames(), second);
     }
     turn ^= 1;
     if (threadIdx.x == 0) {
-      part_tops[part] = top, part_totals[part] = total;
-      if constexpr (REST) part_seconds[part] = second;
+      parts.tops[part] = top, parts.totals[part] = total;
+      if constexpr (REST) parts.seconds[part] = second, parts.rest_tops[part] = rest_top, parts.rests[part] = rest;
     }
   }
 }
@@ -274,40 +312,54 @@ __global__ __launch_bounds__(kPieceThreads) void stats_kernel(Call<T> c, T* __re
 // What a row's pieces add up to, by every wave for itself; a lane's pieces join first,
 // one after the other in 64 bits (join_pieces, with two sums).
 template <typename T, bool REST, typename Scale>
-__device__ __forceinline__ void join_row(const T* tops, const T* totals, const T* seconds, int pieces, Scale scaled, T& top, T& total, T& second) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void join_row(const Statistics<T>& parts, int64_t row, Scale scaled, T& top, T& total, T& rest_top, T& unlisted) {
+  int lane = threadIdx.x & 63;
+  const int pieces = parts.pieces;
+  const int64_t first = row * pieces;
   const T none = -T(__builtin_huge_val());
   const bool has = lane < pieces;
-  T own = has ? tops[lane] : none;
-  double sum = has ? totals[lane] : T(0), other = REST && has ? seconds[lane] : T(0);
-  for (int k = lane + 64; k < pieces; k += 64) {
-    const T next = larger(own, tops[k]);
-    const double before = own == none ? 1.0 : double(hpd::exp_down(scaled(own - next)));
-    const double here = tops[k] == none ? 1.0 : double(hpd::exp_down(scaled(tops[k] - next)));
-    sum = sum * before + double(totals[k]) * here;
-    if constexpr (REST) other = other * before + double(seconds[k]) * here;
-    own = next;
-  }
+  const auto add = [&](const T* tops, const T* sums, const T* others, T& own, double& sum, double& other) __attribute__((always_inline)) {
+    own = has ? tops[lane] : none;
+    sum = has ? sums[lane] : T(0), other = others && has ? others[lane] : T(0);
+    for (int k = lane + 64; k < pieces; k += 64) {
+      const T next = larger(own, tops[k]);
+      const double before = own == none ? 1.0 : double(hpd::exp_down(scaled(own - next)));
+      const double here = tops[k] == none ? 1.0 : double(hpd::exp_down(scaled(tops[k] - next)));
+      sum = sum * before + double(sums[k]) * here;
+      if (others) other = other * before + double(others[k]) * here;
+      own = next;
+    }
+  };
+  T own;
+  double sum, other;
+  add(parts.tops + first, parts.totals + first, REST ? parts.seconds + first : nullptr, own, sum, other);
   join(has, own, T(sum), top, total, scaled);
-  T again;
-  if constexpr (REST) join(has, own, T(other), again, second, scaled);
+  rest_top = top;
+  if constexpr (REST) {
+    T again;
+    join(has, own, T(other), again, unlisted, scaled);
+    if (unlisted < kLeastSecond<T>) {
+      asm volatile("" : "+v"(lane));  // as in Share::apart
+      add(parts.rest_tops + first, parts.rests + first, nullptr, own, sum, other);
+      join(has, own, T(sum), rest_top, unlisted, scaled);
+    }
+  }
 }
 
 // The rows' losses from their pieces, a workgroup each, as wide as piece_grad_kernel, so
 // that both add the losses in one order.
 template <typename T, bool REST>
-__global__ __launch_bounds__(kPieceThreads) void finish_kernel(Call<T> c, const T* __restrict__ part_tops, const T* __restrict__ part_totals,
-                                                               const T* __restrict__ part_seconds, int pieces) {
+__global__ __launch_bounds__(kPieceThreads) void finish_kernel(Call<T> c, Statistics<T> parts) {
   const double factor = scale_of(c);
   const int64_t row = blockIdx.x;
   double loss = 0;
   if (threadIdx.x < 64) {
     if (c.kept(row)) {
-      T top, total, unlisted = T(0);
-      join_row<T, REST>(part_tops + row * pieces, part_totals + row * pieces, part_seconds + row * pieces, pieces, c.scaled(), top, total, unlisted);
+      T top, total, rest_top, unlisted = T(0);
+      join_row<T, REST>(parts, row, c.scaled(), top, total, rest_top, unlisted);
       List<T, 64> list;
       list.read(c, row, threadIdx.x);
-      loss = list.loss(c, row, threadIdx.x, top, total, unlisted);
+      loss = list.loss(c, row, threadIdx.x, top, total, rest_top, unlisted);
     }
     if (threadIdx.x == 0) c.losses[row] = T(loss);
   }
@@ -317,8 +369,7 @@ __global__ __launch_bounds__(kPieceThreads) void finish_kernel(Call<T> c, const 
 // The gradient of one piece of a row from the statistics of its pieces, which every
 // workgroup joins for itself; that of the first piece leaves the row's loss.
 template <typename T, bool REST>
-__global__ __launch_bounds__(kPieceThreads) void piece_grad_kernel(Call<T> c, const T* __restrict__ part_tops, const T* __restrict__ part_totals,
-                                                                   const T* __restrict__ part_seconds, int pieces, int piece) {
+__global__ __launch_bounds__(kPieceThreads, sizeof(T) == 8 && REST ? 3 : 1) void piece_grad_kernel(Call<T> c, Statistics<T> parts) {
   using S = Share<T, kPieceThreads, kPieceLoads>;
   __shared__ unsigned words[kPieceThreads * kPieceLoads * S::W / 32];
   __shared__ T told[2];
@@ -328,11 +379,11 @@ __global__ __launch_bounds__(kPieceThreads) void piece_grad_kernel(Call<T> c, co
   for (unsigned i = threadIdx.x; i < sizeof(words) / 4; i += kPieceThreads) words[i] = 0;
   __syncthreads();
   const double factor = scale_of(c);
-  for (int64_t part = blockIdx.x; part < c.rows * pieces; part += gridDim.x) {
-    const int64_t row = part / pieces;
-    const bool first = part == row * pieces;
-    const int64_t start = (part - row * pieces) * piece;
-    const int length = piece_end(c.vocab - start, piece);
+  for (int64_t part = blockIdx.x; part < c.rows * parts.pieces; part += gridDim.x) {
+    const int64_t row = part / parts.pieces;
+    const bool first = part == row * parts.pieces;
+    const int64_t start = (part - row * parts.pieces) * parts.length;
+    const int length = piece_end(c.vocab - start, parts.length);
     T* out = c.grad + row * c.vocab + start;
     double loss = 0;
     S share;
@@ -344,18 +395,23 @@ __global__ __launch_bounds__(kPieceThreads) void piece_grad_kernel(Call<T> c, co
         list.set(c, bits, row, lane, start, length);
         if (lane == 0) told[0] = list.rest, told[1] = list.spoiled;
       }
-      T top, total, unlisted = T(0);
-      join_row<T, REST>(part_tops + row * pieces, part_totals + row * pieces, part_seconds + row * pieces, pieces, scaled, top, total, unlisted);
+      T top, total, rest_top, unlisted = T(0);
+      join_row<T, REST>(parts, row, scaled, top, total, rest_top, unlisted);
       __syncthreads();
       const T inverse = T(1) / total, weight = T(factor * c.inverse) + told[1];
-      const T inner = inverse * weight, outer = REST ? unlisted_factor(inverse, told[0], unlisted) * weight : inner;
+      const bool apart = REST && rest_top != top;
+      const T inner = inverse * weight, outer = REST && !apart ? unlisted_factor(inverse, told[0], unlisted) * weight : inner;
       share.each_named(length, lane, bits, [&](T& v, bool named, int) { v = hpd::exp_down(scaled(v - top)) * (!REST || named ? inner : outer); });
       share.store(out, length, lane);
       __syncthreads();
+      if (apart) {
+        if (told[0] != T(0) && unlisted != T(0)) correct_rest<kPieceThreads>(c, bits, row, lane, start, length, top, inverse, rest_top, told[0] / unlisted, weight);
+        __syncthreads();  // before the list's bits are cleared
+      }
       if (lane < 64) {
         list.correct(c, row, lane, start, length, top, inverse, weight);
         list.clear(c, bits, row, lane, start, length);
-        if (first) loss = list.loss(c, row, lane, top, total, unlisted);
+        if (first) loss = list.loss(c, row, lane, top, total, rest_top, unlisted);
       }
     } else {
       share.each(length, lane, [](T& v, int, int) { v = T(0); });
@@ -392,15 +448,16 @@ int64_t rows_pass(hp_ctx* ctx, hp::Scratch& scratch, Call<T>& c) {
   }
   const Pieces<T> pieces(c.rows, c.vocab);
   const int64_t parts = c.rows * pieces.count;
-  T *tops = scratch.take<T>(parts), *totals = scratch.take<T>(parts), *seconds = scratch.take<T>(REST ? parts : 1);
+  Statistics<T> found{scratch.take<T>(parts), scratch.take<T>(parts), nullptr, nullptr, nullptr, pieces.count, pieces.length};
+  if constexpr (REST) found.seconds = scratch.take<T>(parts), found.rest_tops = scratch.take<T>(parts), found.rests = scratch.take<T>(parts);
   const unsigned grid = loop_grid(parts);
   hp::require(c.rows <= hp::kMaxGrid, "too many long rows for one launch");
   blocks = unsigned(c.rows);
   plan_losses(ctx, scratch, c, blocks, c.grad ? grid : blocks);
-  stats_kernel<T, REST><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, seconds, pieces.count, pieces.length);
+  stats_kernel<T, REST><<<grid, kPieceThreads, 0, ctx->stream>>>(c, found);
   hp::check_launch("distillation statistics");
-  if (c.grad) piece_grad_kernel<T, REST><<<grid, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, seconds, pieces.count, pieces.length);
-  else finish_kernel<T, REST><<<blocks, kPieceThreads, 0, ctx->stream>>>(c, tops, totals, seconds, pieces.count);
+  if (c.grad) piece_grad_kernel<T, REST><<<grid, kPieceThreads, 0, ctx->stream>>>(c, found);
+  else finish_kernel<T, REST><<<blocks, kPieceThreads, 0, ctx->stream>>>(c, found);
   hp::check_launch("distillation losses");
   return blocks;
 }

@@ -85,14 +85,14 @@ struct Unscaled {
   }
 };
 
-// (m, S) of a row from those of pieces in the lanes that have one.
-template <typename T, typename Scale = Unscaled>
+// (m, S) of a row from those of pieces in the lanes that have one, of L lanes.
+template <int L = 64, typename T, typename Scale = Unscaled>
 __device__ __forceinline__ void join(bool has, T piece_top, T piece_total, T& top, T& total, Scale scaled = {}) {
   const T none = -T(__builtin_huge_val());
-  top = team_reduce<64>(has ? piece_top : none, [](T a, T b) { return larger(a, b); });
+  top = team_reduce<L>(has ? piece_top : none, [](T a, T b) { return larger(a, b); });
   T part = T(0);
   if (has) part = piece_top == none ? piece_total : piece_total * hpd::exp_down(scaled(piece_top - top));
-  total = team_reduce<64>(part, [](T a, T b) { return a + b; });
+  total = team_reduce<L>(part, [](T a, T b) { return a + b; });
 }
 
 // The same from memory, by every wave for itself; a lane's pieces join first, one after
@@ -123,6 +123,12 @@ struct Meet {
 struct NoNames {
   static constexpr bool some = false;
 };
+
+// A second sum (Share::statistics) below this is formed again, relative to the largest of its own logits: relative to
+// the row's its terms have left the type, or are about to. Above it the terms that an exponential rounds to
+// zero (2^-126, 2^-1022 and less each, of no more than 2^31 logits) are 2^-31 of it at most.
+template <typename T>
+constexpr T kLeastSecond = sizeof(T) == 4 ? T(0x1p-64f) : T(0x1p-900);
 
 // A team's share of a row of `length` elements, which it takes in pieces of
 // kPieceThreads x kPieceLoads vectors: kSide pieces side by side by 256 threads each,
@@ -315,6 +321,57 @@ struct Share {
         if (has) part = of_waves(meet.seconds[turn][d], side, plus);
         join(has, piece_top, part, again, second, scaled);
       }
+    }
+  }
+
+  // A second sum of less than kLeastSecond, from another reading of `row`: sum exp(scaled(z - top)) of the values that
+  // `names` leaves out, of which `top` is the largest (-inf and 0 of none). Of several pieces those whose own sum is not as
+  // small keep it. For a whole team, with what statistics() left in `meet`; its other set is free for this.
+  template <typename Scale, typename Names>
+  __device__ __forceinline__ static void apart(const T* row, int length, int lane, Meet<T, kDeep, 2>& meet, int turn, Scale scaled, Names names, T& top, T& sum) {
+    constexpr T kNone = -T(__builtin_huge_val());
+    constexpr int kPiece = kStep * kLoads * W;
+    const auto greater = [](T a, T b) { return larger(a, b); };
+    const auto plus = [](T a, T b) { return a + b; };
+    asm volatile("" : "+v"(lane));  // what follows from it is formed here, not kept from row to row
+#pragma unroll 1
+    for (int d = 0; d < kDeep; ++d) {
+      const int side = kSide > 1 ? lane / kStep : 0, start = (d * kSide + side) * kPiece;
+      T own = kNone, part = T(0);
+      if (kSide * kDeep == 1 || of_waves(meet.seconds[turn][d], side, plus) < kLeastSecond<T>) {
+        for (int i = start + lane % kStep; i < length && i < start + kPiece; i += kStep) {
+          const T z = row[i];
+          if (names.one(i) || z == kNone) continue;
+          if (z > own) part = part * hpd::exp_down(scaled(own - z)) + T(1), own = z;
+          else part += hpd::exp_down(scaled(z - own));
+        }
+      }
+      join<L < 64 ? L : 64>(true, own, part, top, sum, scaled);
+      if constexpr (L > 64) {
+        if ((lane & 63) == 0) meet.tops[turn ^ 1][d][lane >> 6] = top, meet.seconds[turn ^ 1][d][lane >> 6] = sum;
+      }
+    }
+    if constexpr (L > 64) {
+      __syncthreads();
+      const auto joined = [&](int d, int side) {  // from the four waves of a piece
+        const T *tops = meet.tops[turn ^ 1][d] + 4 * side, *sums = meet.seconds[turn ^ 1][d] + 4 * side;
+        top = of_waves(tops - 4 * side, side, greater), sum = T(0);
+        for (int w = 0; w < 4; ++w) sum += tops[w] == kNone ? T(0) : sums[w] * hpd::exp_down(scaled(tops[w] - top));
+      };
+      if constexpr (kSide * kDeep == 1) {
+        joined(0, 0);
+      } else {
+        const int k = lane & 63, d = k / kSide, side = k % kSide;
+        const bool has = k <= rest_piece(length);
+        T piece_top = kNone, piece_sum = T(0);
+        if (has) {
+          piece_top = of_waves(meet.tops[turn][d], side, greater);
+          piece_sum = of_waves(meet.seconds[turn][d], side, plus);
+          if (piece_sum < kLeastSecond<T>) joined(d, side), piece_top = top, piece_sum = sum;
+        }
+        join(has, piece_top, piece_sum, top, sum, scaled);
+      }
+      __syncthreads();  // the set belongs to the next row
     }
   }
 

@@ -354,13 +354,13 @@ def distillation_loss(logits, indices, teacher_logits, teacher_rest, mask, tempe
         log_p = t - t.max(-1, keepdims=True)
         log_p = log_p - np.log(np.exp(log_p).sum(-1, keepdims=True))
         p = np.exp(log_p)
-        z = np.where(kept[..., None], logits, 0)
-        top = z.max(-1, keepdims=True)
+        logits = np.where(kept[..., None], logits, 0)
+        top = logits.max(-1, keepdims=True)
         live = t[..., : indices.shape[-1]] != -np.inf
         named = live & (indices >= 0) & (indices < vocab)
         at = np.where(named, indices, 0)
-        apart = (np.take_along_axis(z, at, -1).astype(np.float64) - top) / temperature
-        z = np.exp((z - top) * dtype.type(1 / temperature))
+        apart = (np.take_along_axis(logits, at, -1).astype(np.float64) - top) / temperature
+        z = np.exp((logits - top) * dtype.type(1 / temperature))
         total = z.sum(-1, keepdims=True)
         log_total = np.log(total.astype(np.float64))
         log_q = apart - log_total
@@ -369,8 +369,13 @@ def distillation_loss(logits, indices, teacher_logits, teacher_rest, mask, tempe
             one = listed.reshape(-1, vocab)
             one[np.arange(len(one)), at[..., k].reshape(-1)] |= named[..., k].reshape(-1)
         if teacher_rest is not None:
-            unlisted = np.where(listed, 0, z).sum(-1, keepdims=True).astype(np.float64)
-            log_q = np.concatenate([log_q, np.log(unlisted) - log_total], -1)
+            # Relative to its own largest logit: relative to the row's all of it may be less than the type has.
+            others = np.where(listed, -np.inf, logits).astype(dtype)
+            other_top = others.max(-1, keepdims=True)
+            others = np.exp((others - np.where(other_top == -np.inf, 0, other_top).astype(dtype)) * dtype.type(1 / temperature))
+            unlisted = others.sum(-1, keepdims=True)
+            log_unlisted = (other_top.astype(np.float64) - top) / temperature + np.log(unlisted.astype(np.float64))
+            log_q = np.concatenate([log_q, log_unlisted - log_total], -1)
         losses = np.where(p != 0, p * (log_p - log_q), 0).sum(-1)
         losses = np.where((live & ~named).any(-1) | np.isnan(p).any(-1), np.nan, losses)
         losses = np.where(kept, losses, 0)
@@ -381,11 +386,11 @@ def distillation_loss(logits, indices, teacher_logits, teacher_rest, mask, tempe
             return loss.reshape(-1), losses.astype(dtype).reshape(-1), None
         weight = (kept / (count * temperature))[..., None]
         lost = np.isnan(losses)[..., None]
-        outside = 1 / total
+        grad = z / total
         if teacher_rest is not None:
             rest = p[..., -1:]
-            outside = outside - np.where((rest == 0) | (unlisted == 0), 0, rest / unlisted)
-        grad = np.where(listed, z / total, z * outside) * weight
+            grad = grad - np.where(listed | (rest == 0) | (unlisted == 0), 0, rest * (others / unlisted))
+        grad = grad * weight
         for k in range(indices.shape[-1]):
             rows = grad.reshape(-1, vocab)
             rows[np.arange(len(rows)), at[..., k].reshape(-1)] -= np.where(named[..., k] & (p[..., k] != 0), p[..., k] * weight[..., 0], 0).reshape(-1)
