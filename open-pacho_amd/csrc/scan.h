@@ -62,8 +62,12 @@ struct Several {
 // by 2^-24 of an exponent whose power is at most 0.37 of its inverse, so by half a unit of 1.
 __device__ __forceinline__ float decay(float dt, float rate) { return __builtin_amdgcn_exp2f(dt * rate); }
 __device__ __forceinline__ double decay(double dt, double rate) { return exp(dt * rate); }
-__device__ __forceinline__ float rate_of(float a_log) { return -(expf(a_log) * 0x1.715476p+0f); }
-__device__ __forceinline__ double rate_of(double a_log) { return -exp(a_log); }
+// Rates end at the type's largest number: in steps that have a dt of 0 to change nothing an infinite one
+// would make NaN, as it would of a decay of 0 in the gradients. A NaN stays one.
+__device__ __forceinline__ float bounded(float rate) { return rate > 0x1.fffffep+127f ? 0x1.fffffep+127f : rate; }
+__device__ __forceinline__ double bounded(double rate) { return rate > 0x1.fffffffffffffp+1023 ? 0x1.fffffffffffffp+1023 : rate; }
+__device__ __forceinline__ float rate_of(float a_log) { return -bounded(expf(a_log) * 0x1.715476p+0f); }
+__device__ __forceinline__ double rate_of(double a_log) { return -bounded(exp(a_log)); }
 // A state passes parts however small the product of its decays is: infinite ones stay so.
 template <typename T>
 __device__ __forceinline__ T passed_decay(T span, T rate) {

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     rate[s] = rate_of(slow[s]);
-    slow[s] = sizeof(T) == 4 ? -T(expf(float(slow[s]))) : rate[s];
+    slow[s] = sizeof(T) == 4 ? -T(bounded(expf(float(slow[s])))) : rate[s];
     e[s] = da[s] = T(0);
   }
   T arrived[S] = {};

@@ -144,7 +144,8 @@ class _Scan(_Sequence):
         with np.errstate(all="ignore"):
             self.raw = delta if delta_bias is None else delta + _view(delta_bias)
             self.dt = (np.maximum(self.raw, 0) + np.log1p(np.exp(-np.abs(self.raw)))).astype(self.x.dtype)
-            self.rates = np.exp(_view(a_log))
+            # Past the type's largest number a decay of 0 times an infinite rate would be NaN.
+            self.rates = np.minimum(np.exp(_view(a_log)), np.finfo(self.x.dtype).max)
 
     def wide(self, projected):
         """(batch, groups, states) for every channel."""
