@@ -68,12 +68,18 @@ __device__ __forceinline__ float bounded(float rate) { return rate > 0x1.fffffep
 __device__ __forceinline__ double bounded(double rate) { return rate > 0x1.fffffffffffffp+1023 ? 0x1.fffffffffffffp+1023 : rate; }
 __device__ __forceinline__ float rate_of(float a_log) { return -bounded(expf(a_log) * 0x1.715476p+0f); }
 __device__ __forceinline__ double rate_of(double a_log) { return -bounded(exp(a_log)); }
-// A state passes parts however small the product of its decays is: infinite ones stay so.
+// What a state is behind steps whose dt add up to `span` (cut_span(): a reset is among them) and which end in
+// `end` from nothing. An infinite one passes them also where the product of their decays is 0 in the type, though
+// none of them is.
 template <typename T>
-__device__ __forceinline__ T passed_decay(T span, T rate) {
-  const T least = sizeof(T) == 4 ? T(0x1p-126f) : T(0x1p-1022);
-  const T found = decay(span, rate);
-  return found < least ? least : found;
+__device__ __forceinline__ T passed(T span, T rate, T state, T end) {
+  T kept = decay(span, rate);
+  kept = kept == T(0) && __builtin_elementwise_abs(state) == T(__builtin_huge_val()) ? T(1) : kept;
+  T behind = __builtin_elementwise_fma(kept, state, end);
+  // Formed by all lanes, without a branch: where registers are short the compiler has put a copy of another value
+  // behind such a branch, before the lanes that skipped it are back (tests/test_build_exec.py looks for that).
+  asm("" : "+v"(behind));
+  return span < T(0) ? end : behind;
 }
 
 // What a workgroup and its lanes work on.
@@ -149,7 +155,7 @@ struct Place {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const T end = state_line(c, c.ended, p, s)[channel];
-        h[s] = span < T(0) ? end : __builtin_elementwise_fma(passed_decay(span, rate[s]), h[s], end);
+        h[s] = passed(span, rate[s], h[s], end);
       }
     }
   }

@@ -268,7 +268,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const T back = at.state_line(c, c.passed, p, s)[at.channel];
-        e[s] = span < T(0) ? back : __builtin_elementwise_fma(passed_decay(span, rate[s]), e[s], back);
+        e[s] = passed(span, rate[s], e[s], back);
       }
     }
   } else if (c.grad_state) {
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(NW * 64) void backward_kernel(Scan<T> c, Grads<T> o
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       r.start[s] = ahead.before[s];
-      if (c.parts > 1) r.start[s] = ahead.since < T(0) ? r.start[s] : __builtin_elementwise_fma(passed_decay(ahead.since, rate[s]), arrived[s], r.start[s]);
+      if (c.parts > 1) r.start[s] = passed(ahead.since, rate[s], arrived[s], r.start[s]);
       if (!at.valid) r.start[s] = T(0);
     }
     r.b = ahead.b, r.c = ahead.c;
