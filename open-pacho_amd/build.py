@@ -38,6 +38,8 @@ FLAGS = [
     "-packed-fp32-ops",
     "-Wall",
     "-Wno-unused-function",
+    # Rows of any length follow each other: a vector that is taken for an aligned one is a mistake.
+    "-Werror=align-mismatch",
     f"-I{REPO / 'include'}",
     f"-I{CSRC}",
 ]

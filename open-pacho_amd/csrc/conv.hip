@@ -57,7 +57,7 @@ struct Value {
 #pragma unroll
       for (int j = 0; j < W; ++j) to[j] = v[j];
     }
-    hpd::put(reinterpret_cast<typename Lane<T, W>::type*>(at), to, past);
+    hpd::put(at, to, past);
   }
 };
 

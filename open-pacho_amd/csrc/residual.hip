@@ -93,7 +93,7 @@ struct Part {
 #pragma unroll
         for (int j = 0; j < W; ++j) to[j] = v[k][j];
       }
-      hpd::put(reinterpret_cast<V*>(row + start(k, length, lane)), to, past);
+      hpd::put(row + start(k, length, lane), to, past);
     }
   }
   // f(k, j) for every value.

@@ -13,9 +13,12 @@ __device__ __forceinline__ int64_t by_die() {
   return int64_t(die) * least + (die < more ? die : more) + blockIdx.x / kDies;
 }
 
-// Stores `value`; with `past` the caches keep no place for it.
-template <typename V>
-__device__ __forceinline__ void put(V* at, V value, bool past) {
+// Stores `value`, a T or a vector of them, which is aligned as its elements are; with `past` the caches keep no
+// place for it.
+template <typename T, typename V>
+__device__ __forceinline__ void put(T* first, V value, bool past) {
+  typedef V Unaligned __attribute__((aligned(sizeof(T))));
+  Unaligned* const at = reinterpret_cast<Unaligned*>(first);
   if (past) {
     asm volatile("");  // else the compiler joins the two stores into a plain one, and without the other from behind
     __builtin_nontemporal_store(value, at);
