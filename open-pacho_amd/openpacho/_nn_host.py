@@ -348,10 +348,15 @@ def distillation_loss(logits, indices, teacher_logits, teacher_rest, mask, tempe
     kept = np.ones(indices.shape[:-1], bool) if mask is None else _view(mask)
     dtype, vocab = logits.dtype, logits.shape[-1]
     with np.errstate(all="ignore"):
-        # The terms of a list in 64 bits; rows that are left out as zeros.
-        t = np.where(kept[..., None], teacher, 0).astype(np.float64) / temperature
+        # The terms of a list in 64 bits; rows that are left out as zeros. Distances from the list's largest logit
+        # are divided by the temperature, as the quotients' own distances would have lost digits.
+        t = np.where(kept[..., None], teacher, 0).astype(np.float64)
+        base = t.max(-1, keepdims=True)
+        base = np.where(base == -np.inf, 0, base)
+        t = (t - base) / temperature
         if teacher_rest is not None:
-            t = np.concatenate([t, np.where(kept, _view(teacher_rest), 0).astype(np.float64)[..., None]], -1)
+            rest = np.where(kept, _view(teacher_rest), 0).astype(np.longdouble)[..., None]
+            t = np.concatenate([t, (rest - base.astype(np.longdouble) / temperature).astype(np.float64)], -1)
         log_p = t - t.max(-1, keepdims=True)
         log_p = log_p - np.log(np.exp(log_p).sum(-1, keepdims=True))
         p = np.exp(log_p)
