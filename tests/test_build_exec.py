@@ -25,30 +25,25 @@ WHOLE_WAVE = ("v_readlane", "v_writelane", "v_readfirstlane")  # whatever EXEC i
 def lost_copies(lines):
     """(kernel, label, instructions) of every block as above in a disassembly with labels for its branches."""
     lines = [line.split("//")[0].strip() for line in lines]
-    kernel, label, early, found = None, None, [], []
-    joins = set()  # of this kernel: labels are its own
-    for number, line in enumerate(lines):
-        head = re.fullmatch(r"(?:[0-9a-f]+ )?<(\S+)>:", line)
-        if head and not re.fullmatch(r"L\d+", head.group(1)):
-            kernel, label = head.group(1), None
-            joins = set()
-            for other in lines[number + 1 :]:
-                if re.fullmatch(r"(?:[0-9a-f]+ )?<(?!L\d+>)\S+>:", other):
+    heads = [(n, m.group(1)) for n, line in enumerate(lines) if line.endswith(">:") for m in [re.search(r"<(\S+)>:$", line)]]
+    labels = {n: name for n, name in heads if re.fullmatch(r"L\d+", name)}
+    kernels = [(n, name) for n, name in heads if n not in labels] + [(len(lines), None)]
+    found = []
+    for (start, kernel), (end, _) in zip(kernels, kernels[1:]):
+        joins = {line.split()[1] for line in lines[start:end] if line.startswith("s_cbranch_execz")}  # labels are a kernel's own
+        for at in range(start, end):
+            if labels.get(at) not in joins:
+                continue
+            early = []
+            for line in lines[at + 1 : end]:
+                if line.startswith("s_or_b64 exec, exec,"):
+                    if early:
+                        found.append((kernel, labels[at], early))
                     break
-                branch = re.match(r"s_cbranch_execz (\S+)", other)
-                if branch:
-                    joins.add(branch.group(1))
-        elif head:
-            label, early = head.group(1) if head.group(1) in joins else None, []
-        elif label and line:
-            if re.match(r"s_or_b64 exec, exec,", line):
-                if early:
-                    found.append((kernel, label, early))
-                label = None
-            elif line.startswith(("s_cbranch", "s_branch", "s_endpgm")) or "exec" in line:
-                label = None
-            elif line.startswith(PER_LANE) and not line.startswith(WHOLE_WAVE):
-                early.append(line)
+                if line.startswith(("s_cbranch", "s_branch", "s_endpgm")) or "exec" in line or line.endswith(">:"):
+                    break
+                if line.startswith(PER_LANE) and not line.startswith(WHOLE_WAVE):
+                    early.append(line)
     return found
 
 
