@@ -9,8 +9,9 @@
 // are not complete yet, through the K - 1 steps behind its run. So only the K - 1 steps
 // around a run are read twice. What a step must not see has left the registers: a reset
 // clears the inputs before it, and a count of visible steps holds its gradient back.
-// Runs' sums for weights and bias meet in the runs' order. Forward 2 x 16387 x 1001 with three taps takes 41 us
-// (6.4 TB/s, partly from the caches), backward 8 x 4096 x 2048 with four 190 (4.2 TB/s).
+// Runs' sums for weights and bias meet in the runs' order. Forward 2 x 16387 x 1001 with three taps takes 40 us
+// (6.5 TB/s, partly from the caches), 8 x 4096 x 2048 with four 130 (4.1 TB/s), backward 202 (4.0 TB/s); as many bytes
+// of doubles 128 and 184.
 #include <type_traits>
 
 #include "exponential.h"
@@ -403,7 +404,8 @@ int hp_causal_conv_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* gra
       c.grad = static_cast<const T*>(grad);
       c.dx = static_cast<T*>(dx);
       c.dinitial = static_cast<T*>(dinitial);
-      // Three arrays, of which the caches would hold none to its next reader: 200 us -> 194 of 8 x 4096 x 2048 float32.
+      // Three arrays, of which the caches would hold none to its next reader: 209 us -> 202 of 8 x 4096 x 2048 float32,
+      // in turn on one card.
       c.past = batch * time * channels * int64_t(3 * sizeof(T)) > hp::kLastCache;
       with_width<T>(channels, [&](auto w) {
         const unsigned blocks = plan(c, w, 64);

@@ -9,16 +9,20 @@
 //
 // with R the sum S without the terms that the list names. R is formed as a sum of its
 // own, not as a difference: where the list holds nearly all of q the rest would lose
-// its digits. Where the list holds all that the type has of q, R is formed again, relative to the largest
-// logit m' that it does not name (Share::apart): log R = (m' - m) / T + log R', and
+// its digits. Where the list holds all that the type has of q, R is formed again, relative to
+// the largest logit m' that it does not name (Share::apart): log R = (m' - m) / T + log R', and
 // exp((z_j - m') / T) / R' takes its place in the gradient. Such rows are read again, and
-// their gradient is stored twice: 8192 x 32000 with 64 entries takes 332 us where no row is so and 1001 where all are. Which logits are named stands in a bit for each of a row, in LDS; a vector's
+// their gradient is stored twice: 8192 x 32000 with 64 entries takes 332 us where no row is
+// so and 1001 where all are.
+//
+// Which logits are named stands in a bit for each of a row, in LDS; a vector's
 // bits are one read, and where a team holds the row the only one: named exponentials carry
 // a sign from there on. (A second read for the gradient, and the bits of all vectors at
 // once, took the values' registers: 451 us in place of 361.) Bound: HBM, each logit read once
 // and each gradient written once, as for the losses of token_loss.hip, whose teams and
 // pieces of rows it shares. 8192 x 32000 float32 with 64 entries and the rest takes
-// 310-361 us with the gradient (5.8-6.8 TB/s).
+// 310-361 us with the gradient (5.8-6.8 TB/s) and 126 without, where a mask leaves rows out that are then not
+// read; 4096 x 32000 float64 588 and 160.
 //
 // The list is the work of one wave, or of a team within one: its softmax, its bits and
 // its terms of the loss, each entry's logit read again. The named places of the

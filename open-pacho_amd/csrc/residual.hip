@@ -13,7 +13,8 @@
 // holds a row in K vectors of 16 bytes of each array, so that each is read once: the
 // squares of x give rms'', then those of the stream rms'. Rows that no team holds are
 // read again from the caches (long_*_kernel). Backward 8 x 4096 x 2048 float32 with a gate
-// for each token takes 411 us (5.2 TB/s).
+// for each token takes 411-424 us (5.1-5.2 TB/s), forward with one for each channel 194 (5.5 TB/s); rows that no team
+// holds, 2048 x 12288, 324 and 143, 3 and 2 times what their bytes would.
 //
 // Backward a team (a worker) takes a run of neighbouring rows and sums over them in
 // registers; the workers' sums meet in worker order (sums_kernel), so that results
@@ -430,8 +431,8 @@ void forward(hp_ctx* ctx, const Norm<T>& c) {
 template <typename T>
 void backward(hp_ctx* ctx, Norm<T> c, T* dweight, T* dpost) {
   hp::Scratch scratch(ctx);
-  // Six arrays, of which the caches would hold none to its next reader: 430 us -> 424 of 8 x 4096 x 2048 float32, and of
-  // rows that are no whole lines 87 -> 72 (3 x 1367 x 1537 float64).
+  // Six arrays, of which the caches would hold none to its next reader: 429 us -> 422 of 8 x 4096 x 2048 float32, and of
+  // rows that are no whole lines 86 -> 74 (3 x 1367 x 1537 float64), each in turn on one card.
   c.past = c.rows * c.channels * int64_t(6 * sizeof(T)) > hp::kLastCache;
   const int64_t groups = c.gate ? c.rows / c.divide : 0;
   const auto plan = [&](int64_t most) {

@@ -7,9 +7,9 @@
 // channels that share b and c. So b and c are the same in a whole wave: a register holds
 // those of four steps in the lanes of each row of 16, and an instruction that multiplies by
 // one of them takes it from its lane on the way (a row broadcast). Bound: vector issue. An
-// exponential, two products and two fused multiply-adds make a state's step: 213 us for 8 x 2048 x
-// 2048 float32 with 16 states, whose bytes would take 89. (Scalar loads of b and c in
-// each step, whose waits no other work covers, took 1458.) Two states a wave leave enough
+// exponential, two products and two fused multiply-adds make a state's step, 10.4 instructions with its
+// share of the rest: 8 x 2048 x 2048 float32 with 16 states takes 230 us, of which 159 are issue, and whose bytes
+// would take 89. (Scalar loads of b and c in each step, whose waits no other work covers, took 1458.) Two states a wave leave enough
 // waves; from 17 states on (33 forward in 16 waves) four save the steps' common work. Only the sums over states meet in LDS, once for a tile of
 // steps: each wave has some of the tile's steps as its own, whose dt and dt x it leaves for
 // all waves before they walk the tile, and whose sums it adds up afterwards. Steps of a
@@ -242,9 +242,11 @@ const T* scan_padded(hp_ctx* ctx, Scratch& scratch, const T* array, int64_t step
 template <typename T>
 void scan_fill(hp_ctx* ctx, T* to, const T* from, int64_t n);
 
-// Parts of rows: one, or as many as make enough workgroups. 128 workgroups in four parts each take 166 us
-// forward and 458 backward where whole rows take 230 and 732 (4 x 2048 x 2048 float32, 16 states); 256 in
-// two parts lose more in the launch before than they gain (380 against 250, and 1371 against 1188).
+// Parts of rows: one, or as many as make enough workgroups. 128 workgroups in four parts each take 165 us
+// forward and 455 backward where whole rows take 230 and 732 (4 x 2048 x 2048 float32, 16 states); 256 in
+// two parts lose more in the launch before than they gain (380 against 250, and 1371 against 1188). Whole rows of 160,
+// 192 and 224 workgroups take 228 and 734-739, in two parts 308-311 and 840-851, in three 277-279 and
+// 861-869 of the last two; three of 160, which fill the chip twice as 128 in four do, would take 217 and 589.
 template <typename T>
 void scan_plan(hpd::Scan<T>& c, int tile) {
   const int64_t blocks = int64_t(c.batch) * c.groups * c.pieces, tiles = ceil_div(c.time, tile);

@@ -1,5 +1,5 @@
-// The selective scan forward (scan.h). Bound: the exponentials of 16 states a channel,
-// about as long as reading x, delta and the gate and writing y takes; for fewer states HBM.
+// The selective scan forward (scan.h). Bound: vector issue, 68% of the SIMDs' cycles for 16 states a
+// channel; waves wait 30% of their time.
 #include "scan.h"
 
 using namespace hpd;

@@ -17,8 +17,9 @@
 // until a register holds a sum in each lane: two or three instructions a value where a sum over
 // 64 lanes by itself takes six times two. Workgroups leave these, and their sums over steps, as parts.
 //
-// Bound: vector issue, 29 instructions a state and step. 8 x 2048 x 2048 float32 with 16 states: 175 us
-// for the first launch, 630-660 for the second, 20 for db and dc, where the call's bytes would take 155.
+// Bound: vector issue, 29 instructions a state and step (32 with resets), 73-76% of the SIMDs' cycles. 8 x 2048 x
+// 2048 float32 with 16 states and resets: 172-184 us for the first launch, 625-671 for the second, 20 for
+// db and dc, where the call's bytes would take 155; 740 in all without resets.
 //
 // Where rows are cut into parts, the first launch also forms what a part passes back from
 // nothing, sum_t D_t c_t g_t with D_t the product of the decays up to t.

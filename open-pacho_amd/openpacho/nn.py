@@ -435,6 +435,8 @@ def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale=1.0
     place of rms(x) post_weight; without ``gate`` it is one. ``gate`` has the
     channels, and any number of x's leading axes followed by axes of 1: one
     factor for each token and channel, each sequence and channel, or each channel.
+    The mean of the squares is formed in the arrays' dtype: a row that it overflows
+    (values past 1.8e19 in float32) has an rms(v) of zero.
     """
     what = "residual_norm"
     ops, x, weight, post_weight, gate, sizes = _norm_operands(what, x, residual, weight, post_weight, gate, scale, eps)
@@ -458,6 +460,7 @@ def residual_norm_grad(grad_stream, grad_normed, x, stream, weight, *, post_weig
     found = ops.backend.residual_norm_grad(grad_stream, grad_normed, x, stream, weight, post_weight, gate, *sizes)
     like = (x, x, weight, post_weight, gate)
     return tuple(None if array is None else ops.result(data, array._shape) for data, array in zip(found, like))
+
 
 # ---- losses from logits ----------------------------------------------------------
 
@@ -603,6 +606,7 @@ def distillation_loss(logits, indices, teacher_logits, teacher_rest=None, *, mas
 def distillation_loss_grad(logits, indices, teacher_logits, teacher_rest=None, *, mask=None, temperature=1.0, count=None):
     """``distillation_loss`` and its gradient: (loss, losses of the tokens, gradient of the logits)."""
     return _distillation("distillation_loss_grad", True, logits, indices, teacher_logits, teacher_rest, mask, temperature, count)
+
 
 # ---- AdamW ---------------------------------------------------------------------
 
