@@ -314,7 +314,7 @@ int hp_causal_conv_grad(hp_ctx* ctx, int dtype, int index_dtype, const void* gra
 
 /* A selective state space scan of x (batch, time, channels): with
  * dt = softplus(delta + delta_bias) each channel's 1 to 256 states are
- * h_t = exp(-dt exp(a_log)) h_{t-1} + dt x_t b_t, and
+ * h_t = exp(-dt exp(a_log)) h_{t-1} + dt x_t b_t (exp(a_log) at most the type's largest number), and
  * y_t = (sum c_t h_t + skip x_t) gate_t sigmoid(gate_t), without the last factor if
  * gate is NULL. delta and gate as x; a_log (channels, states); b, c (batch, time,
  * groups, states), whose groups divide the channels; skip, delta_bias (channels) or

@@ -334,7 +334,8 @@ def selective_scan(x, delta, a_log, b, c, skip=None, gate=None, initial=None, *,
     With ``dt = softplus(delta + delta_bias)`` each channel has ``states`` states
     ``h_t = exp(-dt exp(a_log)) h_{t-1} + dt x_t b_t`` and
     ``y_t = (sum c_t h_t + skip x_t) gate_t sigmoid(gate_t)``, without the last
-    factor if ``gate`` is not given. Shapes: x, delta, gate (..., time, channels);
+    factor if ``gate`` is not given; ``exp(a_log)`` ends at the dtype's largest number.
+    Shapes: x, delta, gate (..., time, channels);
     a_log (channels, states), of 1 to 256 states; b, c (..., time, groups, states),
     whose groups divide the channels; skip, delta_bias (channels,); ``initial``
     (..., channels, states), the states before the first step, zero if not
